@@ -275,6 +275,61 @@ int gl_peak_normalise_static(float* x, long long row_stride, long long len, floa
 int gl_pcm16_encode(gl_plan* plan, const float* x, long long row_stride, long long len, int16_t* pcm,
                     long long pcm_stride, float* peaks, int B, void* stream);
 
+/* ---- learned mel inversion -----------------------------------------------------------------------------------
+ * The reference inverts mel -> linear with one fixed basis (griffin_lim.py:18-19); a learned inversion takes the
+ * log-mel frames the decoder emits (and gl_wav_to_logmel makes, next to the magnitudes to learn from) through dense
+ * layers with group norms between them.  NO COUNTERPART IN THE REFERENCE.  These calls need no plan: they run on
+ * the current device, and scratch is the caller's -- `workspace`, at least gl_*_workspace(...) bytes, 16-byte
+ * aligned, not shared with a call that may run at the same time (so two captured graphs never share hidden state).
+ * They only enqueue kernels: no allocation, no memset node, legal inside a stream capture.  Results do not depend
+ * on timing (no floating-point atomics): equal calls give equal bits.
+ *   dtype of x, weight, bias and gradients: GL_F32, GL_BF16 or GL_F16; sums are 32-bit.
+ *   out_dtype of y, residual, preactivation and dy: dtype, or GL_F32.
+ *   Rows are frames; row strides are in elements, the elements of a row are contiguous.  A row stride may exceed
+ *   the row; elements between rows are neither read into results nor written.                                   */
+enum gl_dtype { GL_F32 = 0, GL_BF16 = 1, GL_F16 = 2 };
+enum gl_activation { GL_ACT_NONE = 0, GL_ACT_RELU = 1, GL_ACT_SILU = 2, GL_ACT_GELU = 3, GL_ACT_TANH = 4, GL_ACT_EXP = 5 };
+
+/* y[r][n] = act(sum_k x[r][k] * weight[n][k] + bias[n]) + residual[r][n], rounded once.
+ *   x [rows][inputs], weight [outputs][inputs], bias [outputs] or NULL, residual [rows][outputs] or NULL,
+ *   y [rows][outputs] (may be the residual itself), preactivation [rows][outputs] or NULL: receives the sum with the
+ *   bias, before act and residual (what gl_dense_backward needs).  gelu is z * Phi(z) (erf form).  rows may be 0. */
+long long gl_dense_workspace(long long rows, int inputs, int outputs, int dtype, int out_dtype);
+int gl_dense(const void* x, long long x_stride, const void* weight, long long w_stride, const void* bias,
+             const void* residual, long long r_stride, void* y, long long y_stride, void* preactivation,
+             long long z_stride, long long rows, int inputs, int outputs, int dtype, int out_dtype, int activation,
+             void* workspace, long long workspace_bytes, void* stream);
+
+/* Gradients of gl_dense: dz = dy * act'(preactivation) (rounded to dtype for the products),
+ *   dx[r][k] = sum_n dz[r][n] weight[n][k],  dweight[n][k] = sum_r dz[r][n] x[r][k],  dbias[n] = sum_r dz[r][n]
+ *   (of the unrounded dz).  dx, dweight, dbias: NULL = not wanted (x may be NULL without dweight, weight without dx).
+ *   The residual's gradient is dy.  preactivation may be NULL for GL_ACT_NONE.  rows == 0 writes zero sums.       */
+long long gl_dense_backward_workspace(long long rows, int inputs, int outputs, int dtype, int out_dtype, int activation);
+int gl_dense_backward(const void* dy, long long dy_stride, const void* x, long long x_stride, const void* weight,
+                      long long w_stride, const void* preactivation, long long z_stride, void* dx, long long dx_stride,
+                      void* dweight, long long dw_stride, void* dbias, long long rows, int inputs, int outputs,
+                      int dtype, int out_dtype, int activation, void* workspace, long long workspace_bytes,
+                      void* stream);
+
+/* Group norm with an activation, channels last: for utterance b and group g of channels / groups channels, over the
+ * frames t < frames[b] (NULL: all T; values are clamped to [0, T]):
+ *   mean, var = mean and biased variance of the group;  y = act((x - mean) / sqrt(var + eps) * gamma[c] + beta[c]).
+ *   Rows t >= frames[b] are not read and are written as zeros, as gl_mask_frames does.  x, y [B][T][channels], row
+ *   (b, t) at (b * T + t) * stride; y may be x.  gamma, beta [channels] or NULL (1 and 0), of x's dtype.
+ *   stats: [B][groups][2] fp32 (mean, 1 / sqrt(var + eps)) or NULL; 0, 0 for an utterance without frames.         */
+long long gl_group_norm_workspace(int B, int T, int channels, int groups, int dtype);
+int gl_group_norm(const void* x, long long x_stride, const void* gamma, const void* beta, const int* frames, void* y,
+                  long long y_stride, float* stats, int B, int T, int channels, int groups, int dtype, int activation,
+                  float eps, void* workspace, long long workspace_bytes, void* stream);
+
+/* Gradients of gl_group_norm, from its input and stats (the activation's argument is recomputed):
+ *   dx [B][T][channels] (rows t >= frames[b] zero; may be dy), dgamma, dbeta [channels] or NULL.                  */
+long long gl_group_norm_backward_workspace(int B, int T, int channels, int groups, int dtype);
+int gl_group_norm_backward(const void* dy, long long dy_stride, const void* x, long long x_stride, const float* stats,
+                           const void* gamma, const void* beta, const int* frames, void* dx, long long dx_stride,
+                           void* dgamma, void* dbeta, int B, int T, int channels, int groups, int dtype,
+                           int activation, void* workspace, long long workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

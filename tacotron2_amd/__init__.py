@@ -8,4 +8,4 @@ or put ``dropin/`` on sys.path so the reference's ``infer.py`` resolves
 """
 __version__ = "0.1.0"
 
-__all__ = ["audio_utilities", "griffin_lim", "params", "filters", "plan"]
+__all__ = ["audio_utilities", "griffin_lim", "params", "filters", "plan", "inversion"]

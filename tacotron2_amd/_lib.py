@@ -15,6 +15,7 @@ LIB_PATH = os.environ.get("GL_HIP_LIB") or os.path.join(_HERE, "libgl_hip.so")  
 
 _c_float_p = ctypes.c_void_p   # device pointers travel as integers
 _plan_p = ctypes.c_void_p
+_int, _i64, _ptr = ctypes.c_int, ctypes.c_longlong, ctypes.c_void_p
 
 # name -> (restype, argtypes); mirrors include/gl_hip.h one to one
 SIGNATURES = {
@@ -66,6 +67,18 @@ SIGNATURES = {
                                                 ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_void_p]),
     "gl_pcm16_encode": (ctypes.c_int, [_plan_p, _c_float_p, ctypes.c_longlong, ctypes.c_longlong, ctypes.c_void_p,
                                        ctypes.c_longlong, _c_float_p, ctypes.c_int, ctypes.c_void_p]),
+    "gl_dense_workspace": (_i64, [_i64, _int, _int, _int, _int]),
+    "gl_dense": (_int, [_ptr, _i64, _ptr, _i64, _ptr, _ptr, _i64, _ptr, _i64, _ptr, _i64, _i64, _int, _int, _int, _int,
+                        _int, _ptr, _i64, _ptr]),
+    "gl_dense_backward_workspace": (_i64, [_i64, _int, _int, _int, _int, _int]),
+    "gl_dense_backward": (_int, [_ptr, _i64, _ptr, _i64, _ptr, _i64, _ptr, _i64, _ptr, _i64, _ptr, _i64, _ptr, _i64,
+                                 _int, _int, _int, _int, _int, _ptr, _i64, _ptr]),
+    "gl_group_norm_workspace": (_i64, [_int, _int, _int, _int, _int]),
+    "gl_group_norm": (_int, [_ptr, _i64, _ptr, _ptr, _ptr, _ptr, _i64, _ptr, _int, _int, _int, _int, _int, _int,
+                             ctypes.c_float, _ptr, _i64, _ptr]),
+    "gl_group_norm_backward_workspace": (_i64, [_int, _int, _int, _int, _int]),
+    "gl_group_norm_backward": (_int, [_ptr, _i64, _ptr, _i64, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _ptr, _ptr, _int,
+                                      _int, _int, _int, _int, _int, _ptr, _i64, _ptr]),
 }
 
 _lib = None

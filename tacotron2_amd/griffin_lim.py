@@ -119,7 +119,7 @@ def mel_to_audio(mel_spectrogram, *, basis=None, n_fft=None, hop=None, iteration
 
 def logmel_to_audio(y_pred_post, *, compression_factor=1.0, basis=None, n_fft=None, hop=None, iterations=None,
                     x_init=None, seed=None, rng="numpy", normalize="reference", device=None, lengths=None,
-                    return_mag=True):
+                    return_mag=True, inversion=None):
     """infer.py:24-29 without the host round trip: the decoder output goes in as it is.
 
     y_pred_post: (B, T, n_mels) or (T, n_mels) natural-log mel (Tacotron2.inference's second
@@ -127,6 +127,8 @@ def logmel_to_audio(y_pred_post, *, compression_factor=1.0, basis=None, n_fft=No
     infer.py:28 and the filterbank contraction run in ONE kernel (gl_logmel_to_mag); then Griffin-Lim
     and the normalisation of save_mel_to_wav.  Unlike the reference (batch forced to 1,
     model.py:530) any batch size is accepted.  return_mag=False: see mel_to_audio.
+    inversion: an ``inversion.MelInversion`` that makes the magnitudes from the log-mels in place of the fixed basis
+    (it learned the compression factor along with the log-mels: neither basis nor compression_factor goes with it).
     Returns (waveforms (B, L), magnitude (B, T, F) or None)."""
     n_fft = int(params.n_fft if n_fft is None else n_fft)
     hop = int(params.frame_hop if hop is None else hop)
@@ -139,7 +141,14 @@ def logmel_to_audio(y_pred_post, *, compression_factor=1.0, basis=None, n_fft=No
         raise ValueError("y_pred_post must be (T, n_mels) or (B, T, n_mels)")
     lm = lm.contiguous()
     B, T, n_mels = lm.shape
-    if basis is None:
+    if inversion is not None:
+        if basis is not None or compression_factor != 1.0:
+            raise ValueError("a learned inversion takes the log-mels as they are: neither basis nor compression_factor")
+        if (inversion.n_mels, inversion.n_bins) != (n_mels, n_fft // 2 + 1):
+            raise ValueError(f"inversion maps {inversion.n_mels} bands to {inversion.n_bins} bins, not {n_mels} to "
+                             f"{n_fft // 2 + 1}")
+        fb_dev = None
+    elif basis is None:
         if n_fft != params.n_fft or n_mels != params.n_mel_channels:
             fb_dev = torch.from_numpy(filters.mel(sr=params.sampling_rate, n_fft=n_fft, n_mels=n_mels,
                                                   fmin=params.f_min, fmax=params.f_max)).to(dev)
@@ -148,13 +157,19 @@ def logmel_to_audio(y_pred_post, *, compression_factor=1.0, basis=None, n_fft=No
     else:
         b, _ = audio_utilities._to_device(basis, dev, torch.float32)
         fb_dev = b.t().contiguous()
-    if tuple(fb_dev.shape) != (n_mels, n_fft // 2 + 1):
+    if fb_dev is not None and tuple(fb_dev.shape) != (n_mels, n_fft // 2 + 1):
         raise ValueError(f"basis/filterbank shape {tuple(fb_dev.shape)} does not match "
                          f"({n_mels}, {n_fft // 2 + 1})")
     plan = get_plan(n_fft, hop, T, B, dev)
     L = plan.signal_length(T)
     x0 = audio_utilities._start_signal(B, L, x_init, seed, rng, plan, dev)
-    if not return_mag and plan.mel_run_supported():
+    if inversion is not None:
+        with torch.no_grad():
+            mag = inversion(lm, lengths=lengths)
+        if lengths is not None:
+            plan.mask_frames(mag, lengths)
+        x = plan.run(mag, x0, iterations, out=x0)
+    elif not return_mag and plan.mel_run_supported():
         mag = None
         x = plan.mel_run(fb_dev, lm, x0, iterations, out=x0, logmel=True, compression_factor=compression_factor,
                          lengths=lengths)

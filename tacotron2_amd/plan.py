@@ -28,6 +28,14 @@ def _require_gpu(device):
     return dev
 
 
+_capture_state = threading.local()
+
+
+def raw_capture_active():
+    """True while this thread is inside Plan.capture(): the recorded calls may not allocate."""
+    return getattr(_capture_state, "depth", 0) > 0
+
+
 class Plan:
     """Owns a gl_plan handle.  Methods take/return fp32 torch tensors on the plan's device."""
 
@@ -353,10 +361,12 @@ class _Capture:
         self._ctx = torch.cuda.stream(self._side)
         self._ctx.__enter__()
         _lib.check(p._lib.gl_graph_begin(ctypes.c_void_p(self._side.cuda_stream)), "gl_graph_begin")
+        _capture_state.depth = getattr(_capture_state, "depth", 0) + 1
         return self.graph
 
     def __exit__(self, et, ev, tb):
         p = self.plan
+        _capture_state.depth -= 1
         h = ctypes.c_void_p()
         rc = p._lib.gl_graph_end(ctypes.c_void_p(self._side.cuda_stream), ctypes.byref(h))
         self._ctx.__exit__(et, ev, tb)
