@@ -11,14 +11,52 @@ __device__ __forceinline__ float gl_to_f32(float v) { return v; }
 __device__ __forceinline__ float gl_to_f32(gl_bf16 v) { return (float)v; }
 __device__ __forceinline__ float gl_to_f32(gl_f16 v) { return (float)v; }
 
-// act(z).  Every branch is uniform: `act` is a kernel argument or a template constant.
+// The exponential, with the reciprocal and the error function built on it, as the 16-bit results need them: relative
+// error below 2^-20 where the result is not subnormal.  exp(z) = 2^n 2^f with n = rint(z log2 e); the product is carried
+// in two floats, so the error does not grow with |z|.
+__device__ __forceinline__ float gl_exp(float z) {
+    const float k = 1.44269504088896341f;                    // log2 e, and what its rounding leaves
+    const float t = z * k;
+    const float lo = fmaf(z, k, -t) + z * 1.92596299e-8f;
+    const bool low = t < -120.0f;                            // subnormal results: 2^64 up, then down with one rounding
+    const float e = __builtin_amdgcn_exp2f(low ? t + 64.0f : t);
+    const float r = fmaf(e, lo * 0.69314718f, e) * (low ? 0x1p-64f : 1.0f);
+    return z < -104.0f ? 0.0f : (e == INFINITY ? e : r);                                   // NaN stays NaN
+}
+
+__device__ __forceinline__ float gl_sigmoid(float z) {
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504088896341f));
+}
+// Phi(-a) = t p exp(-a^2 / 2) for a >= 0: Abramowitz and Stegun 7.1.26, erfc(x) = t (a1 + t (a2 + ...)) exp(-x^2),
+// t = 1 / (1 + p x), with x = a / sqrt 2; |error of erf| <= 1.5e-7.
+__device__ __forceinline__ float gl_phi_poly(float a, float& t) {
+    t = __builtin_amdgcn_rcpf(fmaf(a, 0.3275911f * 0.70710678118654752f, 1.0f));
+    float p = fmaf(t, 1.061405429f * 0.5f, -1.453152027f * 0.5f);
+    p = fmaf(p, t, 1.421413741f * 0.5f);
+    p = fmaf(p, t, -0.284496736f * 0.5f);
+    return fmaf(p, t, 0.254829592f * 0.5f);
+}
+
+// act(z).  Every branch on `act` is uniform: a kernel argument or a template constant.
 __device__ __forceinline__ float gl_act(float z, int act) {
     switch (act) {
         case GL_ACT_RELU: return z < 0.0f ? 0.0f : z;                  // NaN stays NaN
-        case GL_ACT_SILU: return z / (1.0f + expf(-z));
-        case GL_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
-        case GL_ACT_TANH: return tanhf(z);
-        case GL_ACT_EXP: return expf(z);
+        case GL_ACT_SILU: return z * gl_sigmoid(z);
+        case GL_ACT_GELU: {                                            // z Phi(z) = max(z, 0) - |z| Phi(-|z|)
+            const float a = fminf(fabsf(z), 16.0f);                    // Phi(-16) is 0: infinities give z or 0
+            float t;
+            const float p = gl_phi_poly(a, t);
+            return fmaf(-(a * t * p), __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f), fmaxf(z, 0.0f));   // NaN: by z z
+        }
+        case GL_ACT_TANH: {
+            // (1 - e) / (1 + e) with e = exp(-2 |z|); near zero the series z - z^3/3 + 2 z^5/15 - 17 z^7/315
+            const float a = fabsf(z), e = __builtin_amdgcn_exp2f(a * -2.88539008177792681f);
+            const float far = copysignf((1.0f - e) * __builtin_amdgcn_rcpf(1.0f + e), z);
+            const float q = z * z;
+            const float near = fmaf(z * q, fmaf(q, fmaf(q, -0.0539682540f, 0.133333333f), -0.333333333f), z);
+            return a < 0.25f ? near : far;
+        }
+        case GL_ACT_EXP: return gl_exp(z);
         default: return z;
     }
 }
@@ -28,16 +66,21 @@ __device__ __forceinline__ float gl_act_grad(float z, int act) {
     switch (act) {
         case GL_ACT_RELU: return z > 0.0f ? 1.0f : (z != z ? z : 0.0f);
         case GL_ACT_SILU: {
-            const float s = 1.0f / (1.0f + expf(-z));
-            return s * (1.0f + z * (1.0f - s));
+            const float s = gl_sigmoid(z);
+            return fmaf(z * s, 1.0f - s, s);
         }
-        case GL_ACT_GELU:
-            return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * expf(-0.5f * z * z) * 0.39894228040143268f;
-        case GL_ACT_TANH: {
-            const float t = tanhf(z);
-            return 1.0f - t * t;
+        case GL_ACT_GELU: {                                            // Phi(z) + z phi(z)
+            const float a = fabsf(z), e = __builtin_amdgcn_exp2f(a * a * -0.72134752044448170f);
+            float t;
+            const float p = gl_phi_poly(a, t), h = t * p * e;
+            return fmaf(z * e, 0.39894228040143268f, z < 0.0f ? h : 1.0f - h);
         }
-        case GL_ACT_EXP: return expf(z);
+        case GL_ACT_TANH: {                                            // 4 e / (1 + e)^2 with e = exp(-2 |z|)
+            const float e = __builtin_amdgcn_exp2f(fabsf(z) * -2.88539008177792681f);
+            const float r = __builtin_amdgcn_rcpf(1.0f + e);
+            return 4.0f * e * r * r;
+        }
+        case GL_ACT_EXP: return gl_exp(z);
         default: return 1.0f;
     }
 }

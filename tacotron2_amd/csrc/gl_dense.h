@@ -1,0 +1,60 @@
+// Shared by the translation units of the dense layers: the products' operands and their dispatch.
+#pragma once
+#include "gl_internal.h"
+#include "gl_act.h"
+
+struct gl_operand {              // element (i, q) at base[i * is + q * qs], one of is, qs is 1
+    const void* base;
+    long long is, qs;
+    bool padded = false;         // this library's own copy: zeros up to whole multiples of 32 in the contiguous direction
+    bool across() const { return is == 1 && qs != 1; }       // contiguous across the contraction
+};
+
+struct gl_epilogue {
+    const void* bias;            // [J] of T or null
+    const void* residual;        // of TO or null
+    long long r_stride;
+    void* y;
+    long long y_stride;
+    void* z;                     // of TO or null
+    long long z_stride;
+    int act;
+    float* partial;              // [parts][I][J]: sums of one part of the contraction, finished by k_dense_join
+};
+
+static inline long long gl_ceil_div(long long a, long long b) { return (a + b - 1) / b; }
+static inline long long gl_align16(long long b) { return (b + 15) / 16 * 16; }
+
+// How a product of 16-bit operands on 16 bytes is split (gl_mm16_launch.h).  A pure function of the sizes: the workspace
+// query and the call must agree, and results must not depend on the moment.
+struct gl_mm_plan {
+    int kind;                    // 0: 64 x 64 tiles, 1: 128 x 128, 2: 256 x 256 walked by one workgroup a CU
+    int parts;                   // of the contraction
+    long long per;               // contraction indexes in a part
+};
+// any_q: both sides are contiguous across the contraction, which may then have any length.
+gl_mm_plan gl_mm_plan_for(long long I, int J, long long nq, bool any_q);
+// columns the first of the product's two launches takes (the rest has its own plan): all, or a multiple of 256
+int gl_mm_first_columns(long long I, int J, long long nq, bool any_q);
+long long gl_mm_partial_bytes(long long I, int J, long long nq, bool any_q);
+
+// Whether the fast kernels take the operands as they lie, else the strided kernel does.
+bool gl_mm16_takes(const gl_operand& P, const gl_operand& Q, const gl_epilogue& e, long long I, int J, long long nq, int out_size);
+// T: gl_bf16 / gl_f16; TO: T or float
+template <typename T, typename TO>
+int gl_mm16(const gl_operand& P, const gl_operand& Q, gl_epilogue e, long long I, int J, long long nq, float* partial, hipStream_t st);
+
+// sums the parts in their order and finishes the elements
+template <typename T, typename TO>
+int gl_dense_join(const gl_epilogue& e, long long I, int J, int parts, hipStream_t st);
+
+// sum -> (preactivation, y) of element (i, j)
+template <typename T, typename TO>
+__device__ __forceinline__ void gl_finish(const gl_epilogue& e, long long i, int j, float sum) {
+    float z = sum;
+    if (e.bias) z += gl_to_f32(((const T*)e.bias)[j]);
+    if (e.z) ((TO*)e.z)[i * e.z_stride + j] = (TO)z;
+    float y = gl_act(z, e.act);
+    if (e.residual) y += gl_to_f32(((const TO*)e.residual)[i * e.r_stride + j]);
+    ((TO*)e.y)[i * e.y_stride + j] = (TO)y;
+}

@@ -6,8 +6,7 @@
 //   dweight   P(i, q) = dz[q][i],      Q(j, q) = x[q][j]             both contiguous in i / j, q = frames
 // 16-bit types: v_mfma_f32_32x32x16 (8 consecutive q per lane), 32-bit: v_mfma_f32_32x32x2_f32; sums are fp32.  Q is the
 // matrix instruction's A operand: the accumulator's registers then run along j, the contiguous direction of C.
-#include "gl_internal.h"
-#include "gl_act.h"
+#include "gl_dense.h"
 
 namespace {
 
@@ -17,33 +16,8 @@ template <typename T> struct vec8 { typedef T type __attribute__((ext_vector_typ
 constexpr int kTile = 64;        // rows and columns of C per workgroup (4 waves, 32 x 32 each)
 constexpr int kBQ = 32;          // contraction indexes staged per step
 
-struct Operand {                 // element (i, q) at base[i * is + q * qs], one of is, qs is 1
-    const void* base;
-    long long is, qs;
-};
-
-struct Epilogue {
-    const void* bias;            // [J] of T or null
-    const void* residual;        // of TO or null
-    long long r_stride;
-    void* y;
-    long long y_stride;
-    void* z;                     // of TO or null
-    long long z_stride;
-    int act;
-    float* partial;              // [splits][I][J]: sums of one part of the contraction, finished by k_dense_join
-};
-
-// sum -> (preactivation, y) of element (i, j); used by the product kernels and by k_dense_join
-template <typename T, typename TO>
-__device__ __forceinline__ void finish(const Epilogue& e, long long i, int j, float sum) {
-    float z = sum;
-    if (e.bias) z += gl_to_f32(((const T*)e.bias)[j]);
-    if (e.z) ((TO*)e.z)[i * e.z_stride + j] = (TO)z;
-    float y = gl_act(z, e.act);
-    if (e.residual) y += gl_to_f32(((const TO*)e.residual)[i * e.r_stride + j]);
-    ((TO*)e.y)[i * e.y_stride + j] = (TO)y;
-}
+typedef gl_operand Operand;
+typedef gl_epilogue Epilogue;
 
 // Any size, stride and alignment: elements are staged one by one.  grid (tiles, splits).
 template <typename T, typename TO>
@@ -104,7 +78,7 @@ __global__ void __launch_bounds__(256) k_dense_any(Operand P, Operand Q, Epilogu
         const int j = j0 + wj + (r & 3) + 8 * (r >> 2) + 4 * lk;
         if (j >= J) continue;
         if (e.partial) e.partial[((long long)blockIdx.y * I + i) * J + j] = acc[r];
-        else finish<T, TO>(e, i, j, acc[r]);
+        else gl_finish<T, TO>(e, i, j, acc[r]);
     }
 }
 
@@ -116,7 +90,7 @@ __global__ void __launch_bounds__(256) k_dense_join(Epilogue e, long long I, int
         float s = 0.0f;
         for (int p = 0; p < splits; ++p) s += e.partial[p * n + at];
         const long long i = at / J;
-        finish<T, TO>(e, i, (int)(at - i * J), s);
+        gl_finish<T, TO>(e, i, (int)(at - i * J), s);
     }
 }
 
@@ -133,6 +107,8 @@ __global__ void __launch_bounds__(256) k_dense_dz(const TO* __restrict__ dy, lon
     const long long r0 = (long long)blockIdx.y * rows_per_part;
     const long long r1 = r0 + rows_per_part < rows ? r0 + rows_per_part : rows;
     float sum = 0.0f;
+    if (n >= N && n < dz_stride && dz)                        // zeros up to the padded width
+        for (long long i = r0 + r; i < r1; i += 4) dz[i * dz_stride + n] = (T)0.0f;
     if (n < N)
         for (long long i = r0 + r; i < r1; i += 4) {
             float d = gl_to_f32(dy[i * dy_stride + n]);
@@ -161,41 +137,39 @@ __global__ void __launch_bounds__(256) k_dense_zero(T* p, long long stride, int 
 }
 
 constexpr int kCUs = 256;        // compute units of an MI355X: the work split must not depend on the moment
-inline long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
-inline long long align16(long long b) { return (b + 15) / 16 * 16; }
 
 // Parts of the contraction: enough workgroups to fill the chip twice, at least 8 steps each.
 int n_splits(long long I, int J, long long nq) {
-    const long long tiles = ceil_div(I, kTile) * ceil_div(J, kTile);
+    const long long tiles = gl_ceil_div(I, kTile) * gl_ceil_div(J, kTile);
     long long s = 2 * kCUs / tiles;
-    const long long most = ceil_div(nq, 8 * kBQ);
+    const long long most = gl_ceil_div(nq, 8 * kBQ);
     if (s > most) s = most;
     return s < 1 ? 1 : (int)s;
 }
-long long partial_bytes(long long I, int J, long long nq) {
+// workspace of a product's parts: whichever kernel takes it (that goes by alignment too, which the query does not know)
+long long partial_bytes(long long I, int J, long long nq, int dtype, bool any_q = false, bool padded = false) {
     const int s = n_splits(I, J, nq);
-    return s > 1 ? align16((long long)s * I * J * 4) : 0;
+    const long long any = s > 1 ? gl_align16((long long)s * I * J * 4) : 0;
+    const long long mm = dtype == GL_F32 ? 0 : gl_mm_partial_bytes(I, J, padded ? gl_ceil_div(nq, 32) * 32 : nq, any_q);
+    return any > mm ? any : mm;
 }
 
 template <typename T, typename TO>
 int product(const Operand& P, const Operand& Q, Epilogue e, long long I, int J, long long nq, float* partial,
             hipStream_t st) {
+    if constexpr (sizeof(T) == 2) {
+        if (gl_mm16_takes(P, Q, e, I, J, nq, sizeof(TO))) return gl_mm16<T, TO>(P, Q, e, I, J, nq, partial, st);
+    }
     const int splits = n_splits(I, J, nq);
-    const long long per = ceil_div(ceil_div(nq, splits), kBQ) * kBQ;
-    const long long used = ceil_div(nq, per);                 // rounding up to whole steps may leave fewer parts
-    const long long tiles = ceil_div(I, kTile) * ceil_div(J, kTile);
+    const long long per = gl_ceil_div(gl_ceil_div(nq, splits), kBQ) * kBQ;
+    const long long used = gl_ceil_div(nq, per);                 // rounding up to whole steps may leave fewer parts
+    const long long tiles = gl_ceil_div(I, kTile) * gl_ceil_div(J, kTile);
     if (tiles > 0x7fffffffLL) return gl_set_error(GL_ERR_INVALID, "gl_dense: %lld tiles are too many for one launch", tiles);
     e.partial = used > 1 ? partial : nullptr;
     hipLaunchKernelGGL((k_dense_any<T, TO>), dim3((unsigned)tiles, (unsigned)used), dim3(256), 0, st, P, Q, e, I, J, nq, per,
-                       (int)ceil_div(J, kTile));
+                       (int)gl_ceil_div(J, kTile));
     GL_HIP_CHECK(hipGetLastError());
-    if (used > 1) {
-        const long long blocks = ceil_div(I * J, 256);
-        hipLaunchKernelGGL((k_dense_join<T, TO>), dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, e, I, J,
-                           (int)used);
-        GL_HIP_CHECK(hipGetLastError());
-    }
-    return 0;
+    return used > 1 ? gl_dense_join<T, TO>(e, I, J, (int)used, st) : 0;
 }
 
 int check_types(int dtype, int out_dtype, int act, const char* who) {
@@ -233,22 +207,26 @@ int forward(const void* x, long long x_stride, const void* w, long long w_stride
 
 constexpr int kMaxParts = 128;
 int rows_per_part(long long rows) {
-    const long long r = ceil_div(rows, kMaxParts);
+    const long long r = gl_ceil_div(rows, kMaxParts);
     return (int)(r < 64 ? 64 : r);
 }
 
 // workspace of the backward pass: [dz (unless dy serves)] [column-sum parts] [partials of dx and dweight, one after the
 // other on the stream: the larger of the two]
 struct BackLayout {
-    long long dz_bytes, parts_bytes, partial_bytes_;
+    bool own_dz;
+    long long dz_stride, dz_bytes, parts_bytes, partial_bytes_;
     long long total() const { return dz_bytes + parts_bytes + partial_bytes_; }
 };
 int elem_size(int dtype) { return dtype == GL_F32 ? 4 : 2; }
 BackLayout back_layout(long long rows, int inputs, int outputs, int dtype, int out_dtype, int act) {
     BackLayout l;
-    l.dz_bytes = act == GL_ACT_NONE && dtype == out_dtype ? 0 : align16(rows * outputs * elem_size(dtype));
-    l.parts_bytes = align16(ceil_div(rows, rows_per_part(rows)) * outputs * 4);
-    const long long a = partial_bytes(rows, inputs, outputs), b = partial_bytes(outputs, inputs, rows);
+    // dy itself serves where nothing is to be multiplied, converted or padded
+    l.dz_stride = gl_ceil_div(outputs, 32) * 32;
+    l.own_dz = act != GL_ACT_NONE || dtype != out_dtype || (dtype != GL_F32 && outputs % 32);
+    l.dz_bytes = l.own_dz ? gl_align16(rows * l.dz_stride * elem_size(dtype)) : 0;
+    l.parts_bytes = gl_align16(gl_ceil_div(rows, rows_per_part(rows)) * outputs * 4);
+    const long long a = partial_bytes(rows, inputs, outputs, dtype, false, l.own_dz), b = partial_bytes(outputs, inputs, rows, dtype, true);
     l.partial_bytes_ = a > b ? a : b;
     return l;
 }
@@ -258,47 +236,118 @@ int backward(const void* dy, long long dy_stride, const void* x, long long x_str
              const void* z, long long z_stride, void* dx, long long dx_stride, void* dw, long long dw_stride, void* db,
              long long rows, int inputs, int outputs, int act, const BackLayout& l, void* ws, hipStream_t st) {
     char* at = (char*)ws;
-    T* dz = l.dz_bytes ? (T*)at : nullptr;
+    T* dz = l.own_dz ? (T*)at : nullptr;
     float* parts = (float*)(at + l.dz_bytes);
     float* partial = (float*)(at + l.dz_bytes + l.parts_bytes);
     if (dz || db) {
         const int rpp = rows_per_part(rows);
-        const int n_parts = (int)ceil_div(rows, rpp);
-        hipLaunchKernelGGL((k_dense_dz<T, TO>), dim3((unsigned)ceil_div(outputs, 64), (unsigned)n_parts), dim3(256), 0, st,
-                           (const TO*)dy, dy_stride, (const TO*)z, z_stride, dz, (long long)outputs, db ? parts : nullptr,
+        const int n_parts = (int)gl_ceil_div(rows, rpp);
+        hipLaunchKernelGGL((k_dense_dz<T, TO>), dim3((unsigned)gl_ceil_div(outputs, 64), (unsigned)n_parts), dim3(256), 0, st,
+                           (const TO*)dy, dy_stride, (const TO*)z, z_stride, dz, l.dz_stride, db ? parts : nullptr,
                            rows, outputs, rpp, act);
         GL_HIP_CHECK(hipGetLastError());
         if (db) {
-            hipLaunchKernelGGL((k_dense_db<T>), dim3((unsigned)ceil_div(outputs, 256)), dim3(256), 0, st, parts, n_parts,
+            hipLaunchKernelGGL((k_dense_db<T>), dim3((unsigned)gl_ceil_div(outputs, 256)), dim3(256), 0, st, parts, n_parts,
                                (T*)db, outputs);
             GL_HIP_CHECK(hipGetLastError());
         }
     }
     const void* d = dz ? (const void*)dz : dy;
-    const long long d_stride = dz ? outputs : dy_stride;
+    const long long d_stride = dz ? l.dz_stride : dy_stride;
     Epilogue e = {};
     if (dx) {
         e.y = dx;
         e.y_stride = dx_stride;
-        int rc = product<T, T>({d, d_stride, 1}, {w, 1, w_stride}, e, rows, inputs, outputs, partial, st);
+        int rc = product<T, T>({d, d_stride, 1, dz != nullptr}, {w, 1, w_stride}, e, rows, inputs, outputs, partial, st);
         if (rc) return rc;
     }
     if (dw) {
         e.y = dw;
         e.y_stride = dw_stride;
-        return product<T, T>({d, 1, d_stride}, {x, 1, x_stride}, e, outputs, inputs, rows, partial, st);
+        return product<T, T>({d, 1, d_stride, dz != nullptr}, {x, 1, x_stride}, e, outputs, inputs, rows, partial, st);
     }
     return 0;
 }
 
 }  // namespace
 
+template <typename T, typename TO>
+int gl_dense_join(const gl_epilogue& e, long long I, int J, int parts, hipStream_t st) {
+    const long long blocks = gl_ceil_div(I * J, 256);
+    hipLaunchKernelGGL((k_dense_join<T, TO>), dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, e, I, J, parts);
+    GL_HIP_CHECK(hipGetLastError());
+    return 0;
+}
+template int gl_dense_join<float, float>(const gl_epilogue&, long long, int, int, hipStream_t);
+template int gl_dense_join<gl_bf16, gl_bf16>(const gl_epilogue&, long long, int, int, hipStream_t);
+template int gl_dense_join<gl_bf16, float>(const gl_epilogue&, long long, int, int, hipStream_t);
+template int gl_dense_join<gl_f16, gl_f16>(const gl_epilogue&, long long, int, int, hipStream_t);
+template int gl_dense_join<gl_f16, float>(const gl_epilogue&, long long, int, int, hipStream_t);
+
+// 256 x 256 tiles where they fill the chip (parts included), else 128 x 128, else 64 x 64.  A part has at least 512
+// contraction indexes with large tiles and 256 with small ones: shorter ones cost more in the join than they fill.
+gl_mm_plan gl_mm_plan_for(long long I, int J, long long nq, bool any_q) {
+    auto split = [&](int b, long long least) -> gl_mm_plan {
+        const long long tiles = gl_ceil_div(I, b) * gl_ceil_div(J, b);
+        const long long fill = b == 256 ? kCUs : 2 * kCUs;
+        long long parts = tiles * 2 > fill ? 1 : fill / tiles;
+        if (parts > nq / least) parts = nq / least;
+        if (parts > 64) parts = 64;
+        if (parts < 1) parts = 1;
+        const long long per = gl_ceil_div(gl_ceil_div(nq, parts), 64) * 64;
+        return {0, (int)gl_ceil_div(nq, per), per};
+    };
+    if (J % 256 == 0 && I >= 256 && (any_q || nq % 32 == 0)) {
+        gl_mm_plan p = split(256, 512);
+        if (gl_ceil_div(I, 256) * (J / 256) * p.parts >= 128) {
+            p.kind = 2;
+            return p;
+        }
+    }
+    gl_mm_plan p = split(128, 256);
+    if (I >= 96 && J >= 96 && gl_ceil_div(I, 128) * gl_ceil_div(J, 128) * p.parts >= 256) {
+        p.kind = 1;
+        return p;
+    }
+    return split(64, 256);
+}
+
+int gl_mm_first_columns(long long I, int J, long long nq, bool any_q) {
+    const int whole = J / 256 * 256;
+    return whole > 0 && whole < J && gl_mm_plan_for(I, whole, nq, any_q).kind == 2 ? whole : J;
+}
+
+long long gl_mm_partial_bytes(long long I, int J, long long nq, bool any_q) {
+    const int first = gl_mm_first_columns(I, J, nq, any_q);
+    const gl_mm_plan a = gl_mm_plan_for(I, first, nq, any_q);
+    long long bytes = a.parts > 1 ? (long long)a.parts * I * first * 4 : 0;
+    if (first < J) {
+        const gl_mm_plan b = gl_mm_plan_for(I, J - first, nq, any_q);
+        const long long more = b.parts > 1 ? (long long)b.parts * I * (J - first) * 4 : 0;
+        if (more > bytes) bytes = more;
+    }
+    return gl_align16(bytes);
+}
+
+bool gl_mm16_takes(const gl_operand& P, const gl_operand& Q, const gl_epilogue& e, long long I, int J, long long nq, int out_size) {
+    auto side = [&](const gl_operand& o, long long rows) {
+        const long long stride = o.across() ? o.qs : o.is;
+        return (uintptr_t)o.base % 16 == 0 && stride % 8 == 0 && stride <= (1 << 21) && (o.padded || (o.across() ? rows : nq) % 8 == 0);
+    };
+    auto out = [&](const void* p, long long stride) {        // stores of four bytes and more
+        return !p || ((uintptr_t)p % 4 == 0 && stride * out_size % 4 == 0 && stride <= (1 << 20));
+    };
+    if (P.across() && !Q.across()) return false;
+    return side(P, I) && side(Q, J) && out(e.y, e.y_stride) && out(e.z, e.z_stride) && out(e.residual, e.r_stride) && nq < (1LL << 31) &&
+           gl_ceil_div(I, 64) * gl_ceil_div(J, 64) < (1LL << 31) - 8;
+}
+
 extern "C" {
 
 long long gl_dense_workspace(long long rows, int inputs, int outputs, int dtype, int out_dtype) {
     if (check_types(dtype, out_dtype, 0, "gl_dense_workspace") || check_sizes(rows, inputs, outputs, "gl_dense_workspace"))
         return GL_ERR_INVALID;
-    return rows ? partial_bytes(rows, outputs, inputs) : 0;
+    return rows ? partial_bytes(rows, outputs, inputs, dtype) : 0;
 }
 
 int gl_dense(const void* x, long long x_stride, const void* weight, long long w_stride, const void* bias,
@@ -314,7 +363,7 @@ int gl_dense(const void* x, long long x_stride, const void* weight, long long w_
     if (!rc) rc = check_stride(y_stride, outputs, "y", "gl_dense");
     if (!rc && residual) rc = check_stride(r_stride, outputs, "residual", "gl_dense");
     if (!rc && preactivation) rc = check_stride(z_stride, outputs, "preactivation", "gl_dense");
-    if (!rc) rc = check_workspace(workspace, workspace_bytes, partial_bytes(rows, outputs, inputs), "gl_dense");
+    if (!rc) rc = check_workspace(workspace, workspace_bytes, partial_bytes(rows, outputs, inputs, dtype), "gl_dense");
     if (rc) return rc;
     const Epilogue e = {bias, residual, r_stride, y, y_stride, preactivation, z_stride, activation, nullptr};
     const hipStream_t st = (hipStream_t)stream;
@@ -345,7 +394,7 @@ int gl_dense_backward(const void* dy, long long dy_stride, const void* x, long l
     const hipStream_t st = (hipStream_t)stream;
     if (rows == 0) {                                         // empty sums
         auto zero = [&](void* p, long long stride, int r, int c) -> int {
-            const long long blocks = ceil_div((long long)r * c, 256);
+            const long long blocks = gl_ceil_div((long long)r * c, 256);
             const dim3 grid((unsigned)(blocks < 4096 ? blocks : 4096));
             if (dtype == GL_F32) hipLaunchKernelGGL((k_dense_zero<float>), grid, dim3(256), 0, st, (float*)p, stride, r, c);
             else hipLaunchKernelGGL((k_dense_zero<gl_f16>), grid, dim3(256), 0, st, (gl_f16*)p, stride, r, c);

@@ -1,0 +1,497 @@
+// C = P Q^T on the 16-bit matrix instructions, for operands whose rows start on 16 bytes and whose contiguous direction is
+// a multiple of 8 elements (gl_dense.hip uses the strided kernel for the rest).
+//
+// A workgroup of (BM / WM) (BN / WN) waves owns a BM x BN tile; a wave owns WM x WN of it in registers.  Steps of BK run
+// through a ring of ST stages in LDS, filled by buffer loads that write LDS directly (no registers, out-of-range chunks
+// become zeros through the buffer's bounds check), one barrier a step:
+//     wait for the own loads of stage k, barrier (all have landed, all waves are done with stage k - 1),
+//     start the loads of stage k + ST - 1 into the slot of k - 1, read stage k, multiply.
+//
+// Stage layouts.  An operand contiguous in the contraction is [rows][BK] with 16-byte chunk c of row r at c ^ swizzle(r):
+// the 16 rows a matrix instruction reads at one chunk then spread over all banks.  An operand contiguous across the
+// contraction is [BK][columns], read by ds_read_b64_tr_b16 (4 contraction rows x 16 columns per 16 lanes, transposed on the
+// way); its 32-byte pieces are XORed with the row so that the 8 rows of half a wave spread over all banks.  The swizzle is
+// applied to the global address, since direct loads place consecutive lanes' chunks consecutively.
+//
+// v_mfma_f32_16x16x32: A = Q rows (columns j of C), B = P rows (rows i of C): a lane's four accumulator registers are four
+// consecutive j of one i.
+#pragma once
+#include "gl_internal.h"
+#include "gl_act.h"
+
+namespace gl_mm {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+template <typename T, int N> struct vec { typedef T type __attribute__((ext_vector_type(N))); };
+
+struct Side {                    // rows (or columns) of C x contraction
+    const void* base;
+    long long stride;            // elements between rows of the contiguous direction
+    long long rows;              // rows that may be loaded: I (J), or more where zeros pad them
+    int missing;                 // contraction indexes at the end that this side does not have (the other has zeros there)
+};
+
+template <typename T>
+__device__ __forceinline__ f32x4 mfma16(s16x8 a, s16x8 b, f32x4 c) {
+    typedef typename vec<T, 8>::type v8;
+    if constexpr (__is_same(T, gl_bf16))
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
+}
+
+__device__ __forceinline__ void wait_loads(int n) {          // at most n vector memory operations outstanding
+    switch (n) {
+#define GL_WAIT(k) case k: asm volatile("s_waitcnt vmcnt(" #k ")" ::: "memory"); break;
+        GL_WAIT(0) GL_WAIT(2) GL_WAIT(3) GL_WAIT(4) GL_WAIT(5) GL_WAIT(6) GL_WAIT(8) GL_WAIT(10) GL_WAIT(12) GL_WAIT(16) GL_WAIT(18) GL_WAIT(22) GL_WAIT(24) GL_WAIT(38) GL_WAIT(40)
+#undef GL_WAIT
+        default: asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+}
+
+// A workgroup barrier behind which this wave's own LDS reads are done too: their slot may be overwritten
+__device__ __forceinline__ void barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+constexpr int kFlags = 0x00027000;                           // raw 32-bit buffer: bounds-checked, no format conversion
+constexpr int kOutside = 0x7fffff00;                         // an offset beyond every buffer: loads zeros
+
+// One operand of a tile: LDS layout, loads and fragments.
+//   R rows of C's side, TR: contiguous across the contraction
+template <int R, int BK, bool TR, int WAVES, bool TEXT>
+struct Stage {
+    static constexpr int kBytes = R * BK * 2;
+    static constexpr int kLoads = kBytes / (1024 * WAVES);   // 16-byte loads per lane and stage
+    static_assert(kBytes % (1024 * WAVES) == 0, "loads must divide evenly");
+    static constexpr int kRowChunks = TR ? R / 8 : BK / 8;   // chunks per LDS row
+    const char* base;            // first element of the tile at the current step
+    int stride2, n_rows;         // bytes per row of the contiguous direction; rows of C's side that exist
+    int voff[kLoads];
+
+    __device__ __forceinline__ static int swizzle(int row) {
+        return BK == 32 ? (row >> 1) & 3 : row & 7;
+    }
+    __device__ __forceinline__ static int tr_swizzle(int q) { return (((q & 3) | ((q >> 3) & 1) << 2) << 1) & (R / 8 - 1); }
+
+    __device__ __forceinline__ static int chunk_of(int i, int wave, int lane, int& row) {
+        const int slot = (i * WAVES + wave) * 64 + lane;
+        row = slot / kRowChunks;
+        return (slot % kRowChunks) ^ (TR ? tr_swizzle(row) : swizzle(row));
+    }
+    // r0: first row of the tile, q0: first contraction index
+    __device__ __forceinline__ void init(const Side& s, long long r0, long long q0, int wave, int lane) {
+        n_rows = s.rows - r0 < R ? (int)(s.rows - r0) : R;
+        stride2 = (int)s.stride * 2;
+        base = (const char*)s.base + (TR ? q0 * s.stride + r0 : r0 * s.stride + q0) * 2;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            int row;
+            const int ch = chunk_of(i, wave, lane, row);
+            voff[i] = (TR ? ch * 8 < n_rows : row < n_rows) ? row * stride2 + ch * 16 : kOutside;
+        }
+    }
+    // krem: contraction indexes left at this step (<= 0: zeros).  Bytes to the end of the last row that exists; rows and
+    // chunks beyond it load as zeros.
+    __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(int krem) const {
+        const int records = krem <= 0 ? 0 : TR ? (min(krem, BK) - 1) * stride2 + n_rows * 2 : (n_rows - 1) * stride2 + krem * 2;
+        return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, records, kFlags);
+    }
+    // One 16-byte load per lane straight into LDS.  TEXT (where a side is read transposed): with the builtin the compiler
+    // waits for every load in flight before a transposing read, which may alias (dx of 55 104 x 2048 x 512: 210 us, so 127);
+    // as text, wait_loads() and barrier() alone order them.  It has no register result.
+    __device__ __forceinline__ void load_one(__amdgpu_buffer_rsrc_t rs, char* lds, int i, int v, int wave) const {
+        auto at = (__attribute__((address_space(3))) char*)(lds + (i * WAVES + wave) * 1024);
+        if constexpr (TEXT)
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                         : : "s"(__builtin_amdgcn_readfirstlane((unsigned)(unsigned long long)at)), "v"(v), "s"(rs)
+                         : "memory", "m0");
+        else
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)at, 16, v, 0, 0, 0);
+    }
+    __device__ __forceinline__ void advance() { base += TR ? (long long)BK * stride2 : BK * 2; }
+    __device__ __forceinline__ void load(char* lds, int krem, int wave, int lane) {
+        const __amdgpu_buffer_rsrc_t rs = buffer(krem);
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            int v = voff[i];
+            if (!TR && krem < BK) {                          // the last step: chunks past the row's end are another row's
+                int row;
+                if (chunk_of(i, wave, lane, row) * 8 >= krem) v = kOutside;
+            }
+            load_one(rs, lds, i, v, wave);
+        }
+        advance();
+    }
+    // 16 rows from r0 (a multiple of 16), contraction 32 ks .. +32: the lane's row is lane & 15, its 8 indexes 8 (lane >> 4)
+    __device__ __forceinline__ static s16x8 frag(const char* lds, int r0, int ks, int lane) {
+        if constexpr (TR) {
+            const int p = lane & 15, g = lane >> 4;
+            const int q = 32 * ks + 8 * g + (p >> 2);
+            const int ch = (r0 / 8 + ((p & 3) >> 1)) ^ tr_swizzle(q);
+            const char* at = lds + q * (R * 2) + ch * 16 + (p & 1) * 8;
+            typedef __attribute__((address_space(3))) s16x4* lp;
+            const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(at));
+            const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lp)(at + 4 * R * 2));
+            return (s16x8){a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+        } else {
+            const int row = r0 + (lane & 15);
+            const int ch = ((lane >> 4) + 4 * ks) ^ swizzle(row);
+            return *(const s16x8*)(lds + row * (BK * 2) + ch * 16);
+        }
+    }
+};
+
+struct Out {
+    const void* bias;            // [J] of T or null
+    const void* residual;        // of TO or null
+    long long r_stride;
+    void* y;
+    long long y_stride;
+    void* z;                     // of TO or null
+    long long z_stride;
+    int act;                     // where the kernel does not fix it
+    long long part_stride;       // elements of y between the results of two parts of the contraction (bias, residual and z
+                                 // are null then)
+};
+
+template <typename T> struct bits;                          // what a buffer load or store of an element moves
+template <> struct bits<float> { typedef unsigned type; };
+template <> struct bits<gl_bf16> { typedef unsigned short type; };
+template <> struct bits<gl_f16> { typedef unsigned short type; };
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+template <typename T>
+__device__ __forceinline__ T load_at(__amdgpu_buffer_rsrc_t rs, int off) {
+    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b32(rs, off, 0, 0));
+    else return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b16(rs, off, 0, 0));
+}
+template <typename T>
+__device__ __forceinline__ void store_at(T v, __amdgpu_buffer_rsrc_t rs, int off) {
+    if constexpr (sizeof(T) == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, v), rs, off, 0, 0);
+    else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, v), rs, off, 0, 0);
+}
+
+// A wave's bias: NI times four consecutive columns, kept packed until the sums start at it; zero past the last column.
+template <typename T, int NI>
+__device__ __forceinline__ void load_bias(const Out& o, typename vec<T, 4>::type (&bias)[NI], int j0, int J, int lane) {
+    const int n_cols = o.bias && j0 < J ? min(J - j0, 16 * NI) : 0;
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)((const T*)o.bias + (n_cols ? j0 : 0)), 0,
+                                                                        n_cols * (int)sizeof(T), kFlags);
+#pragma unroll
+    for (int n = 0; n < NI; ++n)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) bias[n][r] = load_at<T>(rs, (16 * n + 4 * (lane >> 4) + r) * (int)sizeof(T));
+}
+template <typename T, int MI, int NI>
+__device__ __forceinline__ void start_sums(f32x4 (&acc)[MI][NI], const typename vec<T, 4>::type (&bias)[NI]) {
+#pragma unroll
+    for (int n = 0; n < NI; ++n) {
+        f32x4 b;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) b[r] = gl_to_f32(bias[n][r]);
+#pragma unroll
+        for (int m = 0; m < MI; ++m) acc[m][n] = b;
+    }
+}
+
+// A wave's block of an array with rows on 4 bytes: the buffer ends with the block's last row, so rows past it are dropped.
+template <typename TO, int MI, int NI>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t block_of(const void* p, long long stride, long long i0, int j0, long long I, int J) {
+    const int rows = I - i0 < 16 * MI ? (int)(I - i0) : 16 * MI, cols = J - j0 < 16 * NI ? J - j0 : 16 * NI;
+    return __builtin_amdgcn_make_buffer_rsrc((void*)((const TO*)p + i0 * stride + j0), 0,
+                                             rows > 0 && cols > 0 ? ((rows - 1) * (int)stride + cols) * (int)sizeof(TO) : 0, kFlags);
+}
+
+// Stores a wave's block, rounded to TO; returns how many store instructions that were at least (the caller may leave that
+// many outstanding).  TAIL: columns may end inside the block (a branch that costs registers).
+template <typename TO, bool TAIL, int MI, int NI>
+__device__ __forceinline__ int put_block(TO* dst, long long stride, const f32x4 (&v)[MI][NI], long long i0, int j0, long long I,
+                                         int J, int lane) {
+    typedef typename vec<TO, 4>::type to4;
+    const int il = lane & 15, g4 = lane >> 4;
+    constexpr bool kPair = sizeof(TO) == 2 && NI % 2 == 0;
+    const __amdgpu_buffer_rsrc_t rs = block_of<TO, MI, NI>(dst, stride, i0, j0, I, J);
+    const int stride_b = (int)stride * (int)sizeof(TO);
+    auto round4 = [](const f32x4& f) {
+        to4 t;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) t[r] = (TO)f[r];
+        return t;
+    };
+    if (!TAIL || j0 + 16 * NI <= J) {                        // wave-uniform: whole column blocks
+        int off = il * stride_b + (kPair ? 16 * (g4 & 1) + 8 * (g4 >> 1) : 4 * g4) * (int)sizeof(TO);
+#pragma unroll
+        for (int m = 0; m < MI; ++m) {
+            if constexpr (kPair) {
+                // two 16-column blocks: quarter-waves swapped so that a lane holds 8 consecutive columns
+#pragma unroll
+                for (int n = 0; n < NI; n += 2) {
+                    const u32x2 lo = __builtin_bit_cast(u32x2, round4(v[m][n])), hi = __builtin_bit_cast(u32x2, round4(v[m][n + 1]));
+                    const auto s0 = __builtin_amdgcn_permlane16_swap(lo[0], hi[0], false, false);
+                    const auto s1 = __builtin_amdgcn_permlane16_swap(lo[1], hi[1], false, false);
+                    __builtin_amdgcn_raw_buffer_store_b128((u32x4){s0[0], s1[0], s0[1], s1[1]}, rs, off + 32 * n, 0, 0);
+                }
+            } else {
+#pragma unroll
+                for (int n = 0; n < NI; ++n) {
+                    if constexpr (sizeof(TO) == 4)
+                        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v[m][n]), rs, off + 64 * n, 0, 0);
+                    else
+                        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, round4(v[m][n])), rs, off + 32 * n, 0, 0);
+                }
+            }
+            off += 16 * stride_b;
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        return MI * NI / (kPair ? 2 : 1);
+    }
+    int off = il * stride_b;
+#pragma unroll
+    for (int m = 0; m < MI; ++m) {
+#pragma unroll
+        for (int n = 0; n < NI; ++n)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int j = 16 * n + 4 * g4 + r;
+                store_at<TO>((TO)v[m][n][r], rs, j0 + j < J ? off + j * (int)sizeof(TO) : kOutside);
+            }
+        off += 16 * stride_b;
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    return MI * NI;
+}
+
+// Writes a wave's block at (i0, j0): activation, residual and one rounding.  All loads come before the
+// results' stores: the memory counter runs in order, a load behind a store would wait for it.
+// EXTRA: there may be a residual or a preactivation.
+template <typename T, typename TO, int ACT, bool EXTRA, bool TAIL, int MI, int NI>
+__device__ __forceinline__ int epilogue(const Out& o, f32x4 (&acc)[MI][NI], long long i0, int j0, long long I, int J,
+                                        int part, int lane) {
+    const int il = lane & 15, g4 = lane >> 4;
+    if (EXTRA && o.z) put_block<TO, TAIL, MI, NI>((TO*)o.z, o.z_stride, acc, i0, j0, I, J, lane);
+#pragma unroll
+    for (int m = 0; m < MI; ++m)
+#pragma unroll
+        for (int n = 0; n < NI; ++n) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[m][n][r] = gl_act(acc[m][n][r], ACT < 0 ? o.act : ACT);
+            if (n & 1) __builtin_amdgcn_sched_barrier(0);    // keeps the block's temporaries few
+        }
+    if (EXTRA && o.residual) {
+        const __amdgpu_buffer_rsrc_t rs = block_of<TO, MI, NI>(o.residual, o.r_stride, i0, j0, I, J);
+        const int stride_b = (int)o.r_stride * (int)sizeof(TO);
+        int off = il * stride_b + 4 * g4 * (int)sizeof(TO);
+        const bool whole = !TAIL || j0 + 16 * NI <= J;
+#pragma unroll
+        for (int m = 0; m < MI; ++m) {
+#pragma unroll
+            for (int n = 0; n < NI; ++n) {
+                typename vec<TO, 4>::type rv;
+                if (whole) {
+                    if constexpr (sizeof(TO) == 4)
+                        rv = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, off + 64 * n, 0, 0));
+                    else
+                        rv = __builtin_bit_cast(typename vec<TO, 4>::type, __builtin_amdgcn_raw_buffer_load_b64(rs, off + 32 * n, 0, 0));
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        rv[r] = load_at<TO>(rs, j0 + 16 * n + 4 * g4 + r < J ? off + (16 * n + r) * (int)sizeof(TO) : kOutside);
+                }
+#pragma unroll
+                for (int r = 0; r < 4; ++r) acc[m][n][r] += gl_to_f32(rv[r]);
+            }
+            off += 16 * stride_b;
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    return put_block<TO, TAIL, MI, NI>((TO*)o.y + part * o.part_stride, o.y_stride, acc, i0, j0, I, J, lane);
+}
+
+template <typename T, typename TO, int ACT, int BM, int BN, int WM, int WN, int BK, int ST, bool PT, bool QT, int WPE>
+__global__ void __launch_bounds__(64 * (BM / WM) * (BN / WN), WPE)
+k_mm16(Side P, Side Q, Out o, long long I, int J, long long nq, long long q_per_part, int tiles_j, int n_tiles) {
+    constexpr int WAVES = (BM / WM) * (BN / WN);
+    typedef Stage<BM, BK, PT, WAVES, PT || QT> SP;
+    typedef Stage<BN, BK, QT, WAVES, PT || QT> SQ;
+    constexpr int kStage = SP::kBytes + SQ::kBytes;
+    constexpr int MI = WM / 16, NI = WN / 16;
+    __shared__ __attribute__((aligned(1024))) char lds[ST * kStage];
+
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // consecutive workgroups go to the 8 XCDs in turn: each XCD walks its own run of tiles, j fastest, so the rows of P
+    // it reads and all of Q stay in its L2
+    const int per = (n_tiles + 7) / 8;
+    const int tile = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if ((int)(blockIdx.x >> 3) >= per || tile >= n_tiles) return;
+    const long long i0 = (long long)(tile / tiles_j) * BM;
+    const int j0 = tile % tiles_j * BN;
+    const long long q0 = (long long)blockIdx.y * q_per_part;
+    const long long q1 = q0 + q_per_part < nq ? q0 + q_per_part : nq;
+    const int wi = wave / (BN / WN) * WM, wj = wave % (BN / WN) * WN;
+
+    SP sp;
+    SQ sq;
+    sp.init(P, i0, q0, wave, lane);
+    sq.init(Q, j0, q0, wave, lane);
+    const int steps = (int)((q1 - q0 + BK - 1) / BK);
+    const int missing = (int)max(0LL, q1 - (nq - Q.missing));   // at the end of this part
+    int krem = (int)(q1 - q0);
+    auto load = [&](int slot) {
+        sp.load(lds + slot * kStage, krem, wave, lane);
+        sq.load(lds + slot * kStage + SP::kBytes, krem - missing, wave, lane);
+        krem -= BK;
+    };
+#pragma unroll
+    for (int s = 0; s < ST - 1; ++s) load(s);
+
+    f32x4 acc[MI][NI];
+    typename vec<T, 4>::type bias[NI];
+    load_bias<T, NI>(o, bias, j0 + wj, J, lane);
+    start_sums<T, MI, NI>(acc, bias);
+
+    int slot = 0;
+    for (int k = 0; k < steps; ++k) {
+        wait_loads((SP::kLoads + SQ::kLoads) * (ST - 2));
+        barrier();
+        load(slot == 0 ? ST - 1 : slot - 1);
+        const char* ps = lds + slot * kStage;
+        const char* qs = ps + SP::kBytes;
+#pragma unroll
+        for (int ks = 0; ks < BK / 32; ++ks) {
+            s16x8 a[NI], b[MI];
+#pragma unroll
+            for (int n = 0; n < NI; ++n) a[n] = SQ::frag(qs, wj + 16 * n, ks, lane);
+#pragma unroll
+            for (int m = 0; m < MI; ++m) b[m] = SP::frag(ps, wi + 16 * m, ks, lane);
+#pragma unroll
+            for (int m = 0; m < MI; ++m)
+#pragma unroll
+                for (int n = 0; n < NI; ++n) acc[m][n] = mfma16<T>(a[n], b[m], acc[m][n]);
+        }
+        slot = slot + 1 == ST ? 0 : slot + 1;
+    }
+    wait_loads(0);                                           // nothing may be on its way into LDS when the wave ends
+
+    epilogue<T, TO, ACT, true, true, MI, NI>(o, acc, i0 + wi, j0 + wj, I, J, blockIdx.y, lane);
+}
+
+// The same product for many tiles.  Persistent: WGS workgroups a CU walk over the tiles, the ring running on into the next
+// tile's first stages while a tile's results are written.  A step's fragments are read, and the loads of the step RING
+// ahead started, between the products of the step before.
+// A contraction that one side is contiguous in is a multiple of 32 here, J a multiple of BN.
+template <typename T, typename TO, int ACT, bool EXTRA, int BM, int BN, int WM, int WN, int RING, int WGS, bool PT, bool QT>
+__global__ void __launch_bounds__(64 * (BM / WM) * (BN / WN), WGS * (BM / WM) * (BN / WN) / 4)
+k_mm16_walk(Side P, Side Q, Out o, long long I, int J, long long nq, long long q_per_part, int tiles_j, int n_tiles) {
+    constexpr int BK = 32, WAVES = (BM / WM) * (BN / WN);
+    typedef Stage<BM, BK, PT, WAVES, PT || QT> SP;
+    typedef Stage<BN, BK, QT, WAVES, PT || QT> SQ;
+    constexpr int kStage = SP::kBytes + SQ::kBytes, kLoads = SP::kLoads + SQ::kLoads;
+    constexpr int MI = WM / 16, NI = WN / 16;
+    __shared__ __attribute__((aligned(1024))) char lds[RING * kStage];
+
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wi = wave / (BN / WN) * WM, wj = wave % (BN / WN) * WN;
+    // consecutive workgroups go to the 8 XCDs in turn: each XCD walks its own run of tiles, j fastest
+    const int per = (n_tiles + 7) / 8, walkers = gridDim.x / 8;
+    const int first = (blockIdx.x & 7) * per, end = min(first + per, n_tiles);
+    const long long q0 = (long long)blockIdx.y * q_per_part;
+    const int nk = (int)(nq - q0 < q_per_part ? nq - q0 : q_per_part);
+    const int missing = (int)max(0LL, q0 + nk - (nq - Q.missing));           // of them on Q's side
+    const int pairs = max((RING + 1) / 2, (nk + 2 * BK - 1) / (2 * BK));   // steps run in twos, at least RING of them: the
+                                                                           // extra ones add zeros
+    int tile = first + (blockIdx.x >> 3);
+    if (tile >= end) return;
+    SP sp;
+    SQ sq;
+    int krem = 0;                                            // what is left of the tile the loads are in
+    auto enter = [&](int t) {
+        if (t < end) {
+            sp.init(P, (long long)(t / tiles_j) * BM, q0, wave, lane);
+            sq.init(Q, (long long)(t % tiles_j) * BN, q0, wave, lane);
+        }
+        krem = t < end ? nk : 0;                             // past the last tile: zeros
+    };
+    enter(tile);
+#pragma unroll
+    for (int s = 0; s < RING; ++s) {
+        sp.load(lds + s * kStage, krem, wave, lane);
+        sq.load(lds + s * kStage + SP::kBytes, krem - missing, wave, lane);
+        krem -= BK;
+    }
+    wait_loads(kLoads * (RING - 1));
+    int slot = 0, left = 2 * pairs - RING;                   // loads left in the tile they are in
+    f32x4 acc[MI][NI];
+    s16x8 a[2][NI], b[MI];
+    typename vec<T, 4>::type bias[NI];
+    load_bias<T, NI>(o, bias, tile % tiles_j * BN + wj, J, lane);
+    // Stores of the last tile's results are newer than the first RING stages of this one: while those are waited for
+    // (RING - 1 steps) they may stay outstanding; `old` is how many there are at least, rounded down to 16 or 32.
+    int old = 0, grace = 0;
+    auto step = [&](const s16x8 (&ca)[NI], s16x8 (&na)[NI]) {
+        if (grace > 0 && old >= 32) wait_loads(kLoads * (RING - 2) + 32);
+        else if (grace > 0 && old >= 16) wait_loads(kLoads * (RING - 2) + 16);
+        else wait_loads(kLoads * (RING - 2));
+        --grace;
+        barrier();                                           // step k + 1 has landed, step k has been read by all
+        char* into = lds + slot * kStage;
+        slot = slot + 1 == RING ? 0 : slot + 1;
+        const char* ps = lds + slot * kStage;
+        const __amdgpu_buffer_rsrc_t rp = sp.buffer(krem), rq = sq.buffer(krem - missing);
+        krem -= BK;
+#pragma unroll
+        for (int m = 0; m < MI; ++m) {
+#pragma unroll
+            for (int i = m * kLoads / MI; i < (m + 1) * kLoads / MI; ++i) {
+                if (i < SP::kLoads) sp.load_one(rp, into, i, sp.voff[i < SP::kLoads ? i : 0], wave);
+                else sq.load_one(rq, into + SP::kBytes, i - SP::kLoads, sq.voff[i < SP::kLoads ? 0 : i - SP::kLoads], wave);
+            }
+#pragma unroll
+            for (int n = m * NI / MI; n < (m + 1) * NI / MI; ++n) na[n] = SQ::frag(ps + SP::kBytes, wj + 16 * n, 0, lane);
+#pragma unroll
+            for (int n = 0; n < NI; ++n) acc[m][n] = mfma16<T>(ca[n], b[m], acc[m][n]);
+            b[m] = SP::frag(ps, wi + 16 * m, 0, lane);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        sp.advance();
+        sq.advance();
+    };
+    for (; tile < end; tile += walkers) {
+        barrier();                                           // the tile's first stage has landed
+#pragma unroll
+        for (int n = 0; n < NI; ++n) a[0][n] = SQ::frag(lds + slot * kStage + SP::kBytes, wj + 16 * n, 0, lane);
+#pragma unroll
+        for (int m = 0; m < MI; ++m) b[m] = SP::frag(lds + slot * kStage, wi + 16 * m, 0, lane);
+        start_sums<T, MI, NI>(acc, bias);
+#pragma unroll 1
+        for (int k = pairs; k > 0; --k) {
+            if (left == 0) enter(tile + walkers);
+            step(a[0], a[1]);
+            if (RING % 2 && left == 1) enter(tile + walkers);
+            left -= 2;
+            step(a[1], a[0]);
+        }
+        left = 2 * pairs - RING;
+        wait_loads(kLoads * (RING - 1));
+        if (tile + walkers < end) load_bias<T, NI>(o, bias, (tile + walkers) % tiles_j * BN + wj, J, lane);
+#pragma unroll
+        for (int n = 0; n < NI; ++n) {                       // arrived before the stores below are issued
+            typedef unsigned u2 __attribute__((ext_vector_type(2)));
+            u2 t = __builtin_bit_cast(u2, bias[n]);
+            asm volatile("" : "+v"(t) : : "memory");
+            bias[n] = __builtin_bit_cast(typename vec<T, 4>::type, t);
+        }
+        grace = RING - 1;
+        old = epilogue<T, TO, ACT, EXTRA, false, MI, NI>(o, acc, (long long)(tile / tiles_j) * BM + wi, tile % tiles_j * BN + wj, I, J, blockIdx.y, lane);
+    }
+    wait_loads(0);                                           // nothing may be on its way into LDS when the wave ends
+}
+
+}  // namespace gl_mm

@@ -73,7 +73,7 @@ def close(got, want, tol, what):
 def dense64(x, w, b, name, r, out_dtype):
     """(z, its tolerance, y, its tolerance) in 64 bits; tolerances for results of out_dtype."""
     x, w = x.double(), w.double()
-    b = torch.zeros(w.shape[0], dtype=torch.float64) if b is None else b.double()
+    b = torch.zeros(w.shape[0], dtype=torch.float64, device=w.device) if b is None else b.double()
     z = x @ w.t() + b
     size = x.abs() @ w.abs().t() + b.abs()
     off = (w.shape[1] + 16) * 2.0 ** -23 * size
@@ -252,6 +252,42 @@ def test_dense_backward_strides(M, K, N, name, dtype):
             close(g, v, t, what)
         for wide, n in ((dx_wide, K), (dw_wide, K)):
             assert wide[:, :left].isnan().all() and wide[:, left + n:].isnan().all()
+
+
+# sizes whose tiles fill the chip: the walking kernel (both sides' layouts), a rest of columns, odd and short contractions
+LARGE_SIZES = [(4400, 512, 2048), (33000, 96, 257), (16500, 544, 512), (40000, 32, 256), (33001, 72, 256), (70000, 64, 264)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype,out_dtype,name,extra", [(BF16, BF16, "gelu", False), (F16, F32, "exp", False), (F16, F16, "silu", True),
+                                                        (BF16, F32, None, True), (F32, F32, "tanh", True)])
+@pytest.mark.parametrize("M,K,N", LARGE_SIZES)
+def test_dense_many_rows(M, K, N, dtype, out_dtype, name, extra):
+    """The 64-bit side runs on the GPU here (plain float64 products)."""
+    x, w, b = (t.cuda() for t in (randn((M, K), dtype, 1), randn((N, K), dtype, 2, K ** -0.5), randn((N,), dtype, 3)))
+    r = randn((M, N), out_dtype, 4).cuda() if extra else None
+    z = torch.full((M, N), float("nan"), dtype=out_dtype, device="cuda") if extra else None
+    z64, z_tol, y64, y_tol = dense64(x, w, b, name, r, out_dtype)
+    y = inv.dense(x, w, b, activation=name, residual=r, out_dtype=out_dtype, preactivation=z)
+    close(y, y64.cpu(), y_tol.cpu(), "y")
+    if extra:
+        close(z, z64.cpu(), z_tol.cpu(), "preactivation")
+        inv.dense(x, w, b, activation=name, residual=r, out_dtype=out_dtype, out=r)
+        assert torch.equal(r, y)                                              # the residual stream in place
+
+
+@gpu
+@pytest.mark.parametrize("dtype,out_dtype,name", [(BF16, BF16, "gelu"), (F16, F32, "silu"), (BF16, BF16, None), (F32, F32, "gelu")])
+@pytest.mark.parametrize("M,K,N", [(9001, 1024, 1024), (16500, 512, 264), (33000, 256, 1025), (16400, 264, 512)])
+def test_dense_backward_many_rows(M, K, N, dtype, out_dtype, name):
+    x, w = randn((M, K), dtype, 1).cuda(), randn((N, K), dtype, 2, K ** -0.5).cuda()
+    z, dy = randn((M, N), out_dtype, 3).cuda(), randn((M, N), out_dtype, 4).cuda()
+    want = dense_back64(dy, x, w, z, name, dtype)
+    got = inv.dense_backward(dy, x, w, z if name else None, activation=name)
+    for g, (v, t), what in zip(got, want, ("dx", "dweight", "dbias")):
+        close(g, v.cpu(), t.cpu(), what)
+    again = inv.dense_backward(dy, x, w, z if name else None, activation=name)
+    assert all(torch.equal(a, c) for a, c in zip(got, again))
 
 
 @gpu
