@@ -3,13 +3,254 @@
 //   xh = (x - mean) rstd,  y = act(xh gamma + beta)          mean, rstd per (utterance, group) over its live frames
 //   du = dy act'(xh gamma + beta);  v = du gamma;  p = mean(v), q = mean(v xh) per (utterance, group)
 //   dx = rstd (v - p - xh q);  dgamma = sum du xh,  dbeta = sum du per channel over all live frames
+//
+// Bound by memory: x (and dy) in once, the result out once.  A workgroup that can hold its frames of some whole groups in
+// registers (16 bytes x 8 a thread) does everything in one pass: "slab" kernels.  Longer utterances are cut into chunks of
+// frames: statistics (sums) of the chunks, their join, and a second pass that applies them, the input then coming from the
+// 256 MB cache behind the L2s where it fits.  Variances are sums of squared distances from a mean already known (of the slab
+// or the chunk, joined with the distances between the means), never a difference of large sums.  All sums run in a
+// fixed order.
 #include "gl_internal.h"
 #include "gl_act.h"
 
 namespace {
 
+constexpr int kHeld = 8;                 // vectors of V channels a thread holds
+constexpr int kMaxThreads = 1024;
+
 __device__ __forceinline__ int live_frames(const int* frames, int b, int T) {
     return frames ? max(0, min(frames[b], T)) : T;
+}
+
+template <typename T, int V> struct vec_of { typedef T type __attribute__((ext_vector_type(V))); };
+template <typename T> struct vec_of<T, 1> { typedef T type; };
+template <typename T, int V>
+__device__ __forceinline__ float get(const typename vec_of<T, V>::type& v, int k) {
+    if constexpr (V == 1) return gl_to_f32(v);
+    else return gl_to_f32(v[k]);
+}
+template <typename T, int V>
+__device__ __forceinline__ void set(typename vec_of<T, V>::type& v, int k, float f) {
+    if constexpr (V == 1) v = (T)f;
+    else v[k] = (T)f;
+}
+
+// Where a workgroup works: CB channels from c0 (whole groups), threads as rows x TP vectors.
+struct Place {
+    int CB, TP, RP, r, col;              // channels, threads per row, rows at a time, this thread's row and first channel
+    bool on;
+};
+template <int V>
+__device__ __forceinline__ Place place(int CB) {
+    Place p;
+    p.CB = CB;
+    p.TP = CB / V;
+    p.RP = blockDim.x / p.TP;
+    p.r = threadIdx.x / p.TP;
+    p.col = (threadIdx.x - p.r * p.TP) * V;
+    p.on = p.r < p.RP;
+    return p;
+}
+
+// Sums of v (V channels a thread) over the workgroup's rows, per channel, to tot[CB]; red: blockDim.x * V floats.
+template <int V>
+__device__ __forceinline__ void channel_sums(const float (&v)[V], const Place& p, float* red, float* tot) {
+    __syncthreads();
+    if (p.on)
+#pragma unroll
+        for (int k = 0; k < V; ++k) red[p.r * p.CB + p.col + k] = v[k];
+    __syncthreads();
+    // rows in `segs` interleaved segments first where there are threads for it, then the segments
+    const int nt = blockDim.x;
+    const int segs = min(p.RP, nt / p.CB);
+    if (segs > 1) {
+        const int c = threadIdx.x % p.CB, s = threadIdx.x / p.CB;
+        float a = 0.0f;
+        if (s < segs)
+            for (int r = s; r < p.RP; r += segs) a += red[r * p.CB + c];
+        __syncthreads();
+        if (s < segs) red[s * p.CB + c] = a;
+        __syncthreads();
+    }
+    const int rows = segs > 1 ? segs : p.RP;
+    for (int c = threadIdx.x; c < p.CB; c += nt) {
+        float a = 0.0f;
+        for (int r = 0; r < rows; ++r) a += red[r * p.CB + c];
+        tot[c] = a;
+    }
+    __syncthreads();
+}
+// f(c) summed over the channels of each of the block's groups to out[group], a wave per group
+template <typename F>
+__device__ __forceinline__ void group_sums(const Place& p, int n, float* out, F f) {
+    const int lane = threadIdx.x & 63, waves = blockDim.x / 64;
+    for (int g = threadIdx.x / 64; g < p.CB / n; g += waves) {
+        float a = 0.0f;
+        for (int c = lane; c < n; c += 64) a += f(g * n + c);
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) a += __shfl_xor(a, o);
+        if (lane == 0) out[g] = a;
+    }
+    __syncthreads();
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void load_affine(const T* gamma, const T* beta, int c, float (&ga)[V], float (&be)[V]) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        ga[k] = gamma ? gl_to_f32(gamma[c + k]) : 1.0f;
+        be[k] = beta ? gl_to_f32(beta[c + k]) : 0.0f;
+    }
+}
+
+// One pass: statistics and result of CB channels of utterance b.  grid (blocks of channels x B), see block_of().
+// Neighbouring blocks share cache lines where CB channels are less than 128 bytes: they go to one XCD (ids 8 apart).
+struct Blocks {
+    int per_b, total;                    // blocks of channels per utterance, and in all
+    int CB, C;                           // channels of a block (the last may have fewer), of a row
+};
+__device__ __forceinline__ bool block_of(const Blocks& k, int& b, int& c0, int& CB) {
+    const int per = (k.total + 7) / 8;
+    const int id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if ((int)(blockIdx.x >> 3) >= per || id >= k.total) return false;
+    b = id / k.per_b;
+    c0 = (id - b * k.per_b) * k.CB;
+    CB = min(k.CB, k.C - c0);
+    return true;
+}
+
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(kMaxThreads) k_norm_slab(const T* x, long long x_stride, const T* __restrict__ gamma,
+                                                           const T* __restrict__ beta, const int* __restrict__ frames,
+                                                           T* y, long long y_stride, float* __restrict__ stats, int Tn, int n,
+                                                           int act, float eps, Blocks blocks) {
+    typedef typename vec_of<T, V>::type vT;
+    extern __shared__ float lds[];
+    int b, c0, CB;
+    if (!block_of(blocks, b, c0, CB)) return;
+    const Place p = place<V>(CB);
+    float* red = lds;                                        // [threads * V]
+    float* tot = red + blockDim.x * V;                       // [CB]
+    float* mean_g = tot + CB;                                // [CB / n] each
+    float* rstd_g = mean_g + CB / n;
+    const int live = live_frames(frames, b, Tn);
+    const int c = c0 + p.col;
+    const T* xb = x + (long long)b * Tn * x_stride + c;
+    vT held[kHeld];
+    float v[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[k] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+        const int t = p.r + i * p.RP;
+        if (p.on && t < live) held[i] = *(const vT*)(xb + (long long)t * x_stride);
+    }
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+        if (p.on && p.r + i * p.RP < live)
+#pragma unroll
+            for (int k = 0; k < V; ++k) v[k] += get<T, V>(held[i], k);
+    channel_sums<V>(v, p, red, tot);
+    const float count = (float)((long long)live * n);
+    const float inv = live ? 1.0f / count : 0.0f;
+    group_sums(p, n, mean_g, [&](int k) { return tot[k]; });
+    float mean[V], ga[V], be[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) mean[k] = p.on ? mean_g[(p.col + k) / n] * inv : 0.0f;
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[k] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+        if (p.on && p.r + i * p.RP < live)
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                const float d = get<T, V>(held[i], k) - mean[k];
+                v[k] = fmaf(d, d, v[k]);
+            }
+    channel_sums<V>(v, p, red, tot);
+    group_sums(p, n, rstd_g, [&](int k) { return tot[k]; });
+    const int groups = CB / n;
+    for (int g = threadIdx.x; g < groups; g += blockDim.x) {
+        const float rstd = live ? 1.0f / sqrtf(rstd_g[g] * inv + eps) : 0.0f;
+        rstd_g[g] = rstd;
+        if (stats) {
+            float* o = stats + 2 * ((long long)b * (blocks.C / n) + c0 / n + g);
+            o[0] = mean_g[g] * inv;
+            o[1] = rstd;
+        }
+    }
+    __syncthreads();
+    if (!p.on) return;
+    load_affine<T, V>(gamma, beta, c, ga, be);
+#pragma unroll
+    for (int k = 0; k < V; ++k) ga[k] *= rstd_g[(p.col + k) / n];
+    T* yb = y + (long long)b * Tn * y_stride + c;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+        const int t = p.r + i * p.RP;
+        if (t >= Tn) continue;
+        vT o;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const float u = fmaf(get<T, V>(held[i], k) - mean[k], ga[k], be[k]);
+            set<T, V>(o, k, t < live ? gl_act(u, ACT < 0 ? act : ACT) : 0.0f);
+        }
+        *(vT*)(yb + (long long)t * y_stride) = o;
+    }
+}
+
+// Chunks of RP * kHeld frames, all channels: mean and sum of squared distances per group.  grid (chunks, B);
+// parts [B][groups][chunks][2]
+template <typename T, int V>
+__global__ void __launch_bounds__(kMaxThreads) k_norm_chunk(const T* __restrict__ x, long long x_stride, const int* __restrict__ frames,
+                                                    float* __restrict__ parts, int Tn, int C, int n) {
+    typedef typename vec_of<T, V>::type vT;
+    extern __shared__ float lds[];
+    const Place p = place<V>(C);
+    float* red = lds;
+    float* tot = red + blockDim.x * V;
+    float* mean_g = tot + C;
+    float* m2_g = mean_g + C / n;
+    const int b = blockIdx.y, rows = p.RP * kHeld;
+    const int live = live_frames(frames, b, Tn);
+    const int t0 = blockIdx.x * rows, here = max(0, min(rows, live - t0));
+    const T* xb = x + ((long long)b * Tn + t0) * x_stride + p.col;
+    vT held[kHeld];
+    float v[V], mean[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[k] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+        const int t = p.r + i * p.RP;
+        if (p.on && t < here) held[i] = *(const vT*)(xb + (long long)t * x_stride);
+    }
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+        if (p.on && p.r + i * p.RP < here)
+#pragma unroll
+            for (int k = 0; k < V; ++k) v[k] += get<T, V>(held[i], k);
+    channel_sums<V>(v, p, red, tot);
+    const float inv = here ? 1.0f / (float)(here * n) : 0.0f;
+    group_sums(p, n, mean_g, [&](int k) { return tot[k]; });
+#pragma unroll
+    for (int k = 0; k < V; ++k) mean[k] = p.on ? mean_g[(p.col + k) / n] * inv : 0.0f;
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[k] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+        if (p.on && p.r + i * p.RP < here)
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                const float d = get<T, V>(held[i], k) - mean[k];
+                v[k] = fmaf(d, d, v[k]);
+            }
+    channel_sums<V>(v, p, red, tot);
+    group_sums(p, n, m2_g, [&](int k) { return tot[k]; });
+    for (int g = threadIdx.x; g < C / n; g += blockDim.x) {
+        float* o = parts + 2 * (((long long)b * (C / n) + g) * gridDim.x + blockIdx.x);
+        o[0] = mean_g[g] * inv;
+        o[1] = m2_g[g];
+    }
 }
 
 // Sum over the 256 threads of a workgroup, the same value in every thread; s: 4 floats of LDS.
@@ -22,9 +263,317 @@ __device__ __forceinline__ float block_sum(float v, float* s) {
     return (s[0] + s[1]) + (s[2] + s[3]);
 }
 
+// grid (groups, B): joins the chunks' means and distances.  rows: frames of a chunk
+__global__ void __launch_bounds__(256) k_norm_join(const float* __restrict__ parts, const int* __restrict__ frames,
+                                                   float* __restrict__ stats, int Tn, int n, int chunks, int rows, float eps) {
+    __shared__ float s[4];
+    const int g = blockIdx.x, b = blockIdx.y;
+    const int live = live_frames(frames, b, Tn);
+    const float* in = parts + 2 * ((long long)b * gridDim.x + g) * chunks;
+    auto frames_of = [&](int k) { return (float)max(0, min(rows, live - k * rows)); };
+    float m = 0.0f;
+    for (int k = threadIdx.x; k < chunks; k += 256) m += frames_of(k) * in[2 * k];
+    m = live ? block_sum(m, s) / (float)live : 0.0f;
+    float m2 = 0.0f;
+    for (int k = threadIdx.x; k < chunks; k += 256) {
+        const float d = in[2 * k] - m;
+        m2 += in[2 * k + 1] + frames_of(k) * (float)n * d * d;
+    }
+    m2 = block_sum(m2, s);
+    if (threadIdx.x == 0) {
+        float* o = stats + 2 * ((long long)b * gridDim.x + g);
+        o[0] = m;
+        o[1] = live ? 1.0f / sqrtf(m2 / ((float)live * (float)n) + eps) : 0.0f;
+    }
+}
+
+// grid (row blocks, B): y from x and the statistics
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(kMaxThreads) k_norm_apply(const T* x, long long x_stride, const T* __restrict__ gamma,
+                                                    const T* __restrict__ beta, const int* __restrict__ frames,
+                                                    const float* __restrict__ stats, T* y, long long y_stride, int Tn, int C,
+                                                    int n, int act) {
+    typedef typename vec_of<T, V>::type vT;
+    const Place p = place<V>(C);
+    if (!p.on) return;
+    const int b = blockIdx.y;
+    const int live = live_frames(frames, b, Tn);
+    float ga[V], be[V], mean[V];
+    load_affine<T, V>(gamma, beta, p.col, ga, be);
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        const float* st = stats + 2 * ((long long)b * (C / n) + (p.col + k) / n);
+        mean[k] = st[0];
+        ga[k] *= st[1];
+    }
+    const T* xb = x + (long long)b * Tn * x_stride + p.col;
+    T* yb = y + (long long)b * Tn * y_stride + p.col;
+    const int step = gridDim.x * p.RP;
+#pragma unroll 4
+    for (int t = blockIdx.x * p.RP + p.r; t < Tn; t += step) {
+        vT o = vT{};
+        if (t < live) {
+            const vT in = *(const vT*)(xb + (long long)t * x_stride);
+#pragma unroll
+            for (int k = 0; k < V; ++k)
+                set<T, V>(o, k, gl_act(fmaf(get<T, V>(in, k) - mean[k], ga[k], be[k]), ACT < 0 ? act : ACT));
+        }
+        *(vT*)(yb + (long long)t * y_stride) = o;
+    }
+}
+
+// ---- gradients ----
+
+// du and xh of one vector
+template <typename T, int V, int ACT>
+__device__ __forceinline__ void du_xh(const typename vec_of<T, V>::type& x, const typename vec_of<T, V>::type& dy, int k, float mean,
+                                      float rstd, float ga, float be, int act, float& du, float& xh) {
+    xh = (get<T, V>(x, k) - mean) * rstd;
+    du = get<T, V>(dy, k) * gl_act_grad(fmaf(xh, ga, be), ACT < 0 ? act : ACT);
+}
+
+// One pass, as k_norm_slab.  sums [B][2][C]: sum du xh, sum du per channel of the utterance
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(kMaxThreads) k_norm_back_slab(const T* dy, long long dy_stride, const T* __restrict__ x,
+                                                                long long x_stride, const float* __restrict__ stats,
+                                                                const T* __restrict__ gamma, const T* __restrict__ beta,
+                                                                const int* __restrict__ frames, T* dx, long long dx_stride,
+                                                                float* __restrict__ sums, int Tn, int n, int act, Blocks blocks) {
+    typedef typename vec_of<T, V>::type vT;
+    extern __shared__ float lds[];
+    int b, c0, CB;
+    if (!block_of(blocks, b, c0, CB)) return;
+    const Place p = place<V>(CB);
+    float* red = lds;
+    float* tot = red + blockDim.x * V;                       // [2][CB]
+    float* pq = tot + 2 * CB;                                // [2][CB / n]
+    const int live = live_frames(frames, b, Tn), C = blocks.C;
+    const int c = c0 + p.col;
+    const T* xb = x + (long long)b * Tn * x_stride + c;
+    const T* db = dy + (long long)b * Tn * dy_stride + c;
+    vT hx[kHeld], hd[kHeld];
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+        const int t = p.r + i * p.RP;
+        if (p.on && t < live) {
+            hx[i] = *(const vT*)(xb + (long long)t * x_stride);
+            hd[i] = *(const vT*)(db + (long long)t * dy_stride);
+        }
+    }
+    float ga[V], be[V], mean[V], rstd[V], a0[V], a1[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) a0[k] = a1[k] = 0.0f;
+    if (p.on) {
+        load_affine<T, V>(gamma, beta, c, ga, be);
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const float* st = stats + 2 * ((long long)b * (C / n) + (c + k) / n);
+            mean[k] = st[0];
+            rstd[k] = st[1];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+        if (p.on && p.r + i * p.RP < live)
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                float du, xh;
+                du_xh<T, V, ACT>(hx[i], hd[i], k, mean[k], rstd[k], ga[k], be[k], act, du, xh);
+                a0[k] = fmaf(du, xh, a0[k]);
+                a1[k] += du;
+            }
+    channel_sums<V>(a0, p, red, tot);
+    channel_sums<V>(a1, p, red, tot + CB);
+    for (int k = threadIdx.x; k < CB; k += blockDim.x) {
+        sums[((long long)b * 2 + 0) * C + c0 + k] = tot[k];
+        sums[((long long)b * 2 + 1) * C + c0 + k] = tot[CB + k];
+        const float g = gamma ? gl_to_f32(gamma[c0 + k]) : 1.0f;
+        tot[k] *= g;
+        tot[CB + k] *= g;
+    }
+    if (!dx) return;
+    __syncthreads();
+    group_sums(p, n, pq, [&](int k) { return tot[CB + k]; });
+    group_sums(p, n, pq + CB / n, [&](int k) { return tot[k]; });
+    if (!p.on) return;
+    const float count = (float)((long long)live * n);
+    float gp[V], gq[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        gp[k] = live ? pq[(p.col + k) / n] / count : 0.0f;
+        gq[k] = live ? pq[CB / n + (p.col + k) / n] / count : 0.0f;
+    }
+    T* ob = dx + (long long)b * Tn * dx_stride + c;
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+        const int t = p.r + i * p.RP;
+        if (t >= Tn) continue;
+        vT o = vT{};
+        if (t < live)
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                float du, xh;
+                du_xh<T, V, ACT>(hx[i], hd[i], k, mean[k], rstd[k], ga[k], be[k], act, du, xh);
+                set<T, V>(o, k, rstd[k] * (du * ga[k] - gp[k] - xh * gq[k]));
+            }
+        *(vT*)(ob + (long long)t * dx_stride) = o;
+    }
+}
+
+// grid (chunks, B): per channel sums of a run of `rows` frames to parts [B][chunks][2][C]
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(kMaxThreads) k_norm_back_chunk(const T* __restrict__ dy, long long dy_stride, const T* __restrict__ x,
+                                                         long long x_stride, const float* __restrict__ stats,
+                                                         const T* __restrict__ gamma, const T* __restrict__ beta,
+                                                         const int* __restrict__ frames, float* __restrict__ parts, int Tn, int C,
+                                                         int n, int rows, int act) {
+    typedef typename vec_of<T, V>::type vT;
+    extern __shared__ float lds[];
+    const Place p = place<V>(C);
+    float* red = lds;
+    float* tot = red + blockDim.x * V;
+    const int b = blockIdx.y;
+    const int live = live_frames(frames, b, Tn);
+    const int t0 = blockIdx.x * rows, t1 = min(t0 + rows, live);
+    float ga[V], be[V], mean[V], rstd[V], a0[V], a1[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) a0[k] = a1[k] = 0.0f;
+    if (p.on) {
+        load_affine<T, V>(gamma, beta, p.col, ga, be);
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const float* st = stats + 2 * ((long long)b * (C / n) + (p.col + k) / n);
+            mean[k] = st[0];
+            rstd[k] = st[1];
+        }
+        const T* xb = x + (long long)b * Tn * x_stride + p.col;
+        const T* db = dy + (long long)b * Tn * dy_stride + p.col;
+#pragma unroll 4
+        for (int t = t0 + p.r; t < t1; t += p.RP) {
+            const vT vx = *(const vT*)(xb + (long long)t * x_stride);
+            const vT vd = *(const vT*)(db + (long long)t * dy_stride);
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                float du, xh;
+                du_xh<T, V, ACT>(vx, vd, k, mean[k], rstd[k], ga[k], be[k], act, du, xh);
+                a0[k] = fmaf(du, xh, a0[k]);
+                a1[k] += du;
+            }
+        }
+    }
+    float* o = parts + ((long long)b * gridDim.x + blockIdx.x) * 2 * C;
+    channel_sums<V>(a0, p, red, tot);
+    for (int c = threadIdx.x; c < C; c += blockDim.x) o[c] = tot[c];
+    channel_sums<V>(a1, p, red, tot);
+    for (int c = threadIdx.x; c < C; c += blockDim.x) o[C + c] = tot[c];
+}
+
+// grid (groups, B): sums [B][2][C] over the chunks, and the group's p, q
+template <typename T>
+__global__ void __launch_bounds__(256) k_norm_back_join(const float* __restrict__ parts, const T* __restrict__ gamma,
+                                                        const int* __restrict__ frames, float* __restrict__ sums,
+                                                        float* __restrict__ pq, int Tn, int C, int n, int chunks) {
+    __shared__ float s[4], red[256];
+    const int g = blockIdx.x, b = blockIdx.y;
+    const int live = live_frames(frames, b, Tn);
+    const int w = n < 256 ? n : 256, lanes = 256 / w;        // channels at a time, chunk lanes per channel
+    const int c = threadIdx.x % w, l = threadIdx.x / w;
+    float p = 0.0f, q = 0.0f;
+    for (int c1 = 0; c1 < n; c1 += w)
+        for (int which = 0; which < 2; ++which) {
+            float a = 0.0f;
+            if (c1 + c < n && l < lanes)
+#pragma unroll 4
+                for (int k = l; k < chunks; k += lanes) a += parts[(((long long)b * chunks + k) * 2 + which) * C + g * n + c1 + c];
+            __syncthreads();
+            red[threadIdx.x] = a;
+            __syncthreads();
+            if (l == 0 && c1 + c < n) {
+                for (int k = 1; k < lanes; ++k) a += red[k * w + c];
+                sums[((long long)b * 2 + which) * C + g * n + c1 + c] = a;
+                const float v = a * (gamma ? gl_to_f32(gamma[g * n + c1 + c]) : 1.0f);
+                if (which) p += v;
+                else q += v;
+            }
+        }
+    p = block_sum(p, s);
+    q = block_sum(q, s);
+    if (threadIdx.x == 0) {
+        const float count = (float)live * (float)n;
+        float* o = pq + 2 * ((long long)b * gridDim.x + g);
+        o[0] = live ? p / count : 0.0f;
+        o[1] = live ? q / count : 0.0f;
+    }
+}
+
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(kMaxThreads) k_norm_back_apply(const T* dy, long long dy_stride, const T* __restrict__ x,
+                                                         long long x_stride, const float* __restrict__ stats,
+                                                         const float* __restrict__ pq, const T* __restrict__ gamma,
+                                                         const T* __restrict__ beta, const int* __restrict__ frames, T* dx,
+                                                         long long dx_stride, int Tn, int C, int n, int act) {
+    typedef typename vec_of<T, V>::type vT;
+    const Place p = place<V>(C);
+    if (!p.on) return;
+    const int b = blockIdx.y;
+    const int live = live_frames(frames, b, Tn);
+    float ga[V], be[V], mean[V], rstd[V], gp[V], gq[V];
+    load_affine<T, V>(gamma, beta, p.col, ga, be);
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        const long long at = 2 * ((long long)b * (C / n) + (p.col + k) / n);
+        mean[k] = stats[at];
+        rstd[k] = stats[at + 1];
+        gp[k] = pq[at];
+        gq[k] = pq[at + 1];
+    }
+    const T* xb = x + (long long)b * Tn * x_stride + p.col;
+    const T* db = dy + (long long)b * Tn * dy_stride + p.col;
+    T* ob = dx + (long long)b * Tn * dx_stride + p.col;
+    const int step = gridDim.x * p.RP;
+#pragma unroll 2
+    for (int t = blockIdx.x * p.RP + p.r; t < Tn; t += step) {
+        vT o = vT{};
+        if (t < live) {
+            const vT vx = *(const vT*)(xb + (long long)t * x_stride);
+            const vT vd = *(const vT*)(db + (long long)t * dy_stride);
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                float du, xh;
+                du_xh<T, V, ACT>(vx, vd, k, mean[k], rstd[k], ga[k], be[k], act, du, xh);
+                set<T, V>(o, k, rstd[k] * (du * ga[k] - gp[k] - xh * gq[k]));
+            }
+        }
+        *(vT*)(ob + (long long)t * dx_stride) = o;
+    }
+}
+
+// dgamma, dbeta: sums [B][2][C] over the utterances.  grid (blocks of 64 channels); thread (channel, one of 4 lanes)
+template <typename T>
+__global__ void __launch_bounds__(256) k_norm_back_affine(const float* __restrict__ sums, T* __restrict__ dgamma,
+                                                          T* __restrict__ dbeta, int B, int C) {
+    __shared__ float s[2][4][64];
+    const int k = threadIdx.x & 63, l = threadIdx.x >> 6, c = blockIdx.x * 64 + k;
+    float a0 = 0.0f, a1 = 0.0f;
+    if (c < C)
+#pragma unroll 4
+        for (int b = l; b < B; b += 4) {
+            a0 += sums[((long long)b * 2 + 0) * C + c];
+            a1 += sums[((long long)b * 2 + 1) * C + c];
+        }
+    s[0][l][k] = a0;
+    s[1][l][k] = a1;
+    __syncthreads();
+    if (l || c >= C) return;
+    if (dgamma) dgamma[c] = (T)((s[0][0][k] + s[0][1][k]) + (s[0][2][k] + s[0][3][k]));
+    if (dbeta) dbeta[c] = (T)((s[1][0][k] + s[1][1][k]) + (s[1][2][k] + s[1][3][k]));
+}
+
+// ---- any size and alignment, element by element ----
+
 // grid (groups, B): mean first, then the squared distances from it (no cancellation whatever the level of x)
 template <typename T>
-__global__ void __launch_bounds__(256) k_norm_stats(const T* __restrict__ x, long long stride, const int* __restrict__ frames,
+__global__ void __launch_bounds__(256) k_norm_plain_stats(const T* __restrict__ x, long long stride, const int* __restrict__ frames,
                                                     float* __restrict__ stats, int Tn, int n, float eps) {
     __shared__ float s[4];
     const int g = blockIdx.x, b = blockIdx.y;
@@ -48,9 +597,9 @@ __global__ void __launch_bounds__(256) k_norm_stats(const T* __restrict__ x, lon
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) k_norm_apply(const T* __restrict__ x, long long x_stride, const T* __restrict__ gamma,
+__global__ void __launch_bounds__(256) k_norm_plain_apply(const T* x, long long x_stride, const T* __restrict__ gamma,
                                                     const T* __restrict__ beta, const int* __restrict__ frames,
-                                                    const float* __restrict__ stats, T* __restrict__ y, long long y_stride,
+                                                    const float* __restrict__ stats, T* y, long long y_stride,
                                                     int Tn, int C, int n, int act) {
     const int b = blockIdx.y;
     const int live = live_frames(frames, b, Tn);
@@ -71,7 +620,7 @@ __global__ void __launch_bounds__(256) k_norm_apply(const T* __restrict__ x, lon
 
 // grid (groups, B): per channel sums over the live frames (parts [B][2][C]: sum du xh, sum du) and the group's p, q
 template <typename T>
-__global__ void __launch_bounds__(256) k_norm_back_sums(const T* __restrict__ dy, long long dy_stride, const T* __restrict__ x,
+__global__ void __launch_bounds__(256) k_norm_plain_back_sums(const T* __restrict__ dy, long long dy_stride, const T* __restrict__ x,
                                                         long long x_stride, const float* __restrict__ stats,
                                                         const T* __restrict__ gamma, const T* __restrict__ beta,
                                                         const int* __restrict__ frames, float* __restrict__ parts,
@@ -109,11 +658,11 @@ __global__ void __launch_bounds__(256) k_norm_back_sums(const T* __restrict__ dy
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) k_norm_back_apply(const T* __restrict__ dy, long long dy_stride,
+__global__ void __launch_bounds__(256) k_norm_plain_back_apply(const T* dy, long long dy_stride,
                                                          const T* __restrict__ x, long long x_stride,
                                                          const float* __restrict__ stats, const float* __restrict__ pq,
                                                          const T* __restrict__ gamma, const T* __restrict__ beta,
-                                                         const int* __restrict__ frames, T* __restrict__ dx,
+                                                         const int* __restrict__ frames, T* dx,
                                                          long long dx_stride, int Tn, int C, int n, int act) {
     const int b = blockIdx.y;
     const int live = live_frames(frames, b, Tn);
@@ -135,19 +684,7 @@ __global__ void __launch_bounds__(256) k_norm_back_apply(const T* __restrict__ d
     }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(256) k_norm_back_join(const float* __restrict__ parts, T* __restrict__ dgamma,
-                                                        T* __restrict__ dbeta, int B, int C) {
-    const int c = blockIdx.x * 256 + threadIdx.x;
-    if (c >= C) return;
-    float a0 = 0.0f, a1 = 0.0f;
-    for (int b = 0; b < B; ++b) {
-        a0 += parts[((long long)b * 2 + 0) * C + c];
-        a1 += parts[((long long)b * 2 + 1) * C + c];
-    }
-    if (dgamma) dgamma[c] = (T)a0;
-    if (dbeta) dbeta[c] = (T)a1;
-}
+// ---- host ----
 
 inline long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 inline long long align16(long long b) { return (b + 15) / 16 * 16; }
@@ -173,49 +710,193 @@ int check_workspace(const void* ws, long long have, long long need, const char* 
     if ((uintptr_t)ws % 16) return gl_set_error(GL_ERR_INVALID, "%s: workspace must be 16-byte aligned", who);
     return 0;
 }
+
 long long stats_bytes(int B, int groups) { return align16(8LL * B * groups); }
 
-unsigned apply_blocks(int B, int T, int C) {
+// Channels a load moves: 16 bytes where rows and channels allow, else one.
+bool vector_ok(const void* p, long long stride, int size) { return (uintptr_t)p % 16 == 0 && stride * size % 16 == 0; }
+
+size_t lds_bytes(int threads, int V, int CB, int n, int totals) {
+    return sizeof(float) * ((size_t)threads * V + (size_t)totals * CB + 2 * (size_t)(CB / n));
+}
+constexpr size_t kMaxLds = 65536;
+
+// How a call is cut.  kind 0: slabs, 1: chunks, 2: element by element (rows that no workgroup spans)
+struct Cut {
+    int kind, threads;
+    Blocks blocks;                       // slabs
+    int rows, chunks;                    // chunks: frames of one, and how many
+};
+constexpr int kWorkgroups = 1024;        // four a CU: chunks of the gradients' sums
+int threads_for(int tp, long long rows) {                    // the fewest threads whose rows hold `rows` frames, or 0
+    for (int t = 256; t <= kMaxThreads; t *= 2)
+        if (t >= tp && (long long)(t / tp) * kHeld >= rows) return t;
+    return 0;
+}
+Cut cut_for(int B, int T, int C, int groups, int size, int V) {
+    Cut c = {};
+    const int n = C / groups;
+    int k = 1;
+    while (k < groups && (n * k) % V) ++k;                   // whole groups on whole vectors
+    if (n * k % V == 0 && threads_for(n * k / V, T) && lds_bytes(kMaxThreads, V, n * k, n, 2) <= kMaxLds) {
+        // more groups to a block, to 128 bytes a row, while the slab fits and the blocks fill the chip
+        for (int m = 2 * k; m <= groups && (long long)n * k * size < 128; m += k)
+            if (groups % m == 0 && threads_for(n * m / V, T) && (long long)B * (groups / m) >= 256) k = m;
+        c.kind = 0;
+        c.threads = threads_for(n * k / V, T);
+        c.blocks = {(int)ceil_div(groups, k), 0, n * k, C};
+        c.blocks.total = B * c.blocks.per_b;
+        return c;
+    }
+    if (C / V > kMaxThreads || lds_bytes(kMaxThreads, V, C, n, 1) > kMaxLds) {
+        c.kind = 2;
+        return c;
+    }
+    c.kind = 1;
+    c.threads = C / V > 512 ? 1024 : 512;
+    c.rows = c.threads / (C / V) * kHeld;
+    c.chunks = (int)ceil_div(T, c.rows);
+    return c;
+}
+// frames of a chunk of the gradients' sums: enough chunks to fill the chip, 32 frames at least
+int back_rows(int B, int T) {
+    const long long chunks = B >= kWorkgroups ? 1 : kWorkgroups / B;
+    const long long r = ceil_div(T, chunks);
+    return (int)(r < 32 ? 32 : r);
+}
+unsigned apply_blocks(int B, int T, int rows_at_a_time) {
+    const long long per = ceil_div(T, 4LL * rows_at_a_time), most = 4096 / B;
+    return (unsigned)(per < 1 ? 1 : per < most ? per : most < 1 ? 1 : most);
+}
+unsigned plain_blocks(int B, int T, int C) {
     long long per = ceil_div((long long)T * C, 256 * 8), most = 256 * 16 / B;
     if (most < 1) most = 1;
     return (unsigned)(per < 1 ? 1 : per < most ? per : most);
 }
+template <int ACT> struct act_tag { static constexpr int value = ACT; };
+// f(act_tag<the activation>) where the vector kernels fix it, f(act_tag<-1>) elsewhere
+template <int V, typename F>
+int with_act(int act, F f) {
+    if constexpr (V == 1) return f(act_tag<-1>());
+    else
+        switch (act) {
+            case GL_ACT_RELU: return f(act_tag<GL_ACT_RELU>());
+            case GL_ACT_SILU: return f(act_tag<GL_ACT_SILU>());
+            case GL_ACT_GELU: return f(act_tag<GL_ACT_GELU>());
+            case GL_ACT_TANH: return f(act_tag<GL_ACT_TANH>());
+            case GL_ACT_EXP: return f(act_tag<GL_ACT_EXP>());
+            default: return f(act_tag<GL_ACT_NONE>());
+        }
+}
 
-template <typename T>
-int norm(const void* x, long long x_stride, const void* gamma, const void* beta, const int* frames, void* y,
-         long long y_stride, float* stats, int B, int Tn, int C, int groups, int act, float eps, hipStream_t st) {
-    const int n = C / groups;
-    hipLaunchKernelGGL((k_norm_stats<T>), dim3(groups, B), dim3(256), 0, st, (const T*)x, x_stride, frames, stats, Tn, n, eps);
+// workspace: [statistics where the caller wants none] [parts of the chunks]
+long long parts_bytes(int B, int T, int C, int groups, int dtype) {
+    const int size = dtype == GL_F32 ? 4 : 2;
+    long long most = 0;
+    for (int V : {16 / size, 1}) {                           // alignment is not known to the query
+        if (C % V) continue;
+        const Cut c = cut_for(B, T, C, groups, size, V);
+        if (c.kind == 1 && 8LL * B * groups * c.chunks > most) most = 8LL * B * groups * c.chunks;
+    }
+    return align16(most);
+}
+long long norm_bytes(int B, int T, int C, int groups, int dtype) {
+    return stats_bytes(B, groups) + (B && T ? parts_bytes(B, T, C, groups, dtype) : 0);
+}
+long long back_parts_bytes(int B, int T, int C) {
+    return B && T ? align16(8LL * B * ceil_div(T, back_rows(B, T)) * C) : 0;
+}
+// workspace of the gradients: [p, q] [sums B x 2 x C] [parts of the chunks]
+long long back_bytes(int B, int T, int C, int groups) {
+    return stats_bytes(B, groups) + align16(8LL * B * C) + back_parts_bytes(B, T, C);
+}
+
+struct Norm {
+    const void* x;
+    long long x_stride;
+    const void *gamma, *beta;
+    const int* frames;
+    int B, T, C, groups, act;
+    hipStream_t st;
+};
+
+template <typename T, int V>
+int norm_fwd(const Norm& a, void* y, long long y_stride, float* stats, float* given, float* parts, float eps) {
+    const int n = a.C / a.groups;
+    const T *x = (const T*)a.x, *ga = (const T*)a.gamma, *be = (const T*)a.beta;
+    Cut c = a.T ? cut_for(a.B, a.T, a.C, a.groups, sizeof(T), V) : Cut{2};
+    if (c.kind == 0)
+        return with_act<V>(a.act, [&](auto act) -> int {
+            hipLaunchKernelGGL((k_norm_slab<T, V, decltype(act)::value>), dim3((unsigned)((c.blocks.total + 7) / 8 * 8)),
+                               dim3(c.threads), lds_bytes(c.threads, V, c.blocks.CB, n, 1), a.st, x, a.x_stride, ga, be, a.frames,
+                               (T*)y, y_stride, given, a.T, n, a.act, eps, c.blocks);
+            GL_HIP_CHECK(hipGetLastError());
+            return 0;
+        });
+    if (c.kind == 1) {
+        hipLaunchKernelGGL((k_norm_chunk<T, V>), dim3(c.chunks, a.B), dim3(c.threads), lds_bytes(c.threads, V, a.C, n, 1), a.st, x,
+                           a.x_stride, a.frames, parts, a.T, a.C, n);
+        GL_HIP_CHECK(hipGetLastError());
+        hipLaunchKernelGGL(k_norm_join, dim3(a.groups, a.B), dim3(256), 0, a.st, parts, a.frames, stats, a.T, n, c.chunks, c.rows, eps);
+        GL_HIP_CHECK(hipGetLastError());
+        return with_act<V>(a.act, [&](auto act) -> int {
+            hipLaunchKernelGGL((k_norm_apply<T, V, decltype(act)::value>),
+                               dim3(apply_blocks(a.B, a.T, c.threads / (a.C / V)), a.B), dim3(c.threads), 0, a.st, x, a.x_stride,
+                               ga, be, a.frames, stats, (T*)y, y_stride, a.T, a.C, n, a.act);
+            GL_HIP_CHECK(hipGetLastError());
+            return 0;
+        });
+    }
+    hipLaunchKernelGGL((k_norm_plain_stats<T>), dim3(a.groups, a.B), dim3(256), 0, a.st, x, a.x_stride, a.frames, stats, a.T, n, eps);
     GL_HIP_CHECK(hipGetLastError());
-    hipLaunchKernelGGL((k_norm_apply<T>), dim3(apply_blocks(B, Tn, C), B), dim3(256), 0, st, (const T*)x, x_stride,
-                       (const T*)gamma, (const T*)beta, frames, stats, (T*)y, y_stride, Tn, C, n, act);
+    if (!a.T) return 0;
+    hipLaunchKernelGGL((k_norm_plain_apply<T>), dim3(plain_blocks(a.B, a.T, a.C), a.B), dim3(256), 0, a.st, x, a.x_stride, ga, be,
+                       a.frames, stats, (T*)y, y_stride, a.T, a.C, n, a.act);
     GL_HIP_CHECK(hipGetLastError());
     return 0;
 }
 
-template <typename T>
-int norm_back(const void* dy, long long dy_stride, const void* x, long long x_stride, const float* stats, const void* gamma,
-              const void* beta, const int* frames, void* dx, long long dx_stride, void* dgamma, void* dbeta, int B, int Tn,
-              int C, int groups, int act, void* ws, hipStream_t st) {
-    const int n = C / groups;
-    float* pq = (float*)ws;
-    float* parts = (float*)((char*)ws + stats_bytes(B, groups));
-    if (B > 0 && Tn > 0) {
-        hipLaunchKernelGGL((k_norm_back_sums<T>), dim3(groups, B), dim3(256), 0, st, (const T*)dy, dy_stride, (const T*)x,
-                           x_stride, stats, (const T*)gamma, (const T*)beta, frames, parts, pq, Tn, C, n, act);
-        GL_HIP_CHECK(hipGetLastError());
-        if (dx) {
-            hipLaunchKernelGGL((k_norm_back_apply<T>), dim3(apply_blocks(B, Tn, C), B), dim3(256), 0, st, (const T*)dy, dy_stride,
-                               (const T*)x, x_stride, stats, pq, (const T*)gamma, (const T*)beta, frames, (T*)dx, dx_stride, Tn,
-                               C, n, act);
+template <typename T, int V>
+int norm_back(const Norm& a, const void* dy_, long long dy_stride, const float* stats, void* dx_, long long dx_stride, float* pq,
+              float* sums, float* parts) {
+    const int n = a.C / a.groups;
+    const T *x = (const T*)a.x, *ga = (const T*)a.gamma, *be = (const T*)a.beta, *dy = (const T*)dy_;
+    T* dx = (T*)dx_;
+    const Cut c = cut_for(a.B, a.T, a.C, a.groups, sizeof(T), V);
+    if (c.kind == 0)
+        return with_act<V>(a.act, [&](auto act) -> int {
+            hipLaunchKernelGGL((k_norm_back_slab<T, V, decltype(act)::value>), dim3((unsigned)((c.blocks.total + 7) / 8 * 8)),
+                               dim3(c.threads), lds_bytes(c.threads, V, c.blocks.CB, n, 2), a.st, dy, dy_stride, x, a.x_stride,
+                               stats, ga, be, a.frames, dx, dx_stride, sums, a.T, n, a.act, c.blocks);
             GL_HIP_CHECK(hipGetLastError());
-        }
+            return 0;
+        });
+    if (c.kind == 1) {
+        const int rows = back_rows(a.B, a.T), chunks = (int)ceil_div(a.T, rows);
+        return with_act<V>(a.act, [&](auto act) -> int {
+            constexpr int ACT = decltype(act)::value;
+            hipLaunchKernelGGL((k_norm_back_chunk<T, V, ACT>), dim3(chunks, a.B), dim3(c.threads),
+                               lds_bytes(c.threads, V, a.C, n, 1), a.st, dy, dy_stride, x, a.x_stride, stats, ga, be, a.frames, parts,
+                               a.T, a.C, n, rows, a.act);
+            GL_HIP_CHECK(hipGetLastError());
+            hipLaunchKernelGGL((k_norm_back_join<T>), dim3(a.groups, a.B), dim3(256), 0, a.st, parts, ga, a.frames, sums, pq, a.T,
+                               a.C, n, chunks);
+            GL_HIP_CHECK(hipGetLastError());
+            if (!dx) return 0;
+            hipLaunchKernelGGL((k_norm_back_apply<T, V, ACT>), dim3(apply_blocks(a.B, a.T, c.threads / (a.C / V)), a.B),
+                               dim3(c.threads), 0, a.st, dy, dy_stride, x, a.x_stride, stats, pq, ga, be, a.frames, dx, dx_stride,
+                               a.T, a.C, n, a.act);
+            GL_HIP_CHECK(hipGetLastError());
+            return 0;
+        });
     }
-    if (dgamma || dbeta) {
-        hipLaunchKernelGGL((k_norm_back_join<T>), dim3((unsigned)ceil_div(C, 256)), dim3(256), 0, st, parts, (T*)dgamma,
-                           (T*)dbeta, Tn > 0 ? B : 0, C);
-        GL_HIP_CHECK(hipGetLastError());
-    }
+    hipLaunchKernelGGL((k_norm_plain_back_sums<T>), dim3(a.groups, a.B), dim3(256), 0, a.st, dy, dy_stride, x, a.x_stride, stats, ga,
+                       be, a.frames, sums, pq, a.T, a.C, n, a.act);
+    GL_HIP_CHECK(hipGetLastError());
+    if (!dx) return 0;
+    hipLaunchKernelGGL((k_norm_plain_back_apply<T>), dim3(plain_blocks(a.B, a.T, a.C), a.B), dim3(256), 0, a.st, dy, dy_stride, x,
+                       a.x_stride, stats, pq, ga, be, a.frames, dx, dx_stride, a.T, a.C, n, a.act);
+    GL_HIP_CHECK(hipGetLastError());
     return 0;
 }
 
@@ -225,7 +906,7 @@ extern "C" {
 
 long long gl_group_norm_workspace(int B, int T, int channels, int groups, int dtype) {
     if (check_norm(B, T, channels, groups, dtype, 0, "gl_group_norm_workspace")) return GL_ERR_INVALID;
-    return stats_bytes(B, groups);
+    return norm_bytes(B, T, channels, groups, dtype);
 }
 
 int gl_group_norm(const void* x, long long x_stride, const void* gamma, const void* beta, const int* frames, void* y,
@@ -237,20 +918,24 @@ int gl_group_norm(const void* x, long long x_stride, const void* gamma, const vo
     if (T > 0 && (!x || !y)) return gl_set_error(GL_ERR_INVALID, "gl_group_norm: NULL buffer");
     rc = check_stride(x_stride, channels, "x", "gl_group_norm");
     if (!rc) rc = check_stride(y_stride, channels, "y", "gl_group_norm");
-    if (!rc) rc = check_workspace(workspace, workspace_bytes, stats_bytes(B, groups), "gl_group_norm");
+    if (!rc) rc = check_workspace(workspace, workspace_bytes, norm_bytes(B, T, channels, groups, dtype), "gl_group_norm");
     if (rc) return rc;
     if (T == 0 && !stats) return 0;
     float* s = stats ? stats : (float*)workspace;
-    const hipStream_t st = (hipStream_t)stream;
-#define GL_NORM(T_)                                                                                                     \
-    norm<T_>(x, x_stride, gamma, beta, frames, y, y_stride, s, B, T, channels, groups, activation, eps, st)
-    return dtype == GL_F32 ? GL_NORM(float) : dtype == GL_BF16 ? GL_NORM(gl_bf16) : GL_NORM(gl_f16);
+    float* parts = (float*)((char*)workspace + stats_bytes(B, groups));
+    const Norm a = {x, x_stride, gamma, beta, frames, B, T, channels, groups, activation, (hipStream_t)stream};
+    const int size = dtype == GL_F32 ? 4 : 2, full = 16 / size;
+    const bool wide = channels % full == 0 && vector_ok(x, x_stride, size) && vector_ok(y, y_stride, size);
+#define GL_NORM(T_, V) norm_fwd<T_, V>(a, y, y_stride, s, stats, parts, eps)
+    if (dtype == GL_F32) return wide ? GL_NORM(float, 4) : GL_NORM(float, 1);
+    if (dtype == GL_BF16) return wide ? GL_NORM(gl_bf16, 8) : GL_NORM(gl_bf16, 1);
+    return wide ? GL_NORM(gl_f16, 8) : GL_NORM(gl_f16, 1);
 #undef GL_NORM
 }
 
 long long gl_group_norm_backward_workspace(int B, int T, int channels, int groups, int dtype) {
     if (check_norm(B, T, channels, groups, dtype, 0, "gl_group_norm_backward_workspace")) return GL_ERR_INVALID;
-    return stats_bytes(B, groups) + align16(8LL * B * channels);
+    return back_bytes(B, T, channels, groups);
 }
 
 int gl_group_norm_backward(const void* dy, long long dy_stride, const void* x, long long x_stride, const float* stats,
@@ -259,22 +944,38 @@ int gl_group_norm_backward(const void* dy, long long dy_stride, const void* x, l
                            int activation, void* workspace, long long workspace_bytes, void* stream) {
     int rc = check_norm(B, T, channels, groups, dtype, activation, "gl_group_norm_backward");
     if (rc) return rc;
+    const hipStream_t st = (hipStream_t)stream;
+    float* pq = (float*)workspace;
+    float* sums = (float*)((char*)workspace + stats_bytes(B, groups));
     if (B > 0 && T > 0) {
         if (!dy || !x || !stats) return gl_set_error(GL_ERR_INVALID, "gl_group_norm_backward: NULL buffer");
         rc = check_stride(dy_stride, channels, "dy", "gl_group_norm_backward");
         if (!rc) rc = check_stride(x_stride, channels, "x", "gl_group_norm_backward");
         if (!rc && dx) rc = check_stride(dx_stride, channels, "dx", "gl_group_norm_backward");
         if (!rc)
-            rc = check_workspace(workspace, workspace_bytes,
-                                 gl_group_norm_backward_workspace(B, T, channels, groups, dtype), "gl_group_norm_backward");
+            rc = check_workspace(workspace, workspace_bytes, back_bytes(B, T, channels, groups), "gl_group_norm_backward");
+        if (rc) return rc;
+        float* parts = (float*)((char*)sums + align16(8LL * B * channels));
+        const Norm a = {x, x_stride, gamma, beta, frames, B, T, channels, groups, activation, st};
+        const int size = dtype == GL_F32 ? 4 : 2, full = 16 / size;
+        const bool wide = channels % full == 0 && vector_ok(x, x_stride, size) && vector_ok(dy, dy_stride, size) &&
+                          (!dx || vector_ok(dx, dx_stride, size));
+#define GL_NORM(T_, V) norm_back<T_, V>(a, dy, dy_stride, stats, dx, dx_stride, pq, sums, parts)
+        if (dtype == GL_F32) rc = wide ? GL_NORM(float, 4) : GL_NORM(float, 1);
+        else if (dtype == GL_BF16) rc = wide ? GL_NORM(gl_bf16, 8) : GL_NORM(gl_bf16, 1);
+        else rc = wide ? GL_NORM(gl_f16, 8) : GL_NORM(gl_f16, 1);
+#undef GL_NORM
         if (rc) return rc;
     }
-    const hipStream_t st = (hipStream_t)stream;
-#define GL_NORM(T_)                                                                                                     \
-    norm_back<T_>(dy, dy_stride, x, x_stride, stats, gamma, beta, frames, dx, dx_stride, dgamma, dbeta, B, T, channels, \
-                  groups, activation, workspace, st)
-    return dtype == GL_F32 ? GL_NORM(float) : dtype == GL_BF16 ? GL_NORM(gl_bf16) : GL_NORM(gl_f16);
-#undef GL_NORM
+    if (dgamma || dbeta) {
+        const dim3 grid((unsigned)ceil_div(channels, 64));
+        const int rows = T > 0 ? B : 0;
+        if (dtype == GL_F32) hipLaunchKernelGGL((k_norm_back_affine<float>), grid, dim3(256), 0, st, sums, (float*)dgamma, (float*)dbeta, rows, channels);
+        else if (dtype == GL_BF16) hipLaunchKernelGGL((k_norm_back_affine<gl_bf16>), grid, dim3(256), 0, st, sums, (gl_bf16*)dgamma, (gl_bf16*)dbeta, rows, channels);
+        else hipLaunchKernelGGL((k_norm_back_affine<gl_f16>), grid, dim3(256), 0, st, sums, (gl_f16*)dgamma, (gl_f16*)dbeta, rows, channels);
+        GL_HIP_CHECK(hipGetLastError());
+    }
+    return 0;
 }
 
 }  // extern "C"
