@@ -6,6 +6,7 @@
 struct gl_operand {              // element (i, q) at base[i * is + q * qs], one of is, qs is 1
     const void* base;
     long long is, qs;
+    long long plane = 0;         // elements between the three planes of a float32 operand
     bool padded = false;         // this library's own copy: zeros up to whole multiples of 32 in the contiguous direction
     bool across() const { return is == 1 && qs != 1; }       // contiguous across the contraction
 };
@@ -20,6 +21,10 @@ struct gl_epilogue {
     long long z_stride;
     int act;
     float* partial;              // [parts][I][J]: sums of one part of the contraction, finished by k_dense_join
+    // float32 through planes: the operands themselves, for the sums that are not finite, and the flags of their blocks
+    const float *exact_p, *exact_q;
+    long long exact_p_is, exact_p_qs, exact_q_is, exact_q_qs, exact_nq;
+    int* flags;
 };
 
 static inline long long gl_ceil_div(long long a, long long b) { return (a + b - 1) / b; }
@@ -32,21 +37,24 @@ struct gl_mm_plan {
     int parts;                   // of the contraction
     long long per;               // contraction indexes in a part
 };
-// any_q: both sides are contiguous across the contraction, which may then have any length.
+// any_q: both sides are contiguous across the contraction, which may then have any length.  out_size: bytes of a result.
 gl_mm_plan gl_mm_plan_for(long long I, int J, long long nq, bool any_q);
 // columns the first of the product's two launches takes (the rest has its own plan): all, or a multiple of 256
-int gl_mm_first_columns(long long I, int J, long long nq, bool any_q);
+int gl_mm_first_columns(long long I, int J, long long nq, bool any_q, int out_size);
 long long gl_mm_partial_bytes(long long I, int J, long long nq, bool any_q);
 
 // Whether the fast kernels take the operands as they lie, else the strided kernel does.
 bool gl_mm16_takes(const gl_operand& P, const gl_operand& Q, const gl_epilogue& e, long long I, int J, long long nq, int out_size);
-// T: gl_bf16 / gl_f16; TO: T or float
-template <typename T, typename TO>
+// T: gl_bf16 / gl_f16; TO: T or float; TB: type of the bias; SEG 6: planes of float32 operands, else 1
+template <typename T, typename TO, typename TB, int SEG>
 int gl_mm16(const gl_operand& P, const gl_operand& Q, gl_epilogue e, long long I, int J, long long nq, float* partial, hipStream_t st);
 
 // sums the parts in their order and finishes the elements
 template <typename T, typename TO>
 int gl_dense_join(const gl_epilogue& e, long long I, int J, int parts, hipStream_t st);
+
+// computes the 64 x 64 blocks that are flagged, on the float32 operands
+int gl_dense_flagged(const gl_epilogue& e, long long I, int J, long long nq, hipStream_t st);
 
 // sum -> (preactivation, y) of element (i, j)
 template <typename T, typename TO>

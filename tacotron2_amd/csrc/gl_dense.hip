@@ -4,40 +4,40 @@
 //   forward   P = x  [rows][inputs],   Q = W  [outputs][inputs]      both contiguous in q
 //   dx        P = dz [rows][outputs],  Q(j, q) = W[q][j]             Q contiguous in j
 //   dweight   P(i, q) = dz[q][i],      Q(j, q) = x[q][j]             both contiguous in i / j, q = frames
-// 16-bit types: v_mfma_f32_32x32x16 (8 consecutive q per lane), 32-bit: v_mfma_f32_32x32x2_f32; sums are fp32.  Q is the
-// matrix instruction's A operand: the accumulator's registers then run along j, the contiguous direction of C.
+// Which kernel, by sizes alone (the workspace query and the call must agree):
+//   up to 8 rows (forward): k_dense_few, one wave (or part of one) a column: W is read once, nothing else counts;
+//   16-bit types: the tiles of gl_mm16.h, on copies padded to whole chunks where a width is not a multiple of 8;
+//   float32 with enough work: the same tiles on three bfloat16 planes;
+//   the rest, and operands whose rows start off 16 bytes against their widths: k_dense_any, element by element, on
+//   v_mfma_f32_32x32x16 or, for float32, v_mfma_f32_32x32x2_f32.
+// Sums are float32 everywhere.  Q is the matrix instruction's A operand: the accumulator's registers then run along j, the
+// contiguous direction of C.
 #include "gl_dense.h"
 
 namespace {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-template <typename T> struct vec8 { typedef T type __attribute__((ext_vector_type(8))); };
-
-constexpr int kTile = 64;        // rows and columns of C per workgroup (4 waves, 32 x 32 each)
-constexpr int kBQ = 32;          // contraction indexes staged per step
-
+template <typename T, int N> struct vecn { typedef T type __attribute__((ext_vector_type(N))); };
 typedef gl_operand Operand;
 typedef gl_epilogue Epilogue;
 
-// Any size, stride and alignment: elements are staged one by one.  grid (tiles, splits).
+constexpr int kTile = 64;        // rows and columns of C per workgroup (4 waves, 32 x 32 each)
+constexpr int kBQ = 32;          // contraction indexes staged per step
+constexpr int kCUs = 256;        // compute units of an MI355X: the work split must not depend on the moment
+
+// Any size, stride and alignment: elements are staged one by one.  grid (workgroups, parts); workgroups walk over the tiles.
+// flags: only the tiles whose flag is set.
 template <typename T, typename TO>
 __global__ void __launch_bounds__(256) k_dense_any(Operand P, Operand Q, Epilogue e, long long I, int J, long long nq,
-                                                   long long q_per_split, int tiles_j) {
+                                                   long long q_per_part, int tiles_j, int n_tiles, const int* __restrict__ flags) {
     constexpr bool k16 = sizeof(T) == 2;
     constexpr int kPitch = k16 ? kBQ + 8 : kBQ + 1;
     __shared__ __attribute__((aligned(16))) T Ps[kTile * kPitch];
     __shared__ __attribute__((aligned(16))) T Qs[kTile * kPitch];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 31, lk = lane >> 5;
-    const long long i0 = (long long)(blockIdx.x / tiles_j) * kTile;
-    const int j0 = (int)(blockIdx.x % tiles_j) * kTile;
-    const long long q_begin = (long long)blockIdx.y * q_per_split;
-    const long long q_end = q_begin + q_per_split < nq ? q_begin + q_per_split : nq;
+    const long long q_begin = (long long)blockIdx.y * q_per_part;
+    const long long q_end = q_begin + q_per_part < nq ? q_begin + q_per_part : nq;
     const int wi = (wave >> 1) * 32, wj = (wave & 1) * 32;
-
-    f32x16 acc;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) acc[r] = 0.0f;
-
     auto stage = [&](T* dst, const Operand& o, long long r0, long long rn, long long q0) {
         for (int e8 = threadIdx.x; e8 < kTile * kBQ; e8 += 256) {
             // consecutive threads along the contiguous direction
@@ -48,86 +48,220 @@ __global__ void __launch_bounds__(256) k_dense_any(Operand P, Operand Q, Epilogu
             dst[r * kPitch + q] = v;
         }
     };
-    for (long long q0 = q_begin; q0 < q_end; q0 += kBQ) {
-        __syncthreads();
-        stage(Ps, P, i0, I, q0);
-        stage(Qs, Q, j0, J, q0);
-        __syncthreads();
-        if constexpr (k16) {
-            typedef typename vec8<T>::type v8;
+    for (long long tile = blockIdx.x; tile < n_tiles; tile += gridDim.x) {
+        if (flags && !flags[tile]) continue;                 // uniform over the workgroup
+        const long long i0 = tile / tiles_j * kTile;
+        const int j0 = (int)(tile % tiles_j) * kTile;
+        f32x16 acc;
 #pragma unroll
-            for (int s = 0; s < kBQ; s += 16) {
-                const v8 a = *(const v8*)(Qs + (wj + li) * kPitch + s + 8 * lk);
-                const v8 b = *(const v8*)(Ps + (wi + li) * kPitch + s + 8 * lk);
-                if constexpr (__is_same(T, gl_bf16))
-                    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, acc, 0, 0, 0);
-                else
-                    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, acc, 0, 0, 0);
+        for (int r = 0; r < 16; ++r) acc[r] = 0.0f;
+        for (long long q0 = q_begin; q0 < q_end; q0 += kBQ) {
+            __syncthreads();
+            stage(Ps, P, i0, I, q0);
+            stage(Qs, Q, j0, J, q0);
+            __syncthreads();
+            if constexpr (k16) {
+                typedef typename vecn<T, 8>::type v8;
+#pragma unroll
+                for (int s = 0; s < kBQ; s += 16) {
+                    const v8 a = *(const v8*)(Qs + (wj + li) * kPitch + s + 8 * lk);
+                    const v8 b = *(const v8*)(Ps + (wi + li) * kPitch + s + 8 * lk);
+                    if constexpr (__is_same(T, gl_bf16))
+                        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, acc, 0, 0, 0);
+                    else
+                        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, acc, 0, 0, 0);
+                }
+            } else {
+#pragma unroll
+                for (int s = 0; s < kBQ; s += 2)
+                    acc = __builtin_amdgcn_mfma_f32_32x32x2f32(Qs[(wj + li) * kPitch + s + lk], Ps[(wi + li) * kPitch + s + lk],
+                                                               acc, 0, 0, 0);
             }
-        } else {
+        }
+        const long long i = i0 + wi + li;
+        if (i >= I) continue;
 #pragma unroll
-            for (int s = 0; s < kBQ; s += 2)
-                acc = __builtin_amdgcn_mfma_f32_32x32x2f32(Qs[(wj + li) * kPitch + s + lk], Ps[(wi + li) * kPitch + s + lk],
-                                                           acc, 0, 0, 0);
+        for (int r = 0; r < 16; ++r) {
+            const int j = j0 + wj + (r & 3) + 8 * (r >> 2) + 4 * lk;
+            if (j >= J) continue;
+            if (e.partial) e.partial[((long long)blockIdx.y * I + i) * J + j] = acc[r];
+            else gl_finish<T, TO>(e, i, j, acc[r]);
         }
     }
-    const long long i = i0 + wi + li;
-    if (i >= I) return;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-        const int j = j0 + wj + (r & 3) + 8 * (r >> 2) + 4 * lk;
-        if (j >= J) continue;
-        if (e.partial) e.partial[((long long)blockIdx.y * I + i) * J + j] = acc[r];
-        else gl_finish<T, TO>(e, i, j, acc[r]);
-    }
 }
 
-// Sums the parts of a split contraction in their order and finishes the element.
-template <typename T, typename TO>
-__global__ void __launch_bounds__(256) k_dense_join(Epilogue e, long long I, int J, int splits) {
+// Sums the parts of a split contraction in their order and finishes the elements, V at a time.
+template <typename T, typename TO, int V>
+__global__ void __launch_bounds__(256) k_dense_join(Epilogue e, long long I, int J, int parts) {
+    typedef typename vecn<float, V>::type vf;
     const long long n = I * J;
-    for (long long at = (long long)blockIdx.x * 256 + threadIdx.x; at < n; at += (long long)gridDim.x * 256) {
-        float s = 0.0f;
-        for (int p = 0; p < splits; ++p) s += e.partial[p * n + at];
+    for (long long at = ((long long)blockIdx.x * 256 + threadIdx.x) * V; at < n; at += (long long)gridDim.x * 256 * V) {
+        vf s = *(const vf*)(e.partial + at);
+#pragma unroll 4
+        for (int p = 1; p < parts; ++p) s += *(const vf*)(e.partial + p * n + at);
         const long long i = at / J;
-        gl_finish<T, TO>(e, i, (int)(at - i * J), s);
+        const int j = (int)(at - i * J);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            float sum = s[v];
+            if (e.exact_p && !(fabsf(sum) < INFINITY)) {     // float32 through planes, not finite: once more from the operands
+                sum = 0.0f;
+                for (long long q = 0; q < e.exact_nq && sum == sum; ++q)
+                    sum = fmaf(e.exact_p[i * e.exact_p_is + q * e.exact_p_qs], e.exact_q[(j + v) * e.exact_q_is + q * e.exact_q_qs], sum);
+            }
+            gl_finish<T, TO>(e, i, j + v, sum);
+        }
     }
 }
 
-// dz = dy act'(z), rounded to T for the products that read it, and column sums over this workgroup's frames.
-// grid (column blocks of 64, parts); thread = (column, one of 4 frame lanes).
-template <typename T, typename TO>
+// Up to ROWS frames: L lanes a column (as many as 16-byte pieces of its weights, to 64), 64 / L columns a wave.  W streams
+// through once.
+template <typename T, typename TO, int ROWS, bool VEC>
+__global__ void __launch_bounds__(256) k_dense_few(const T* __restrict__ x, long long x_stride, const T* __restrict__ w,
+                                                   long long w_stride, Epilogue e, int rows, int K, int N, int L) {
+    constexpr int V = VEC ? 16 / sizeof(T) : 1;
+    typedef typename vecn<T, V>::type vT;
+    const int lane = threadIdx.x & 63, l = lane & (L - 1);
+    const int n = (blockIdx.x * 4 + (threadIdx.x >> 6)) * (64 / L) + lane / L;
+    float acc[ROWS];
+#pragma unroll
+    for (int m = 0; m < ROWS; ++m) acc[m] = 0.0f;
+    if (n < N) {
+        const T* wn = w + n * w_stride;
+#pragma unroll 2
+        for (int k = l * V; k < K; k += L * V) {
+            const vT wv = *(const vT*)(wn + k);
+#pragma unroll
+            for (int m = 0; m < ROWS; ++m) {
+                if (m >= rows) break;                        // uniform
+                const vT xv = *(const vT*)(x + m * x_stride + k);
+#pragma unroll
+                for (int v = 0; v < V; ++v) acc[m] = fmaf(gl_to_f32(xv[v]), gl_to_f32(wv[v]), acc[m]);
+            }
+        }
+    }
+#pragma unroll
+    for (int m = 0; m < ROWS; ++m)
+        for (int o = L / 2; o > 0; o >>= 1) acc[m] += __shfl_xor(acc[m], o);
+    if (n >= N) return;
+#pragma unroll
+    for (int m = 0; m < ROWS; ++m)
+        if (m < rows && l == m) gl_finish<T, TO>(e, m, n, acc[m]);
+}
+
+// Copies a matrix into rows of whole chunks: zeros up to `padded` columns.  PLANES 3: float32 into three bfloat16 planes.
+template <typename T, int PLANES>
+__global__ void __launch_bounds__(256) k_dense_pack(const T* __restrict__ in, long long in_stride, void* __restrict__ out, long long rows,
+                                                    int cols, int padded, long long plane) {
+    const int per_row = padded / 8;
+    const long long n = rows * per_row;
+    for (long long at = (long long)blockIdx.x * 256 + threadIdx.x; at < n; at += (long long)gridDim.x * 256) {
+        const long long r = at / per_row;
+        const int c = (int)(at - r * per_row) * 8;
+        const T* src = in + r * in_stride + c;
+        T v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = c + k < cols ? src[k] : (T)0.0f;
+        if constexpr (PLANES == 1) {
+            typename vecn<T, 8>::type o;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) o[k] = v[k];
+            *(typename vecn<T, 8>::type*)((T*)out + r * padded + c) = o;
+        } else {
+            typedef typename vecn<gl_bf16, 8>::type v8;
+            v8 h, m, l;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                h[k] = (gl_bf16)v[k];
+                const float d = v[k] - (float)h[k];          // exact
+                m[k] = (gl_bf16)d;
+                l[k] = (gl_bf16)(d - (float)m[k]);
+            }
+            gl_bf16* o = (gl_bf16*)out + r * padded + c;
+            *(v8*)o = h;
+            *(v8*)(o + plane) = m;
+            *(v8*)(o + 2 * plane) = l;
+        }
+    }
+}
+
+// dz = dy act'(z), rounded for the products that read it (to T, or into three planes), zeros up to dz_stride columns, and
+// column sums of the unrounded dz over this workgroup's frames.  grid (blocks of 64 V columns, parts of the frames); thread =
+// (V columns, one of 4 frame lanes).
+template <typename T, typename TO, int V, int PLANES>
 __global__ void __launch_bounds__(256) k_dense_dz(const TO* __restrict__ dy, long long dy_stride, const TO* __restrict__ z,
-                                                  long long z_stride, T* __restrict__ dz, long long dz_stride,
-                                                  float* __restrict__ parts, long long rows, int N, int rows_per_part,
-                                                  int act) {
-    __shared__ float s[4][64];
+                                                  long long z_stride, void* __restrict__ dz_, long long dz_stride, long long plane,
+                                                  float* __restrict__ parts, long long rows, int N, int rows_per_part, int act) {
+    typedef typename vecn<TO, V>::type vI;
+    __shared__ float s[4][64 * V];
     const int c = threadIdx.x & 63, r = threadIdx.x >> 6;
-    const int n = blockIdx.x * 64 + c;
+    const int n = (blockIdx.x * 64 + c) * V;                 // V divides N: a thread's columns exist or are padding, all of them
     const long long r0 = (long long)blockIdx.y * rows_per_part;
     const long long r1 = r0 + rows_per_part < rows ? r0 + rows_per_part : rows;
-    float sum = 0.0f;
-    if (n >= N && n < dz_stride && dz)                        // zeros up to the padded width
-        for (long long i = r0 + r; i < r1; i += 4) dz[i * dz_stride + n] = (T)0.0f;
-    if (n < N)
+    const bool real = n < N;
+    float sum[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) sum[v] = 0.0f;
+    if (real || (dz_ && n < dz_stride))
+#pragma unroll 2
         for (long long i = r0 + r; i < r1; i += 4) {
-            float d = gl_to_f32(dy[i * dy_stride + n]);
-            if (act != GL_ACT_NONE) d *= gl_act_grad(gl_to_f32(z[i * z_stride + n]), act);
-            if (dz) dz[i * dz_stride + n] = (T)d;
-            sum += d;
+            float d[V];
+#pragma unroll
+            for (int v = 0; v < V; ++v) d[v] = 0.0f;
+            if (real) {
+                const vI g = *(const vI*)(dy + i * dy_stride + n);
+                vI zz = vI{};
+                if (act != GL_ACT_NONE) zz = *(const vI*)(z + i * z_stride + n);
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    d[v] = gl_to_f32(g[v]);
+                    if (act != GL_ACT_NONE) d[v] *= gl_act_grad(gl_to_f32(zz[v]), act);
+                    sum[v] += d[v];
+                }
+            }
+            if (!dz_) continue;
+            if constexpr (PLANES == 1) {
+                typename vecn<T, V>::type o;
+#pragma unroll
+                for (int v = 0; v < V; ++v) o[v] = (T)d[v];
+                *(typename vecn<T, V>::type*)((T*)dz_ + i * dz_stride + n) = o;
+            } else {
+                typename vecn<gl_bf16, V>::type h, m, l;
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    h[v] = (gl_bf16)d[v];
+                    const float e = d[v] - (float)h[v];
+                    m[v] = (gl_bf16)e;
+                    l[v] = (gl_bf16)(e - (float)m[v]);
+                }
+                gl_bf16* o = (gl_bf16*)dz_ + i * dz_stride + n;
+                *(typename vecn<gl_bf16, V>::type*)o = h;
+                *(typename vecn<gl_bf16, V>::type*)(o + plane) = m;
+                *(typename vecn<gl_bf16, V>::type*)(o + 2 * plane) = l;
+            }
         }
-    s[r][c] = sum;
+    if (!parts) return;
+#pragma unroll
+    for (int v = 0; v < V; ++v) s[r][c * V + v] = sum[v];
     __syncthreads();
-    if (parts && r == 0 && n < N) parts[(long long)blockIdx.y * N + n] = (s[0][c] + s[1][c]) + (s[2][c] + s[3][c]);
+    for (int k = threadIdx.x; k < 64 * V; k += 256) {
+        const int col = blockIdx.x * 64 * V + k;
+        if (col < N) parts[(long long)blockIdx.y * N + col] = (s[0][k] + s[1][k]) + (s[2][k] + s[3][k]);
+    }
 }
 
+// column sums over the parts; thread (column, one of 4 part lanes)
 template <typename T>
 __global__ void __launch_bounds__(256) k_dense_db(const float* __restrict__ parts, int n_parts, T* __restrict__ db, int N) {
-    const int n = blockIdx.x * 256 + threadIdx.x;
-    if (n >= N) return;
-    float s = 0.0f;
-    for (int p = 0; p < n_parts; ++p) s += parts[(long long)p * N + n];
-    db[n] = (T)s;
+    __shared__ float s[4][64];
+    const int c = threadIdx.x & 63, r = threadIdx.x >> 6, n = blockIdx.x * 64 + c;
+    float a = 0.0f;
+    if (n < N)
+#pragma unroll 4
+        for (int p = r; p < n_parts; p += 4) a += parts[(long long)p * N + n];
+    s[r][c] = a;
+    __syncthreads();
+    if (r == 0 && n < N) db[n] = (T)((s[0][c] + s[1][c]) + (s[2][c] + s[3][c]));
 }
 
 template <typename T>
@@ -135,8 +269,6 @@ __global__ void __launch_bounds__(256) k_dense_zero(T* p, long long stride, int 
     for (long long at = (long long)blockIdx.x * 256 + threadIdx.x; at < (long long)rows * cols; at += (long long)gridDim.x * 256)
         p[at / cols * stride + at % cols] = (T)0.0f;
 }
-
-constexpr int kCUs = 256;        // compute units of an MI355X: the work split must not depend on the moment
 
 // Parts of the contraction: enough workgroups to fill the chip twice, at least 8 steps each.
 int n_splits(long long I, int J, long long nq) {
@@ -146,30 +278,74 @@ int n_splits(long long I, int J, long long nq) {
     if (s > most) s = most;
     return s < 1 ? 1 : (int)s;
 }
-// workspace of a product's parts: whichever kernel takes it (that goes by alignment too, which the query does not know)
-long long partial_bytes(long long I, int J, long long nq, int dtype, bool any_q = false, bool padded = false) {
+long long any_bytes(long long I, int J, long long nq) {
     const int s = n_splits(I, J, nq);
-    const long long any = s > 1 ? gl_align16((long long)s * I * J * 4) : 0;
-    const long long mm = dtype == GL_F32 ? 0 : gl_mm_partial_bytes(I, J, padded ? gl_ceil_div(nq, 32) * 32 : nq, any_q);
-    return any > mm ? any : mm;
+    return s > 1 ? gl_align16((long long)s * I * J * 4) : 0;
 }
 
 template <typename T, typename TO>
-int product(const Operand& P, const Operand& Q, Epilogue e, long long I, int J, long long nq, float* partial,
-            hipStream_t st) {
-    if constexpr (sizeof(T) == 2) {
-        if (gl_mm16_takes(P, Q, e, I, J, nq, sizeof(TO))) return gl_mm16<T, TO>(P, Q, e, I, J, nq, partial, st);
-    }
+int any_product(const Operand& P, const Operand& Q, Epilogue e, long long I, int J, long long nq, float* partial, hipStream_t st) {
     const int splits = n_splits(I, J, nq);
     const long long per = gl_ceil_div(gl_ceil_div(nq, splits), kBQ) * kBQ;
-    const long long used = gl_ceil_div(nq, per);                 // rounding up to whole steps may leave fewer parts
+    const long long used = gl_ceil_div(nq, per);             // rounding up to whole steps may leave fewer parts
     const long long tiles = gl_ceil_div(I, kTile) * gl_ceil_div(J, kTile);
     if (tiles > 0x7fffffffLL) return gl_set_error(GL_ERR_INVALID, "gl_dense: %lld tiles are too many for one launch", tiles);
     e.partial = used > 1 ? partial : nullptr;
+    e.exact_p = nullptr;
     hipLaunchKernelGGL((k_dense_any<T, TO>), dim3((unsigned)tiles, (unsigned)used), dim3(256), 0, st, P, Q, e, I, J, nq, per,
-                       (int)gl_ceil_div(J, kTile));
+                       (int)gl_ceil_div(J, kTile), (int)tiles, (const int*)nullptr);
     GL_HIP_CHECK(hipGetLastError());
     return used > 1 ? gl_dense_join<T, TO>(e, I, J, (int)used, st) : 0;
+}
+
+// Products of fewer multiplications than this go to k_dense_any as they are where the tiles would need copies.
+constexpr double kCopyWork = 1 << 27;
+bool enough(long long rows, int inputs, int outputs) { return (double)rows * inputs * outputs >= kCopyWork; }
+int pad_to(int n) { return (n + 63) / 64 * 64; }
+bool copies(int dtype, int width, bool enough_) { return enough_ && (dtype == GL_F32 || width % 8 != 0); }
+long long copy_bytes(int dtype, long long rows, int cols) {
+    return gl_align16(rows * pad_to(cols) * (dtype == GL_F32 ? 6LL : 2LL));
+}
+long long flag_bytes(int dtype, long long I, int J) { return dtype == GL_F32 ? gl_align16(gl_ceil_div(I, 64) * gl_ceil_div(J, 64) * 4) : 0; }
+// flags and parts of a product, whichever kernel takes it
+long long partial_bytes(int dtype, long long I, int J, long long nq, bool any_q, bool fast) {
+    const long long any = any_bytes(I, J, nq);
+    const long long mm = dtype == GL_F32 && !fast ? 0 : gl_mm_partial_bytes(I, J, nq, any_q);
+    return (any > mm ? any : mm) + (fast ? flag_bytes(dtype, I, J) : 0);
+}
+
+// Copies `rows` x `cols` of o to `out` and points o at the copy.
+template <typename T>
+int pack(Operand& o, bool across, long long stride, long long rows, int cols, void* out, hipStream_t st) {
+    const int padded = pad_to(cols);
+    const long long plane = rows * padded, blocks = gl_ceil_div(rows * (padded / 8), 256);
+    hipLaunchKernelGGL((k_dense_pack<T, sizeof(T) == 4 ? 3 : 1>), dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, st,
+                       (const T*)o.base, stride, out, rows, cols, padded, plane);
+    GL_HIP_CHECK(hipGetLastError());
+    o = across ? Operand{out, 1, padded, plane, true} : Operand{out, padded, 1, plane, true};
+    return 0;
+}
+
+// The product on prepared operands (16-bit as they lie or copied, float32 in planes), else on the originals (P0, Q0).
+template <typename T, typename TO>
+int product(const Operand& P, const Operand& Q, const Operand& P0, const Operand& Q0, Epilogue e, long long I, int J, long long nq,
+            float* partial, bool fast, hipStream_t st) {
+    if constexpr (sizeof(T) == 2) {
+        if (gl_mm16_takes(P, Q, e, I, J, nq, sizeof(TO))) return gl_mm16<T, TO, T, 1>(P, Q, e, I, J, nq, partial, st);
+    } else {
+        if (fast && gl_mm16_takes(P, Q, e, I, J, nq, sizeof(TO))) {
+            e.exact_p = (const float*)P0.base;
+            e.exact_q = (const float*)Q0.base;
+            e.exact_p_is = P0.is;
+            e.exact_p_qs = P0.qs;
+            e.exact_q_is = Q0.is;
+            e.exact_q_qs = Q0.qs;
+            e.exact_nq = nq;
+            e.flags = (int*)partial;
+            return gl_mm16<gl_bf16, float, float, 6>(P, Q, e, I, J, nq, partial + flag_bytes(GL_F32, I, J) / 4, st);
+        }
+    }
+    return any_product<T, TO>(P0, Q0, e, I, J, nq, partial, st);
 }
 
 int check_types(int dtype, int out_dtype, int act, const char* who) {
@@ -199,36 +375,113 @@ int check_workspace(const void* ws, long long have, long long need, const char* 
     return 0;
 }
 
-template <typename T, typename TO>
-int forward(const void* x, long long x_stride, const void* w, long long w_stride, const Epilogue& e, long long rows,
-            int inputs, int outputs, void* ws, hipStream_t st) {
-    return product<T, TO>({x, x_stride, 1}, {w, w_stride, 1}, e, rows, outputs, inputs, (float*)ws, st);
+// ---- forward ----
+constexpr int kFewRows = 8;
+
+// workspace: [copy of x] [copy of weight] [flags and parts]
+struct FrontLayout {
+    bool fast, copy;
+    long long x_bytes, w_bytes, partial;
+    long long total() const { return x_bytes + w_bytes + partial; }
+};
+FrontLayout front_layout(long long rows, int inputs, int outputs, int dtype) {
+    FrontLayout l = {};
+    if (rows <= kFewRows) return l;
+    l.fast = enough(rows, inputs, outputs);
+    l.copy = copies(dtype, inputs, l.fast);
+    if (l.copy) {
+        l.x_bytes = copy_bytes(dtype, rows, inputs);
+        l.w_bytes = copy_bytes(dtype, outputs, inputs);
+    }
+    l.partial = partial_bytes(dtype, rows, outputs, l.copy ? pad_to(inputs) : inputs, false, l.fast);
+    return l;
 }
 
+template <typename T, typename TO, int ROWS>
+int few(const void* x, long long x_stride, const void* w, long long w_stride, const Epilogue& e, int rows, int K, int N, hipStream_t st) {
+    const int V = 16 / sizeof(T);
+    const bool vec = K % V == 0 && (uintptr_t)x % 16 == 0 && (uintptr_t)w % 16 == 0 && x_stride % V == 0 && w_stride % V == 0;
+    const int pieces = vec ? K / V : K;
+    int L = kFewRows;                    // a lane for every row's result at least
+    while (L < 64 && L < pieces) L *= 2;
+    const unsigned grid = (unsigned)gl_ceil_div(N, 4 * (64 / L));
+    if (vec) hipLaunchKernelGGL((k_dense_few<T, TO, ROWS, true>), dim3(grid), dim3(256), 0, st, (const T*)x, x_stride, (const T*)w,
+                                w_stride, e, rows, K, N, L);
+    else hipLaunchKernelGGL((k_dense_few<T, TO, ROWS, false>), dim3(grid), dim3(256), 0, st, (const T*)x, x_stride, (const T*)w,
+                            w_stride, e, rows, K, N, L);
+    GL_HIP_CHECK(hipGetLastError());
+    return 0;
+}
+
+template <typename T, typename TO>
+int forward(const void* x, long long x_stride, const void* w, long long w_stride, const Epilogue& e, long long rows,
+            int inputs, int outputs, const FrontLayout& l, void* ws, hipStream_t st) {
+    if (rows == 1) return few<T, TO, 1>(x, x_stride, w, w_stride, e, 1, inputs, outputs, st);
+    if (rows <= kFewRows) return few<T, TO, kFewRows>(x, x_stride, w, w_stride, e, (int)rows, inputs, outputs, st);
+    const Operand P0 = {x, x_stride, 1}, Q0 = {w, w_stride, 1};
+    Operand P = P0, Q = Q0;
+    char* at = (char*)ws;
+    if (l.copy) {
+        int rc = pack<T>(P, false, x_stride, rows, inputs, at, st);
+        if (!rc) rc = pack<T>(Q, false, w_stride, outputs, inputs, at + l.x_bytes, st);
+        if (rc) return rc;
+    }
+    return product<T, TO>(P, Q, P0, Q0, e, rows, outputs, inputs, (float*)(at + l.x_bytes + l.w_bytes), l.fast, st);
+}
+
+// ---- backward ----
 constexpr int kMaxParts = 128;
 int rows_per_part(long long rows) {
     const long long r = gl_ceil_div(rows, kMaxParts);
     return (int)(r < 64 ? 64 : r);
 }
 
-// workspace of the backward pass: [dz (unless dy serves)] [column-sum parts] [partials of dx and dweight, one after the
-// other on the stream: the larger of the two]
+// workspace: [dz (unless dy serves), or its planes] [with planes: dz itself, for sums that are not finite] [copy of x]
+// [copy of weight] [column-sum parts] [flags and parts of dx and dweight, one after the other on the stream: the larger]
 struct BackLayout {
-    bool own_dz;
-    long long dz_stride, dz_bytes, parts_bytes, partial_bytes_;
-    long long total() const { return dz_bytes + parts_bytes + partial_bytes_; }
+    bool fast, own_dz, copy, planes;
+    long long dz_stride, dz_bytes, dz32_bytes, x_bytes, w_bytes, parts_bytes, partial;
+    long long total() const { return dz_bytes + dz32_bytes + x_bytes + w_bytes + parts_bytes + partial; }
 };
-int elem_size(int dtype) { return dtype == GL_F32 ? 4 : 2; }
 BackLayout back_layout(long long rows, int inputs, int outputs, int dtype, int out_dtype, int act) {
-    BackLayout l;
+    BackLayout l = {};
+    l.fast = enough(rows, inputs, outputs);
+    l.planes = dtype == GL_F32 && l.fast;
     // dy itself serves where nothing is to be multiplied, converted or padded
-    l.dz_stride = gl_ceil_div(outputs, 32) * 32;
-    l.own_dz = act != GL_ACT_NONE || dtype != out_dtype || (dtype != GL_F32 && outputs % 32);
-    l.dz_bytes = l.own_dz ? gl_align16(rows * l.dz_stride * elem_size(dtype)) : 0;
+    l.own_dz = act != GL_ACT_NONE || dtype != out_dtype || (dtype != GL_F32 && outputs % 32) || l.planes;
+    l.dz_stride = pad_to(outputs);
+    if (l.own_dz) l.dz_bytes = gl_align16(rows * l.dz_stride * (l.planes ? 6 : dtype == GL_F32 ? 4 : 2));
+    if (l.planes && act != GL_ACT_NONE) l.dz32_bytes = gl_align16(rows * l.dz_stride * 4);
+    l.copy = copies(dtype, inputs, l.fast);
+    if (l.copy) {
+        l.x_bytes = copy_bytes(dtype, rows, inputs);
+        l.w_bytes = copy_bytes(dtype, outputs, inputs);
+    }
     l.parts_bytes = gl_align16(gl_ceil_div(rows, rows_per_part(rows)) * outputs * 4);
-    const long long a = partial_bytes(rows, inputs, outputs, dtype, false, l.own_dz), b = partial_bytes(outputs, inputs, rows, dtype, true);
-    l.partial_bytes_ = a > b ? a : b;
+    const long long a = partial_bytes(dtype, rows, inputs, l.own_dz ? l.dz_stride : outputs, false, l.fast);
+    const long long b = partial_bytes(dtype, outputs, inputs, rows, true, l.fast);
+    l.partial = a > b ? a : b;
     return l;
+}
+
+template <typename T, typename TO, int V, int PLANES>
+int dz_launch(const void* dy, long long dy_stride, const void* z, long long z_stride, void* dz, long long dz_stride, float* parts,
+              long long rows, int outputs, int act, hipStream_t st) {
+    const int rpp = rows_per_part(rows);
+    hipLaunchKernelGGL((k_dense_dz<T, TO, V, PLANES>), dim3((unsigned)gl_ceil_div(dz ? dz_stride : outputs, 64 * V),
+                       (unsigned)gl_ceil_div(rows, rpp)), dim3(256), 0, st, (const TO*)dy, dy_stride, (const TO*)z, z_stride, dz,
+                       dz_stride, rows * dz_stride, parts, rows, outputs, rpp, act);
+    GL_HIP_CHECK(hipGetLastError());
+    return 0;
+}
+template <typename T, typename TO, int PLANES>
+int dz_pass(const void* dy, long long dy_stride, const void* z, long long z_stride, void* dz, long long dz_stride, float* parts,
+            long long rows, int outputs, int act, hipStream_t st) {
+    constexpr int V = 16 / sizeof(TO);   // 16 bytes at a time where rows and columns allow
+    auto wide = [&](const void* p, long long stride) { return (uintptr_t)p % 16 == 0 && stride % V == 0; };
+    if (outputs % V == 0 && wide(dy, dy_stride) && (act == GL_ACT_NONE || wide(z, z_stride)))
+        return dz_launch<T, TO, V, PLANES>(dy, dy_stride, z, z_stride, dz, dz_stride, parts, rows, outputs, act, st);
+    return dz_launch<T, TO, 1, PLANES>(dy, dy_stride, z, z_stride, dz, dz_stride, parts, rows, outputs, act, st);
 }
 
 template <typename T, typename TO>
@@ -236,45 +489,68 @@ int backward(const void* dy, long long dy_stride, const void* x, long long x_str
              const void* z, long long z_stride, void* dx, long long dx_stride, void* dw, long long dw_stride, void* db,
              long long rows, int inputs, int outputs, int act, const BackLayout& l, void* ws, hipStream_t st) {
     char* at = (char*)ws;
-    T* dz = l.own_dz ? (T*)at : nullptr;
-    float* parts = (float*)(at + l.dz_bytes);
-    float* partial = (float*)(at + l.dz_bytes + l.parts_bytes);
+    const bool products = dx || dw;
+    void* dz = l.own_dz && products ? at : nullptr;
+    float* dz32 = l.dz32_bytes && products ? (float*)(at + l.dz_bytes) : nullptr;
+    char* x_copy = at + l.dz_bytes + l.dz32_bytes;
+    char* w_copy = x_copy + l.x_bytes;
+    float* parts = (float*)(w_copy + l.w_bytes);
+    float* partial = (float*)((char*)parts + l.parts_bytes);
+    int rc = 0;
     if (dz || db) {
-        const int rpp = rows_per_part(rows);
-        const int n_parts = (int)gl_ceil_div(rows, rpp);
-        hipLaunchKernelGGL((k_dense_dz<T, TO>), dim3((unsigned)gl_ceil_div(outputs, 64), (unsigned)n_parts), dim3(256), 0, st,
-                           (const TO*)dy, dy_stride, (const TO*)z, z_stride, dz, l.dz_stride, db ? parts : nullptr,
-                           rows, outputs, rpp, act);
-        GL_HIP_CHECK(hipGetLastError());
-        if (db) {
-            hipLaunchKernelGGL((k_dense_db<T>), dim3((unsigned)gl_ceil_div(outputs, 256)), dim3(256), 0, st, parts, n_parts,
-                               (T*)db, outputs);
-            GL_HIP_CHECK(hipGetLastError());
+        float* sums = db ? parts : nullptr;
+        if constexpr (sizeof(T) == 4) {
+            if (l.planes) rc = dz_pass<T, TO, 3>(dy, dy_stride, z, z_stride, dz, l.dz_stride, sums, rows, outputs, act, st);
+            else rc = dz_pass<T, TO, 1>(dy, dy_stride, z, z_stride, dz, l.dz_stride, sums, rows, outputs, act, st);
+            if (!rc && dz32) rc = dz_pass<T, TO, 1>(dy, dy_stride, z, z_stride, dz32, l.dz_stride, nullptr, rows, outputs, act, st);
+        } else {
+            rc = dz_pass<T, TO, 1>(dy, dy_stride, z, z_stride, dz, l.dz_stride, sums, rows, outputs, act, st);
         }
+        if (rc) return rc;
     }
+    if (db) {
+        hipLaunchKernelGGL((k_dense_db<T>), dim3((unsigned)gl_ceil_div(outputs, 64)), dim3(256), 0, st, parts,
+                           (int)gl_ceil_div(rows, rows_per_part(rows)), (T*)db, outputs);
+        GL_HIP_CHECK(hipGetLastError());
+    }
+    // dz as the products read it, and as it is
     const void* d = dz ? (const void*)dz : dy;
-    const long long d_stride = dz ? l.dz_stride : dy_stride;
+    const long long d_stride = dz ? l.dz_stride : dy_stride, plane = rows * l.dz_stride;
+    const bool padded = dz != nullptr;
+    const void* d0 = !l.planes ? d : dz32 ? (const void*)dz32 : dy;
+    const long long d0_stride = !l.planes ? d_stride : dz32 ? l.dz_stride : dy_stride;
     Epilogue e = {};
     if (dx) {
+        const Operand Q0 = {w, 1, w_stride};
+        Operand Q = Q0;
+        if (l.copy) rc = pack<T>(Q, true, w_stride, outputs, inputs, w_copy, st);
+        if (rc) return rc;
         e.y = dx;
         e.y_stride = dx_stride;
-        int rc = product<T, T>({d, d_stride, 1, dz != nullptr}, {w, 1, w_stride}, e, rows, inputs, outputs, partial, st);
+        rc = product<T, T>({d, d_stride, 1, plane, padded}, Q, {d0, d0_stride, 1}, Q0, e, rows, inputs, outputs, partial, l.fast, st);
         if (rc) return rc;
     }
     if (dw) {
+        const Operand Q0 = {x, 1, x_stride};
+        Operand Q = Q0;
+        if (l.copy) rc = pack<T>(Q, true, x_stride, rows, inputs, x_copy, st);
+        if (rc) return rc;
         e.y = dw;
         e.y_stride = dw_stride;
-        return product<T, T>({d, 1, d_stride, dz != nullptr}, {x, 1, x_stride}, e, outputs, inputs, rows, partial, st);
+        rc = product<T, T>({d, 1, d_stride, plane, padded}, Q, {d0, 1, d0_stride}, Q0, e, outputs, inputs, rows, partial, l.fast, st);
     }
-    return 0;
+    return rc;
 }
 
 }  // namespace
 
 template <typename T, typename TO>
 int gl_dense_join(const gl_epilogue& e, long long I, int J, int parts, hipStream_t st) {
-    const long long blocks = gl_ceil_div(I * J, 256);
-    hipLaunchKernelGGL((k_dense_join<T, TO>), dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, e, I, J, parts);
+    const int V = J % 4 == 0 ? 4 : 1;
+    const long long blocks = gl_ceil_div(I * J, 256 * V);
+    const dim3 grid((unsigned)(blocks < 4096 ? blocks : 4096));
+    if (V == 4) hipLaunchKernelGGL((k_dense_join<T, TO, 4>), grid, dim3(256), 0, st, e, I, J, parts);
+    else hipLaunchKernelGGL((k_dense_join<T, TO, 1>), grid, dim3(256), 0, st, e, I, J, parts);
     GL_HIP_CHECK(hipGetLastError());
     return 0;
 }
@@ -283,6 +559,17 @@ template int gl_dense_join<gl_bf16, gl_bf16>(const gl_epilogue&, long long, int,
 template int gl_dense_join<gl_bf16, float>(const gl_epilogue&, long long, int, int, hipStream_t);
 template int gl_dense_join<gl_f16, gl_f16>(const gl_epilogue&, long long, int, int, hipStream_t);
 template int gl_dense_join<gl_f16, float>(const gl_epilogue&, long long, int, int, hipStream_t);
+
+int gl_dense_flagged(const gl_epilogue& e, long long I, int J, long long nq, hipStream_t st) {
+    const long long tiles = gl_ceil_div(I, kTile) * gl_ceil_div(J, kTile);
+    gl_epilogue f = e;
+    f.partial = nullptr;
+    hipLaunchKernelGGL((k_dense_any<float, float>), dim3((unsigned)(tiles < 512 ? tiles : 512)), dim3(256), 0, st,
+                       Operand{e.exact_p, e.exact_p_is, e.exact_p_qs}, Operand{e.exact_q, e.exact_q_is, e.exact_q_qs}, f, I, J, nq, nq,
+                       (int)gl_ceil_div(J, kTile), (int)tiles, e.flags);
+    GL_HIP_CHECK(hipGetLastError());
+    return 0;
+}
 
 // 256 x 256 tiles where they fill the chip (parts included), else 128 x 128, else 64 x 64.  A part has at least 512
 // contraction indexes with large tiles and 256 with small ones: shorter ones cost more in the join than they fill.
@@ -312,21 +599,24 @@ gl_mm_plan gl_mm_plan_for(long long I, int J, long long nq, bool any_q) {
     return split(64, 256);
 }
 
-int gl_mm_first_columns(long long I, int J, long long nq, bool any_q) {
+int gl_mm_first_columns(long long I, int J, long long nq, bool any_q, int out_size) {
+    // columns that end inside a tile, and rows that start off 4 bytes, go to smaller tiles: the large ones have no registers
+    // for a second way to store
     const int whole = J / 256 * 256;
+    if (J % 2 && out_size == 2) return J;
     return whole > 0 && whole < J && gl_mm_plan_for(I, whole, nq, any_q).kind == 2 ? whole : J;
 }
 
 long long gl_mm_partial_bytes(long long I, int J, long long nq, bool any_q) {
-    const int first = gl_mm_first_columns(I, J, nq, any_q);
-    const gl_mm_plan a = gl_mm_plan_for(I, first, nq, any_q);
-    long long bytes = a.parts > 1 ? (long long)a.parts * I * first * 4 : 0;
-    if (first < J) {
-        const gl_mm_plan b = gl_mm_plan_for(I, J - first, nq, any_q);
-        const long long more = b.parts > 1 ? (long long)b.parts * I * (J - first) * 4 : 0;
-        if (more > bytes) bytes = more;
-    }
-    return gl_align16(bytes);
+    auto bytes = [&](int cols) {
+        const gl_mm_plan p = gl_mm_plan_for(I, cols, nq, any_q);
+        return p.parts > 1 ? (long long)p.parts * I * cols * 4 : 0;
+    };
+    const int first = gl_mm_first_columns(I, J, nq, any_q, 4);
+    long long most = bytes(J);                               // in one launch, or in two: that goes by the result's type
+    if (bytes(first) > most) most = bytes(first);
+    if (first < J && bytes(J - first) > most) most = bytes(J - first);
+    return gl_align16(most);
 }
 
 bool gl_mm16_takes(const gl_operand& P, const gl_operand& Q, const gl_epilogue& e, long long I, int J, long long nq, int out_size) {
@@ -334,11 +624,11 @@ bool gl_mm16_takes(const gl_operand& P, const gl_operand& Q, const gl_epilogue& 
         const long long stride = o.across() ? o.qs : o.is;
         return (uintptr_t)o.base % 16 == 0 && stride % 8 == 0 && stride <= (1 << 21) && (o.padded || (o.across() ? rows : nq) % 8 == 0);
     };
-    auto out = [&](const void* p, long long stride) {        // stores of four bytes and more
-        return !p || ((uintptr_t)p % 4 == 0 && stride * out_size % 4 == 0 && stride <= (1 << 20));
+    auto out = [&](const void* p, long long stride) {        // stores of four bytes and more; single elements where J is odd
+        return !p || (stride <= (1 << 20) && (J % 2 || ((uintptr_t)p % 4 == 0 && stride * out_size % 4 == 0)));
     };
     if (P.across() && !Q.across()) return false;
-    return side(P, I) && side(Q, J) && out(e.y, e.y_stride) && out(e.z, e.z_stride) && out(e.residual, e.r_stride) && nq < (1LL << 31) &&
+    return side(P, I) && side(Q, J) && out(e.y, e.y_stride) && out(e.z, e.z_stride) && out(e.residual, e.r_stride) && nq < (1LL << 31) - 64 &&
            gl_ceil_div(I, 64) * gl_ceil_div(J, 64) < (1LL << 31) - 8;
 }
 
@@ -347,7 +637,7 @@ extern "C" {
 long long gl_dense_workspace(long long rows, int inputs, int outputs, int dtype, int out_dtype) {
     if (check_types(dtype, out_dtype, 0, "gl_dense_workspace") || check_sizes(rows, inputs, outputs, "gl_dense_workspace"))
         return GL_ERR_INVALID;
-    return rows ? partial_bytes(rows, outputs, inputs, dtype) : 0;
+    return rows ? front_layout(rows, inputs, outputs, dtype).total() : 0;
 }
 
 int gl_dense(const void* x, long long x_stride, const void* weight, long long w_stride, const void* bias,
@@ -363,16 +653,24 @@ int gl_dense(const void* x, long long x_stride, const void* weight, long long w_
     if (!rc) rc = check_stride(y_stride, outputs, "y", "gl_dense");
     if (!rc && residual) rc = check_stride(r_stride, outputs, "residual", "gl_dense");
     if (!rc && preactivation) rc = check_stride(z_stride, outputs, "preactivation", "gl_dense");
-    if (!rc) rc = check_workspace(workspace, workspace_bytes, partial_bytes(rows, outputs, inputs, dtype), "gl_dense");
+    const FrontLayout l = front_layout(rows, inputs, outputs, dtype);
+    if (!rc) rc = check_workspace(workspace, workspace_bytes, l.total(), "gl_dense");
     if (rc) return rc;
-    const Epilogue e = {bias, residual, r_stride, y, y_stride, preactivation, z_stride, activation, nullptr};
+    Epilogue e = {};
+    e.bias = bias;
+    e.residual = residual;
+    e.r_stride = r_stride;
+    e.y = y;
+    e.y_stride = y_stride;
+    e.z = preactivation;
+    e.z_stride = z_stride;
+    e.act = activation;
     const hipStream_t st = (hipStream_t)stream;
-    if (dtype == GL_F32) return forward<float, float>(x, x_stride, weight, w_stride, e, rows, inputs, outputs, workspace, st);
-    if (dtype == GL_BF16)
-        return out_dtype == GL_F32 ? forward<gl_bf16, float>(x, x_stride, weight, w_stride, e, rows, inputs, outputs, workspace, st)
-                                   : forward<gl_bf16, gl_bf16>(x, x_stride, weight, w_stride, e, rows, inputs, outputs, workspace, st);
-    return out_dtype == GL_F32 ? forward<gl_f16, float>(x, x_stride, weight, w_stride, e, rows, inputs, outputs, workspace, st)
-                               : forward<gl_f16, gl_f16>(x, x_stride, weight, w_stride, e, rows, inputs, outputs, workspace, st);
+#define GL_FRONT(T, TO) forward<T, TO>(x, x_stride, weight, w_stride, e, rows, inputs, outputs, l, workspace, st)
+    if (dtype == GL_F32) return GL_FRONT(float, float);
+    if (dtype == GL_BF16) return out_dtype == GL_F32 ? GL_FRONT(gl_bf16, float) : GL_FRONT(gl_bf16, gl_bf16);
+    return out_dtype == GL_F32 ? GL_FRONT(gl_f16, float) : GL_FRONT(gl_f16, gl_f16);
+#undef GL_FRONT
 }
 
 long long gl_dense_backward_workspace(long long rows, int inputs, int outputs, int dtype, int out_dtype, int activation) {

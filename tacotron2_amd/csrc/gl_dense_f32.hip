@@ -1,0 +1,4 @@
+// The products of the dense layers on float32 operands in three bfloat16 planes.
+#include "gl_mm16_launch.h"
+
+template int gl_mm16<gl_bf16, float, float, 6>(const gl_operand&, const gl_operand&, gl_epilogue, long long, int, long long, float*, hipStream_t);

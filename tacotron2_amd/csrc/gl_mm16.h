@@ -13,6 +13,11 @@
 // way); its 32-byte pieces are XORed with the row so that the 8 rows of half a wave spread over all banks.  The swizzle is
 // applied to the global address, since direct loads place consecutive lanes' chunks consecutively.
 //
+// float32 operands come as three planes of bfloat16, x = h + m + l with h = bf16(x), m = bf16(x - h), l = bf16(x - h - m):
+// 24 bits, exact up to the last half bit.  C is the sum of six products (SEG): hh, hm, mh, mm, hl, lh; what is left out (ml, lm,
+// ll) is below 2^-24 of |x| |y|, as one rounding of a product is.  A block with a sum that is not finite is not written but
+// flagged, and the float32 kernel computes it: an infinity times a zero plane would be NaN.
+//
 // v_mfma_f32_16x16x32: A = Q rows (columns j of C), B = P rows (rows i of C): a lane's four accumulator registers are four
 // consecutive j of one i.
 #pragma once
@@ -30,6 +35,7 @@ struct Side {                    // rows (or columns) of C x contraction
     const void* base;
     long long stride;            // elements between rows of the contiguous direction
     long long rows;              // rows that may be loaded: I (J), or more where zeros pad them
+    long long plane;             // elements between the planes of a float32 operand
     int missing;                 // contraction indexes at the end that this side does not have (the other has zeros there)
 };
 
@@ -58,6 +64,11 @@ __device__ __forceinline__ void barrier() {
     asm volatile("" ::: "memory");
 }
 
+// The planes of the six products of float32 operands, two bits each: hh, hm, mh, mm, hl, lh
+constexpr int kPlanesP = 0 | 0 << 2 | 1 << 4 | 1 << 6 | 0 << 8 | 2 << 10;
+constexpr int kPlanesQ = 0 | 1 << 2 | 0 << 4 | 1 << 6 | 2 << 8 | 0 << 10;
+__device__ __forceinline__ int plane_of(int planes, int seg) { return planes >> (2 * seg) & 3; }
+
 constexpr int kFlags = 0x00027000;                           // raw 32-bit buffer: bounds-checked, no format conversion
 constexpr int kOutside = 0x7fffff00;                         // an offset beyond every buffer: loads zeros
 
@@ -70,6 +81,7 @@ struct Stage {
     static_assert(kBytes % (1024 * WAVES) == 0, "loads must divide evenly");
     static constexpr int kRowChunks = TR ? R / 8 : BK / 8;   // chunks per LDS row
     const char* base;            // first element of the tile at the current step
+    const char* start;           // and at the first one
     int stride2, n_rows;         // bytes per row of the contiguous direction; rows of C's side that exist
     int voff[kLoads];
 
@@ -88,6 +100,7 @@ struct Stage {
         n_rows = s.rows - r0 < R ? (int)(s.rows - r0) : R;
         stride2 = (int)s.stride * 2;
         base = (const char*)s.base + (TR ? q0 * s.stride + r0 : r0 * s.stride + q0) * 2;
+        start = base;
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
             int row;
@@ -147,7 +160,7 @@ struct Stage {
 };
 
 struct Out {
-    const void* bias;            // [J] of T or null
+    const void* bias;            // [J] of TB or null
     const void* residual;        // of TO or null
     long long r_stride;
     void* y;
@@ -155,8 +168,10 @@ struct Out {
     void* z;                     // of TO or null
     long long z_stride;
     int act;                     // where the kernel does not fix it
+    int* flags;                  // SEG > 1: per 64 x 64 block of C, whether it is left to the float32 kernel; or null
     long long part_stride;       // elements of y between the results of two parts of the contraction (bias, residual and z
                                  // are null then)
+    int odd;                     // rows start off 4 bytes: elements are stored one by one (TAIL kernels)
 };
 
 template <typename T> struct bits;                          // what a buffer load or store of an element moves
@@ -178,18 +193,18 @@ __device__ __forceinline__ void store_at(T v, __amdgpu_buffer_rsrc_t rs, int off
 }
 
 // A wave's bias: NI times four consecutive columns, kept packed until the sums start at it; zero past the last column.
-template <typename T, int NI>
-__device__ __forceinline__ void load_bias(const Out& o, typename vec<T, 4>::type (&bias)[NI], int j0, int J, int lane) {
+template <typename TB, int NI>
+__device__ __forceinline__ void load_bias(const Out& o, typename vec<TB, 4>::type (&bias)[NI], int j0, int J, int lane) {
     const int n_cols = o.bias && j0 < J ? min(J - j0, 16 * NI) : 0;
-    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)((const T*)o.bias + (n_cols ? j0 : 0)), 0,
-                                                                        n_cols * (int)sizeof(T), kFlags);
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)((const TB*)o.bias + (n_cols ? j0 : 0)), 0,
+                                                                        n_cols * (int)sizeof(TB), kFlags);
 #pragma unroll
     for (int n = 0; n < NI; ++n)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) bias[n][r] = load_at<T>(rs, (16 * n + 4 * (lane >> 4) + r) * (int)sizeof(T));
+        for (int r = 0; r < 4; ++r) bias[n][r] = load_at<TB>(rs, (16 * n + 4 * (lane >> 4) + r) * (int)sizeof(TB));
 }
-template <typename T, int MI, int NI>
-__device__ __forceinline__ void start_sums(f32x4 (&acc)[MI][NI], const typename vec<T, 4>::type (&bias)[NI]) {
+template <typename TB, int MI, int NI>
+__device__ __forceinline__ void start_sums(f32x4 (&acc)[MI][NI], const typename vec<TB, 4>::type (&bias)[NI]) {
 #pragma unroll
     for (int n = 0; n < NI; ++n) {
         f32x4 b;
@@ -212,7 +227,7 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t block_of(const void* p, long l
 // many outstanding).  TAIL: columns may end inside the block (a branch that costs registers).
 template <typename TO, bool TAIL, int MI, int NI>
 __device__ __forceinline__ int put_block(TO* dst, long long stride, const f32x4 (&v)[MI][NI], long long i0, int j0, long long I,
-                                         int J, int lane) {
+                                         int J, int lane, bool odd) {
     typedef typename vec<TO, 4>::type to4;
     const int il = lane & 15, g4 = lane >> 4;
     constexpr bool kPair = sizeof(TO) == 2 && NI % 2 == 0;
@@ -224,7 +239,7 @@ __device__ __forceinline__ int put_block(TO* dst, long long stride, const f32x4 
         for (int r = 0; r < 4; ++r) t[r] = (TO)f[r];
         return t;
     };
-    if (!TAIL || j0 + 16 * NI <= J) {                        // wave-uniform: whole column blocks
+    if (!TAIL || (j0 + 16 * NI <= J && !odd)) {              // wave-uniform: whole column blocks
         int off = il * stride_b + (kPair ? 16 * (g4 & 1) + 8 * (g4 >> 1) : 4 * g4) * (int)sizeof(TO);
 #pragma unroll
         for (int m = 0; m < MI; ++m) {
@@ -267,6 +282,23 @@ __device__ __forceinline__ int put_block(TO* dst, long long stride, const f32x4 
     return MI * NI;
 }
 
+// Whether all sums of a wave's block are finite; writes the flags of its 64 x 64 blocks.
+template <int MI, int NI>
+__device__ __forceinline__ bool all_finite(int* flags, const f32x4 (&acc)[MI][NI], long long i0, int j0, long long I, int J, int lane) {
+    static_assert(MI % 4 == 0 && NI == 4, "whole blocks of flags");
+    float worst = 0.0f;                                      // 0 x finite = 0, 0 x (infinity or NaN) = NaN
+#pragma unroll
+    for (int m = 0; m < MI; ++m)
+#pragma unroll
+        for (int n = 0; n < NI; ++n)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) worst = fmaf(acc[m][n][r], 0.0f, worst);
+    const bool bad = __any(worst != 0.0f);
+    const int per_row = (J + 63) / 64;
+    if (lane < MI / 4 && i0 + 64 * lane < I && j0 < J) flags[(i0 / 64 + lane) * per_row + j0 / 64] = bad;
+    return !bad;
+}
+
 // Writes a wave's block at (i0, j0): activation, residual and one rounding.  All loads come before the
 // results' stores: the memory counter runs in order, a load behind a store would wait for it.
 // EXTRA: there may be a residual or a preactivation.
@@ -274,7 +306,7 @@ template <typename T, typename TO, int ACT, bool EXTRA, bool TAIL, int MI, int N
 __device__ __forceinline__ int epilogue(const Out& o, f32x4 (&acc)[MI][NI], long long i0, int j0, long long I, int J,
                                         int part, int lane) {
     const int il = lane & 15, g4 = lane >> 4;
-    if (EXTRA && o.z) put_block<TO, TAIL, MI, NI>((TO*)o.z, o.z_stride, acc, i0, j0, I, J, lane);
+    if (EXTRA && o.z) put_block<TO, TAIL, MI, NI>((TO*)o.z, o.z_stride, acc, i0, j0, I, J, lane, o.odd);
 #pragma unroll
     for (int m = 0; m < MI; ++m)
 #pragma unroll
@@ -287,7 +319,7 @@ __device__ __forceinline__ int epilogue(const Out& o, f32x4 (&acc)[MI][NI], long
         const __amdgpu_buffer_rsrc_t rs = block_of<TO, MI, NI>(o.residual, o.r_stride, i0, j0, I, J);
         const int stride_b = (int)o.r_stride * (int)sizeof(TO);
         int off = il * stride_b + 4 * g4 * (int)sizeof(TO);
-        const bool whole = !TAIL || j0 + 16 * NI <= J;
+        const bool whole = !TAIL || (j0 + 16 * NI <= J && !o.odd);
 #pragma unroll
         for (int m = 0; m < MI; ++m) {
 #pragma unroll
@@ -310,10 +342,10 @@ __device__ __forceinline__ int epilogue(const Out& o, f32x4 (&acc)[MI][NI], long
             __builtin_amdgcn_sched_barrier(0);
         }
     }
-    return put_block<TO, TAIL, MI, NI>((TO*)o.y + part * o.part_stride, o.y_stride, acc, i0, j0, I, J, lane);
+    return put_block<TO, TAIL, MI, NI>((TO*)o.y + part * o.part_stride, o.y_stride, acc, i0, j0, I, J, lane, o.odd);
 }
 
-template <typename T, typename TO, int ACT, int BM, int BN, int WM, int WN, int BK, int ST, bool PT, bool QT, int WPE>
+template <typename T, typename TO, typename TB, int SEG, int ACT, int BM, int BN, int WM, int WN, int BK, int ST, bool PT, bool QT, int WPE>
 __global__ void __launch_bounds__(64 * (BM / WM) * (BN / WN), WPE)
 k_mm16(Side P, Side Q, Out o, long long I, int J, long long nq, long long q_per_part, int tiles_j, int n_tiles) {
     constexpr int WAVES = (BM / WM) * (BN / WN);
@@ -340,21 +372,26 @@ k_mm16(Side P, Side Q, Out o, long long I, int J, long long nq, long long q_per_
     SQ sq;
     sp.init(P, i0, q0, wave, lane);
     sq.init(Q, j0, q0, wave, lane);
-    const int steps = (int)((q1 - q0 + BK - 1) / BK);
+    const int steps = SEG * (int)((q1 - q0 + BK - 1) / BK);
     const int missing = (int)max(0LL, q1 - (nq - Q.missing));   // at the end of this part
-    int krem = (int)(q1 - q0);
+    int krem = (int)(q1 - q0), seg = 0;
     auto load = [&](int slot) {
         sp.load(lds + slot * kStage, krem, wave, lane);
         sq.load(lds + slot * kStage + SP::kBytes, krem - missing, wave, lane);
         krem -= BK;
+        if (SEG > 1 && krem <= 0 && ++seg < SEG) {
+            krem = (int)(q1 - q0);
+            sp.base = sp.start + plane_of(kPlanesP, seg) * P.plane * 2;
+            sq.base = sq.start + plane_of(kPlanesQ, seg) * Q.plane * 2;
+        }
     };
 #pragma unroll
     for (int s = 0; s < ST - 1; ++s) load(s);
 
     f32x4 acc[MI][NI];
-    typename vec<T, 4>::type bias[NI];
-    load_bias<T, NI>(o, bias, j0 + wj, J, lane);
-    start_sums<T, MI, NI>(acc, bias);
+    typename vec<TB, 4>::type bias[NI];
+    load_bias<TB, NI>(o, bias, j0 + wj, J, lane);
+    start_sums<TB, MI, NI>(acc, bias);
 
     int slot = 0;
     for (int k = 0; k < steps; ++k) {
@@ -379,6 +416,9 @@ k_mm16(Side P, Side Q, Out o, long long I, int J, long long nq, long long q_per_
     }
     wait_loads(0);                                           // nothing may be on its way into LDS when the wave ends
 
+    if constexpr (SEG > 1) {
+        if (o.flags && !all_finite<MI, NI>(o.flags, acc, i0 + wi, j0 + wj, I, J, lane)) return;
+    }
     epilogue<T, TO, ACT, true, true, MI, NI>(o, acc, i0 + wi, j0 + wj, I, J, blockIdx.y, lane);
 }
 
@@ -386,7 +426,7 @@ k_mm16(Side P, Side Q, Out o, long long I, int J, long long nq, long long q_per_
 // tile's first stages while a tile's results are written.  A step's fragments are read, and the loads of the step RING
 // ahead started, between the products of the step before.
 // A contraction that one side is contiguous in is a multiple of 32 here, J a multiple of BN.
-template <typename T, typename TO, int ACT, bool EXTRA, int BM, int BN, int WM, int WN, int RING, int WGS, bool PT, bool QT>
+template <typename T, typename TO, typename TB, int SEG, int ACT, bool EXTRA, int BM, int BN, int WM, int WN, int RING, int WGS, bool PT, bool QT>
 __global__ void __launch_bounds__(64 * (BM / WM) * (BN / WN), WGS * (BM / WM) * (BN / WN) / 4)
 k_mm16_walk(Side P, Side Q, Out o, long long I, int J, long long nq, long long q_per_part, int tiles_j, int n_tiles) {
     constexpr int BK = 32, WAVES = (BM / WM) * (BN / WN);
@@ -405,14 +445,24 @@ k_mm16_walk(Side P, Side Q, Out o, long long I, int J, long long nq, long long q
     const long long q0 = (long long)blockIdx.y * q_per_part;
     const int nk = (int)(nq - q0 < q_per_part ? nq - q0 : q_per_part);
     const int missing = (int)max(0LL, q0 + nk - (nq - Q.missing));           // of them on Q's side
-    const int pairs = max((RING + 1) / 2, (nk + 2 * BK - 1) / (2 * BK));   // steps run in twos, at least RING of them: the
+    const int steps = SEG * ((nk + BK - 1) / BK);
+    const int pairs = max((RING + 1) / 2, (steps + 1) / 2);   // steps run in twos, at least RING of them: the
                                                                            // extra ones add zeros
     int tile = first + (blockIdx.x >> 3);
     if (tile >= end) return;
     SP sp;
     SQ sq;
-    int krem = 0;                                            // what is left of the tile the loads are in
+    int krem = 0, seg = 0;                                   // what is left of the tile (its product) the loads are in
+    auto move = [&] {
+        krem -= BK;
+        if (SEG > 1 && krem <= 0 && ++seg < SEG) {
+            krem = nk;
+            sp.base = sp.start + plane_of(kPlanesP, seg) * P.plane * 2;
+            sq.base = sq.start + plane_of(kPlanesQ, seg) * Q.plane * 2;
+        }
+    };
     auto enter = [&](int t) {
+        seg = 0;
         if (t < end) {
             sp.init(P, (long long)(t / tiles_j) * BM, q0, wave, lane);
             sq.init(Q, (long long)(t % tiles_j) * BN, q0, wave, lane);
@@ -424,14 +474,14 @@ k_mm16_walk(Side P, Side Q, Out o, long long I, int J, long long nq, long long q
     for (int s = 0; s < RING; ++s) {
         sp.load(lds + s * kStage, krem, wave, lane);
         sq.load(lds + s * kStage + SP::kBytes, krem - missing, wave, lane);
-        krem -= BK;
+        move();
     }
     wait_loads(kLoads * (RING - 1));
     int slot = 0, left = 2 * pairs - RING;                   // loads left in the tile they are in
     f32x4 acc[MI][NI];
     s16x8 a[2][NI], b[MI];
-    typename vec<T, 4>::type bias[NI];
-    load_bias<T, NI>(o, bias, tile % tiles_j * BN + wj, J, lane);
+    typename vec<TB, 4>::type bias[NI];
+    load_bias<TB, NI>(o, bias, tile % tiles_j * BN + wj, J, lane);
     // Stores of the last tile's results are newer than the first RING stages of this one: while those are waited for
     // (RING - 1 steps) they may stay outstanding; `old` is how many there are at least, rounded down to 16 or 32.
     int old = 0, grace = 0;
@@ -445,7 +495,6 @@ k_mm16_walk(Side P, Side Q, Out o, long long I, int J, long long nq, long long q
         slot = slot + 1 == RING ? 0 : slot + 1;
         const char* ps = lds + slot * kStage;
         const __amdgpu_buffer_rsrc_t rp = sp.buffer(krem), rq = sq.buffer(krem - missing);
-        krem -= BK;
 #pragma unroll
         for (int m = 0; m < MI; ++m) {
 #pragma unroll
@@ -462,6 +511,7 @@ k_mm16_walk(Side P, Side Q, Out o, long long I, int J, long long nq, long long q
         }
         sp.advance();
         sq.advance();
+        move();
     };
     for (; tile < end; tile += walkers) {
         barrier();                                           // the tile's first stage has landed
@@ -469,7 +519,7 @@ k_mm16_walk(Side P, Side Q, Out o, long long I, int J, long long nq, long long q
         for (int n = 0; n < NI; ++n) a[0][n] = SQ::frag(lds + slot * kStage + SP::kBytes, wj + 16 * n, 0, lane);
 #pragma unroll
         for (int m = 0; m < MI; ++m) b[m] = SP::frag(lds + slot * kStage, wi + 16 * m, 0, lane);
-        start_sums<T, MI, NI>(acc, bias);
+        start_sums<TB, MI, NI>(acc, bias);
 #pragma unroll 1
         for (int k = pairs; k > 0; --k) {
             if (left == 0) enter(tile + walkers);
@@ -480,15 +530,21 @@ k_mm16_walk(Side P, Side Q, Out o, long long I, int J, long long nq, long long q
         }
         left = 2 * pairs - RING;
         wait_loads(kLoads * (RING - 1));
-        if (tile + walkers < end) load_bias<T, NI>(o, bias, (tile + walkers) % tiles_j * BN + wj, J, lane);
+        if (tile + walkers < end) load_bias<TB, NI>(o, bias, (tile + walkers) % tiles_j * BN + wj, J, lane);
 #pragma unroll
         for (int n = 0; n < NI; ++n) {                       // arrived before the stores below are issued
-            typedef unsigned u2 __attribute__((ext_vector_type(2)));
-            u2 t = __builtin_bit_cast(u2, bias[n]);
+            typedef unsigned uB __attribute__((ext_vector_type(sizeof(TB))));
+            uB t = __builtin_bit_cast(uB, bias[n]);
             asm volatile("" : "+v"(t) : : "memory");
-            bias[n] = __builtin_bit_cast(typename vec<T, 4>::type, t);
+            bias[n] = __builtin_bit_cast(typename vec<TB, 4>::type, t);
         }
         grace = RING - 1;
+        if constexpr (SEG > 1) {
+            if (o.flags && !all_finite<MI, NI>(o.flags, acc, (long long)(tile / tiles_j) * BM + wi, tile % tiles_j * BN + wj, I, J, lane)) {
+                old = 0;
+                continue;
+            }
+        }
         old = epilogue<T, TO, ACT, EXTRA, false, MI, NI>(o, acc, (long long)(tile / tiles_j) * BM + wi, tile % tiles_j * BN + wj, I, J, blockIdx.y, lane);
     }
     wait_loads(0);                                           // nothing may be on its way into LDS when the wave ends

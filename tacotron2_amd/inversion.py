@@ -17,18 +17,20 @@ with a row stride (``h[..., :512]``); anything that is not one row stride over c
 refuses to run under a stream capture: autograd's own bookkeeping for leaves that already live in an eager graph ends
 the process there; capture the explicit forward and backward calls instead.
 """
-import ctypes
+import contextlib
+import functools
 
 import torch
 
 from . import _lib
-from .plan import _require_gpu, _stream_ptr, raw_capture_active
+from .plan import _require_gpu, raw_capture_active
 
 ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "silu": 2, "gelu": 3, "tanh": 4, "exp": 5}
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
 # -- argument plumbing -----------------------------------------------------------------------------------------
+# Small calls are bound by this file, so its checks are few attribute reads each.
 def _activation(name):
     try:
         return ACTIVATIONS[name]
@@ -44,10 +46,11 @@ def _tensor(t, what, device=None, dtype=None, shape=None):
     if dtype is not None and t.dtype != dtype:
         raise ValueError(f"{what} must be {dtype}, got {t.dtype}")
     if device is None:
-        _require_gpu(t.device)
+        if not t.is_cuda:
+            _require_gpu(t.device)
     elif t.device != device:
         raise ValueError(f"{what} is on {t.device}, expected {device}")
-    if shape is not None and tuple(t.shape) != tuple(shape):
+    if shape is not None and t.shape != shape:
         raise ValueError(f"{what}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
     return t
 
@@ -55,6 +58,8 @@ def _tensor(t, what, device=None, dtype=None, shape=None):
 def _row_stride(t):
     """Elements between the rows of t (..., cols) when all its rows lie at one stride and are contiguous, else None."""
     cols = t.shape[-1]
+    if t.is_contiguous():
+        return cols
     if cols > 1 and t.stride(-1) != 1:
         return None
     step, span = None, 1
@@ -87,11 +92,11 @@ def _copy(t):
 
 
 def _vector(t):
-    return t if t.stride(0) == 1 or t.numel() <= 1 else _copy(t)
+    return t if t.is_contiguous() else _copy(t)
 
 
 def _p(t):
-    return None if t is None else ctypes.c_void_p(t.data_ptr())
+    return None if t is None else t.data_ptr()
 
 
 def _span(t):
@@ -131,10 +136,13 @@ def _output(out, shape, dtype, device, what):
     return out, stride
 
 
+@functools.lru_cache(maxsize=4096)
+def _bytes_of(query, *args):
+    """What a gl_*_workspace query says: a function of its arguments alone."""
+    return _lib.check(getattr(_lib.lib(), query)(*args), query)
+
+
 def _scratch(workspace, need, device):
-    need = int(need)
-    if need < 0:
-        _lib.check(need, "workspace query")
     if need == 0:
         return None, 0
     if workspace is None:
@@ -145,12 +153,24 @@ def _scratch(workspace, need, device):
     return workspace, workspace.numel()
 
 
+_no_switch = contextlib.nullcontext()
+
+
+def _on(device):
+    """Makes `device` the current one for a launch (a no-op where it is)."""
+    return _no_switch if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _stream(device):
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
 def _needs_grad(*tensors):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 def _eager_only(device, what):
-    with torch.cuda.device(device):
+    with _on(device):
         capturing = torch.cuda.is_current_stream_capturing()
     if capturing:
         raise RuntimeError(f"the differentiable {what}() cannot be captured into a graph: capture {what}() without "
@@ -161,16 +181,14 @@ def _eager_only(device, what):
 def dense_workspace(rows, inputs, outputs, dtype=torch.float32, out_dtype=None):
     """Bytes of workspace :func:`dense` needs for (rows, inputs) @ (outputs, inputs).T."""
     out_dtype = dtype if out_dtype is None else out_dtype
-    return _lib.check(_lib.lib().gl_dense_workspace(int(rows), int(inputs), int(outputs), _DTYPES[dtype],
-                                                    _DTYPES[out_dtype]), "gl_dense_workspace")
+    return _bytes_of("gl_dense_workspace", int(rows), int(inputs), int(outputs), _DTYPES[dtype], _DTYPES[out_dtype])
 
 
 def dense_backward_workspace(rows, inputs, outputs, dtype=torch.float32, out_dtype=None, activation=None):
     """Bytes of workspace :func:`dense_backward` needs."""
     out_dtype = dtype if out_dtype is None else out_dtype
-    return _lib.check(_lib.lib().gl_dense_backward_workspace(int(rows), int(inputs), int(outputs), _DTYPES[dtype],
-                                                             _DTYPES[out_dtype], _activation(activation)),
-                      "gl_dense_backward_workspace")
+    return _bytes_of("gl_dense_backward_workspace", int(rows), int(inputs), int(outputs), _DTYPES[dtype],
+                     _DTYPES[out_dtype], _activation(activation))
 
 
 def _dense_args(x, weight, bias, residual, out_dtype):
@@ -211,11 +229,11 @@ def _dense(x, weight, bias, act, residual, out_dtype, out, preactivation, worksp
     bias = None if bias is None else _vector(bias)
     lib = _lib.lib()
     d, od = _DTYPES[x.dtype], _DTYPES[out_dtype]
-    ws, ws_bytes = _scratch(workspace, lib.gl_dense_workspace(rows, x.shape[-1], shape[-1], d, od), x.device)
-    with torch.cuda.device(x.device):
+    ws, ws_bytes = _scratch(workspace, _bytes_of("gl_dense_workspace", rows, x.shape[-1], shape[-1], d, od), x.device)
+    with _on(x.device):
         _lib.check(lib.gl_dense(_p(x), x_stride, _p(weight), w_stride, _p(bias), _p(residual), r_stride, _p(y), y_stride,
                                 _p(z), z_stride, rows, x.shape[-1], shape[-1], d, od, act, _p(ws), ws_bytes,
-                                _stream_ptr(x.device)), "gl_dense")
+                                _stream(x.device)), "gl_dense")
     return y
 
 
@@ -278,10 +296,10 @@ def _dense_backward(dy, x, weight, z, act, need, outs, workspace):
     inputs = [("dy", dy), ("x", x), ("weight", weight), ("preactivation", z)]
     made = []
     if need[0]:
-        dx, dx_stride = _output(outs[0], tuple(x.shape), x.dtype, x.device, "dx")
+        dx, dx_stride = _output(outs[0], x.shape, x.dtype, x.device, "dx")
         made.append(("dx", dx))
     if need[1]:
-        dw, dw_stride = _output(outs[1], tuple(weight.shape), x.dtype, x.device, "dweight")
+        dw, dw_stride = _output(outs[1], weight.shape, x.dtype, x.device, "dweight")
         made.append(("dweight", dw))
     if need[2]:
         db, _ = _output(outs[2], (weight.shape[0],), x.dtype, x.device, "dbias")
@@ -300,11 +318,11 @@ def _dense_backward(dy, x, weight, z, act, need, outs, workspace):
         z, z_stride = _rows(z)
     lib = _lib.lib()
     d, od, K, N = _DTYPES[x.dtype], _DTYPES[dy.dtype], x.shape[-1], weight.shape[0]
-    ws, ws_bytes = _scratch(workspace, lib.gl_dense_backward_workspace(rows, K, N, d, od, act), x.device)
-    with torch.cuda.device(x.device):
+    ws, ws_bytes = _scratch(workspace, _bytes_of("gl_dense_backward_workspace", rows, K, N, d, od, act), x.device)
+    with _on(x.device):
         _lib.check(lib.gl_dense_backward(_p(dy), dy_stride, _p(x), x_stride, _p(weight), w_stride, _p(z), z_stride,
                                          _p(dx), dx_stride, _p(dw), dw_stride, _p(db), rows, K, N, d, od, act, _p(ws),
-                                         ws_bytes, _stream_ptr(x.device)), "gl_dense_backward")
+                                         ws_bytes, _stream(x.device)), "gl_dense_backward")
     return dx, dw, db
 
 
@@ -322,14 +340,13 @@ def dense_backward(dy, x, weight, preactivation=None, *, activation=None, needs=
 # -- group norm ------------------------------------------------------------------------------------------------
 def group_norm_workspace(batch, frames, channels, groups, dtype=torch.float32):
     """Bytes of workspace :func:`group_norm` needs."""
-    return _lib.check(_lib.lib().gl_group_norm_workspace(int(batch), int(frames), int(channels), int(groups),
-                                                         _DTYPES[dtype]), "gl_group_norm_workspace")
+    return _bytes_of("gl_group_norm_workspace", int(batch), int(frames), int(channels), int(groups), _DTYPES[dtype])
 
 
 def group_norm_backward_workspace(batch, frames, channels, groups, dtype=torch.float32):
     """Bytes of workspace :func:`group_norm_backward` needs."""
-    return _lib.check(_lib.lib().gl_group_norm_backward_workspace(int(batch), int(frames), int(channels), int(groups),
-                                                                  _DTYPES[dtype]), "gl_group_norm_backward_workspace")
+    return _bytes_of("gl_group_norm_backward_workspace", int(batch), int(frames), int(channels), int(groups),
+                     _DTYPES[dtype])
 
 
 def _norm_args(x, groups, weight, bias, lengths):
@@ -349,8 +366,11 @@ def _norm_args(x, groups, weight, bias, lengths):
         if raw_capture_active() and not (isinstance(lengths, torch.Tensor) and lengths.device == x.device
                                          and lengths.dtype == torch.int32 and lengths.is_contiguous()):
             raise RuntimeError("inside Plan.capture() lengths must be a contiguous int32 tensor on the device")
-        lens = torch.as_tensor(lengths, dtype=torch.int32).to(x.device).contiguous()
-        if tuple(lens.shape) != (B,):
+        lens = lengths
+        if not (isinstance(lens, torch.Tensor) and lens.dtype == torch.int32 and lens.device == x.device
+                and lens.is_contiguous()):
+            lens = torch.as_tensor(lengths, dtype=torch.int32).to(x.device).contiguous()
+        if lens.shape != (B,):
             raise ValueError(f"lengths must have shape ({B},)")
     return groups, B, T, C, lens
 
@@ -359,7 +379,7 @@ def _group_norm(x, groups, weight, bias, eps, act, lengths, out, stats, workspac
     groups, B, T, C, lens = _norm_args(x, groups, weight, bias, lengths)
     if not eps >= 0:
         raise ValueError(f"eps must be >= 0, got {eps}")
-    y, y_stride = _output(out, tuple(x.shape), x.dtype, x.device, "out")
+    y, y_stride = _output(out, x.shape, x.dtype, x.device, "out")
     inputs = [("weight", weight), ("bias", bias), ("lengths", lens)]
     if out is not None:
         _apart(y, "out", inputs + [("x", x)], same=(x,))
@@ -373,10 +393,10 @@ def _group_norm(x, groups, weight, bias, eps, act, lengths, out, stats, workspac
     bias = None if bias is None else _vector(bias)
     lib = _lib.lib()
     d = _DTYPES[x.dtype]
-    ws, ws_bytes = _scratch(workspace, lib.gl_group_norm_workspace(B, T, C, groups, d), x.device)
-    with torch.cuda.device(x.device):
+    ws, ws_bytes = _scratch(workspace, _bytes_of("gl_group_norm_workspace", B, T, C, groups, d), x.device)
+    with _on(x.device):
         _lib.check(lib.gl_group_norm(_p(x), x_stride, _p(weight), _p(bias), _p(lens), _p(y), y_stride, _p(stats), B, T, C,
-                                     groups, d, act, float(eps), _p(ws), ws_bytes, _stream_ptr(x.device)),
+                                     groups, d, act, float(eps), _p(ws), ws_bytes, _stream(x.device)),
                    "gl_group_norm")
     return y
 
@@ -420,7 +440,7 @@ def group_norm(x, groups, weight=None, bias=None, *, eps=1e-5, activation=None, 
 
 def _group_norm_backward(dy, x, groups, stats, weight, bias, act, lengths, need, outs, workspace):
     groups, B, T, C, lens = _norm_args(x, groups, weight, bias, lengths)
-    _tensor(dy, "dy", x.device, x.dtype, tuple(x.shape))
+    _tensor(dy, "dy", x.device, x.dtype, x.shape)
     _tensor(stats, "stats", x.device, torch.float32, (B, groups, 2))
     stats = stats.contiguous()
     dx = dg = db = None
@@ -428,7 +448,7 @@ def _group_norm_backward(dy, x, groups, stats, weight, bias, act, lengths, need,
     inputs = [("x", x), ("stats", stats), ("weight", weight), ("bias", bias), ("lengths", lens), ("dy", dy)]
     made = []
     if need[0]:
-        dx, dx_stride = _output(outs[0], tuple(x.shape), x.dtype, x.device, "dx")
+        dx, dx_stride = _output(outs[0], x.shape, x.dtype, x.device, "dx")
         made.append(("dx", dx))
     if need[1] and weight is not None:
         dg, _ = _output(outs[1], (C,), x.dtype, x.device, "dweight")
@@ -447,11 +467,11 @@ def _group_norm_backward(dy, x, groups, stats, weight, bias, act, lengths, need,
     bias = None if bias is None else _vector(bias)
     lib = _lib.lib()
     d = _DTYPES[x.dtype]
-    ws, ws_bytes = _scratch(workspace, lib.gl_group_norm_backward_workspace(B, T, C, groups, d), x.device)
-    with torch.cuda.device(x.device):
+    ws, ws_bytes = _scratch(workspace, _bytes_of("gl_group_norm_backward_workspace", B, T, C, groups, d), x.device)
+    with _on(x.device):
         _lib.check(lib.gl_group_norm_backward(_p(dy), dy_stride, _p(x), x_stride, _p(stats), _p(weight), _p(bias), _p(lens),
                                               _p(dx), dx_stride, _p(dg), _p(db), B, T, C, groups, d, act, _p(ws), ws_bytes,
-                                              _stream_ptr(x.device)), "gl_group_norm_backward")
+                                              _stream(x.device)), "gl_group_norm_backward")
     return dx, dg, db
 
 

@@ -693,7 +693,7 @@ def test_refusals_of_the_python_calls():
     for bad in (dict(weight=w[:, :7]), dict(weight=w.half()), dict(bias=b[:5]), dict(weight=w.cpu()), dict(x=x.double()),
                 dict(activation="swish"), dict(activation=["relu"]), dict(residual=y[:3]), dict(residual=y.half()),
                 dict(out_dtype=F16), dict(out=y[:3]), dict(out=torch.zeros(6, 4, device="cuda").t()), dict(out=y.half()),
-                dict(workspace=torch.zeros(4, device="cuda"), x=torch.zeros(1, 4096, device="cuda"),
+                dict(workspace=torch.zeros(4, device="cuda"), x=torch.zeros(16, 4096, device="cuda"),
                      weight=torch.zeros(6, 4096, device="cuda")),
                 dict(preactivation=y, out=y), dict(weight=torch.zeros(0, 8, device="cuda"), bias=None), dict(weight=w[0])):
         with pytest.raises(ValueError):
@@ -745,9 +745,9 @@ def test_refusals_of_the_c_calls():
         assert call(**bad) == -1, bad
         assert b"gl_dense" in lib.gl_last_error()
     assert call(rows=0) == 0
-    need = lib.gl_dense_workspace(1, 4096, 6, 0, 0)
+    need = lib.gl_dense_workspace(16, 4096, 6, 0, 0)
     assert need > 0 and lib.gl_dense_workspace(0, 4096, 6, 0, 0) == 0 and lib.gl_dense_workspace(1, 0, 6, 0, 0) == -1
-    big = dict(rows=1, k=4096, xs=4096, ws=4096)
+    big = dict(rows=16, k=4096, xs=4096, ws=4096)
     assert call(**big, wb=need - 1) == -1 and b"workspace" in lib.gl_last_error()
     assert call(**big, wk=None) == -1 and call(**big, wk=ctypes.c_void_p(4104)) == -1
     back = dict(dy=p, dys=6, x=p, xs=8, w=p, ws=8, z=p, zs=6, dx=p, dxs=8, dw=p, dws=8, db=p, rows=4, k=8, n=6, d=0, od=0,
