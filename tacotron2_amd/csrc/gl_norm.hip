@@ -94,13 +94,98 @@ __device__ __forceinline__ void group_sums(const Place& p, int n, float* out, F 
     __syncthreads();
 }
 
+// V values of gamma or beta from channel c on
+template <typename T, int V>
+__device__ __forceinline__ void load_vector(const T* p, int c, float none, float (&v)[V]) {
+    typedef typename vec_of<T, V>::type vT;
+    if (!p) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[k] = none;
+    } else if ((uintptr_t)p % sizeof(vT) == 0) {             // c is a multiple of V
+        const vT t = *(const vT*)(p + c);
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[k] = get<T, V>(t, k);
+    } else {
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[k] = gl_to_f32(p[c + k]);
+    }
+}
 template <typename T, int V>
 __device__ __forceinline__ void load_affine(const T* gamma, const T* beta, int c, float (&ga)[V], float (&be)[V]) {
+    load_vector<T, V>(gamma, c, 1.0f, ga);
+    load_vector<T, V>(beta, c, 0.0f, be);
+}
+// pairs [group][2] of the groups of channels c .. c + V - 1
+template <int V>
+__device__ __forceinline__ void load_pairs(const float* pairs, int c, int n, float (&first)[V], float (&second)[V]) {
+    if (n % V == 0) {                                        // one group
+        const float f = pairs[2 * (c / n)], g = pairs[2 * (c / n) + 1];
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-        ga[k] = gamma ? gl_to_f32(gamma[c + k]) : 1.0f;
-        be[k] = beta ? gl_to_f32(beta[c + k]) : 0.0f;
+        for (int k = 0; k < V; ++k) {
+            first[k] = f;
+            second[k] = g;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            first[k] = pairs[2 * ((c + k) / n)];
+            second[k] = pairs[2 * ((c + k) / n) + 1];
+        }
     }
+}
+
+// Vectors inside one group, rows and groups on whole powers of two of lanes: sums run through shuffles.
+struct Lanes {
+    bool even;
+    int gl;                              // lanes of a row that share a group
+};
+template <int V>
+__device__ __forceinline__ Lanes lanes_of(const Place& p, int n) {
+    Lanes l;
+    l.gl = n / V;
+    l.even = n % V == 0 && (p.TP & (p.TP - 1)) == 0 && (l.gl & (l.gl - 1)) == 0 && l.gl <= 64;
+    return l;
+}
+// The sum over rows and channels of this thread's group, in every thread.  red: floats, waves x lanes of a row's groups.
+// Alternate two buffers between calls: only one barrier is inside.
+__device__ __forceinline__ float group_total(float s, const Place& p, const Lanes& l, float* red) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    for (int o = 1; o < l.gl; o <<= 1) s += __shfl_xor(s, o);
+    for (int o = p.TP; o < 64; o <<= 1) s += __shfl_xor(s, o);
+    const int per = min(p.TP, 64);                           // lanes of a row in a wave; TP / per waves make a row
+    const int slot = (lane & (per - 1)) / l.gl, slots = per / l.gl;
+    if (lane < per && (lane & (l.gl - 1)) == 0) red[wave * slots + slot] = s;
+    __syncthreads();
+    const int seg = p.TP / per;
+    s = 0.0f;
+    for (int w = wave % seg; w < waves; w += seg) s += red[w * slots + slot];
+    return s;
+}
+template <int V>
+__device__ __forceinline__ float total(const float (&v)[V]) {
+    float s = v[0];
+#pragma unroll
+    for (int k = 1; k < V; ++k) s += v[k];
+    return s;
+}
+// Sums over rows per channel, where rows are whole powers of two of lanes: tot[CB] written, a barrier behind it.  red: waves x CB
+template <int V>
+__device__ __forceinline__ void channel_totals(float (&v)[V], const Place& p, float* red, float* tot) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    for (int o = p.TP; o < 64; o <<= 1)
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[k] += __shfl_xor(v[k], o);
+    const int seg = max(1, p.TP / 64), width = p.CB / seg;   // channels of a wave
+    if (lane < p.TP)
+#pragma unroll
+        for (int k = 0; k < V; ++k) red[wave * width + (lane & 63) * V + k] = v[k];
+    __syncthreads();
+    for (int c = threadIdx.x; c < p.CB; c += blockDim.x) {
+        float a = 0.0f;
+        for (int w = c / width; w < waves; w += seg) a += red[w * width + c % width];
+        tot[c] = a;
+    }
+    __syncthreads();
 }
 
 // One pass: statistics and result of CB channels of utterance b.  grid (blocks of channels x B), see block_of().
@@ -130,7 +215,7 @@ __global__ void __launch_bounds__(kMaxThreads) k_norm_slab(const T* x, long long
     if (!block_of(blocks, b, c0, CB)) return;
     const Place p = place<V>(CB);
     float* red = lds;                                        // [threads * V]
-    float* tot = red + blockDim.x * V;                       // [CB]
+    float* tot = red + blockDim.x * (V > 1 ? V : 2);                       // [CB]
     float* mean_g = tot + CB;                                // [CB / n] each
     float* rstd_g = mean_g + CB / n;
     const int live = live_frames(frames, b, Tn);
@@ -150,40 +235,60 @@ __global__ void __launch_bounds__(kMaxThreads) k_norm_slab(const T* x, long long
         if (p.on && p.r + i * p.RP < live)
 #pragma unroll
             for (int k = 0; k < V; ++k) v[k] += get<T, V>(held[i], k);
-    channel_sums<V>(v, p, red, tot);
     const float count = (float)((long long)live * n);
     const float inv = live ? 1.0f / count : 0.0f;
-    group_sums(p, n, mean_g, [&](int k) { return tot[k]; });
+    const Lanes l = lanes_of<V>(p, n);
     float mean[V], ga[V], be[V];
+    if (p.on) load_affine<T, V>(gamma, beta, c, ga, be);     // arrives under the sums
+    const auto squares = [&] {
 #pragma unroll
-    for (int k = 0; k < V; ++k) mean[k] = p.on ? mean_g[(p.col + k) / n] * inv : 0.0f;
+        for (int k = 0; k < V; ++k) v[k] = 0.0f;
 #pragma unroll
-    for (int k = 0; k < V; ++k) v[k] = 0.0f;
+        for (int i = 0; i < kHeld; ++i)
+            if (p.on && p.r + i * p.RP < live)
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i)
-        if (p.on && p.r + i * p.RP < live)
+                for (int k = 0; k < V; ++k) {
+                    const float d = get<T, V>(held[i], k) - mean[k];
+                    v[k] = fmaf(d, d, v[k]);
+                }
+    };
+    if (l.even) {
+        const float m = group_total(total<V>(v), p, l, red) * inv;
 #pragma unroll
-            for (int k = 0; k < V; ++k) {
-                const float d = get<T, V>(held[i], k) - mean[k];
-                v[k] = fmaf(d, d, v[k]);
-            }
-    channel_sums<V>(v, p, red, tot);
-    group_sums(p, n, rstd_g, [&](int k) { return tot[k]; });
-    const int groups = CB / n;
-    for (int g = threadIdx.x; g < groups; g += blockDim.x) {
-        const float rstd = live ? 1.0f / sqrtf(rstd_g[g] * inv + eps) : 0.0f;
-        rstd_g[g] = rstd;
-        if (stats) {
-            float* o = stats + 2 * ((long long)b * (blocks.C / n) + c0 / n + g);
-            o[0] = mean_g[g] * inv;
+        for (int k = 0; k < V; ++k) mean[k] = m;
+        squares();
+        const float m2 = group_total(total<V>(v), p, l, red + blockDim.x);
+        const float rstd = live ? 1.0f / sqrtf(m2 * inv + eps) : 0.0f;
+        if (stats && p.r == 0 && p.col % n == 0) {
+            float* o = stats + 2 * ((long long)b * (blocks.C / n) + c / n);
+            o[0] = m;
             o[1] = rstd;
         }
-    }
-    __syncthreads();
-    if (!p.on) return;
-    load_affine<T, V>(gamma, beta, c, ga, be);
 #pragma unroll
-    for (int k = 0; k < V; ++k) ga[k] *= rstd_g[(p.col + k) / n];
+        for (int k = 0; k < V; ++k) ga[k] *= rstd;
+    } else {
+        channel_sums<V>(v, p, red, tot);
+        group_sums(p, n, mean_g, [&](int k) { return tot[k]; });
+#pragma unroll
+        for (int k = 0; k < V; ++k) mean[k] = p.on ? mean_g[(p.col + k) / n] * inv : 0.0f;
+        squares();
+        channel_sums<V>(v, p, red, tot);
+        group_sums(p, n, rstd_g, [&](int k) { return tot[k]; });
+        for (int g = threadIdx.x; g < CB / n; g += blockDim.x) {
+            const float rstd = live ? 1.0f / sqrtf(rstd_g[g] * inv + eps) : 0.0f;
+            rstd_g[g] = rstd;
+            if (stats) {
+                float* o = stats + 2 * ((long long)b * (blocks.C / n) + c0 / n + g);
+                o[0] = mean_g[g] * inv;
+                o[1] = rstd;
+            }
+        }
+        __syncthreads();
+        if (p.on)
+#pragma unroll
+            for (int k = 0; k < V; ++k) ga[k] *= rstd_g[(p.col + k) / n];
+    }
+    if (!p.on) return;
     T* yb = y + (long long)b * Tn * y_stride + c;
 #pragma unroll
     for (int i = 0; i < kHeld; ++i) {
@@ -208,7 +313,7 @@ __global__ void __launch_bounds__(kMaxThreads) k_norm_chunk(const T* __restrict_
     extern __shared__ float lds[];
     const Place p = place<V>(C);
     float* red = lds;
-    float* tot = red + blockDim.x * V;
+    float* tot = red + blockDim.x * (V > 1 ? V : 2);
     float* mean_g = tot + C;
     float* m2_g = mean_g + C / n;
     const int b = blockIdx.y, rows = p.RP * kHeld;
@@ -229,21 +334,38 @@ __global__ void __launch_bounds__(kMaxThreads) k_norm_chunk(const T* __restrict_
         if (p.on && p.r + i * p.RP < here)
 #pragma unroll
             for (int k = 0; k < V; ++k) v[k] += get<T, V>(held[i], k);
-    channel_sums<V>(v, p, red, tot);
     const float inv = here ? 1.0f / (float)(here * n) : 0.0f;
+    const Lanes l = lanes_of<V>(p, n);
+    const auto squares = [&] {
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[k] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i)
+            if (p.on && p.r + i * p.RP < here)
+#pragma unroll
+                for (int k = 0; k < V; ++k) {
+                    const float d = get<T, V>(held[i], k) - mean[k];
+                    v[k] = fmaf(d, d, v[k]);
+                }
+    };
+    if (l.even) {
+        const float m = group_total(total<V>(v), p, l, red) * inv;
+#pragma unroll
+        for (int k = 0; k < V; ++k) mean[k] = m;
+        squares();
+        const float m2 = group_total(total<V>(v), p, l, red + blockDim.x);
+        if (p.r == 0 && p.col % n == 0) {
+            float* o = parts + 2 * (((long long)b * (C / n) + p.col / n) * gridDim.x + blockIdx.x);
+            o[0] = m;
+            o[1] = m2;
+        }
+        return;
+    }
+    channel_sums<V>(v, p, red, tot);
     group_sums(p, n, mean_g, [&](int k) { return tot[k]; });
 #pragma unroll
     for (int k = 0; k < V; ++k) mean[k] = p.on ? mean_g[(p.col + k) / n] * inv : 0.0f;
-#pragma unroll
-    for (int k = 0; k < V; ++k) v[k] = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kHeld; ++i)
-        if (p.on && p.r + i * p.RP < here)
-#pragma unroll
-            for (int k = 0; k < V; ++k) {
-                const float d = get<T, V>(held[i], k) - mean[k];
-                v[k] = fmaf(d, d, v[k]);
-            }
+    squares();
     channel_sums<V>(v, p, red, tot);
     group_sums(p, n, m2_g, [&](int k) { return tot[k]; });
     for (int g = threadIdx.x; g < C / n; g += blockDim.x) {
@@ -300,11 +422,11 @@ __global__ void __launch_bounds__(kMaxThreads) k_norm_apply(const T* x, long lon
     const int live = live_frames(frames, b, Tn);
     float ga[V], be[V], mean[V];
     load_affine<T, V>(gamma, beta, p.col, ga, be);
+    {
+        float rstd[V];
+        load_pairs<V>(stats + 2 * (long long)b * (C / n), p.col, n, mean, rstd);
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-        const float* st = stats + 2 * ((long long)b * (C / n) + (p.col + k) / n);
-        mean[k] = st[0];
-        ga[k] *= st[1];
+        for (int k = 0; k < V; ++k) ga[k] *= rstd[k];
     }
     const T* xb = x + (long long)b * Tn * x_stride + p.col;
     T* yb = y + (long long)b * Tn * y_stride + p.col;
@@ -345,7 +467,7 @@ __global__ void __launch_bounds__(kMaxThreads) k_norm_back_slab(const T* dy, lon
     if (!block_of(blocks, b, c0, CB)) return;
     const Place p = place<V>(CB);
     float* red = lds;
-    float* tot = red + blockDim.x * V;                       // [2][CB]
+    float* tot = red + blockDim.x * (V > 1 ? V : 2);                       // [2][CB]
     float* pq = tot + 2 * CB;                                // [2][CB / n]
     const int live = live_frames(frames, b, Tn), C = blocks.C;
     const int c = c0 + p.col;
@@ -365,12 +487,7 @@ __global__ void __launch_bounds__(kMaxThreads) k_norm_back_slab(const T* dy, lon
     for (int k = 0; k < V; ++k) a0[k] = a1[k] = 0.0f;
     if (p.on) {
         load_affine<T, V>(gamma, beta, c, ga, be);
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-            const float* st = stats + 2 * ((long long)b * (C / n) + (c + k) / n);
-            mean[k] = st[0];
-            rstd[k] = st[1];
-        }
+        load_pairs<V>(stats + 2 * (long long)b * (C / n), c, n, mean, rstd);
     }
 #pragma unroll
     for (int i = 0; i < kHeld; ++i)
@@ -382,26 +499,50 @@ __global__ void __launch_bounds__(kMaxThreads) k_norm_back_slab(const T* dy, lon
                 a0[k] = fmaf(du, xh, a0[k]);
                 a1[k] += du;
             }
-    channel_sums<V>(a0, p, red, tot);
-    channel_sums<V>(a1, p, red, tot + CB);
-    for (int k = threadIdx.x; k < CB; k += blockDim.x) {
-        sums[((long long)b * 2 + 0) * C + c0 + k] = tot[k];
-        sums[((long long)b * 2 + 1) * C + c0 + k] = tot[CB + k];
-        const float g = gamma ? gl_to_f32(gamma[c0 + k]) : 1.0f;
-        tot[k] *= g;
-        tot[CB + k] *= g;
-    }
-    if (!dx) return;
-    __syncthreads();
-    group_sums(p, n, pq, [&](int k) { return tot[CB + k]; });
-    group_sums(p, n, pq + CB / n, [&](int k) { return tot[k]; });
-    if (!p.on) return;
-    const float count = (float)((long long)live * n);
+    const Lanes l = lanes_of<V>(p, n);
+    const float scale = live ? 1.0f / (float)((long long)live * n) : 0.0f;
     float gp[V], gq[V];
+    if (l.even) {
+        float vp = 0.0f, vq = 0.0f;
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-        gp[k] = live ? pq[(p.col + k) / n] / count : 0.0f;
-        gq[k] = live ? pq[CB / n + (p.col + k) / n] / count : 0.0f;
+        for (int k = 0; k < V; ++k) {
+            vp = fmaf(a1[k], ga[k], vp);
+            vq = fmaf(a0[k], ga[k], vq);
+        }
+        channel_totals<V>(a0, p, red, tot);
+        channel_totals<V>(a1, p, red, tot + CB);
+        for (int k = threadIdx.x; k < CB; k += blockDim.x) {
+            sums[((long long)b * 2 + 0) * C + c0 + k] = tot[k];
+            sums[((long long)b * 2 + 1) * C + c0 + k] = tot[CB + k];
+        }
+        if (!dx) return;
+        vp = group_total(vp, p, l, red) * scale;
+        vq = group_total(vq, p, l, red + blockDim.x) * scale;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            gp[k] = vp;
+            gq[k] = vq;
+        }
+    } else {
+        channel_sums<V>(a0, p, red, tot);
+        channel_sums<V>(a1, p, red, tot + CB);
+        for (int k = threadIdx.x; k < CB; k += blockDim.x) {
+            sums[((long long)b * 2 + 0) * C + c0 + k] = tot[k];
+            sums[((long long)b * 2 + 1) * C + c0 + k] = tot[CB + k];
+            const float g = gamma ? gl_to_f32(gamma[c0 + k]) : 1.0f;
+            tot[k] *= g;
+            tot[CB + k] *= g;
+        }
+        if (!dx) return;
+        __syncthreads();
+        group_sums(p, n, pq, [&](int k) { return tot[CB + k]; });
+        group_sums(p, n, pq + CB / n, [&](int k) { return tot[k]; });
+        if (!p.on) return;
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            gp[k] = pq[(p.col + k) / n] * scale;
+            gq[k] = pq[CB / n + (p.col + k) / n] * scale;
+        }
     }
     T* ob = dx + (long long)b * Tn * dx_stride + c;
 #pragma unroll
@@ -431,7 +572,7 @@ __global__ void __launch_bounds__(kMaxThreads) k_norm_back_chunk(const T* __rest
     extern __shared__ float lds[];
     const Place p = place<V>(C);
     float* red = lds;
-    float* tot = red + blockDim.x * V;
+    float* tot = red + blockDim.x * (V > 1 ? V : 2);
     const int b = blockIdx.y;
     const int live = live_frames(frames, b, Tn);
     const int t0 = blockIdx.x * rows, t1 = min(t0 + rows, live);
@@ -440,12 +581,7 @@ __global__ void __launch_bounds__(kMaxThreads) k_norm_back_chunk(const T* __rest
     for (int k = 0; k < V; ++k) a0[k] = a1[k] = 0.0f;
     if (p.on) {
         load_affine<T, V>(gamma, beta, p.col, ga, be);
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-            const float* st = stats + 2 * ((long long)b * (C / n) + (p.col + k) / n);
-            mean[k] = st[0];
-            rstd[k] = st[1];
-        }
+        load_pairs<V>(stats + 2 * (long long)b * (C / n), p.col, n, mean, rstd);
         const T* xb = x + (long long)b * Tn * x_stride + p.col;
         const T* db = dy + (long long)b * Tn * dy_stride + p.col;
 #pragma unroll 4
@@ -462,71 +598,83 @@ __global__ void __launch_bounds__(kMaxThreads) k_norm_back_chunk(const T* __rest
         }
     }
     float* o = parts + ((long long)b * gridDim.x + blockIdx.x) * 2 * C;
-    channel_sums<V>(a0, p, red, tot);
+    const bool even = (p.TP & (p.TP - 1)) == 0;
+    if (even) channel_totals<V>(a0, p, red, tot);
+    else channel_sums<V>(a0, p, red, tot);
     for (int c = threadIdx.x; c < C; c += blockDim.x) o[c] = tot[c];
-    channel_sums<V>(a1, p, red, tot);
+    __syncthreads();
+    if (even) channel_totals<V>(a1, p, red, tot);
+    else channel_sums<V>(a1, p, red, tot);
     for (int c = threadIdx.x; c < C; c += blockDim.x) o[C + c] = tot[c];
 }
 
-// grid (groups, B): sums [B][2][C] over the chunks, and the group's p, q
+// grid (blocks of 64 of the 2 C columns, B): sums [B][2][C] over the chunks; thread (column, one of 16 chunk lanes).  With one
+// utterance they are dgamma and dbeta already.
 template <typename T>
-__global__ void __launch_bounds__(256) k_norm_back_join(const float* __restrict__ parts, const T* __restrict__ gamma,
-                                                        const int* __restrict__ frames, float* __restrict__ sums,
-                                                        float* __restrict__ pq, int Tn, int C, int n, int chunks) {
-    __shared__ float s[4], red[256];
-    const int g = blockIdx.x, b = blockIdx.y;
-    const int live = live_frames(frames, b, Tn);
-    const int w = n < 256 ? n : 256, lanes = 256 / w;        // channels at a time, chunk lanes per channel
-    const int c = threadIdx.x % w, l = threadIdx.x / w;
-    float p = 0.0f, q = 0.0f;
-    for (int c1 = 0; c1 < n; c1 += w)
-        for (int which = 0; which < 2; ++which) {
-            float a = 0.0f;
-            if (c1 + c < n && l < lanes)
-#pragma unroll 4
-                for (int k = l; k < chunks; k += lanes) a += parts[(((long long)b * chunks + k) * 2 + which) * C + g * n + c1 + c];
-            __syncthreads();
-            red[threadIdx.x] = a;
-            __syncthreads();
-            if (l == 0 && c1 + c < n) {
-                for (int k = 1; k < lanes; ++k) a += red[k * w + c];
-                sums[((long long)b * 2 + which) * C + g * n + c1 + c] = a;
-                const float v = a * (gamma ? gl_to_f32(gamma[g * n + c1 + c]) : 1.0f);
-                if (which) p += v;
-                else q += v;
-            }
-        }
-    p = block_sum(p, s);
-    q = block_sum(q, s);
-    if (threadIdx.x == 0) {
-        const float count = (float)live * (float)n;
-        float* o = pq + 2 * ((long long)b * gridDim.x + g);
-        o[0] = live ? p / count : 0.0f;
-        o[1] = live ? q / count : 0.0f;
+__global__ void __launch_bounds__(1024) k_norm_back_join(const float* __restrict__ parts, float* __restrict__ sums,
+                                                         T* __restrict__ dgamma, T* __restrict__ dbeta, int C, int chunks) {
+    __shared__ float s[16][64];
+    const int k = threadIdx.x & 63, l = threadIdx.x >> 6, c = blockIdx.x * 64 + k, b = blockIdx.y;
+    float a = 0.0f;
+    if (c < 2 * C) {
+        const float* in = parts + (long long)b * chunks * 2 * C + c;
+#pragma unroll 8
+        for (int j = l; j < chunks; j += 16) a += in[(long long)j * 2 * C];
     }
+    s[l][k] = a;
+    __syncthreads();
+    if (l || c >= 2 * C) return;
+#pragma unroll
+    for (int j = 1; j < 16; ++j) a += s[j][k];
+    sums[(long long)b * 2 * C + c] = a;
+    if (gridDim.y > 1) return;
+    if (c < C && dgamma) dgamma[c] = (T)a;
+    if (c >= C && dbeta) dbeta[c - C] = (T)a;
 }
 
 template <typename T, int V, int ACT>
 __global__ void __launch_bounds__(kMaxThreads) k_norm_back_apply(const T* dy, long long dy_stride, const T* __restrict__ x,
                                                          long long x_stride, const float* __restrict__ stats,
-                                                         const float* __restrict__ pq, const T* __restrict__ gamma,
+                                                         const float* __restrict__ sums, const T* __restrict__ gamma,
                                                          const T* __restrict__ beta, const int* __restrict__ frames, T* dx,
                                                          long long dx_stride, int Tn, int C, int n, int act) {
     typedef typename vec_of<T, V>::type vT;
+    extern __shared__ float lds[];                           // [2][C] weighted sums, [groups][2] p, q
     const Place p = place<V>(C);
-    if (!p.on) return;
     const int b = blockIdx.y;
     const int live = live_frames(frames, b, Tn);
     float ga[V], be[V], mean[V], rstd[V], gp[V], gq[V];
-    load_affine<T, V>(gamma, beta, p.col, ga, be);
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-        const long long at = 2 * ((long long)b * (C / n) + (p.col + k) / n);
-        mean[k] = stats[at];
-        rstd[k] = stats[at + 1];
-        gp[k] = pq[at];
-        gq[k] = pq[at + 1];
+    if (p.on) {
+        load_affine<T, V>(gamma, beta, p.col, ga, be);
+        load_pairs<V>(stats + 2 * (long long)b * (C / n), p.col, n, mean, rstd);
     }
+    float* pairs = lds + 2 * C;
+    for (int c = threadIdx.x; c < C; c += blockDim.x) {
+        const float g = gamma ? gl_to_f32(gamma[c]) : 1.0f;
+        lds[c] = sums[((long long)b * 2 + 0) * C + c] * g;
+        lds[C + c] = sums[((long long)b * 2 + 1) * C + c] * g;
+    }
+    __syncthreads();
+    const float scale = live ? 1.0f / (float)((long long)live * n) : 0.0f;
+    for (int g = threadIdx.x >> 6; g < C / n; g += blockDim.x >> 6) {
+        float sp = 0.0f, sq = 0.0f;
+        for (int c = threadIdx.x & 63; c < n; c += 64) {
+            sp += lds[C + g * n + c];
+            sq += lds[g * n + c];
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+            sp += __shfl_xor(sp, o);
+            sq += __shfl_xor(sq, o);
+        }
+        if ((threadIdx.x & 63) == 0) {
+            pairs[2 * g] = sp * scale;
+            pairs[2 * g + 1] = sq * scale;
+        }
+    }
+    __syncthreads();
+    if (!p.on) return;
+    load_pairs<V>(pairs, p.col, n, gp, gq);
     const T* xb = x + (long long)b * Tn * x_stride + p.col;
     const T* db = dy + (long long)b * Tn * dy_stride + p.col;
     T* ob = dx + (long long)b * Tn * dx_stride + p.col;
@@ -705,6 +853,7 @@ int check_stride(long long stride, int cols, const char* what, const char* who) 
     return 0;
 }
 int check_workspace(const void* ws, long long have, long long need, const char* who) {
+    if (need == 0) return 0;
     if (!ws || have < need)
         return gl_set_error(GL_ERR_INVALID, "%s: workspace of %lld bytes needed, %lld given", who, need, ws ? have : 0LL);
     if ((uintptr_t)ws % 16) return gl_set_error(GL_ERR_INVALID, "%s: workspace must be 16-byte aligned", who);
@@ -717,7 +866,7 @@ long long stats_bytes(int B, int groups) { return align16(8LL * B * groups); }
 bool vector_ok(const void* p, long long stride, int size) { return (uintptr_t)p % 16 == 0 && stride * size % 16 == 0; }
 
 size_t lds_bytes(int threads, int V, int CB, int n, int totals) {
-    return sizeof(float) * ((size_t)threads * V + (size_t)totals * CB + 2 * (size_t)(CB / n));
+    return sizeof(float) * ((size_t)threads * (V > 1 ? V : 2) + (size_t)totals * CB + 2 * (size_t)(CB / n));
 }
 constexpr size_t kMaxLds = 65536;
 
@@ -765,7 +914,7 @@ int back_rows(int B, int T) {
     return (int)(r < 32 ? 32 : r);
 }
 unsigned apply_blocks(int B, int T, int rows_at_a_time) {
-    const long long per = ceil_div(T, 4LL * rows_at_a_time), most = 4096 / B;
+    const long long per = ceil_div(T, 8LL * rows_at_a_time), most = 4096 / B;
     return (unsigned)(per < 1 ? 1 : per < most ? per : most < 1 ? 1 : most);
 }
 unsigned plain_blocks(int B, int T, int C) {
@@ -801,7 +950,11 @@ long long parts_bytes(int B, int T, int C, int groups, int dtype) {
     return align16(most);
 }
 long long norm_bytes(int B, int T, int C, int groups, int dtype) {
-    return stats_bytes(B, groups) + (B && T ? parts_bytes(B, T, C, groups, dtype) : 0);
+    const int size = dtype == GL_F32 ? 4 : 2;
+    bool slabs = B && T;
+    for (int V : {16 / size, 1})
+        if (slabs && C % V == 0) slabs = cut_for(B, T, C, groups, size, V).kind == 0;
+    return slabs ? 0 : stats_bytes(B, groups) + (B && T ? parts_bytes(B, T, C, groups, dtype) : 0);
 }
 long long back_parts_bytes(int B, int T, int C) {
     return B && T ? align16(8LL * B * ceil_div(T, back_rows(B, T)) * C) : 0;
@@ -858,7 +1011,7 @@ int norm_fwd(const Norm& a, void* y, long long y_stride, float* stats, float* gi
 
 template <typename T, int V>
 int norm_back(const Norm& a, const void* dy_, long long dy_stride, const float* stats, void* dx_, long long dx_stride, float* pq,
-              float* sums, float* parts) {
+              float* sums, float* parts, void* dgamma, void* dbeta, bool* done) {
     const int n = a.C / a.groups;
     const T *x = (const T*)a.x, *ga = (const T*)a.gamma, *be = (const T*)a.beta, *dy = (const T*)dy_;
     T* dx = (T*)dx_;
@@ -873,19 +1026,20 @@ int norm_back(const Norm& a, const void* dy_, long long dy_stride, const float* 
         });
     if (c.kind == 1) {
         const int rows = back_rows(a.B, a.T), chunks = (int)ceil_div(a.T, rows);
+        *done = a.B == 1;                                    // the join writes dgamma and dbeta
         return with_act<V>(a.act, [&](auto act) -> int {
             constexpr int ACT = decltype(act)::value;
             hipLaunchKernelGGL((k_norm_back_chunk<T, V, ACT>), dim3(chunks, a.B), dim3(c.threads),
                                lds_bytes(c.threads, V, a.C, n, 1), a.st, dy, dy_stride, x, a.x_stride, stats, ga, be, a.frames, parts,
                                a.T, a.C, n, rows, a.act);
             GL_HIP_CHECK(hipGetLastError());
-            hipLaunchKernelGGL((k_norm_back_join<T>), dim3(a.groups, a.B), dim3(256), 0, a.st, parts, ga, a.frames, sums, pq, a.T,
-                               a.C, n, chunks);
+            hipLaunchKernelGGL((k_norm_back_join<T>), dim3((unsigned)ceil_div(2 * a.C, 64), a.B), dim3(1024), 0, a.st, parts, sums,
+                               (T*)dgamma, (T*)dbeta, a.C, chunks);
             GL_HIP_CHECK(hipGetLastError());
             if (!dx) return 0;
             hipLaunchKernelGGL((k_norm_back_apply<T, V, ACT>), dim3(apply_blocks(a.B, a.T, c.threads / (a.C / V)), a.B),
-                               dim3(c.threads), 0, a.st, dy, dy_stride, x, a.x_stride, stats, pq, ga, be, a.frames, dx, dx_stride,
-                               a.T, a.C, n, a.act);
+                               dim3(c.threads), sizeof(float) * (2 * a.C + 2 * (a.C / n)), a.st, dy, dy_stride, x, a.x_stride, stats,
+                               sums, ga, be, a.frames, dx, dx_stride, a.T, a.C, n, a.act);
             GL_HIP_CHECK(hipGetLastError());
             return 0;
         });
@@ -947,6 +1101,7 @@ int gl_group_norm_backward(const void* dy, long long dy_stride, const void* x, l
     const hipStream_t st = (hipStream_t)stream;
     float* pq = (float*)workspace;
     float* sums = (float*)((char*)workspace + stats_bytes(B, groups));
+    bool done = false;
     if (B > 0 && T > 0) {
         if (!dy || !x || !stats) return gl_set_error(GL_ERR_INVALID, "gl_group_norm_backward: NULL buffer");
         rc = check_stride(dy_stride, channels, "dy", "gl_group_norm_backward");
@@ -960,14 +1115,14 @@ int gl_group_norm_backward(const void* dy, long long dy_stride, const void* x, l
         const int size = dtype == GL_F32 ? 4 : 2, full = 16 / size;
         const bool wide = channels % full == 0 && vector_ok(x, x_stride, size) && vector_ok(dy, dy_stride, size) &&
                           (!dx || vector_ok(dx, dx_stride, size));
-#define GL_NORM(T_, V) norm_back<T_, V>(a, dy, dy_stride, stats, dx, dx_stride, pq, sums, parts)
+#define GL_NORM(T_, V) norm_back<T_, V>(a, dy, dy_stride, stats, dx, dx_stride, pq, sums, parts, dgamma, dbeta, &done)
         if (dtype == GL_F32) rc = wide ? GL_NORM(float, 4) : GL_NORM(float, 1);
         else if (dtype == GL_BF16) rc = wide ? GL_NORM(gl_bf16, 8) : GL_NORM(gl_bf16, 1);
         else rc = wide ? GL_NORM(gl_f16, 8) : GL_NORM(gl_f16, 1);
 #undef GL_NORM
         if (rc) return rc;
     }
-    if (dgamma || dbeta) {
+    if ((dgamma || dbeta) && !done) {
         const dim3 grid((unsigned)ceil_div(channels, 64));
         const int rows = T > 0 ? B : 0;
         if (dtype == GL_F32) hipLaunchKernelGGL((k_norm_back_affine<float>), grid, dim3(256), 0, st, sums, (float*)dgamma, (float*)dbeta, rows, channels);

@@ -757,7 +757,7 @@ def test_refusals_of_the_c_calls():
                 dict(dxs=7), dict(dws=7), dict(rows=-2), dict(od=2), dict(act=9), dict(wb=0), dict(wk=None)):
         assert call(**bad) == -1, bad
     assert call(dx=None, dw=None, db=None) == 0
-    norm = dict(x=p, xs=12, ga=p, be=p, f=p, y=p, ys=12, s=p, B=2, T=5, C=12, G=3, d=0, act=0, eps=1e-5, wk=p, wb=1 << 30,
+    norm = dict(x=p, xs=12, ga=p, be=p, f=p, y=p, ys=12, s=p, B=2, T=50000, C=12, G=3, d=0, act=0, eps=1e-5, wk=p, wb=1 << 30,
                 st=None)
     call = lambda **k: lib.gl_group_norm(*{**norm, **k}.values())                      # noqa: E731
     for bad in (dict(x=None), dict(y=None), dict(xs=11), dict(ys=11), dict(B=-1), dict(B=65536), dict(T=-1), dict(C=0),
@@ -771,7 +771,7 @@ def test_refusals_of_the_c_calls():
     for bad in (dict(dy=None), dict(x=None), dict(s=None), dict(dys=3), dict(xs=11), dict(dxs=11), dict(G=5), dict(wb=8),
                 dict(wk=None), dict(act=-1), dict(d=9)):
         assert call(**bad) == -1, bad
-    assert lib.gl_group_norm_workspace(2, 5, 12, 5, 0) == -1 and lib.gl_group_norm_workspace(2, 5, 12, 3, 0) > 0
+    assert lib.gl_group_norm_workspace(2, 5, 12, 5, 0) == -1 and lib.gl_group_norm_workspace(2, 50000, 12, 3, 0) > 0
 
 
 def test_row_strides_of_views():
