@@ -17,6 +17,10 @@ namespace {
 
 constexpr int kHeld = 8;                 // vectors of V channels a thread holds
 constexpr int kMaxThreads = 1024;
+constexpr int kRowBytes = 64;            // of a slab's rows where whole groups and the chip allow: 64 ragged utterances of 861 x 512
+                                         // bf16 with 32: 28.9 us, 64: 28.3, 128: 32
+// threads of a gradient slab: it holds x and du in registers (16-bit: 96 of them, 1024 threads would spill)
+template <typename T> constexpr int kBackThreads = sizeof(T) == 2 ? 512 : 1024;
 
 __device__ __forceinline__ int live_frames(const int* frames, int b, int T) {
     return frames ? max(0, min(frames[b], T)) : T;
@@ -204,7 +208,8 @@ __device__ __forceinline__ bool block_of(const Blocks& k, int& b, int& c0, int& 
     return true;
 }
 
-template <typename T, int V, int ACT>
+// EVEN: see Lanes; one group a vector then, so its mean and deviation are single registers.
+template <typename T, int V, int ACT, bool EVEN>
 __global__ void __launch_bounds__(kMaxThreads) k_norm_slab(const T* x, long long x_stride, const T* __restrict__ gamma,
                                                            const T* __restrict__ beta, const int* __restrict__ frames,
                                                            T* y, long long y_stride, float* __restrict__ stats, int Tn, int n,
@@ -252,7 +257,7 @@ __global__ void __launch_bounds__(kMaxThreads) k_norm_slab(const T* x, long long
                     v[k] = fmaf(d, d, v[k]);
                 }
     };
-    if (l.even) {
+    if constexpr (EVEN) {
         const float m = group_total(total<V>(v), p, l, red) * inv;
 #pragma unroll
         for (int k = 0; k < V; ++k) mean[k] = m;
@@ -455,8 +460,8 @@ __device__ __forceinline__ void du_xh(const typename vec_of<T, V>::type& x, cons
 }
 
 // One pass, as k_norm_slab.  sums [B][2][C]: sum du xh, sum du per channel of the utterance
-template <typename T, int V, int ACT>
-__global__ void __launch_bounds__(kMaxThreads) k_norm_back_slab(const T* dy, long long dy_stride, const T* __restrict__ x,
+template <typename T, int V, int ACT, bool EVEN>
+__global__ void __launch_bounds__(kBackThreads<T>) k_norm_back_slab(const T* dy, long long dy_stride, const T* __restrict__ x,
                                                                 long long x_stride, const float* __restrict__ stats,
                                                                 const T* __restrict__ gamma, const T* __restrict__ beta,
                                                                 const int* __restrict__ frames, T* dx, long long dx_stride,
@@ -482,27 +487,39 @@ __global__ void __launch_bounds__(kMaxThreads) k_norm_back_slab(const T* dy, lon
             hd[i] = *(const vT*)(db + (long long)t * dy_stride);
         }
     }
+    float du[kHeld][V];                                      // in place of dy from here on: the activation's slope is
+                                                             // worked out once
     float ga[V], be[V], mean[V], rstd[V], a0[V], a1[V];
 #pragma unroll
     for (int k = 0; k < V; ++k) a0[k] = a1[k] = 0.0f;
     if (p.on) {
         load_affine<T, V>(gamma, beta, c, ga, be);
-        load_pairs<V>(stats + 2 * (long long)b * (C / n), c, n, mean, rstd);
+        if constexpr (EVEN) {
+            const float* st = stats + 2 * ((long long)b * (C / n) + c / n);
+            const float m = st[0], r = st[1];
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                mean[k] = m;
+                rstd[k] = r;
+            }
+        } else {
+            load_pairs<V>(stats + 2 * (long long)b * (C / n), c, n, mean, rstd);
+        }
     }
 #pragma unroll
     for (int i = 0; i < kHeld; ++i)
         if (p.on && p.r + i * p.RP < live)
 #pragma unroll
             for (int k = 0; k < V; ++k) {
-                float du, xh;
-                du_xh<T, V, ACT>(hx[i], hd[i], k, mean[k], rstd[k], ga[k], be[k], act, du, xh);
-                a0[k] = fmaf(du, xh, a0[k]);
-                a1[k] += du;
+                float xh;
+                du_xh<T, V, ACT>(hx[i], hd[i], k, mean[k], rstd[k], ga[k], be[k], act, du[i][k], xh);
+                a0[k] = fmaf(du[i][k], xh, a0[k]);
+                a1[k] += du[i][k];
             }
     const Lanes l = lanes_of<V>(p, n);
     const float scale = live ? 1.0f / (float)((long long)live * n) : 0.0f;
     float gp[V], gq[V];
-    if (l.even) {
+    if constexpr (EVEN) {
         float vp = 0.0f, vq = 0.0f;
 #pragma unroll
         for (int k = 0; k < V; ++k) {
@@ -553,9 +570,8 @@ __global__ void __launch_bounds__(kMaxThreads) k_norm_back_slab(const T* dy, lon
         if (t < live)
 #pragma unroll
             for (int k = 0; k < V; ++k) {
-                float du, xh;
-                du_xh<T, V, ACT>(hx[i], hd[i], k, mean[k], rstd[k], ga[k], be[k], act, du, xh);
-                set<T, V>(o, k, rstd[k] * (du * ga[k] - gp[k] - xh * gq[k]));
+                const float xh = (get<T, V>(hx[i], k) - mean[k]) * rstd[k];
+                set<T, V>(o, k, rstd[k] * (du[i][k] * ga[k] - gp[k] - xh * gq[k]));
             }
         *(vT*)(ob + (long long)t * dx_stride) = o;
     }
@@ -877,22 +893,22 @@ struct Cut {
     int rows, chunks;                    // chunks: frames of one, and how many
 };
 constexpr int kWorkgroups = 1024;        // four a CU: chunks of the gradients' sums
-int threads_for(int tp, long long rows) {                    // the fewest threads whose rows hold `rows` frames, or 0
-    for (int t = 256; t <= kMaxThreads; t *= 2)
+int threads_for(int tp, long long rows, int most) {          // the fewest threads whose rows hold `rows` frames, or 0
+    for (int t = 256; t <= most; t *= 2)
         if (t >= tp && (long long)(t / tp) * kHeld >= rows) return t;
     return 0;
 }
-Cut cut_for(int B, int T, int C, int groups, int size, int V) {
+Cut cut_for(int B, int T, int C, int groups, int size, int V, int most) {
     Cut c = {};
     const int n = C / groups;
     int k = 1;
     while (k < groups && (n * k) % V) ++k;                   // whole groups on whole vectors
-    if (n * k % V == 0 && threads_for(n * k / V, T) && lds_bytes(kMaxThreads, V, n * k, n, 2) <= kMaxLds) {
+    if (n * k % V == 0 && threads_for(n * k / V, T, most) && lds_bytes(kMaxThreads, V, n * k, n, 2) <= kMaxLds) {
         // more groups to a block, to 128 bytes a row, while the slab fits and the blocks fill the chip
-        for (int m = 2 * k; m <= groups && (long long)n * k * size < 128; m += k)
-            if (groups % m == 0 && threads_for(n * m / V, T) && (long long)B * (groups / m) >= 256) k = m;
+        for (int m = 2 * k; m <= groups && (long long)n * k * size < kRowBytes; m += k)
+            if (groups % m == 0 && threads_for(n * m / V, T, most) && (long long)B * (groups / m) >= 256) k = m;
         c.kind = 0;
-        c.threads = threads_for(n * k / V, T);
+        c.threads = threads_for(n * k / V, T, most);
         c.blocks = {(int)ceil_div(groups, k), 0, n * k, C};
         c.blocks.total = B * c.blocks.per_b;
         return c;
@@ -922,6 +938,13 @@ unsigned plain_blocks(int B, int T, int C) {
     if (most < 1) most = 1;
     return (unsigned)(per < 1 ? 1 : per < most ? per : most);
 }
+// Lanes::even of every block of a cut (the last block of an utterance may have fewer groups: powers of two divide them too)
+bool even_blocks(const Cut& c, int C, int n, int V) {
+    auto pow2 = [](int v) { return v > 0 && (v & (v - 1)) == 0; };
+    const int last = C - (c.blocks.per_b - 1) * c.blocks.CB;
+    return n % V == 0 && pow2(n / V) && n / V <= 64 && pow2(c.blocks.CB / V) && pow2(last / V);
+}
+
 template <int ACT> struct act_tag { static constexpr int value = ACT; };
 // f(act_tag<the activation>) where the vector kernels fix it, f(act_tag<-1>) elsewhere
 template <int V, typename F>
@@ -944,7 +967,7 @@ long long parts_bytes(int B, int T, int C, int groups, int dtype) {
     long long most = 0;
     for (int V : {16 / size, 1}) {                           // alignment is not known to the query
         if (C % V) continue;
-        const Cut c = cut_for(B, T, C, groups, size, V);
+        const Cut c = cut_for(B, T, C, groups, size, V, kMaxThreads);
         if (c.kind == 1 && 8LL * B * groups * c.chunks > most) most = 8LL * B * groups * c.chunks;
     }
     return align16(most);
@@ -953,7 +976,7 @@ long long norm_bytes(int B, int T, int C, int groups, int dtype) {
     const int size = dtype == GL_F32 ? 4 : 2;
     bool slabs = B && T;
     for (int V : {16 / size, 1})
-        if (slabs && C % V == 0) slabs = cut_for(B, T, C, groups, size, V).kind == 0;
+        if (slabs && C % V == 0) slabs = cut_for(B, T, C, groups, size, V, kMaxThreads).kind == 0;
     return slabs ? 0 : stats_bytes(B, groups) + (B && T ? parts_bytes(B, T, C, groups, dtype) : 0);
 }
 long long back_parts_bytes(int B, int T, int C) {
@@ -977,11 +1000,12 @@ template <typename T, int V>
 int norm_fwd(const Norm& a, void* y, long long y_stride, float* stats, float* given, float* parts, float eps) {
     const int n = a.C / a.groups;
     const T *x = (const T*)a.x, *ga = (const T*)a.gamma, *be = (const T*)a.beta;
-    Cut c = a.T ? cut_for(a.B, a.T, a.C, a.groups, sizeof(T), V) : Cut{2};
+    Cut c = a.T ? cut_for(a.B, a.T, a.C, a.groups, sizeof(T), V, kMaxThreads) : Cut{2};
     if (c.kind == 0)
         return with_act<V>(a.act, [&](auto act) -> int {
-            hipLaunchKernelGGL((k_norm_slab<T, V, decltype(act)::value>), dim3((unsigned)((c.blocks.total + 7) / 8 * 8)),
-                               dim3(c.threads), lds_bytes(c.threads, V, c.blocks.CB, n, 1), a.st, x, a.x_stride, ga, be, a.frames,
+            const bool even = even_blocks(c, a.C, n, V);
+            auto kernel = even ? k_norm_slab<T, V, decltype(act)::value, true> : k_norm_slab<T, V, decltype(act)::value, false>;
+            hipLaunchKernelGGL(kernel, dim3((unsigned)((c.blocks.total + 7) / 8 * 8)), dim3(c.threads), lds_bytes(c.threads, V, c.blocks.CB, n, 1), a.st, x, a.x_stride, ga, be, a.frames,
                                (T*)y, y_stride, given, a.T, n, a.act, eps, c.blocks);
             GL_HIP_CHECK(hipGetLastError());
             return 0;
@@ -1015,11 +1039,12 @@ int norm_back(const Norm& a, const void* dy_, long long dy_stride, const float* 
     const int n = a.C / a.groups;
     const T *x = (const T*)a.x, *ga = (const T*)a.gamma, *be = (const T*)a.beta, *dy = (const T*)dy_;
     T* dx = (T*)dx_;
-    const Cut c = cut_for(a.B, a.T, a.C, a.groups, sizeof(T), V);
+    const Cut c = cut_for(a.B, a.T, a.C, a.groups, sizeof(T), V, kBackThreads<T>);
     if (c.kind == 0)
         return with_act<V>(a.act, [&](auto act) -> int {
-            hipLaunchKernelGGL((k_norm_back_slab<T, V, decltype(act)::value>), dim3((unsigned)((c.blocks.total + 7) / 8 * 8)),
-                               dim3(c.threads), lds_bytes(c.threads, V, c.blocks.CB, n, 2), a.st, dy, dy_stride, x, a.x_stride,
+            const bool even = even_blocks(c, a.C, n, V);
+            auto kernel = even ? k_norm_back_slab<T, V, decltype(act)::value, true> : k_norm_back_slab<T, V, decltype(act)::value, false>;
+            hipLaunchKernelGGL(kernel, dim3((unsigned)((c.blocks.total + 7) / 8 * 8)), dim3(c.threads), lds_bytes(c.threads, V, c.blocks.CB, n, 2), a.st, dy, dy_stride, x, a.x_stride,
                                stats, ga, be, a.frames, dx, dx_stride, sums, a.T, n, a.act, c.blocks);
             GL_HIP_CHECK(hipGetLastError());
             return 0;
