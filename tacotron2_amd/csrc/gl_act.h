@@ -11,17 +11,12 @@ __device__ __forceinline__ float gl_to_f32(float v) { return v; }
 __device__ __forceinline__ float gl_to_f32(gl_bf16 v) { return (float)v; }
 __device__ __forceinline__ float gl_to_f32(gl_f16 v) { return (float)v; }
 
-// The exponential, with the reciprocal and the error function built on it, as the 16-bit results need them: relative
-// error below 2^-20 where the result is not subnormal.  exp(z) = 2^n 2^f with n = rint(z log2 e); the product is carried
-// in two floats, so the error does not grow with |z|.
+// exp(z) = 2^(z log2 e).  The product's rounding moves the result by |z| 2^-24 of it, as half a step of z itself does: a sum z
+// is not known better than that, so it is not carried further.
 __device__ __forceinline__ float gl_exp(float z) {
-    const float k = 1.44269504088896341f;                    // log2 e, and what its rounding leaves
-    const float t = z * k;
-    const float lo = fmaf(z, k, -t) + z * 1.92596299e-8f;
+    const float t = z * 1.44269504088896341f;
     const bool low = t < -120.0f;                            // subnormal results: 2^64 up, then down with one rounding
-    const float e = __builtin_amdgcn_exp2f(low ? t + 64.0f : t);
-    const float r = fmaf(e, lo * 0.69314718f, e) * (low ? 0x1p-64f : 1.0f);
-    return z < -104.0f ? 0.0f : (e == INFINITY ? e : r);                                   // NaN stays NaN
+    return __builtin_amdgcn_exp2f(t + (low ? 64.0f : 0.0f)) * (low ? 0x1p-64f : 1.0f);
 }
 
 __device__ __forceinline__ float gl_sigmoid(float z) {
@@ -42,11 +37,10 @@ __device__ __forceinline__ float gl_act(float z, int act) {
     switch (act) {
         case GL_ACT_RELU: return z < 0.0f ? 0.0f : z;                  // NaN stays NaN
         case GL_ACT_SILU: return z * gl_sigmoid(z);
-        case GL_ACT_GELU: {                                            // z Phi(z) = max(z, 0) - |z| Phi(-|z|)
-            const float a = fminf(fabsf(z), 16.0f);                    // Phi(-16) is 0: infinities give z or 0
+        case GL_ACT_GELU: {                                            // z Phi(z) = z / 2 + |z| (1 / 2 - Phi(-|z|))
             float t;
-            const float p = gl_phi_poly(a, t);
-            return fmaf(-(a * t * p), __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f), fmaxf(z, 0.0f));   // NaN: by z z
+            const float p = gl_phi_poly(fabsf(z), t), e = __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f);
+            return fmaf(fabsf(z), fmaf(-(t * p), e, 0.5f), 0.5f * z);
         }
         case GL_ACT_TANH: {
             // (1 - e) / (1 + e) with e = exp(-2 |z|); near zero the series z - z^3/3 + 2 z^5/15 - 17 z^7/315

@@ -25,28 +25,51 @@ constexpr int kTile = 64;        // rows and columns of C per workgroup (4 waves
 constexpr int kBQ = 32;          // contraction indexes staged per step
 constexpr int kCUs = 256;        // compute units of an MI355X: the work split must not depend on the moment
 
-// Any size, stride and alignment: elements are staged one by one.  grid (workgroups, parts); workgroups walk over the tiles.
-// flags: only the tiles whose flag is set.
-template <typename T, typename TO>
+// Any size, stride and alignment.  A thread stages eight consecutive elements of each side, the next step's while this one's
+// products run.  grid (workgroups, parts); workgroups walk over the tiles.  flags: only the tiles whose flag is set.
+// V: how many elements a load may take (the sides' rows and pointers allow it), 1 or 16 bytes of them.
+template <typename T, typename TO, int V>
 __global__ void __launch_bounds__(256) k_dense_any(Operand P, Operand Q, Epilogue e, long long I, int J, long long nq,
                                                    long long q_per_part, int tiles_j, int n_tiles, const int* __restrict__ flags) {
     constexpr bool k16 = sizeof(T) == 2;
     constexpr int kPitch = k16 ? kBQ + 8 : kBQ + 1;
+    typedef typename vecn<T, V>::type vT;
     __shared__ __attribute__((aligned(16))) T Ps[kTile * kPitch];
     __shared__ __attribute__((aligned(16))) T Qs[kTile * kPitch];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 31, lk = lane >> 5;
     const long long q_begin = (long long)blockIdx.y * q_per_part;
     const long long q_end = q_begin + q_per_part < nq ? q_begin + q_per_part : nq;
     const int wi = (wave >> 1) * 32, wj = (wave & 1) * 32;
-    auto stage = [&](T* dst, const Operand& o, long long r0, long long rn, long long q0) {
-        for (int e8 = threadIdx.x; e8 < kTile * kBQ; e8 += 256) {
-            // consecutive threads along the contiguous direction
-            const int r = o.qs == 1 ? e8 / kBQ : e8 % kTile;
-            const int q = o.qs == 1 ? e8 % kBQ : e8 / kTile;
-            T v = (T)0.0f;
-            if (r0 + r < rn && q0 + q < q_end) v = ((const T*)o.base)[(r0 + r) * o.is + (q0 + q) * o.qs];
-            dst[r * kPitch + q] = v;
+    // this thread's eight elements: of row r along q, or of contraction index q across rows
+    auto spot = [&](const Operand& o, int& r, int& q) {
+        r = o.qs == 1 ? threadIdx.x >> 2 : (threadIdx.x & 7) * 8;
+        q = o.qs == 1 ? (threadIdx.x & 3) * 8 : threadIdx.x >> 3;
+    };
+    auto fetch = [&](T (&v)[8], const Operand& o, long long r0, long long rn, long long q0) {
+        int r, q;
+        spot(o, r, q);
+        const bool along = o.qs == 1;
+        const T* at = (const T*)o.base + (r0 + r) * o.is + (q0 + q) * o.qs;
+        // how many of the eight exist
+        const long long have = along ? (r0 + r < rn ? q_end - (q0 + q) : 0) : (q0 + q < q_end ? rn - (r0 + r) : 0);
+        if (V > 1 && have >= 8) {
+#pragma unroll
+            for (int k = 0; k < 8; k += V) {
+                const vT t = *(const vT*)(at + k);
+#pragma unroll
+                for (int u = 0; u < V; ++u) v[k + u] = t[u];
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = k < have ? at[k] : (T)0.0f;
         }
+    };
+    auto deposit = [&](T* dst, const Operand& o, const T (&v)[8]) {
+        int r, q;
+        spot(o, r, q);
+        const int step = o.qs == 1 ? 1 : kPitch;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) dst[r * kPitch + q + k * step] = v[k];
     };
     for (long long tile = blockIdx.x; tile < n_tiles; tile += gridDim.x) {
         if (flags && !flags[tile]) continue;                 // uniform over the workgroup
@@ -55,11 +78,18 @@ __global__ void __launch_bounds__(256) k_dense_any(Operand P, Operand Q, Epilogu
         f32x16 acc;
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[r] = 0.0f;
+        T pv[8], qv[8];
+        fetch(pv, P, i0, I, q_begin);
+        fetch(qv, Q, j0, J, q_begin);
         for (long long q0 = q_begin; q0 < q_end; q0 += kBQ) {
             __syncthreads();
-            stage(Ps, P, i0, I, q0);
-            stage(Qs, Q, j0, J, q0);
+            deposit(Ps, P, pv);
+            deposit(Qs, Q, qv);
             __syncthreads();
+            if (q0 + kBQ < q_end) {
+                fetch(pv, P, i0, I, q0 + kBQ);
+                fetch(qv, Q, j0, J, q0 + kBQ);
+            }
             if constexpr (k16) {
                 typedef typename vecn<T, 8>::type v8;
 #pragma unroll
@@ -250,18 +280,21 @@ __global__ void __launch_bounds__(256) k_dense_dz(const TO* __restrict__ dy, lon
     }
 }
 
-// column sums over the parts; thread (column, one of 4 part lanes)
+// column sums over the parts; thread (column, one of 16 part lanes)
 template <typename T>
-__global__ void __launch_bounds__(256) k_dense_db(const float* __restrict__ parts, int n_parts, T* __restrict__ db, int N) {
-    __shared__ float s[4][64];
+__global__ void __launch_bounds__(1024) k_dense_db(const float* __restrict__ parts, int n_parts, T* __restrict__ db, int N) {
+    __shared__ float s[16][64];
     const int c = threadIdx.x & 63, r = threadIdx.x >> 6, n = blockIdx.x * 64 + c;
     float a = 0.0f;
     if (n < N)
-#pragma unroll 4
-        for (int p = r; p < n_parts; p += 4) a += parts[(long long)p * N + n];
+#pragma unroll 8
+        for (int p = r; p < n_parts; p += 16) a += parts[(long long)p * N + n];
     s[r][c] = a;
     __syncthreads();
-    if (r == 0 && n < N) db[n] = (T)((s[0][c] + s[1][c]) + (s[2][c] + s[3][c]));
+    if (r || n >= N) return;
+#pragma unroll
+    for (int k = 1; k < 16; ++k) a += s[k][c];
+    db[n] = (T)a;
 }
 
 template <typename T>
@@ -270,17 +303,25 @@ __global__ void __launch_bounds__(256) k_dense_zero(T* p, long long stride, int 
         p[at / cols * stride + at % cols] = (T)0.0f;
 }
 
-// Parts of the contraction: enough workgroups to fill the chip twice, at least 8 steps each.
+// Parts of the contraction for k_dense_any: enough workgroups to fill half the chip, at least 4 steps each.
 int n_splits(long long I, int J, long long nq) {
     const long long tiles = gl_ceil_div(I, kTile) * gl_ceil_div(J, kTile);
-    long long s = 2 * kCUs / tiles;
-    const long long most = gl_ceil_div(nq, 8 * kBQ);
+    long long s = kCUs / tiles;
+    const long long most = gl_ceil_div(nq, 4 * kBQ);
     if (s > most) s = most;
+    if (s > 16) s = 16;
     return s < 1 ? 1 : (int)s;
 }
 long long any_bytes(long long I, int J, long long nq) {
     const int s = n_splits(I, J, nq);
     return s > 1 ? gl_align16((long long)s * I * J * 4) : 0;
+}
+
+// 16-byte loads: rows on 16 bytes (eight elements from a multiple of eight on)
+template <typename T>
+bool wide_loads(const Operand& o) {
+    const long long stride = o.qs == 1 ? o.is : o.qs;
+    return (uintptr_t)o.base % 16 == 0 && stride * sizeof(T) % 16 == 0;
 }
 
 template <typename T, typename TO>
@@ -292,7 +333,9 @@ int any_product(const Operand& P, const Operand& Q, Epilogue e, long long I, int
     if (tiles > 0x7fffffffLL) return gl_set_error(GL_ERR_INVALID, "gl_dense: %lld tiles are too many for one launch", tiles);
     e.partial = used > 1 ? partial : nullptr;
     e.exact_p = nullptr;
-    hipLaunchKernelGGL((k_dense_any<T, TO>), dim3((unsigned)tiles, (unsigned)used), dim3(256), 0, st, P, Q, e, I, J, nq, per,
+    const bool wide = wide_loads<T>(P) && wide_loads<T>(Q);
+    auto kernel = wide ? k_dense_any<T, TO, 16 / sizeof(T)> : k_dense_any<T, TO, 1>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)tiles, (unsigned)used), dim3(256), 0, st, P, Q, e, I, J, nq, per,
                        (int)gl_ceil_div(J, kTile), (int)tiles, (const int*)nullptr);
     GL_HIP_CHECK(hipGetLastError());
     return used > 1 ? gl_dense_join<T, TO>(e, I, J, (int)used, st) : 0;
@@ -430,10 +473,11 @@ int forward(const void* x, long long x_stride, const void* w, long long w_stride
 }
 
 // ---- backward ----
-constexpr int kMaxParts = 128;
-int rows_per_part(long long rows) {
-    const long long r = gl_ceil_div(rows, kMaxParts);
-    return (int)(r < 64 ? 64 : r);
+// Frames of a part of the column sums: about 2048 workgroups of k_dense_dz in all (its loads in flight then reach what the
+// memory needs: 55 104 x 2048 bf16 gelu 190 us with 512 of them), 16 frames at least.
+int rows_per_part(long long rows, int outputs) {
+    const long long r = gl_ceil_div(rows, 2048 / gl_ceil_div(outputs, 512) + 1);
+    return (int)(r < 16 ? 16 : r);
 }
 
 // workspace: [dz (unless dy serves), or its planes] [with planes: dz itself, for sums that are not finite] [copy of x]
@@ -457,7 +501,7 @@ BackLayout back_layout(long long rows, int inputs, int outputs, int dtype, int o
         l.x_bytes = copy_bytes(dtype, rows, inputs);
         l.w_bytes = copy_bytes(dtype, outputs, inputs);
     }
-    l.parts_bytes = gl_align16(gl_ceil_div(rows, rows_per_part(rows)) * outputs * 4);
+    l.parts_bytes = gl_align16(gl_ceil_div(rows, rows_per_part(rows, outputs)) * outputs * 4);
     const long long a = partial_bytes(dtype, rows, inputs, l.own_dz ? l.dz_stride : outputs, false, l.fast);
     const long long b = partial_bytes(dtype, outputs, inputs, rows, true, l.fast);
     l.partial = a > b ? a : b;
@@ -467,7 +511,7 @@ BackLayout back_layout(long long rows, int inputs, int outputs, int dtype, int o
 template <typename T, typename TO, int V, int PLANES>
 int dz_launch(const void* dy, long long dy_stride, const void* z, long long z_stride, void* dz, long long dz_stride, float* parts,
               long long rows, int outputs, int act, hipStream_t st) {
-    const int rpp = rows_per_part(rows);
+    const int rpp = rows_per_part(rows, outputs);
     hipLaunchKernelGGL((k_dense_dz<T, TO, V, PLANES>), dim3((unsigned)gl_ceil_div(dz ? dz_stride : outputs, 64 * V),
                        (unsigned)gl_ceil_div(rows, rpp)), dim3(256), 0, st, (const TO*)dy, dy_stride, (const TO*)z, z_stride, dz,
                        dz_stride, rows * dz_stride, parts, rows, outputs, rpp, act);
@@ -509,8 +553,8 @@ int backward(const void* dy, long long dy_stride, const void* x, long long x_str
         if (rc) return rc;
     }
     if (db) {
-        hipLaunchKernelGGL((k_dense_db<T>), dim3((unsigned)gl_ceil_div(outputs, 64)), dim3(256), 0, st, parts,
-                           (int)gl_ceil_div(rows, rows_per_part(rows)), (T*)db, outputs);
+        hipLaunchKernelGGL((k_dense_db<T>), dim3((unsigned)gl_ceil_div(outputs, 64)), dim3(1024), 0, st, parts,
+                           (int)gl_ceil_div(rows, rows_per_part(rows, outputs)), (T*)db, outputs);
         GL_HIP_CHECK(hipGetLastError());
     }
     // dz as the products read it, and as it is
@@ -564,15 +608,16 @@ int gl_dense_flagged(const gl_epilogue& e, long long I, int J, long long nq, hip
     const long long tiles = gl_ceil_div(I, kTile) * gl_ceil_div(J, kTile);
     gl_epilogue f = e;
     f.partial = nullptr;
-    hipLaunchKernelGGL((k_dense_any<float, float>), dim3((unsigned)(tiles < 512 ? tiles : 512)), dim3(256), 0, st,
+    hipLaunchKernelGGL((k_dense_any<float, float, 1>), dim3((unsigned)(tiles < 512 ? tiles : 512)), dim3(256), 0, st,
                        Operand{e.exact_p, e.exact_p_is, e.exact_p_qs}, Operand{e.exact_q, e.exact_q_is, e.exact_q_qs}, f, I, J, nq, nq,
                        (int)gl_ceil_div(J, kTile), (int)tiles, e.flags);
     GL_HIP_CHECK(hipGetLastError());
     return 0;
 }
 
-// 256 x 256 tiles where they fill the chip (parts included), else 128 x 128, else 64 x 64.  A part has at least 512
-// contraction indexes with large tiles and 256 with small ones: shorter ones cost more in the join than they fill.
+// 256 x 256 tiles where they fill half the chip (parts included), else 128 x 128, else 64 x 64.  A part of the contraction has
+// at least 2048 indexes with large tiles, 512 with medium and 256 with small ones: shorter ones cost more in the join than
+// they fill (6888 x 1024 x 1024 float32 in two parts of large tiles 120 us, in one of medium ones 92).
 gl_mm_plan gl_mm_plan_for(long long I, int J, long long nq, bool any_q) {
     auto split = [&](int b, long long least) -> gl_mm_plan {
         const long long tiles = gl_ceil_div(I, b) * gl_ceil_div(J, b);
@@ -585,13 +630,13 @@ gl_mm_plan gl_mm_plan_for(long long I, int J, long long nq, bool any_q) {
         return {0, (int)gl_ceil_div(nq, per), per};
     };
     if (J % 256 == 0 && I >= 256 && (any_q || nq % 32 == 0)) {
-        gl_mm_plan p = split(256, 512);
+        gl_mm_plan p = split(256, 2048);
         if (gl_ceil_div(I, 256) * (J / 256) * p.parts >= 128) {
             p.kind = 2;
             return p;
         }
     }
-    gl_mm_plan p = split(128, 256);
+    gl_mm_plan p = split(128, 512);
     if (I >= 96 && J >= 96 && gl_ceil_div(I, 128) * gl_ceil_div(J, 128) * p.parts >= 256) {
         p.kind = 1;
         return p;

@@ -51,7 +51,7 @@ __device__ __forceinline__ f32x4 mfma16(s16x8 a, s16x8 b, f32x4 c) {
 __device__ __forceinline__ void wait_loads(int n) {          // at most n vector memory operations outstanding
     switch (n) {
 #define GL_WAIT(k) case k: asm volatile("s_waitcnt vmcnt(" #k ")" ::: "memory"); break;
-        GL_WAIT(0) GL_WAIT(2) GL_WAIT(3) GL_WAIT(4) GL_WAIT(5) GL_WAIT(6) GL_WAIT(8) GL_WAIT(10) GL_WAIT(12) GL_WAIT(16) GL_WAIT(18) GL_WAIT(22) GL_WAIT(24) GL_WAIT(38) GL_WAIT(40)
+        GL_WAIT(0) GL_WAIT(2) GL_WAIT(3) GL_WAIT(4) GL_WAIT(5) GL_WAIT(6) GL_WAIT(8) GL_WAIT(10) GL_WAIT(12) GL_WAIT(16) GL_WAIT(18) GL_WAIT(22) GL_WAIT(24) GL_WAIT(28) GL_WAIT(38) GL_WAIT(40) GL_WAIT(44)
 #undef GL_WAIT
         default: asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
@@ -70,6 +70,7 @@ constexpr int kPlanesQ = 0 | 1 << 2 | 0 << 4 | 1 << 6 | 2 << 8 | 0 << 10;
 __device__ __forceinline__ int plane_of(int planes, int seg) { return planes >> (2 * seg) & 3; }
 
 constexpr int kFlags = 0x00027000;                           // raw 32-bit buffer: bounds-checked, no format conversion
+constexpr int kStream = 2;                                   // cache policy: non-temporal
 constexpr int kOutside = 0x7fffff00;                         // an offset beyond every buffer: loads zeros
 
 // One operand of a tile: LDS layout, loads and fragments.
@@ -224,8 +225,10 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t block_of(const void* p, long l
 }
 
 // Stores a wave's block, rounded to TO; returns how many store instructions that were at least (the caller may leave that
-// many outstanding).  TAIL: columns may end inside the block (a branch that costs registers).
-template <typename TO, bool TAIL, int MI, int NI>
+// many outstanding).  TAIL: columns may end inside the block (a branch that costs registers).  LINES: rows on 128 bytes; the
+// result then streams past the L2s, which keep Q and the rows of P (55 104 x 2048 x 512 bf16: 149 us, so 128; rows off 128 bytes
+// would lose that way what the L2s merge: 55 104 x 1025 float32 105 us, so 132).
+template <typename TO, bool TAIL, bool LINES, int MI, int NI>
 __device__ __forceinline__ int put_block(TO* dst, long long stride, const f32x4 (&v)[MI][NI], long long i0, int j0, long long I,
                                          int J, int lane, bool odd) {
     typedef typename vec<TO, 4>::type to4;
@@ -240,28 +243,49 @@ __device__ __forceinline__ int put_block(TO* dst, long long stride, const f32x4 
         return t;
     };
     if (!TAIL || (j0 + 16 * NI <= J && !odd)) {              // wave-uniform: whole column blocks
-        int off = il * stride_b + (kPair ? 16 * (g4 & 1) + 8 * (g4 >> 1) : 4 * g4) * (int)sizeof(TO);
+        // A lane's 16 bytes of two column groups: neighbouring lanes (rows 2 k and 2 k + 1) swap one, so that a store writes
+        // 128 contiguous bytes of eight rows instead of 64 of sixteen: whole cache lines.
+        const bool hi = lane & 1;
+        constexpr int kCols = kPair ? 32 : 16;               // columns from one group to the other
+        const int c0 = kPair ? 16 * (g4 & 1) + 8 * (g4 >> 1) : 4 * g4;
+        int off_a = (il & ~1) * stride_b + (c0 + (hi ? kCols : 0)) * (int)sizeof(TO), off_b = off_a + stride_b;
+        auto store2 = [&](const u32x4& x, const u32x4& y, int at) {
+            u32x4 a, b;
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+                const unsigned got = __builtin_amdgcn_mov_dpp(hi ? x[d] : y[d], 0xB1, 0xF, 0xF, true);   // the lane beside
+                a[d] = hi ? got : x[d];
+                b[d] = hi ? y[d] : got;
+            }
+            __builtin_amdgcn_raw_buffer_store_b128(a, rs, off_a + at, 0, LINES ? kStream : 0);
+            __builtin_amdgcn_raw_buffer_store_b128(b, rs, off_b + at, 0, LINES ? kStream : 0);
+        };
 #pragma unroll
         for (int m = 0; m < MI; ++m) {
             if constexpr (kPair) {
                 // two 16-column blocks: quarter-waves swapped so that a lane holds 8 consecutive columns
+                auto eight = [&](int n) -> u32x4 {
+                    const u32x2 lo = __builtin_bit_cast(u32x2, round4(v[m][n])), up = __builtin_bit_cast(u32x2, round4(v[m][n + 1]));
+                    const auto s0 = __builtin_amdgcn_permlane16_swap(lo[0], up[0], false, false);
+                    const auto s1 = __builtin_amdgcn_permlane16_swap(lo[1], up[1], false, false);
+                    return (u32x4){s0[0], s1[0], s0[1], s1[1]};
+                };
+                if constexpr (NI % 4 == 0) {
 #pragma unroll
-                for (int n = 0; n < NI; n += 2) {
-                    const u32x2 lo = __builtin_bit_cast(u32x2, round4(v[m][n])), hi = __builtin_bit_cast(u32x2, round4(v[m][n + 1]));
-                    const auto s0 = __builtin_amdgcn_permlane16_swap(lo[0], hi[0], false, false);
-                    const auto s1 = __builtin_amdgcn_permlane16_swap(lo[1], hi[1], false, false);
-                    __builtin_amdgcn_raw_buffer_store_b128((u32x4){s0[0], s1[0], s0[1], s1[1]}, rs, off + 32 * n, 0, 0);
+                    for (int n = 0; n < NI; n += 4) store2(eight(n), eight(n + 2), 32 * n);
+                } else {
+#pragma unroll
+                    for (int n = 0; n < NI; n += 2)
+                        __builtin_amdgcn_raw_buffer_store_b128(eight(n), rs, (16 * m + il) * stride_b + (c0 + 16 * n) * 2, 0, 0);
                 }
             } else {
+                static_assert(sizeof(TO) == 4 && NI % 2 == 0, "columns in pairs of blocks");
 #pragma unroll
-                for (int n = 0; n < NI; ++n) {
-                    if constexpr (sizeof(TO) == 4)
-                        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v[m][n]), rs, off + 64 * n, 0, 0);
-                    else
-                        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, round4(v[m][n])), rs, off + 32 * n, 0, 0);
-                }
+                for (int n = 0; n < NI; n += 2)
+                    store2(__builtin_bit_cast(u32x4, v[m][n]), __builtin_bit_cast(u32x4, v[m][n + 1]), 64 * n);
             }
-            off += 16 * stride_b;
+            off_a += 16 * stride_b;
+            off_b += 16 * stride_b;
             __builtin_amdgcn_sched_barrier(0);
         }
         return MI * NI / (kPair ? 2 : 1);
@@ -302,11 +326,11 @@ __device__ __forceinline__ bool all_finite(int* flags, const f32x4 (&acc)[MI][NI
 // Writes a wave's block at (i0, j0): activation, residual and one rounding.  All loads come before the
 // results' stores: the memory counter runs in order, a load behind a store would wait for it.
 // EXTRA: there may be a residual or a preactivation.
-template <typename T, typename TO, int ACT, bool EXTRA, bool TAIL, int MI, int NI>
+template <typename T, typename TO, int ACT, bool EXTRA, bool TAIL, bool LINES, int MI, int NI>
 __device__ __forceinline__ int epilogue(const Out& o, f32x4 (&acc)[MI][NI], long long i0, int j0, long long I, int J,
                                         int part, int lane) {
     const int il = lane & 15, g4 = lane >> 4;
-    if (EXTRA && o.z) put_block<TO, TAIL, MI, NI>((TO*)o.z, o.z_stride, acc, i0, j0, I, J, lane, o.odd);
+    if (EXTRA && o.z) put_block<TO, TAIL, LINES, MI, NI>((TO*)o.z, o.z_stride, acc, i0, j0, I, J, lane, o.odd);
 #pragma unroll
     for (int m = 0; m < MI; ++m)
 #pragma unroll
@@ -342,7 +366,7 @@ __device__ __forceinline__ int epilogue(const Out& o, f32x4 (&acc)[MI][NI], long
             __builtin_amdgcn_sched_barrier(0);
         }
     }
-    return put_block<TO, TAIL, MI, NI>((TO*)o.y + part * o.part_stride, o.y_stride, acc, i0, j0, I, J, lane, o.odd);
+    return put_block<TO, TAIL, LINES, MI, NI>((TO*)o.y + part * o.part_stride, o.y_stride, acc, i0, j0, I, J, lane, o.odd);
 }
 
 template <typename T, typename TO, typename TB, int SEG, int ACT, int BM, int BN, int WM, int WN, int BK, int ST, bool PT, bool QT, int WPE>
@@ -419,14 +443,14 @@ k_mm16(Side P, Side Q, Out o, long long I, int J, long long nq, long long q_per_
     if constexpr (SEG > 1) {
         if (o.flags && !all_finite<MI, NI>(o.flags, acc, i0 + wi, j0 + wj, I, J, lane)) return;
     }
-    epilogue<T, TO, ACT, true, true, MI, NI>(o, acc, i0 + wi, j0 + wj, I, J, blockIdx.y, lane);
+    epilogue<T, TO, ACT, true, true, false, MI, NI>(o, acc, i0 + wi, j0 + wj, I, J, blockIdx.y, lane);
 }
 
 // The same product for many tiles.  Persistent: WGS workgroups a CU walk over the tiles, the ring running on into the next
 // tile's first stages while a tile's results are written.  A step's fragments are read, and the loads of the step RING
 // ahead started, between the products of the step before.
 // A contraction that one side is contiguous in is a multiple of 32 here, J a multiple of BN.
-template <typename T, typename TO, typename TB, int SEG, int ACT, bool EXTRA, int BM, int BN, int WM, int WN, int RING, int WGS, bool PT, bool QT>
+template <typename T, typename TO, typename TB, int SEG, int ACT, bool EXTRA, bool LINES, int BM, int BN, int WM, int WN, int RING, int WGS, bool PT, bool QT>
 __global__ void __launch_bounds__(64 * (BM / WM) * (BN / WN), WGS * (BM / WM) * (BN / WN) / 4)
 k_mm16_walk(Side P, Side Q, Out o, long long I, int J, long long nq, long long q_per_part, int tiles_j, int n_tiles) {
     constexpr int BK = 32, WAVES = (BM / WM) * (BN / WN);
@@ -545,7 +569,7 @@ k_mm16_walk(Side P, Side Q, Out o, long long I, int J, long long nq, long long q
                 continue;
             }
         }
-        old = epilogue<T, TO, ACT, EXTRA, false, MI, NI>(o, acc, (long long)(tile / tiles_j) * BM + wi, tile % tiles_j * BN + wj, I, J, blockIdx.y, lane);
+        old = epilogue<T, TO, ACT, EXTRA, false, LINES, MI, NI>(o, acc, (long long)(tile / tiles_j) * BM + wi, tile % tiles_j * BN + wj, I, J, blockIdx.y, lane);
     }
     wait_loads(0);                                           // nothing may be on its way into LDS when the wave ends
 }

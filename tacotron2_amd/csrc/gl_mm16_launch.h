@@ -17,18 +17,26 @@ static inline long long padded_q(const gl_operand& P, long long nq) {
     return P.padded && !P.across() ? (nq + 63) / 64 * 64 : nq;
 }
 
-template <typename T, typename TO, typename TB, int SEG, int ACT, bool EXTRA, bool PT, bool QT>
-int walk(const gl_operand& P, const gl_operand& Q, const Out& o, long long I, int J, long long nq, const gl_mm_plan& p, hipStream_t st) {
+template <typename T, typename TO, typename TB, int SEG, int ACT, bool EXTRA, bool LINES, bool PT, bool QT>
+int walk_as(const gl_operand& P, const gl_operand& Q, const Out& o, long long I, int J, long long nq, const gl_mm_plan& p, hipStream_t st) {
     const long long pad = padded_q(P, nq);
     const int tiles_j = J / 256;
     const long long tiles = gl_ceil_div(I, 256) * tiles_j;
     long long walkers = 256 / p.parts / 8 * 8;               // one workgroup a CU in all, whole rounds of the 8 XCDs
     if (walkers > (tiles + 7) / 8 * 8) walkers = (tiles + 7) / 8 * 8;
     if (walkers < 8) walkers = 8;
-    hipLaunchKernelGGL((k_mm16_walk<T, TO, TB, SEG, ACT, EXTRA, 256, 256, 128, 64, 4, 1, PT, QT>), dim3((unsigned)walkers, p.parts), dim3(512),
+    hipLaunchKernelGGL((k_mm16_walk<T, TO, TB, SEG, ACT, EXTRA, LINES, 256, 256, 128, 64, 4, 1, PT, QT>), dim3((unsigned)walkers, p.parts), dim3(512),
                        0, st, side(P, I, nq, pad), side(Q, J, nq, pad), o, I, J, pad, p.per, tiles_j, (int)tiles);
     GL_HIP_CHECK(hipGetLastError());
     return 0;
+}
+
+template <typename T, typename TO, typename TB, int SEG, int ACT, bool EXTRA, bool PT, bool QT>
+int walk(const gl_operand& P, const gl_operand& Q, const Out& o, long long I, int J, long long nq, const gl_mm_plan& p, hipStream_t st) {
+    auto on_lines = [](const void* q, long long stride) { return !q || ((uintptr_t)q % 128 == 0 && stride * (long long)sizeof(TO) % 128 == 0); };
+    if (p.parts == 1 && on_lines(o.y, o.y_stride) && on_lines(o.z, o.z_stride))
+        return walk_as<T, TO, TB, SEG, ACT, EXTRA, true, PT, QT>(P, Q, o, I, J, nq, p, st);
+    return walk_as<T, TO, TB, SEG, ACT, EXTRA, false, PT, QT>(P, Q, o, I, J, nq, p, st);
 }
 
 template <typename T, typename TO, typename TB, int SEG, int B, int W, bool PT, bool QT>

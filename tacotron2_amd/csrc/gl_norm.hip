@@ -17,8 +17,9 @@ namespace {
 
 constexpr int kHeld = 8;                 // vectors of V channels a thread holds
 constexpr int kMaxThreads = 1024;
-constexpr int kRowBytes = 64;            // of a slab's rows where whole groups and the chip allow: 64 ragged utterances of 861 x 512
-                                         // bf16 with 32: 28.9 us, 64: 28.3, 128: 32
+// Bytes of a slab's rows where whole groups and the chip allow.  64 ragged utterances of 861 x 512 bf16 with 32: 28.9 us, 64: 28.3,
+// 128: 32; their gradients 58, 62, 70.
+constexpr int kRowBytes = 64, kBackRowBytes = 32;
 // threads of a gradient slab: it holds x and du in registers (16-bit: 96 of them, 1024 threads would spill)
 template <typename T> constexpr int kBackThreads = sizeof(T) == 2 ? 512 : 1024;
 
@@ -898,14 +899,14 @@ int threads_for(int tp, long long rows, int most) {          // the fewest threa
         if (t >= tp && (long long)(t / tp) * kHeld >= rows) return t;
     return 0;
 }
-Cut cut_for(int B, int T, int C, int groups, int size, int V, int most) {
+Cut cut_for(int B, int T, int C, int groups, int size, int V, int most, int row_bytes) {
     Cut c = {};
     const int n = C / groups;
     int k = 1;
     while (k < groups && (n * k) % V) ++k;                   // whole groups on whole vectors
     if (n * k % V == 0 && threads_for(n * k / V, T, most) && lds_bytes(kMaxThreads, V, n * k, n, 2) <= kMaxLds) {
         // more groups to a block, to 128 bytes a row, while the slab fits and the blocks fill the chip
-        for (int m = 2 * k; m <= groups && (long long)n * k * size < kRowBytes; m += k)
+        for (int m = 2 * k; m <= groups && (long long)n * k * size < row_bytes; m += k)
             if (groups % m == 0 && threads_for(n * m / V, T, most) && (long long)B * (groups / m) >= 256) k = m;
         c.kind = 0;
         c.threads = threads_for(n * k / V, T, most);
@@ -967,7 +968,7 @@ long long parts_bytes(int B, int T, int C, int groups, int dtype) {
     long long most = 0;
     for (int V : {16 / size, 1}) {                           // alignment is not known to the query
         if (C % V) continue;
-        const Cut c = cut_for(B, T, C, groups, size, V, kMaxThreads);
+        const Cut c = cut_for(B, T, C, groups, size, V, kMaxThreads, kRowBytes);
         if (c.kind == 1 && 8LL * B * groups * c.chunks > most) most = 8LL * B * groups * c.chunks;
     }
     return align16(most);
@@ -976,7 +977,7 @@ long long norm_bytes(int B, int T, int C, int groups, int dtype) {
     const int size = dtype == GL_F32 ? 4 : 2;
     bool slabs = B && T;
     for (int V : {16 / size, 1})
-        if (slabs && C % V == 0) slabs = cut_for(B, T, C, groups, size, V, kMaxThreads).kind == 0;
+        if (slabs && C % V == 0) slabs = cut_for(B, T, C, groups, size, V, kMaxThreads, kRowBytes).kind == 0;
     return slabs ? 0 : stats_bytes(B, groups) + (B && T ? parts_bytes(B, T, C, groups, dtype) : 0);
 }
 long long back_parts_bytes(int B, int T, int C) {
@@ -1000,7 +1001,7 @@ template <typename T, int V>
 int norm_fwd(const Norm& a, void* y, long long y_stride, float* stats, float* given, float* parts, float eps) {
     const int n = a.C / a.groups;
     const T *x = (const T*)a.x, *ga = (const T*)a.gamma, *be = (const T*)a.beta;
-    Cut c = a.T ? cut_for(a.B, a.T, a.C, a.groups, sizeof(T), V, kMaxThreads) : Cut{2};
+    Cut c = a.T ? cut_for(a.B, a.T, a.C, a.groups, sizeof(T), V, kMaxThreads, kRowBytes) : Cut{2};
     if (c.kind == 0)
         return with_act<V>(a.act, [&](auto act) -> int {
             const bool even = even_blocks(c, a.C, n, V);
@@ -1039,7 +1040,7 @@ int norm_back(const Norm& a, const void* dy_, long long dy_stride, const float* 
     const int n = a.C / a.groups;
     const T *x = (const T*)a.x, *ga = (const T*)a.gamma, *be = (const T*)a.beta, *dy = (const T*)dy_;
     T* dx = (T*)dx_;
-    const Cut c = cut_for(a.B, a.T, a.C, a.groups, sizeof(T), V, kBackThreads<T>);
+    const Cut c = cut_for(a.B, a.T, a.C, a.groups, sizeof(T), V, kBackThreads<T>, kBackRowBytes);
     if (c.kind == 0)
         return with_act<V>(a.act, [&](auto act) -> int {
             const bool even = even_blocks(c, a.C, n, V);
