@@ -77,9 +77,9 @@ constexpr int kOutside = 0x7fffff00;                         // an offset beyond
 //   R rows of C's side, TR: contiguous across the contraction
 template <int R, int BK, bool TR, int WAVES, bool TEXT>
 struct Stage {
-    static constexpr int kBytes = R * BK * 2;
-    static constexpr int kLoads = kBytes / (1024 * WAVES);   // 16-byte loads per lane and stage
-    static_assert(kBytes % (1024 * WAVES) == 0, "loads must divide evenly");
+    static constexpr int kLoads = (R * BK * 2 + 1024 * WAVES - 1) / (1024 * WAVES);   // 16-byte loads per lane and stage
+    static constexpr int kBytes = kLoads * 1024 * WAVES;     // with whole loads of all waves: rows past R are zeros
+    static_assert(!TR || R % 32 == 0 && (R & (R - 1)) == 0, "pieces of 32 bytes are exchanged within a row");
     static constexpr int kRowChunks = TR ? R / 8 : BK / 8;   // chunks per LDS row
     const char* base;            // first element of the tile at the current step
     const char* start;           // and at the first one
