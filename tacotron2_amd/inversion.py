@@ -39,6 +39,8 @@ def _activation(name):
 
 
 def _tensor(t, what, device=None, dtype=None, shape=None):
+    if device is not None and isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.device == device:
+        return t
     if not isinstance(t, torch.Tensor):
         raise ValueError(f"{what} must be a torch tensor, got {type(t).__name__}")
     if t.dtype not in _DTYPES:
@@ -166,7 +168,11 @@ def _stream(device):
 
 
 def _needs_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and getattr(t, "requires_grad", False):
+                return True
+    return False
 
 
 def _eager_only(device, what):
@@ -192,56 +198,61 @@ def dense_backward_workspace(rows, inputs, outputs, dtype=torch.float32, out_dty
 
 
 def _dense_args(x, weight, bias, residual, out_dtype):
+    """(result's shape, its type, device) of checked arguments."""
     _tensor(x, "x")
     if x.dim() < 1 or not isinstance(weight, torch.Tensor) or weight.dim() != 2:
         raise ValueError("x must be (..., inputs) and weight (outputs, inputs)")
-    out_dtype = x.dtype if out_dtype is None else out_dtype
-    if out_dtype not in (x.dtype, torch.float32):
-        raise ValueError(f"out_dtype must be {x.dtype} or float32, got {out_dtype}")
-    _tensor(weight, "weight", x.device, x.dtype, (weight.shape[0], x.shape[-1]))
-    if weight.numel() == 0:
+    dtype, device, width = x.dtype, x.device, weight.shape
+    if out_dtype is None:
+        out_dtype = dtype
+    elif out_dtype is not dtype and out_dtype is not torch.float32:
+        raise ValueError(f"out_dtype must be {dtype} or float32, got {out_dtype}")
+    _tensor(weight, "weight", device, dtype, (width[0], x.shape[-1]))
+    if width[0] == 0 or width[1] == 0:
         raise ValueError("weight has no elements")
-    shape = tuple(x.shape[:-1]) + (weight.shape[0],)
+    shape = x.shape[:-1] + width[:1]
     if bias is not None:
-        _tensor(bias, "bias", x.device, x.dtype, shape[-1:])
+        _tensor(bias, "bias", device, dtype, width[:1])
     if residual is not None:
-        _tensor(residual, "residual", x.device, out_dtype, shape)
-    return shape, out_dtype
+        _tensor(residual, "residual", device, out_dtype, shape)
+    return shape, out_dtype, device
 
 
 def _dense(x, weight, bias, act, residual, out_dtype, out, preactivation, workspace):
-    shape, out_dtype = _dense_args(x, weight, bias, residual, out_dtype)
-    y, y_stride = _output(out, shape, out_dtype, x.device, "out")
+    shape, out_dtype, device = _dense_args(x, weight, bias, residual, out_dtype)
+    y, y_stride = _output(out, shape, out_dtype, device, "out")
     z, z_stride = None, 0
     if preactivation is not None:
-        z, z_stride = _output(preactivation, shape, out_dtype, x.device, "preactivation")
-    inputs = [("x", x), ("weight", weight), ("bias", bias), ("residual", residual)]
-    if out is not None:
-        _apart(y, "out", inputs, same=(residual,))
-    if z is not None:
-        _apart(z, "preactivation", inputs + [("out", y)])
-    rows = x.numel() // x.shape[-1]
+        z, z_stride = _output(preactivation, shape, out_dtype, device, "preactivation")
+    if out is not None or z is not None:
+        inputs = [("x", x), ("weight", weight), ("bias", bias), ("residual", residual)]
+        if out is not None:
+            _apart(y, "out", inputs, same=(residual,))
+        if z is not None:
+            _apart(z, "preactivation", inputs + [("out", y)])
+    K, N = x.shape[-1], shape[-1]
+    rows = x.numel() // K
     x, x_stride = _rows(x)
     weight, w_stride = _rows(weight)
     r_stride = 0
     if residual is not None:
         residual, r_stride = _rows(residual)
-    bias = None if bias is None else _vector(bias)
-    lib = _lib.lib()
+    if bias is not None:
+        bias = _vector(bias)
     d, od = _DTYPES[x.dtype], _DTYPES[out_dtype]
-    ws, ws_bytes = _scratch(workspace, _bytes_of("gl_dense_workspace", rows, x.shape[-1], shape[-1], d, od), x.device)
-    with _on(x.device):
-        _lib.check(lib.gl_dense(_p(x), x_stride, _p(weight), w_stride, _p(bias), _p(residual), r_stride, _p(y), y_stride,
-                                _p(z), z_stride, rows, x.shape[-1], shape[-1], d, od, act, _p(ws), ws_bytes,
-                                _stream(x.device)), "gl_dense")
+    ws, ws_bytes = _scratch(workspace, _bytes_of("gl_dense_workspace", rows, K, N, d, od), device)
+    with _on(device):
+        _lib.check(_lib.lib().gl_dense(_p(x), x_stride, _p(weight), w_stride, _p(bias), _p(residual), r_stride, _p(y),
+                                       y_stride, _p(z), z_stride, rows, K, N, d, od, act, _p(ws), ws_bytes,
+                                       _stream(device)), "gl_dense")
     return y
 
 
 class _Dense(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act, out_dtype):
-        shape, out_dtype = _dense_args(x, weight, bias, residual, out_dtype)
-        z = torch.empty(shape, dtype=out_dtype, device=x.device) if act else None
+        shape, out_dtype, device = _dense_args(x, weight, bias, residual, out_dtype)
+        z = torch.empty(shape, dtype=out_dtype, device=device) if act else None
         y = _dense(x, weight, bias, act, residual, out_dtype, None, z, None)
         ctx.act = act
         ctx.save_for_backward(x, weight, z)
@@ -357,9 +368,10 @@ def _norm_args(x, groups, weight, bias, lengths):
     C = x.shape[-1]
     if groups < 1 or C % groups:
         raise ValueError(f"{C} channels do not divide into {groups} groups")
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None:
-            _tensor(t, name, x.device, x.dtype, (C,))
+    if weight is not None:
+        _tensor(weight, "weight", x.device, x.dtype, (C,))
+    if bias is not None:
+        _tensor(bias, "bias", x.device, x.dtype, (C,))
     B, T = (1, x.shape[0]) if x.dim() == 2 else x.shape[:2]
     lens = None
     if lengths is not None:
@@ -379,24 +391,27 @@ def _group_norm(x, groups, weight, bias, eps, act, lengths, out, stats, workspac
     groups, B, T, C, lens = _norm_args(x, groups, weight, bias, lengths)
     if not eps >= 0:
         raise ValueError(f"eps must be >= 0, got {eps}")
-    y, y_stride = _output(out, x.shape, x.dtype, x.device, "out")
-    inputs = [("weight", weight), ("bias", bias), ("lengths", lens)]
-    if out is not None:
-        _apart(y, "out", inputs + [("x", x)], same=(x,))
-    if stats is not None:
-        _tensor(stats, "stats", x.device, torch.float32, (B, groups, 2))
-        if not stats.is_contiguous():
-            raise ValueError("stats must be contiguous")
-        _apart(stats, "stats", inputs + [("x", x), ("out", y)])
+    device, dtype = x.device, x.dtype
+    y, y_stride = _output(out, x.shape, dtype, device, "out")
+    if out is not None or stats is not None:
+        inputs = [("weight", weight), ("bias", bias), ("lengths", lens)]
+        if out is not None:
+            _apart(y, "out", inputs + [("x", x)], same=(x,))
+        if stats is not None:
+            _tensor(stats, "stats", device, torch.float32, (B, groups, 2))
+            if not stats.is_contiguous():
+                raise ValueError("stats must be contiguous")
+            _apart(stats, "stats", inputs + [("x", x), ("out", y)])
     x, x_stride = _rows(x)
-    weight = None if weight is None else _vector(weight)
-    bias = None if bias is None else _vector(bias)
-    lib = _lib.lib()
-    d = _DTYPES[x.dtype]
-    ws, ws_bytes = _scratch(workspace, _bytes_of("gl_group_norm_workspace", B, T, C, groups, d), x.device)
-    with _on(x.device):
-        _lib.check(lib.gl_group_norm(_p(x), x_stride, _p(weight), _p(bias), _p(lens), _p(y), y_stride, _p(stats), B, T, C,
-                                     groups, d, act, float(eps), _p(ws), ws_bytes, _stream(x.device)),
+    if weight is not None:
+        weight = _vector(weight)
+    if bias is not None:
+        bias = _vector(bias)
+    d = _DTYPES[dtype]
+    ws, ws_bytes = _scratch(workspace, _bytes_of("gl_group_norm_workspace", B, T, C, groups, d), device)
+    with _on(device):
+        _lib.check(_lib.lib().gl_group_norm(_p(x), x_stride, _p(weight), _p(bias), _p(lens), _p(y), y_stride, _p(stats), B,
+                                            T, C, groups, d, act, eps, _p(ws), ws_bytes, _stream(device)),
                    "gl_group_norm")
     return y
 

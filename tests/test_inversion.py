@@ -255,7 +255,7 @@ def test_dense_backward_strides(M, K, N, name, dtype):
 
 
 # sizes whose tiles fill the chip: the walking kernel (both sides' layouts), a rest of columns, odd and short contractions
-LARGE_SIZES = [(4400, 512, 2048), (33000, 96, 257), (16500, 544, 512), (40000, 32, 256), (33001, 72, 256), (70000, 64, 264)]
+LARGE_SIZES = [(4400, 512, 2048), (33000, 96, 257), (16500, 544, 512), (40000, 32, 256), (33001, 72, 256), (70000, 64, 264), (65500, 64, 256)]
 
 
 @gpu
