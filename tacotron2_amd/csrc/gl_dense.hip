@@ -12,6 +12,8 @@
 //   v_mfma_f32_32x32x16 or, for float32, v_mfma_f32_32x32x2_f32.
 // Sums are float32 everywhere.  Q is the matrix instruction's A operand: the accumulator's registers then run along j, the
 // contiguous direction of C.
+#include <type_traits>
+
 #include "gl_dense.h"
 
 namespace {
@@ -23,83 +25,113 @@ typedef gl_epilogue Epilogue;
 
 constexpr int kTile = 64;        // rows and columns of C per workgroup (4 waves, 32 x 32 each)
 constexpr int kBQ = 32;          // contraction indexes staged per step
+constexpr long long kMostBlocks = 1 << 23;   // of 256 threads: a launch has less than 2^32
 constexpr int kCUs = 256;        // compute units of an MI355X: the work split must not depend on the moment
 
+// A product of k_dense_any.  With DZ, P is dy and Z the preactivation: the first factor is dz = dy act'(z), rounded to T, and
+// `sums` ([parts][I]) or, without parts, `db` gets the unrounded dz's sums over q, from the tiles at j = 0.
+struct AnyArgs {
+    Operand P, Q, Z;             // base null: zeros
+    Epilogue e;
+    long long I, nq, q_per_part;
+    int J, tiles_j, n_tiles, act;
+    bool p_along, q_along;       // staged along q (P and Z alike), or eight rows of one q
+    float* sums;
+    void* db;
+};
+
 // Any size, stride and alignment.  A thread stages eight consecutive elements of each side, the next step's while this one's
-// products run.  grid (workgroups, parts); workgroups walk over the tiles.  flags: only the tiles whose flag is set.
-// V: how many elements a load may take (the sides' rows and pointers allow it), 1 or 16 bytes of them.
-template <typename T, typename TO, int V>
-__global__ void __launch_bounds__(256) k_dense_any(Operand P, Operand Q, Epilogue e, long long I, int J, long long nq,
-                                                   long long q_per_part, int tiles_j, int n_tiles, const int* __restrict__ flags) {
+// products run.  V: 1, or 16 bytes of T: loads are 16 bytes wide (the sides' rows and pointers allow it).
+// T: what is multiplied, TY: what is written, TD: what dy and z are.
+template <typename T, typename TY, typename TD, int V, bool DZ>
+__device__ __forceinline__ void any_tiles(const AnyArgs& a, long long first, long long step, int part, const int* __restrict__ flags) {
     constexpr bool k16 = sizeof(T) == 2;
     constexpr int kPitch = k16 ? kBQ + 8 : kBQ + 1;
-    typedef typename vecn<T, V>::type vT;
     __shared__ __attribute__((aligned(16))) T Ps[kTile * kPitch];
     __shared__ __attribute__((aligned(16))) T Qs[kTile * kPitch];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 31, lk = lane >> 5;
-    const long long q_begin = (long long)blockIdx.y * q_per_part;
-    const long long q_end = q_begin + q_per_part < nq ? q_begin + q_per_part : nq;
+    const long long q_begin = (long long)part * a.q_per_part;
+    const long long q_end = q_begin + a.q_per_part < a.nq ? q_begin + a.q_per_part : a.nq;
     const int wi = (wave >> 1) * 32, wj = (wave & 1) * 32;
     // this thread's eight elements: of row r along q, or of contraction index q across rows
-    auto spot = [&](const Operand& o, int& r, int& q) {
-        r = o.qs == 1 ? threadIdx.x >> 2 : (threadIdx.x & 7) * 8;
-        q = o.qs == 1 ? (threadIdx.x & 3) * 8 : threadIdx.x >> 3;
+    auto spot = [&](bool along, int& r, int& q) {
+        r = along ? threadIdx.x >> 2 : (threadIdx.x & 7) * 8;
+        q = along ? (threadIdx.x & 3) * 8 : threadIdx.x >> 3;
     };
-    auto fetch = [&](T (&v)[8], const Operand& o, long long r0, long long rn, long long q0) {
+    auto fetch = [&](auto (&v)[8], const Operand& o, bool along, long long r0, long long rn, long long q0) {
+        typedef typename std::remove_reference<decltype(v[0])>::type U;
+        constexpr int VU = V > 1 ? 16 / sizeof(U) : 1;
+        typedef typename vecn<U, VU>::type vU;
         int r, q;
-        spot(o, r, q);
-        const bool along = o.qs == 1;
-        const T* at = (const T*)o.base + (r0 + r) * o.is + (q0 + q) * o.qs;
+        spot(along, r, q);
+        const U* at = (const U*)o.base + (r0 + r) * o.is + (q0 + q) * o.qs;
         // how many of the eight exist
-        const long long have = along ? (r0 + r < rn ? q_end - (q0 + q) : 0) : (q0 + q < q_end ? rn - (r0 + r) : 0);
+        const long long have = !o.base ? 0 : along ? (r0 + r < rn ? q_end - (q0 + q) : 0) : (q0 + q < q_end ? rn - (r0 + r) : 0);
         if (V > 1 && have >= 8) {
 #pragma unroll
-            for (int k = 0; k < 8; k += V) {
-                const vT t = *(const vT*)(at + k);
+            for (int k = 0; k < 8; k += VU) {
+                const vU t = *(const vU*)(at + k);
 #pragma unroll
-                for (int u = 0; u < V; ++u) v[k + u] = t[u];
+                for (int u = 0; u < VU; ++u) v[k + u] = t[u];
             }
         } else {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = k < have ? at[k] : (T)0.0f;
+            for (int k = 0; k < 8; ++k) v[k] = k < have ? at[k] : (U)0.0f;
         }
     };
-    auto deposit = [&](T* dst, const Operand& o, const T (&v)[8]) {
+    auto deposit = [&](T* dst, bool along, const T (&v)[8]) {
         int r, q;
-        spot(o, r, q);
-        const int step = o.qs == 1 ? 1 : kPitch;
+        spot(along, r, q);
+        const int across = along ? 1 : kPitch;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) dst[r * kPitch + q + k * step] = v[k];
+        for (int k = 0; k < 8; ++k) dst[r * kPitch + q + k * across] = v[k];
     };
-    for (long long tile = blockIdx.x; tile < n_tiles; tile += gridDim.x) {
+    for (long long tile = first; tile < a.n_tiles; tile += step) {
         if (flags && !flags[tile]) continue;                 // uniform over the workgroup
-        const long long i0 = tile / tiles_j * kTile;
-        const int j0 = (int)(tile % tiles_j) * kTile;
+        const long long i0 = tile / a.tiles_j * kTile;
+        const int j0 = (int)(tile % a.tiles_j) * kTile;
         f32x16 acc;
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[r] = 0.0f;
-        T pv[8], qv[8];
-        fetch(pv, P, i0, I, q_begin);
-        fetch(qv, Q, j0, J, q_begin);
+        TD pv[8], zv[8];
+        T qv[8];
+        float sum[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) sum[k] = 0.0f;
+        auto load = [&](long long q0) {
+            fetch(pv, a.P, a.p_along, i0, a.I, q0);
+            if (DZ && a.act != GL_ACT_NONE) fetch(zv, a.Z, a.p_along, i0, a.I, q0);
+            fetch(qv, a.Q, a.q_along, j0, a.J, q0);
+        };
+        load(q_begin);
         for (long long q0 = q_begin; q0 < q_end; q0 += kBQ) {
-            __syncthreads();
-            deposit(Ps, P, pv);
-            deposit(Qs, Q, qv);
-            __syncthreads();
-            if (q0 + kBQ < q_end) {
-                fetch(pv, P, i0, I, q0 + kBQ);
-                fetch(qv, Q, j0, J, q0 + kBQ);
+            T pt[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                if constexpr (DZ) {
+                    float d = gl_to_f32(pv[k]);
+                    if (a.act != GL_ACT_NONE) d *= gl_act_grad(gl_to_f32(zv[k]), a.act);
+                    sum[k] += d;
+                    pt[k] = (T)d;
+                } else {
+                    pt[k] = pv[k];
+                }
             }
+            __syncthreads();
+            deposit(Ps, a.p_along, pt);
+            deposit(Qs, a.q_along, qv);
+            __syncthreads();
+            if (q0 + kBQ < q_end) load(q0 + kBQ);
             if constexpr (k16) {
                 typedef typename vecn<T, 8>::type v8;
 #pragma unroll
                 for (int s = 0; s < kBQ; s += 16) {
-                    const v8 a = *(const v8*)(Qs + (wj + li) * kPitch + s + 8 * lk);
-                    const v8 b = *(const v8*)(Ps + (wi + li) * kPitch + s + 8 * lk);
+                    const v8 x = *(const v8*)(Qs + (wj + li) * kPitch + s + 8 * lk);
+                    const v8 y = *(const v8*)(Ps + (wi + li) * kPitch + s + 8 * lk);
                     if constexpr (__is_same(T, gl_bf16))
-                        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, acc, 0, 0, 0);
+                        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, acc, 0, 0, 0);
                     else
-                        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, acc, 0, 0, 0);
+                        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, y, acc, 0, 0, 0);
                 }
             } else {
 #pragma unroll
@@ -108,15 +140,91 @@ __global__ void __launch_bounds__(256) k_dense_any(Operand P, Operand Q, Epilogu
                                                                acc, 0, 0, 0);
             }
         }
+        if constexpr (DZ) {
+            if ((a.sums || a.db) && j0 == 0) {               // not p_along: thread = (8 rows, one of 32 indexes)
+                __shared__ float red[4][kTile];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    sum[k] += __shfl_xor(sum[k], 8);
+                    sum[k] += __shfl_xor(sum[k], 16);
+                    sum[k] += __shfl_xor(sum[k], 32);
+                }
+                __syncthreads();
+                if (lane < 8)
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) red[wave][lane * 8 + k] = sum[k];
+                __syncthreads();
+                const int c = threadIdx.x;
+                if (c < kTile && i0 + c < a.I) {
+                    const float s = (red[0][c] + red[1][c]) + (red[2][c] + red[3][c]);
+                    if (a.sums) a.sums[part * a.I + i0 + c] = s;
+                    else ((T*)a.db)[i0 + c] = (T)s;
+                }
+            }
+        }
         const long long i = i0 + wi + li;
-        if (i >= I) continue;
+        if (i >= a.I || !(a.e.partial || a.e.y)) continue;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             const int j = j0 + wj + (r & 3) + 8 * (r >> 2) + 4 * lk;
-            if (j >= J) continue;
-            if (e.partial) e.partial[((long long)blockIdx.y * I + i) * J + j] = acc[r];
-            else gl_finish<T, TO>(e, i, j, acc[r]);
+            if (j >= a.J) continue;
+            if (a.e.partial) a.e.partial[((long long)part * a.I + i) * a.J + j] = acc[r];
+            else gl_finish<T, TY>(a.e, i, j, acc[r]);
         }
+    }
+}
+
+// grid (workgroups, parts); workgroups walk over the tiles.  flags: only the tiles whose flag is set.
+template <typename T, typename TO, int V>
+__global__ void __launch_bounds__(256) k_dense_any(AnyArgs a, const int* __restrict__ flags) {
+    any_tiles<T, TO, T, V, false>(a, blockIdx.x, gridDim.x, blockIdx.y, flags);
+}
+
+// The gradients of a small layer in one launch: tiles (times parts) of dx, then of dweight, whose first ones sum dz for dbias.
+// dz is worked out from dy and z by every tile that reads it.
+template <typename T, typename TO, int V>
+__global__ void __launch_bounds__(256) k_dense_back_small(AnyArgs x, AnyArgs w, int x_blocks) {
+    const bool second = (int)blockIdx.x >= x_blocks;
+    const AnyArgs a = second ? w : x;
+    const int block = blockIdx.x - (second ? x_blocks : 0), part = block / a.n_tiles;
+    any_tiles<T, T, TO, V, true>(a, block - part * a.n_tiles, a.n_tiles, part, nullptr);
+}
+
+// Its join: elements of dx, then of dweight (where there are parts of them), then of dbias.  V divides `inputs`.
+struct BackJoin {
+    const float *x, *w, *d;              // parts
+    int x_parts, w_parts;
+    long long x_n, w_n;                  // elements of a part; 0: written already
+    void *dx, *dw, *db;
+    long long dx_stride, dw_stride;
+    int inputs, outputs;                 // outputs: of dbias to sum
+};
+template <typename T, int V>
+__global__ void __launch_bounds__(256) k_dense_back_join(BackJoin k) {
+    typedef typename vecn<float, V>::type vf;
+    const long long n = k.x_n + k.w_n + k.outputs;
+    for (long long at = ((long long)blockIdx.x * 256 + threadIdx.x) * V; at < n; at += (long long)gridDim.x * 256 * V) {
+        if (at >= k.x_n + k.w_n) {
+            const int c0 = (int)(at - k.x_n - k.w_n);
+            for (int c = c0; c < c0 + V && c < k.outputs; ++c) {
+                float s = 0.0f;
+#pragma unroll 8
+                for (int p = 0; p < k.w_parts; ++p) s += k.d[(long long)p * k.outputs + c];
+                ((T*)k.db)[c] = (T)s;
+            }
+            continue;
+        }
+        const bool second = at >= k.x_n;
+        const long long e = second ? at - k.x_n : at, part = second ? k.w_n : k.x_n;
+        const float* in = (second ? k.w : k.x) + e;
+        const int parts = second ? k.w_parts : k.x_parts;
+        vf s = *(const vf*)in;
+#pragma unroll 8
+        for (int p = 1; p < parts; ++p) s += *(const vf*)(in + p * part);
+        const long long i = e / k.inputs;
+        T* o = (T*)(second ? k.dw : k.dx) + i * (second ? k.dw_stride : k.dx_stride) + (e - i * k.inputs);
+#pragma unroll
+        for (int v = 0; v < V; ++v) o[v] = (T)s[v];
     }
 }
 
@@ -280,18 +388,21 @@ __global__ void __launch_bounds__(256) k_dense_dz(const TO* __restrict__ dy, lon
     }
 }
 
-// column sums over the parts; thread (column, one of 16 part lanes)
+// Column sums over the parts: grid (blocks of 16 columns), thread (column, one of 64 lanes over the parts)
 template <typename T>
 __global__ void __launch_bounds__(1024) k_dense_db(const float* __restrict__ parts, int n_parts, T* __restrict__ db, int N) {
-    __shared__ float s[16][64];
-    const int c = threadIdx.x & 63, r = threadIdx.x >> 6, n = blockIdx.x * 64 + c;
+    __shared__ float s[16][16];
+    const int c = threadIdx.x & 15, l = threadIdx.x >> 4, n = blockIdx.x * 16 + c;
     float a = 0.0f;
     if (n < N)
 #pragma unroll 8
-        for (int p = r; p < n_parts; p += 16) a += parts[(long long)p * N + n];
-    s[r][c] = a;
+        for (int p = l; p < n_parts; p += 64) a += parts[(long long)p * N + n];
+    a += __shfl_xor(a, 16);
+    a += __shfl_xor(a, 32);
+    if ((l & 3) == 0) s[l >> 2][c] = a;
     __syncthreads();
-    if (r || n >= N) return;
+    if (l || n >= N) return;
+    a = s[0][c];
 #pragma unroll
     for (int k = 1; k < 16; ++k) a += s[k][c];
     db[n] = (T)a;
@@ -309,7 +420,6 @@ int n_splits(long long I, int J, long long nq) {
     long long s = kCUs / tiles;
     const long long most = gl_ceil_div(nq, 4 * kBQ);
     if (s > most) s = most;
-    if (s > 16) s = 16;
     return s < 1 ? 1 : (int)s;
 }
 long long any_bytes(long long I, int J, long long nq) {
@@ -335,17 +445,30 @@ int any_product(const Operand& P, const Operand& Q, Epilogue e, long long I, int
     e.exact_p = nullptr;
     const bool wide = wide_loads<T>(P) && wide_loads<T>(Q);
     auto kernel = wide ? k_dense_any<T, TO, 16 / sizeof(T)> : k_dense_any<T, TO, 1>;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)tiles, (unsigned)used), dim3(256), 0, st, P, Q, e, I, J, nq, per,
-                       (int)gl_ceil_div(J, kTile), (int)tiles, (const int*)nullptr);
+    const AnyArgs a = {P, Q, {}, e, I, nq, per, J, (int)gl_ceil_div(J, kTile), (int)tiles, GL_ACT_NONE, P.qs == 1,
+                       Q.qs == 1, nullptr, nullptr};
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(tiles < kMostBlocks ? tiles : kMostBlocks), (unsigned)used), dim3(256), 0, st, a,
+                       (const int*)nullptr);
     GL_HIP_CHECK(hipGetLastError());
     return used > 1 ? gl_dense_join<T, TO>(e, I, J, (int)used, st) : 0;
 }
 
-// Products of fewer multiplications than this go to k_dense_any as they are where the tiles would need copies.
-constexpr double kCopyWork = 1 << 27;
-bool enough(long long rows, int inputs, int outputs) { return (double)rows * inputs * outputs >= kCopyWork; }
+// Layers of fewer multiplications than this go as they are to k_dense_any (forward, where the tiles would need copies) and
+// k_dense_back_small.  Microseconds there / on the tiles:
+//   float32, widths on 16 bytes   forward 2000 x 1024 -> 1024 58 / 61, 6888 x 1024 -> 512 90 / 87
+//                                 backward 2000 x 1024 -> 1024 122 / 153, 6888 x 1024 -> 512 240 / 179
+//   float32, others               forward 2000 x 501 -> 701 53 / 51, backward 641 x 512 -> 1025 79 / 84, 2000 x 501 -> 701 104 / 98
+//   16 bits forward               641 x 257 -> 513 18 / 18, 2000 x 501 -> 701 41 / 21
+//   16 bits backward              641 x 512 -> 512 29 / 38, 6888 x 80 -> 512 45 / 38
+double small_layer(int dtype, int inputs, int outputs, bool back) {
+    if (dtype == GL_F32) return inputs % 4 || outputs % 4 ? 1LL << 29 : 1LL << 31;
+    return back ? 3 << 26 : 1 << 27;
+}
+bool is_small(long long rows, int inputs, int outputs, int dtype, bool back) {
+    return (double)rows * inputs * outputs < small_layer(dtype, inputs, outputs, back);
+}
 int pad_to(int n) { return (n + 63) / 64 * 64; }
-bool copies(int dtype, int width, bool enough_) { return enough_ && (dtype == GL_F32 || width % 8 != 0); }
+bool copies(int dtype, int width) { return dtype == GL_F32 || width % 8 != 0; }
 long long copy_bytes(int dtype, long long rows, int cols) {
     return gl_align16(rows * pad_to(cols) * (dtype == GL_F32 ? 6LL : 2LL));
 }
@@ -430,8 +553,8 @@ struct FrontLayout {
 FrontLayout front_layout(long long rows, int inputs, int outputs, int dtype) {
     FrontLayout l = {};
     if (rows <= kFewRows) return l;
-    l.fast = enough(rows, inputs, outputs);
-    l.copy = copies(dtype, inputs, l.fast);
+    l.fast = !is_small(rows, inputs, outputs, dtype, false);
+    l.copy = l.fast && copies(dtype, inputs);
     if (l.copy) {
         l.x_bytes = copy_bytes(dtype, rows, inputs);
         l.w_bytes = copy_bytes(dtype, outputs, inputs);
@@ -480,30 +603,58 @@ int rows_per_part(long long rows, int outputs) {
     return (int)(r < 16 ? 16 : r);
 }
 
-// workspace: [dz (unless dy serves), or its planes] [with planes: dz itself, for sums that are not finite] [copy of x]
+// One product of k_dense_back_small: parts for one workgroup a CU, of two steps at least, or for two, of eight.
+struct SmallSplit {
+    long long tiles, per;
+    int parts;
+};
+SmallSplit small_split(long long I, int J, long long nq) {
+    SmallSplit s;
+    s.tiles = gl_ceil_div(I, kTile) * gl_ceil_div(J, kTile);
+    auto parts = [&](long long workgroups, int steps) {
+        const long long fill = workgroups / s.tiles, most = nq / (steps * kBQ);
+        return fill < most ? fill : most;
+    };
+    const long long one = parts(kCUs, 2), two = parts(2 * kCUs, 8), most = one > two ? one : two;
+    s.per = gl_ceil_div(gl_ceil_div(nq, most > 1 ? most : 1), kBQ) * kBQ;
+    s.parts = (int)gl_ceil_div(nq, s.per);
+    return s;
+}
+
+// workspace of a small layer: [parts of dx] [parts of dweight] [parts of dbias]; else
+// [dz (unless dy serves), or its planes] [with planes: dz itself, for sums that are not finite] [copy of x]
 // [copy of weight] [column-sum parts] [flags and parts of dx and dweight, one after the other on the stream: the larger]
 struct BackLayout {
-    bool fast, own_dz, copy, planes;
+    bool small, own_dz, copy, planes;
+    SmallSplit x, w;
     long long dz_stride, dz_bytes, dz32_bytes, x_bytes, w_bytes, parts_bytes, partial;
     long long total() const { return dz_bytes + dz32_bytes + x_bytes + w_bytes + parts_bytes + partial; }
 };
 BackLayout back_layout(long long rows, int inputs, int outputs, int dtype, int out_dtype, int act) {
     BackLayout l = {};
-    l.fast = enough(rows, inputs, outputs);
-    l.planes = dtype == GL_F32 && l.fast;
+    l.small = is_small(rows, inputs, outputs, dtype, true);
+    if (l.small) {
+        l.x = small_split(rows, inputs, outputs);
+        l.w = small_split(outputs, inputs, rows);
+        if (l.x.parts > 1) l.x_bytes = gl_align16(4LL * l.x.parts * rows * inputs);
+        if (l.w.parts > 1) l.w_bytes = gl_align16(4LL * l.w.parts * outputs * inputs);
+        if (l.w.parts > 1) l.parts_bytes = gl_align16(4LL * l.w.parts * outputs);
+        return l;
+    }
+    l.planes = dtype == GL_F32;
     // dy itself serves where nothing is to be multiplied, converted or padded
     l.own_dz = act != GL_ACT_NONE || dtype != out_dtype || (dtype != GL_F32 && outputs % 32) || l.planes;
     l.dz_stride = pad_to(outputs);
-    if (l.own_dz) l.dz_bytes = gl_align16(rows * l.dz_stride * (l.planes ? 6 : dtype == GL_F32 ? 4 : 2));
+    if (l.own_dz) l.dz_bytes = gl_align16(rows * l.dz_stride * (l.planes ? 6 : 2));
     if (l.planes && act != GL_ACT_NONE) l.dz32_bytes = gl_align16(rows * l.dz_stride * 4);
-    l.copy = copies(dtype, inputs, l.fast);
+    l.copy = copies(dtype, inputs);
     if (l.copy) {
         l.x_bytes = copy_bytes(dtype, rows, inputs);
         l.w_bytes = copy_bytes(dtype, outputs, inputs);
     }
     l.parts_bytes = gl_align16(gl_ceil_div(rows, rows_per_part(rows, outputs)) * outputs * 4);
-    const long long a = partial_bytes(dtype, rows, inputs, l.own_dz ? l.dz_stride : outputs, false, l.fast);
-    const long long b = partial_bytes(dtype, outputs, inputs, rows, true, l.fast);
+    const long long a = partial_bytes(dtype, rows, inputs, l.own_dz ? l.dz_stride : outputs, false, true);
+    const long long b = partial_bytes(dtype, outputs, inputs, rows, true, true);
     l.partial = a > b ? a : b;
     return l;
 }
@@ -529,6 +680,50 @@ int dz_pass(const void* dy, long long dy_stride, const void* z, long long z_stri
 }
 
 template <typename T, typename TO>
+int backward_small(const void* dy, long long dy_stride, const void* x, long long x_stride, const void* w, long long w_stride,
+                   const void* z, long long z_stride, void* dx, long long dx_stride, void* dw, long long dw_stride, void* db,
+                   long long rows, int inputs, int outputs, int act, const BackLayout& l, void* ws, hipStream_t st) {
+    char* at = (char*)ws;
+    AnyArgs a = {{dy, dy_stride, 1}, {w, 1, w_stride}, {z, z_stride, 1}, {}, rows, outputs, l.x.per, inputs,
+                 (int)gl_ceil_div(inputs, kTile), (int)l.x.tiles, act, true, false, nullptr, nullptr};
+    AnyArgs b = {{dy, 1, dy_stride}, {x, 1, x_stride}, {z, 1, z_stride}, {}, outputs, rows, l.w.per, inputs,
+                 (int)gl_ceil_div(inputs, kTile), (int)l.w.tiles, act, false, false, nullptr, nullptr};
+    a.e.y = dx;
+    a.e.y_stride = dx_stride;
+    b.e.y = dw;
+    b.e.y_stride = dw_stride;
+    if (!dw) {                           // sums of dz alone: one column of tiles
+        b.Q.base = nullptr;
+        b.tiles_j = 1;
+        b.n_tiles = (int)gl_ceil_div(outputs, kTile);
+    }
+    if (dx && l.x.parts > 1) a.e.partial = (float*)at;
+    if (dw && l.w.parts > 1) b.e.partial = (float*)(at + l.x_bytes);
+    if (db && l.w.parts > 1) b.sums = (float*)(at + l.x_bytes + l.w_bytes);
+    else b.db = db;
+    const long long x_blocks = dx ? l.x.tiles * l.x.parts : 0, w_blocks = dw || db ? (long long)b.n_tiles * l.w.parts : 0;
+    auto wide = [](const Operand& o, int size) {
+        return !o.base || ((uintptr_t)o.base % 16 == 0 && (o.qs == 1 ? o.is : o.qs) * size % 16 == 0);
+    };
+    const bool v = wide(a.P, sizeof(TO)) && (act == GL_ACT_NONE || wide(a.Z, sizeof(TO))) && (!dx || wide(a.Q, sizeof(T))) &&
+                   (!dw || wide(b.Q, sizeof(T)));
+    auto kernel = v ? k_dense_back_small<T, TO, 16 / sizeof(T)> : k_dense_back_small<T, TO, 1>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(x_blocks + w_blocks)), dim3(256), 0, st, a, b, (int)x_blocks);
+    GL_HIP_CHECK(hipGetLastError());
+    BackJoin j = {a.e.partial, b.e.partial, b.sums, l.x.parts, l.w.parts, a.e.partial ? rows * inputs : 0,
+                  b.e.partial ? (long long)outputs * inputs : 0, dx, dw, db, dx_stride, dw_stride, inputs, b.sums ? outputs : 0};
+    const long long n = j.x_n + j.w_n + j.outputs;
+    if (n == 0) return 0;
+    const int V = inputs % 4 == 0 ? 4 : 1;
+    const long long blocks = gl_ceil_div(n, 256 * V);
+    const dim3 grid((unsigned)(blocks < 4096 ? blocks : 4096));
+    if (V == 4) hipLaunchKernelGGL((k_dense_back_join<T, 4>), grid, dim3(256), 0, st, j);
+    else hipLaunchKernelGGL((k_dense_back_join<T, 1>), grid, dim3(256), 0, st, j);
+    GL_HIP_CHECK(hipGetLastError());
+    return 0;
+}
+
+template <typename T, typename TO>
 int backward(const void* dy, long long dy_stride, const void* x, long long x_stride, const void* w, long long w_stride,
              const void* z, long long z_stride, void* dx, long long dx_stride, void* dw, long long dw_stride, void* db,
              long long rows, int inputs, int outputs, int act, const BackLayout& l, void* ws, hipStream_t st) {
@@ -544,8 +739,7 @@ int backward(const void* dy, long long dy_stride, const void* x, long long x_str
     if (dz || db) {
         float* sums = db ? parts : nullptr;
         if constexpr (sizeof(T) == 4) {
-            if (l.planes) rc = dz_pass<T, TO, 3>(dy, dy_stride, z, z_stride, dz, l.dz_stride, sums, rows, outputs, act, st);
-            else rc = dz_pass<T, TO, 1>(dy, dy_stride, z, z_stride, dz, l.dz_stride, sums, rows, outputs, act, st);
+            rc = dz_pass<T, TO, 3>(dy, dy_stride, z, z_stride, dz, l.dz_stride, sums, rows, outputs, act, st);
             if (!rc && dz32) rc = dz_pass<T, TO, 1>(dy, dy_stride, z, z_stride, dz32, l.dz_stride, nullptr, rows, outputs, act, st);
         } else {
             rc = dz_pass<T, TO, 1>(dy, dy_stride, z, z_stride, dz, l.dz_stride, sums, rows, outputs, act, st);
@@ -553,7 +747,7 @@ int backward(const void* dy, long long dy_stride, const void* x, long long x_str
         if (rc) return rc;
     }
     if (db) {
-        hipLaunchKernelGGL((k_dense_db<T>), dim3((unsigned)gl_ceil_div(outputs, 64)), dim3(1024), 0, st, parts,
+        hipLaunchKernelGGL((k_dense_db<T>), dim3((unsigned)gl_ceil_div(outputs, 16)), dim3(1024), 0, st, parts,
                            (int)gl_ceil_div(rows, rows_per_part(rows, outputs)), (T*)db, outputs);
         GL_HIP_CHECK(hipGetLastError());
     }
@@ -571,7 +765,7 @@ int backward(const void* dy, long long dy_stride, const void* x, long long x_str
         if (rc) return rc;
         e.y = dx;
         e.y_stride = dx_stride;
-        rc = product<T, T>({d, d_stride, 1, plane, padded}, Q, {d0, d0_stride, 1}, Q0, e, rows, inputs, outputs, partial, l.fast, st);
+        rc = product<T, T>({d, d_stride, 1, plane, padded}, Q, {d0, d0_stride, 1}, Q0, e, rows, inputs, outputs, partial, true, st);
         if (rc) return rc;
     }
     if (dw) {
@@ -581,7 +775,7 @@ int backward(const void* dy, long long dy_stride, const void* x, long long x_str
         if (rc) return rc;
         e.y = dw;
         e.y_stride = dw_stride;
-        rc = product<T, T>({d, 1, d_stride, plane, padded}, Q, {d0, 1, d0_stride}, Q0, e, outputs, inputs, rows, partial, l.fast, st);
+        rc = product<T, T>({d, 1, d_stride, plane, padded}, Q, {d0, 1, d0_stride}, Q0, e, outputs, inputs, rows, partial, true, st);
     }
     return rc;
 }
@@ -608,9 +802,9 @@ int gl_dense_flagged(const gl_epilogue& e, long long I, int J, long long nq, hip
     const long long tiles = gl_ceil_div(I, kTile) * gl_ceil_div(J, kTile);
     gl_epilogue f = e;
     f.partial = nullptr;
-    hipLaunchKernelGGL((k_dense_any<float, float, 1>), dim3((unsigned)(tiles < 512 ? tiles : 512)), dim3(256), 0, st,
-                       Operand{e.exact_p, e.exact_p_is, e.exact_p_qs}, Operand{e.exact_q, e.exact_q_is, e.exact_q_qs}, f, I, J, nq, nq,
-                       (int)gl_ceil_div(J, kTile), (int)tiles, e.flags);
+    const AnyArgs a = {{e.exact_p, e.exact_p_is, e.exact_p_qs}, {e.exact_q, e.exact_q_is, e.exact_q_qs}, {}, f, I, nq, nq, J,
+                       (int)gl_ceil_div(J, kTile), (int)tiles, GL_ACT_NONE, e.exact_p_qs == 1, e.exact_q_qs == 1, nullptr, nullptr};
+    hipLaunchKernelGGL((k_dense_any<float, float, 1>), dim3((unsigned)(tiles < 512 ? tiles : 512)), dim3(256), 0, st, a, e.flags);
     GL_HIP_CHECK(hipGetLastError());
     return 0;
 }
@@ -760,8 +954,8 @@ int gl_dense_backward(const void* dy, long long dy_stride, const void* x, long l
     if (!rc) rc = check_workspace(workspace, workspace_bytes, l.total(), "gl_dense_backward");
     if (rc) return rc;
 #define GL_BACK(T, TO)                                                                                                    \
-    backward<T, TO>(dy, dy_stride, x, x_stride, weight, w_stride, preactivation, z_stride, dx, dx_stride, dweight,        \
-                    dw_stride, dbias, rows, inputs, outputs, activation, l, workspace, st)
+    (l.small ? backward_small<T, TO> : backward<T, TO>)(dy, dy_stride, x, x_stride, weight, w_stride, preactivation,      \
+        z_stride, dx, dx_stride, dweight, dw_stride, dbias, rows, inputs, outputs, activation, l, workspace, st)
     if (dtype == GL_F32) return GL_BACK(float, float);
     if (dtype == GL_BF16) return out_dtype == GL_F32 ? GL_BACK(gl_bf16, float) : GL_BACK(gl_bf16, gl_bf16);
     return out_dtype == GL_F32 ? GL_BACK(gl_f16, float) : GL_BACK(gl_f16, gl_f16);

@@ -255,7 +255,8 @@ def test_dense_backward_strides(M, K, N, name, dtype):
 
 
 # sizes whose tiles fill the chip: the walking kernel (both sides' layouts), a rest of columns, odd and short contractions
-LARGE_SIZES = [(4400, 512, 2048), (33000, 96, 257), (16500, 544, 512), (40000, 32, 256), (33001, 72, 256), (70000, 64, 264), (65500, 64, 256)]
+LARGE_SIZES = [(4400, 512, 2048), (33000, 96, 257), (16500, 544, 512), (40000, 32, 256), (33001, 72, 256), (70000, 64, 264), (65500, 64, 256),
+               (33000, 130, 600)]
 
 
 @gpu
@@ -288,6 +289,61 @@ def test_dense_backward_many_rows(M, K, N, dtype, out_dtype, name):
         close(g, v.cpu(), t.cpu(), what)
     again = inv.dense_backward(dy, x, w, z if name else None, activation=name)
     assert all(torch.equal(a, c) for a, c in zip(got, again))
+
+
+@gpu
+def test_dense_full_precision_values_that_are_not_finite():
+    """Large float32 products run on 16-bit planes: what those cannot hold has to come out as float32 has it."""
+    M, K, N = 4400, 512, 2048
+    x, w = randn((M, K), F32, 1).cuda(), randn((N, K), F32, 2, K ** -0.5).abs().cuda()
+    z64, z_tol, _, _ = dense64(x, w, None, None, None, F32)
+    x[3, 5], x[2000, 100], x[M - 1, K - 1] = float("inf"), float("nan"), -float("inf")
+    y = inv.dense(x, w)
+    assert (y[3] == float("inf")).all() and y[2000].isnan().all() and (y[M - 1] == -float("inf")).all()
+    rest = torch.ones(M, dtype=torch.bool, device="cuda")
+    rest[[3, 2000, M - 1]] = False
+    close(y[rest], z64[rest].cpu(), z_tol[rest].cpu(), "the other rows")
+    x = randn((M, K), F32, 1).cuda()
+    x[50], x[51], x[4000] = 0.0, 0.0, 0.0
+    x[50, 7], x[51, 8], x[4000, 9] = 3.4e38, -torch.finfo(F32).max, 1e-30        # the first two round up to infinity in 16 bits
+    z64, z_tol, _, _ = dense64(x, w, None, None, None, F32)
+    close(inv.dense(x, w), z64.cpu(), z_tol.cpu(), "product")
+
+
+@gpu
+def test_dense_backward_full_precision_values_that_are_not_finite():
+    M, K, N = 16500, 512, 264                                                  # dweight: parts of the frames, joined
+    x, w, dy = randn((M, K), F32, 1).cuda(), randn((N, K), F32, 2).cuda(), randn((M, N), F32, 3).cuda()
+    want = dense_back64(dy, x, w, None, None, F32)
+    dy[7, 3], dy[16000, 200] = float("inf"), float("nan")
+    dx, dw, db = inv.dense_backward(dy, x, w)
+    assert torch.equal(dx[7], float("inf") * w[3]) and dx[16000].isnan().all()
+    assert torch.equal(dw[3], float("inf") * x[7]) and dw[200].isnan().all()
+    assert db[3] == float("inf") and db[200].isnan()
+    for got, (v, t), gone, what in ((dx, want[0], (7, 16000), "dx"), (dw, want[1], (3, 200), "dweight"), (db, want[2], (3, 200), "dbias")):
+        rest = torch.ones(got.shape[0], dtype=torch.bool, device="cuda")
+        rest[list(gone)] = False
+        close(got[rest], v[rest].cpu(), t[rest].cpu(), what)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("M,K,N", [(70, 1, 1), (70, 1, 3), (70, 5, 1), (1, 1, 9), (1, 9, 1), (200, 2, 130)])
+@pytest.mark.parametrize("apart", [0, 4])
+def test_dense_backward_narrow(M, K, N, apart, dtype):
+    """One column, next to each other or a stride apart: which direction is contiguous does not show in the strides."""
+    def view(t, more):
+        wide = torch.full((t.shape[0], t.shape[1] + more), float("nan"), dtype=t.dtype, device="cuda")
+        wide[:, :t.shape[1]] = t.cuda()
+        return wide[:, :t.shape[1]]
+
+    x, w = randn((M, K), dtype, 1), randn((N, K), dtype, 2)
+    z, dy = randn((M, N), dtype, 3), randn((M, N), dtype, 4)
+    want = dense_back64(dy, x, w, z, "silu", dtype)
+    for mix in ((0, apart), (apart, 0), (apart, apart)):
+        got = inv.dense_backward(view(dy, mix[0]), view(x, mix[1]), view(w, mix[0]), view(z, mix[1]), activation="silu")
+        for g, (v, t), what in zip(got, want, ("dx", "dweight", "dbias")):
+            close(g, v, t, what)
 
 
 @gpu
