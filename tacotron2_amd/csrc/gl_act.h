@@ -32,7 +32,8 @@ __device__ __forceinline__ float gl_phi_poly(float a, float& t) {
     return fmaf(p, t, 0.254829592f * 0.5f);
 }
 
-// act(z).  Every branch on `act` is uniform: a kernel argument or a template constant.
+// act(z).  Every branch on `act` is uniform: a kernel argument or a template constant.  For many values at once take
+// gl_with_act around the loop: a branch a value scatters the code that runs over all activations of all values.
 __device__ __forceinline__ float gl_act(float z, int act) {
     switch (act) {
         case GL_ACT_RELU: return z < 0.0f ? 0.0f : z;                  // NaN stays NaN
@@ -76,5 +77,18 @@ __device__ __forceinline__ float gl_act_grad(float z, int act) {
         }
         case GL_ACT_EXP: return gl_exp(z);
         default: return 1.0f;
+    }
+}
+
+// f(gl_int<the activation>)
+template <typename F>
+__device__ __forceinline__ void gl_with_act(int act, F f) {
+    switch (act) {
+        case GL_ACT_RELU: f(gl_int<GL_ACT_RELU>()); break;
+        case GL_ACT_SILU: f(gl_int<GL_ACT_SILU>()); break;
+        case GL_ACT_GELU: f(gl_int<GL_ACT_GELU>()); break;
+        case GL_ACT_TANH: f(gl_int<GL_ACT_TANH>()); break;
+        case GL_ACT_EXP: f(gl_int<GL_ACT_EXP>()); break;
+        default: f(gl_int<GL_ACT_NONE>());
     }
 }

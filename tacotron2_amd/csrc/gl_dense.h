@@ -20,6 +20,7 @@ struct gl_epilogue {
     void* z;                     // of TO or null
     long long z_stride;
     int act;
+    bool quads;                  // k_dense_any: four columns of y, z and residual lie on whole vectors
     float* partial;              // [parts][I][J]: sums of one part of the contraction, finished by k_dense_join
     // float32 through planes: the operands themselves, for the sums that are not finite, and the flags of their blocks
     const float *exact_p, *exact_q;

@@ -18,6 +18,7 @@
 
 namespace {
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 template <typename T, int N> struct vecn { typedef T type __attribute__((ext_vector_type(N))); };
 typedef gl_operand Operand;
@@ -40,8 +41,8 @@ struct AnyArgs {
     void* db;
 };
 
-// Any size, stride and alignment.  A thread stages eight consecutive elements of each side, the next step's while this one's
-// products run.  V: 1, or 16 bytes of T: loads are 16 bytes wide (the sides' rows and pointers allow it).
+// Any size, stride and alignment.  A thread stages eight consecutive elements of each side, two steps ahead of the
+// products.  V: 1, or 16 bytes of T: loads are 16 bytes wide (the sides' pointers, strides and sizes allow it).
 // T: what is multiplied, TY: what is written, TD: what dy and z are.
 template <typename T, typename TY, typename TD, int V, bool DZ>
 __device__ __forceinline__ void any_tiles(const AnyArgs& a, long long first, long long step, int part, const int* __restrict__ flags) {
@@ -58,26 +59,26 @@ __device__ __forceinline__ void any_tiles(const AnyArgs& a, long long first, lon
         r = along ? threadIdx.x >> 2 : (threadIdx.x & 7) * 8;
         q = along ? (threadIdx.x & 3) * 8 : threadIdx.x >> 3;
     };
-    auto fetch = [&](auto (&v)[8], const Operand& o, bool along, long long r0, long long rn, long long q0) {
+    // Loads them and says how many exist.  No branch around a load: one would have to wait for it.
+    auto fetch = [&](auto (&v)[8], const Operand& o, bool along, long long r0, long long rn, long long q0) -> int {
         typedef typename std::remove_reference<decltype(v[0])>::type U;
         constexpr int VU = V > 1 ? 16 / sizeof(U) : 1;
         typedef typename vecn<U, VU>::type vU;
         int r, q;
         spot(along, r, q);
         const U* at = (const U*)o.base + (r0 + r) * o.is + (q0 + q) * o.qs;
-        // how many of the eight exist
-        const long long have = !o.base ? 0 : along ? (r0 + r < rn ? q_end - (q0 + q) : 0) : (q0 + q < q_end ? rn - (r0 + r) : 0);
-        if (V > 1 && have >= 8) {
+        const long long left = along ? (r0 + r < rn ? q_end - (q0 + q) : 0) : (q0 + q < q_end ? rn - (r0 + r) : 0);
+        const int have = (int)min(max(left, 0LL), 8LL);
 #pragma unroll
-            for (int k = 0; k < 8; k += VU) {
-                const vU t = *(const vU*)(at + k);
+        for (int k = 0; k < 8; k += VU) {
+            const vU t = *(const vU*)(k < have ? at + k : (const U*)o.base);
 #pragma unroll
-                for (int u = 0; u < VU; ++u) v[k + u] = t[u];
+            for (int u = 0; u < VU; ++u) {
+                if constexpr (VU == 1) v[k] = t[0];
+                else v[k + u] = t[u];
             }
-        } else {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = k < have ? at[k] : (U)0.0f;
         }
+        return have;
     };
     auto deposit = [&](T* dst, bool along, const T (&v)[8]) {
         int r, q;
@@ -93,35 +94,55 @@ __device__ __forceinline__ void any_tiles(const AnyArgs& a, long long first, lon
         f32x16 acc;
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[r] = 0.0f;
-        TD pv[8], zv[8];
-        T qv[8];
+        float bias[16];                                      // arrives under the products
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int j = j0 + wj + (r & 3) + 8 * (r >> 2) + 4 * lk;
+            bias[r] = !DZ && a.e.bias && !a.e.partial && j < a.J ? gl_to_f32(((const T*)a.e.bias)[j]) : 0.0f;
+        }
+        struct Staged {
+            TD p[8], z[8];
+            T q[8];
+            int p_have, q_have;
+        };
         float sum[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) sum[k] = 0.0f;
-        auto load = [&](long long q0) {
-            fetch(pv, a.P, a.p_along, i0, a.I, q0);
-            if (DZ && a.act != GL_ACT_NONE) fetch(zv, a.Z, a.p_along, i0, a.I, q0);
-            fetch(qv, a.Q, a.q_along, j0, a.J, q0);
+        auto load = [&](Staged& t, long long q0) {
+            if (q0 >= q_end) return;                         // uniform, as all conditions outside of fetch
+            t.p_have = fetch(t.p, a.P, a.p_along, i0, a.I, q0);
+            if (DZ && a.act != GL_ACT_NONE) fetch(t.z, a.Z, a.p_along, i0, a.I, q0);
+            t.q_have = a.Q.base ? fetch(t.q, a.Q, a.q_along, j0, a.J, q0) : 0;
         };
-        load(q_begin);
-        for (long long q0 = q_begin; q0 < q_end; q0 += kBQ) {
+        auto multiply = [&](Staged& t, long long q0) {
+            if (q0 >= q_end) return;
             T pt[8];
+            if constexpr (DZ) {
+                float d[8];
+                gl_with_act(a.act, [&](auto act) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                if constexpr (DZ) {
-                    float d = gl_to_f32(pv[k]);
-                    if (a.act != GL_ACT_NONE) d *= gl_act_grad(gl_to_f32(zv[k]), a.act);
-                    sum[k] += d;
-                    pt[k] = (T)d;
-                } else {
-                    pt[k] = pv[k];
+                    for (int k = 0; k < 8; ++k) {
+                        d[k] = gl_to_f32(t.p[k]);
+                        if constexpr (decltype(act)::value != GL_ACT_NONE) d[k] *= gl_act_grad(gl_to_f32(t.z[k]), decltype(act)::value);
+                    }
+                });
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    d[k] = k < t.p_have ? d[k] : 0.0f;
+                    sum[k] += d[k];
+                    pt[k] = (T)d[k];
                 }
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) pt[k] = k < t.p_have ? t.p[k] : (T)0.0f;
             }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) t.q[k] = k < t.q_have ? t.q[k] : (T)0.0f;
             __syncthreads();
             deposit(Ps, a.p_along, pt);
-            deposit(Qs, a.q_along, qv);
+            deposit(Qs, a.q_along, t.q);
             __syncthreads();
-            if (q0 + kBQ < q_end) load(q0 + kBQ);
+            load(t, q0 + 2 * kBQ);
             if constexpr (k16) {
                 typedef typename vecn<T, 8>::type v8;
 #pragma unroll
@@ -139,6 +160,13 @@ __device__ __forceinline__ void any_tiles(const AnyArgs& a, long long first, lon
                     acc = __builtin_amdgcn_mfma_f32_32x32x2f32(Qs[(wj + li) * kPitch + s + lk], Ps[(wi + li) * kPitch + s + lk],
                                                                acc, 0, 0, 0);
             }
+        };
+        Staged even, odd;
+        load(even, q_begin);
+        load(odd, q_begin + kBQ);
+        for (long long q0 = q_begin; q0 < q_end; q0 += 2 * kBQ) {
+            multiply(even, q0);
+            multiply(odd, q0 + kBQ);
         }
         if constexpr (DZ) {
             if ((a.sums || a.db) && j0 == 0) {               // not p_along: thread = (8 rows, one of 32 indexes)
@@ -164,13 +192,51 @@ __device__ __forceinline__ void any_tiles(const AnyArgs& a, long long first, lon
         }
         const long long i = i0 + wi + li;
         if (i >= a.I || !(a.e.partial || a.e.y)) continue;
+        const Epilogue& e = a.e;
+        typedef typename vecn<TY, 4>::type v4;
+        // four columns next to each other: f(first column, how many exist, the sums)
+        auto quads = [&](auto f) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const int j = j0 + wj + (r & 3) + 8 * (r >> 2) + 4 * lk;
-            if (j >= a.J) continue;
-            if (a.e.partial) a.e.partial[((long long)part * a.I + i) * a.J + j] = acc[r];
-            else gl_finish<T, TY>(a.e, i, j, acc[r]);
+            for (int g = 0; g < 4; ++g) {
+                const int j = j0 + wj + 8 * g + 4 * lk;
+                if (j < a.J) f(j, min(a.J - j, 4), 4 * g);
+            }
+        };
+        auto put = [&](TY* o, int n, int r) {
+            v4 t;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) t[k] = (TY)acc[r + k];
+            if (e.quads) *(v4*)o = t;
+            else
+                for (int k = 0; k < n; ++k) o[k] = t[k];
+        };
+        if (e.partial) {
+            quads([&](int j, int n, int r) {
+                float* o = e.partial + ((long long)part * a.I + i) * a.J + j;
+                if (a.J % 4 == 0) *(f32x4*)o = f32x4{acc[r], acc[r + 1], acc[r + 2], acc[r + 3]};
+                else
+                    for (int k = 0; k < n; ++k) o[k] = acc[r + k];
+            });
+            continue;
         }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[r] += bias[r];
+        if (e.z) quads([&](int j, int n, int r) { put((TY*)e.z + i * e.z_stride + j, n, r); });
+        gl_with_act(e.act, [&](auto act) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[r] = gl_act(acc[r], decltype(act)::value);
+        });
+        if (e.residual)
+            quads([&](int j, int n, int r) {
+                const TY* from = (const TY*)e.residual + i * e.r_stride + j;
+                v4 t = v4{};
+                if (e.quads) t = *(const v4*)from;
+                else
+                    for (int k = 0; k < n; ++k) t[k] = from[k];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) acc[r + k] += gl_to_f32(t[k]);
+            });
+        quads([&](int j, int n, int r) { put((TY*)e.y + i * e.y_stride + j, n, r); });
     }
 }
 
@@ -340,7 +406,8 @@ __global__ void __launch_bounds__(256) k_dense_dz(const TO* __restrict__ dy, lon
     float sum[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) sum[v] = 0.0f;
-    if (real || (dz_ && n < dz_stride))
+    auto frames = [&](auto act) {
+        constexpr int ACT = decltype(act)::value;
 #pragma unroll 2
         for (long long i = r0 + r; i < r1; i += 4) {
             float d[V];
@@ -349,11 +416,11 @@ __global__ void __launch_bounds__(256) k_dense_dz(const TO* __restrict__ dy, lon
             if (real) {
                 const vI g = *(const vI*)(dy + i * dy_stride + n);
                 vI zz = vI{};
-                if (act != GL_ACT_NONE) zz = *(const vI*)(z + i * z_stride + n);
+                if constexpr (ACT != GL_ACT_NONE) zz = *(const vI*)(z + i * z_stride + n);
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
                     d[v] = gl_to_f32(g[v]);
-                    if (act != GL_ACT_NONE) d[v] *= gl_act_grad(gl_to_f32(zz[v]), act);
+                    if constexpr (ACT != GL_ACT_NONE) d[v] *= gl_act_grad(gl_to_f32(zz[v]), ACT);
                     sum[v] += d[v];
                 }
             }
@@ -378,6 +445,8 @@ __global__ void __launch_bounds__(256) k_dense_dz(const TO* __restrict__ dy, lon
                 *(typename vecn<gl_bf16, V>::type*)(o + 2 * plane) = l;
             }
         }
+    };
+    if (real || (dz_ && n < dz_stride)) gl_with_act(act, frames);
     if (!parts) return;
 #pragma unroll
     for (int v = 0; v < V; ++v) s[r][c * V + v] = sum[v];
@@ -427,11 +496,17 @@ long long any_bytes(long long I, int J, long long nq) {
     return s > 1 ? gl_align16((long long)s * I * J * 4) : 0;
 }
 
-// 16-byte loads: rows on 16 bytes (eight elements from a multiple of eight on)
-template <typename T>
-bool wide_loads(const Operand& o) {
+// 16-byte loads: pointer, rows and their length on 16 bytes.  length: of the contiguous direction
+bool wide_loads(const Operand& o, long long length, int size) {
     const long long stride = o.qs == 1 ? o.is : o.qs;
-    return (uintptr_t)o.base % 16 == 0 && stride * sizeof(T) % 16 == 0;
+    return !o.base || ((uintptr_t)o.base % 16 == 0 && stride * size % 16 == 0 && length * size % 16 == 0);
+}
+
+// Whether four columns of every array of results can be moved at once.
+template <typename TO>
+bool quads(const Epilogue& e, int J) {
+    auto whole = [](const void* p, long long stride) { return !p || ((uintptr_t)p % (4 * sizeof(TO)) == 0 && stride % 4 == 0); };
+    return J % 4 == 0 && whole(e.y, e.y_stride) && whole(e.z, e.z_stride) && whole(e.residual, e.r_stride);
 }
 
 template <typename T, typename TO>
@@ -443,7 +518,8 @@ int any_product(const Operand& P, const Operand& Q, Epilogue e, long long I, int
     if (tiles > 0x7fffffffLL) return gl_set_error(GL_ERR_INVALID, "gl_dense: %lld tiles are too many for one launch", tiles);
     e.partial = used > 1 ? partial : nullptr;
     e.exact_p = nullptr;
-    const bool wide = wide_loads<T>(P) && wide_loads<T>(Q);
+    e.quads = quads<TO>(e, J);
+    const bool wide = wide_loads(P, P.qs == 1 ? nq : I, sizeof(T)) && wide_loads(Q, Q.qs == 1 ? nq : J, sizeof(T));
     auto kernel = wide ? k_dense_any<T, TO, 16 / sizeof(T)> : k_dense_any<T, TO, 1>;
     const AnyArgs a = {P, Q, {}, e, I, nq, per, J, (int)gl_ceil_div(J, kTile), (int)tiles, GL_ACT_NONE, P.qs == 1,
                        Q.qs == 1, nullptr, nullptr};
@@ -697,16 +773,15 @@ int backward_small(const void* dy, long long dy_stride, const void* x, long long
         b.tiles_j = 1;
         b.n_tiles = (int)gl_ceil_div(outputs, kTile);
     }
+    a.e.quads = quads<T>(a.e, inputs);
+    b.e.quads = quads<T>(b.e, inputs);
     if (dx && l.x.parts > 1) a.e.partial = (float*)at;
     if (dw && l.w.parts > 1) b.e.partial = (float*)(at + l.x_bytes);
     if (db && l.w.parts > 1) b.sums = (float*)(at + l.x_bytes + l.w_bytes);
     else b.db = db;
     const long long x_blocks = dx ? l.x.tiles * l.x.parts : 0, w_blocks = dw || db ? (long long)b.n_tiles * l.w.parts : 0;
-    auto wide = [](const Operand& o, int size) {
-        return !o.base || ((uintptr_t)o.base % 16 == 0 && (o.qs == 1 ? o.is : o.qs) * size % 16 == 0);
-    };
-    const bool v = wide(a.P, sizeof(TO)) && (act == GL_ACT_NONE || wide(a.Z, sizeof(TO))) && (!dx || wide(a.Q, sizeof(T))) &&
-                   (!dw || wide(b.Q, sizeof(T)));
+    const bool v = wide_loads(a.P, outputs, sizeof(TO)) && (act == GL_ACT_NONE || wide_loads(a.Z, outputs, sizeof(TO))) &&
+                   (!dx || wide_loads(a.Q, inputs, sizeof(T))) && (!dw || wide_loads(b.Q, inputs, sizeof(T)));
     auto kernel = v ? k_dense_back_small<T, TO, 16 / sizeof(T)> : k_dense_back_small<T, TO, 1>;
     hipLaunchKernelGGL(kernel, dim3((unsigned)(x_blocks + w_blocks)), dim3(256), 0, st, a, b, (int)x_blocks);
     GL_HIP_CHECK(hipGetLastError());
@@ -802,6 +877,7 @@ int gl_dense_flagged(const gl_epilogue& e, long long I, int J, long long nq, hip
     const long long tiles = gl_ceil_div(I, kTile) * gl_ceil_div(J, kTile);
     gl_epilogue f = e;
     f.partial = nullptr;
+    f.quads = quads<float>(e, J);
     const AnyArgs a = {{e.exact_p, e.exact_p_is, e.exact_p_qs}, {e.exact_q, e.exact_q_is, e.exact_q_qs}, {}, f, I, nq, nq, J,
                        (int)gl_ceil_div(J, kTile), (int)tiles, GL_ACT_NONE, e.exact_p_qs == 1, e.exact_q_qs == 1, nullptr, nullptr};
     hipLaunchKernelGGL((k_dense_any<float, float, 1>), dim3((unsigned)(tiles < 512 ? tiles : 512)), dim3(256), 0, st, a, e.flags);

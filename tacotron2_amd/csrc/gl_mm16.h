@@ -331,14 +331,18 @@ __device__ __forceinline__ int epilogue(const Out& o, f32x4 (&acc)[MI][NI], long
                                         int part, int lane) {
     const int il = lane & 15, g4 = lane >> 4;
     if (EXTRA && o.z) put_block<TO, TAIL, LINES, MI, NI>((TO*)o.z, o.z_stride, acc, i0, j0, I, J, lane, o.odd);
+    auto activate = [&](auto act) {
 #pragma unroll
-    for (int m = 0; m < MI; ++m)
+        for (int m = 0; m < MI; ++m)
 #pragma unroll
-        for (int n = 0; n < NI; ++n) {
+            for (int n = 0; n < NI; ++n) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) acc[m][n][r] = gl_act(acc[m][n][r], ACT < 0 ? o.act : ACT);
-            if (n & 1) __builtin_amdgcn_sched_barrier(0);    // keeps the block's temporaries few
-        }
+                for (int r = 0; r < 4; ++r) acc[m][n][r] = gl_act(acc[m][n][r], decltype(act)::value);
+                if (n & 1) __builtin_amdgcn_sched_barrier(0);    // keeps the block's temporaries few
+            }
+    };
+    if constexpr (ACT < 0) gl_with_act(o.act, activate);
+    else activate(gl_int<ACT>());
     if (EXTRA && o.residual) {
         const __amdgpu_buffer_rsrc_t rs = block_of<TO, MI, NI>(o.residual, o.r_stride, i0, j0, I, J);
         const int stride_b = (int)o.r_stride * (int)sizeof(TO);

@@ -90,7 +90,7 @@ def _rows(t):
 def _copy(t):
     if raw_capture_active():
         raise RuntimeError("inside Plan.capture() nothing may be copied: pass inputs with contiguous rows at one stride")
-    return t.contiguous()
+    return t.detach().contiguous()
 
 
 def _vector(t):
@@ -144,14 +144,16 @@ def _bytes_of(query, *args):
     return _lib.check(getattr(_lib.lib(), query)(*args), query)
 
 
-def _scratch(workspace, need, device):
+def _scratch(workspace, need, device, *others):
+    """(workspace, its bytes): new, or the caller's, which none of the other tensors may reach into."""
     if need == 0:
         return None, 0
     if workspace is None:
-        workspace = _new((need,), torch.uint8, device, "workspace")
-    elif not isinstance(workspace, torch.Tensor) or workspace.dtype != torch.uint8 or workspace.device != device \
+        return _new((need,), torch.uint8, device, "workspace"), need
+    if not isinstance(workspace, torch.Tensor) or workspace.dtype != torch.uint8 or workspace.device != device \
             or not workspace.is_contiguous() or workspace.numel() < need or workspace.data_ptr() % 16:
         raise ValueError(f"workspace must be a contiguous, 16-byte aligned uint8 tensor of at least {need} bytes on {device}")
+    _apart(workspace, "workspace", [("an input or an output", t) for t in others])
     return workspace, workspace.numel()
 
 
@@ -240,7 +242,8 @@ def _dense(x, weight, bias, act, residual, out_dtype, out, preactivation, worksp
     if bias is not None:
         bias = _vector(bias)
     d, od = _DTYPES[x.dtype], _DTYPES[out_dtype]
-    ws, ws_bytes = _scratch(workspace, _bytes_of("gl_dense_workspace", rows, K, N, d, od), device)
+    ws, ws_bytes = _scratch(workspace, _bytes_of("gl_dense_workspace", rows, K, N, d, od), device, x, weight, bias,
+                            residual, y, z)
     with _on(device):
         _lib.check(_lib.lib().gl_dense(_p(x), x_stride, _p(weight), w_stride, _p(bias), _p(residual), r_stride, _p(y),
                                        y_stride, _p(z), z_stride, rows, K, N, d, od, act, _p(ws), ws_bytes,
@@ -285,55 +288,57 @@ def dense(x, weight, bias=None, *, activation=None, residual=None, out_dtype=Non
     return _dense(x, weight, bias, act, residual, out_dtype, out, preactivation, workspace)
 
 
+def _apart_from_all(outs, made, inputs, same=()):
+    """_apart for the caller's own gradients; made, inputs: (name, tensor)."""
+    for k, (name, t) in enumerate(made):
+        if t is not None and any(o is t for o in outs):
+            _apart(t, name, inputs + made[:k], same if k == 0 else ())
+
+
 def _dense_backward(dy, x, weight, z, act, need, outs, workspace):
     _tensor(x, "x")
-    if not isinstance(weight, torch.Tensor) or weight.dim() != 2:
-        raise ValueError("weight must be (outputs, inputs)")
-    _tensor(weight, "weight", x.device, x.dtype, (weight.shape[0], x.shape[-1]))
-    if weight.numel() == 0:
+    if x.dim() < 1 or not isinstance(weight, torch.Tensor) or weight.dim() != 2:
+        raise ValueError("x must be (..., inputs) and weight (outputs, inputs)")
+    dtype, device, width = x.dtype, x.device, weight.shape
+    N, K = width
+    _tensor(weight, "weight", device, dtype, (N, x.shape[-1]))
+    if N == 0 or K == 0:
         raise ValueError("weight has no elements")
-    shape = tuple(x.shape[:-1]) + (weight.shape[0],)
-    _tensor(dy, "dy", x.device, None, shape)
-    if dy.dtype not in (x.dtype, torch.float32):
-        raise ValueError(f"dy must be {x.dtype} or float32, got {dy.dtype}")
+    shape = x.shape[:-1] + width[:1]
+    dy_dtype = torch.float32 if isinstance(dy, torch.Tensor) and dy.dtype is torch.float32 else dtype
+    _tensor(dy, "dy", device, dy_dtype, shape)
+    z_stride = dx_stride = dw_stride = 0
     if act:
         if z is None:
             raise ValueError("dense_backward needs the preactivation of an activation's forward pass")
-        _tensor(z, "preactivation", x.device, dy.dtype, shape)
+        _tensor(z, "preactivation", device, dy_dtype, shape)
     else:
         z = None
     dx = dw = db = None
-    dx_stride = dw_stride = 0
-    inputs = [("dy", dy), ("x", x), ("weight", weight), ("preactivation", z)]
-    made = []
     if need[0]:
-        dx, dx_stride = _output(outs[0], x.shape, x.dtype, x.device, "dx")
-        made.append(("dx", dx))
+        dx, dx_stride = _output(outs[0], x.shape, dtype, device, "dx")
     if need[1]:
-        dw, dw_stride = _output(outs[1], weight.shape, x.dtype, x.device, "dweight")
-        made.append(("dweight", dw))
+        dw, dw_stride = _output(outs[1], width, dtype, device, "dweight")
     if need[2]:
-        db, _ = _output(outs[2], (weight.shape[0],), x.dtype, x.device, "dbias")
-        made.append(("dbias", db))
-    for k, (name, t) in enumerate(made):
-        if any(o is t for o in outs):
-            _apart(t, name, inputs + made[:k])
-    if not made:
+        db, _ = _output(outs[2], width[:1], dtype, device, "dbias")
+    if outs[0] is not None or outs[1] is not None or outs[2] is not None:
+        _apart_from_all(outs, [("dx", dx), ("dweight", dw), ("dbias", db)],
+                        [("dy", dy), ("x", x), ("weight", weight), ("preactivation", z)])
+    if not any(need):
         return dx, dw, db
-    rows = x.numel() // x.shape[-1]
+    rows = x.numel() // K
     dy, dy_stride = _rows(dy)
     x, x_stride = _rows(x)
     weight, w_stride = _rows(weight)
-    z_stride = 0
     if z is not None:
         z, z_stride = _rows(z)
-    lib = _lib.lib()
-    d, od, K, N = _DTYPES[x.dtype], _DTYPES[dy.dtype], x.shape[-1], weight.shape[0]
-    ws, ws_bytes = _scratch(workspace, _bytes_of("gl_dense_backward_workspace", rows, K, N, d, od, act), x.device)
-    with _on(x.device):
-        _lib.check(lib.gl_dense_backward(_p(dy), dy_stride, _p(x), x_stride, _p(weight), w_stride, _p(z), z_stride,
-                                         _p(dx), dx_stride, _p(dw), dw_stride, _p(db), rows, K, N, d, od, act, _p(ws),
-                                         ws_bytes, _stream(x.device)), "gl_dense_backward")
+    d, od = _DTYPES[dtype], _DTYPES[dy_dtype]
+    ws, ws_bytes = _scratch(workspace, _bytes_of("gl_dense_backward_workspace", rows, K, N, d, od, act), device, dy, x,
+                            weight, z, dx, dw, db)
+    with _on(device):
+        _lib.check(_lib.lib().gl_dense_backward(_p(dy), dy_stride, _p(x), x_stride, _p(weight), w_stride, _p(z), z_stride,
+                                                _p(dx), dx_stride, _p(dw), dw_stride, _p(db), rows, K, N, d, od, act,
+                                                _p(ws), ws_bytes, _stream(device)), "gl_dense_backward")
     return dx, dw, db
 
 
@@ -343,9 +348,7 @@ def dense_backward(dy, x, weight, preactivation=None, *, activation=None, needs=
 
     dy, preactivation: (..., outputs), of dense's result type.  needs: which of the three are wanted (None comes back
     for the others).  dx, dweight, dbias: tensors that receive them."""
-    with torch.no_grad():
-        return _dense_backward(dy, x, weight, preactivation, _activation(activation), tuple(needs), (dx, dweight, dbias),
-                               workspace)
+    return _dense_backward(dy, x, weight, preactivation, _activation(activation), needs, (dx, dweight, dbias), workspace)
 
 
 # -- group norm ------------------------------------------------------------------------------------------------
@@ -408,7 +411,8 @@ def _group_norm(x, groups, weight, bias, eps, act, lengths, out, stats, workspac
     if bias is not None:
         bias = _vector(bias)
     d = _DTYPES[dtype]
-    ws, ws_bytes = _scratch(workspace, _bytes_of("gl_group_norm_workspace", B, T, C, groups, d), device)
+    ws, ws_bytes = _scratch(workspace, _bytes_of("gl_group_norm_workspace", B, T, C, groups, d), device, x, weight,
+                            bias, lens, y, stats)
     with _on(device):
         _lib.check(_lib.lib().gl_group_norm(_p(x), x_stride, _p(weight), _p(bias), _p(lens), _p(y), y_stride, _p(stats), B,
                                             T, C, groups, d, act, eps, _p(ws), ws_bytes, _stream(device)),
@@ -455,38 +459,36 @@ def group_norm(x, groups, weight=None, bias=None, *, eps=1e-5, activation=None, 
 
 def _group_norm_backward(dy, x, groups, stats, weight, bias, act, lengths, need, outs, workspace):
     groups, B, T, C, lens = _norm_args(x, groups, weight, bias, lengths)
-    _tensor(dy, "dy", x.device, x.dtype, x.shape)
-    _tensor(stats, "stats", x.device, torch.float32, (B, groups, 2))
-    stats = stats.contiguous()
+    device, dtype = x.device, x.dtype
+    _tensor(dy, "dy", device, dtype, x.shape)
+    _tensor(stats, "stats", device, torch.float32, (B, groups, 2))
+    stats = _vector(stats)
     dx = dg = db = None
     dx_stride = 0
-    inputs = [("x", x), ("stats", stats), ("weight", weight), ("bias", bias), ("lengths", lens), ("dy", dy)]
-    made = []
     if need[0]:
-        dx, dx_stride = _output(outs[0], x.shape, x.dtype, x.device, "dx")
-        made.append(("dx", dx))
+        dx, dx_stride = _output(outs[0], x.shape, dtype, device, "dx")
     if need[1] and weight is not None:
-        dg, _ = _output(outs[1], (C,), x.dtype, x.device, "dweight")
-        made.append(("dweight", dg))
+        dg, _ = _output(outs[1], (C,), dtype, device, "dweight")
     if need[2] and bias is not None:
-        db, _ = _output(outs[2], (C,), x.dtype, x.device, "dbias")
-        made.append(("dbias", db))
-    for k, (name, t) in enumerate(made):
-        if any(o is t for o in outs):
-            _apart(t, name, inputs + made[:k], same=(dy,) if t is dx else ())
-    if not made:
+        db, _ = _output(outs[2], (C,), dtype, device, "dbias")
+    if outs[0] is not None or outs[1] is not None or outs[2] is not None:
+        _apart_from_all(outs, [("dx", dx), ("dweight", dg), ("dbias", db)],
+                        [("x", x), ("stats", stats), ("weight", weight), ("bias", bias), ("lengths", lens), ("dy", dy)], (dy,))
+    if dx is None and dg is None and db is None:
         return dx, dg, db
     dy, dy_stride = _rows(dy)
     x, x_stride = _rows(x)
-    weight = None if weight is None else _vector(weight)
-    bias = None if bias is None else _vector(bias)
-    lib = _lib.lib()
-    d = _DTYPES[x.dtype]
-    ws, ws_bytes = _scratch(workspace, _bytes_of("gl_group_norm_backward_workspace", B, T, C, groups, d), x.device)
-    with _on(x.device):
-        _lib.check(lib.gl_group_norm_backward(_p(dy), dy_stride, _p(x), x_stride, _p(stats), _p(weight), _p(bias), _p(lens),
-                                              _p(dx), dx_stride, _p(dg), _p(db), B, T, C, groups, d, act, _p(ws), ws_bytes,
-                                              _stream(x.device)), "gl_group_norm_backward")
+    if weight is not None:
+        weight = _vector(weight)
+    if bias is not None:
+        bias = _vector(bias)
+    d = _DTYPES[dtype]
+    ws, ws_bytes = _scratch(workspace, _bytes_of("gl_group_norm_backward_workspace", B, T, C, groups, d), device, dy, x, stats,
+                            weight, bias, lens, dx, dg, db)
+    with _on(device):
+        _lib.check(_lib.lib().gl_group_norm_backward(_p(dy), dy_stride, _p(x), x_stride, _p(stats), _p(weight), _p(bias),
+                                                     _p(lens), _p(dx), dx_stride, _p(dg), _p(db), B, T, C, groups, d, act,
+                                                     _p(ws), ws_bytes, _stream(device)), "gl_group_norm_backward")
     return dx, dg, db
 
 
@@ -495,9 +497,8 @@ def group_norm_backward(dy, x, groups, stats, weight=None, bias=None, *, activat
     """Gradients (dx, dweight, dbias) of :func:`group_norm` from its input and stats (gl_group_norm_backward).
 
     dx is zero in frames past an utterance's end and may be dy.  dweight / dbias are None where weight / bias is."""
-    with torch.no_grad():
-        return _group_norm_backward(dy, x, groups, stats, weight, bias, _activation(activation), lengths, tuple(needs),
-                                    (dx, dweight, dbias), workspace)
+    return _group_norm_backward(dy, x, groups, stats, weight, bias, _activation(activation), lengths, needs,
+                                (dx, dweight, dbias), workspace)
 
 
 # -- the network -----------------------------------------------------------------------------------------------

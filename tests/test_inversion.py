@@ -759,6 +759,14 @@ def test_refusals_of_the_python_calls():
         inv.dense(both[:32].view(4, 8), w, out=both[20:44].view(4, 6))
     with pytest.raises(ValueError, match="overlaps"):
         inv.dense(x, w, residual=both[:24].view(4, 6), out=both[1:25].view(4, 6))
+    space = torch.zeros(1 << 23, dtype=torch.uint8, device="cuda")
+    with pytest.raises(ValueError, match="workspace overlaps"):
+        inv.dense(torch.zeros(16, 4096, device="cuda"), torch.zeros(6, 4096, device="cuda"),
+                  out=space[:384].view(torch.float32).view(16, 6), workspace=space)
+    with pytest.raises(ValueError, match="workspace overlaps"):
+        inv.dense_backward(torch.zeros(700, 512, device="cuda"), torch.zeros(700, 80, device="cuda"),
+                           torch.zeros(512, 80, device="cuda"), dbias=space[-2048:].view(torch.float32),
+                           workspace=space)
     with pytest.raises(ValueError, match="preactivation"):
         inv.dense_backward(y, x, w, activation="silu")
     with pytest.raises(ValueError):
@@ -810,14 +818,19 @@ def test_refusals_of_the_c_calls():
                 act=2, wk=p, wb=1 << 30, st=None)
     call = lambda **k: lib.gl_dense_backward(*{**back, **k}.values())                  # noqa: E731
     for bad in (dict(dy=None), dict(x=None), dict(w=None), dict(z=None), dict(dys=5), dict(xs=7), dict(ws=7), dict(zs=5),
-                dict(dxs=7), dict(dws=7), dict(rows=-2), dict(od=2), dict(act=9), dict(wb=0), dict(wk=None)):
+                dict(dxs=7), dict(dws=7), dict(rows=-2), dict(od=2), dict(act=9)):
         assert call(**bad) == -1, bad
+    assert lib.gl_dense_backward_workspace(4, 8, 6, 0, 0, 2) == 0                       # one part each: nothing to join
+    big = dict(rows=700, k=80, n=512, dys=512, xs=80, ws=80, zs=512, dxs=80, dws=80)
+    need = lib.gl_dense_backward_workspace(700, 80, 512, 0, 0, 2)
+    assert need > 0 and call(**big, wb=need - 1) == -1 and b"workspace" in lib.gl_last_error()
+    assert call(**big, wk=None) == -1 and call(**big, wk=ctypes.c_void_p(4104)) == -1
     assert call(dx=None, dw=None, db=None) == 0
     norm = dict(x=p, xs=12, ga=p, be=p, f=p, y=p, ys=12, s=p, B=2, T=50000, C=12, G=3, d=0, act=0, eps=1e-5, wk=p, wb=1 << 30,
                 st=None)
     call = lambda **k: lib.gl_group_norm(*{**norm, **k}.values())                      # noqa: E731
     for bad in (dict(x=None), dict(y=None), dict(xs=11), dict(ys=11), dict(B=-1), dict(B=65536), dict(T=-1), dict(C=0),
-                dict(G=5), dict(G=0), dict(G=24), dict(d=4), dict(act=7), dict(eps=-1.0), dict(eps=float("nan")), dict(wb=1),
+                dict(T=(1 << 30) + 1), dict(G=5), dict(G=0), dict(G=24), dict(d=4), dict(act=7), dict(eps=-1.0), dict(eps=float("nan")), dict(wb=1),
                 dict(wk=None), dict(wk=ctypes.c_void_p(4100))):
         assert call(**bad) == -1, bad
     assert call(B=0) == 0 and call(T=0, s=None) == 0
