@@ -22,11 +22,29 @@ struct gl_epilogue {
     int act;
     bool quads;                  // k_dense_any: four columns of y, z and residual lie on whole vectors
     float* partial;              // [parts][I][J]: sums of one part of the contraction, finished by k_dense_join
-    // float32 through planes: the operands themselves, for the sums that are not finite, and the flags of their blocks
+    // float32 through planes: the operands themselves, for the sums the planes do not give, and the flags of their blocks
     const float *exact_p, *exact_q;
     long long exact_p_is, exact_p_qs, exact_q_is, exact_q_qs, exact_nq;
     int* flags;
+    const int *scale_p, *scale_q;    // float32 through halves: gl_scale of P's and Q's rows, else null
 };
+
+// A row of a float32 matrix in two planes of f16: x 2^e = h + l 2^-12 with h = f16(x 2^e), l = f16((x 2^e - h) 2^12) and the row's
+// largest |x| 2^e in [2^14, 2^15).  Values of at least 2^-13 have 24 bits in it, smaller ones are off by 2^-37 at most: `small`
+// says that there are such.  `wild`: the row holds an infinity or a NaN, and its planes zeros.
+struct gl_scale {
+    int bits;                    // e, small, wild
+    static __host__ __device__ gl_scale of(int e, bool small, bool wild) { return {e * 4 + (small ? 1 : 0) + (wild ? 2 : 0)}; }
+    __device__ int e() const { return bits >> 2; }
+    __device__ bool small() const { return bits & 1; }
+    __device__ bool wild() const { return bits & 2; }
+};
+// Whether the planes give a sum of nq products, `sum` = C 2^(e of P's row + e of Q's).  Small values move it by at most
+// 3 nq 2^-37 2^15 in all; where that is more than 2^-23 of it, it is for the operands themselves.
+__device__ __forceinline__ bool gl_halves_give(float sum, gl_scale p, gl_scale q, float nq) {
+    const gl_scale both = {p.bits | q.bits};
+    return !both.wild() && !(both.small() && fabsf(sum) < 6.0f * nq);
+}
 
 static inline long long gl_ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 static inline long long gl_align16(long long b) { return (b + 15) / 16 * 16; }
@@ -46,7 +64,7 @@ long long gl_mm_partial_bytes(long long I, int J, long long nq, bool any_q);
 
 // Whether the fast kernels take the operands as they lie, else the strided kernel does.
 bool gl_mm16_takes(const gl_operand& P, const gl_operand& Q, const gl_epilogue& e, long long I, int J, long long nq, int out_size);
-// T: gl_bf16 / gl_f16; TO: T or float; TB: type of the bias; SEG 6: planes of float32 operands, else 1
+// T: gl_bf16 / gl_f16; TO: T or float; TB: type of the bias; SEG 6 (gl_bf16), 3 (gl_f16): planes of float32 operands, else 1
 template <typename T, typename TO, typename TB, int SEG>
 int gl_mm16(const gl_operand& P, const gl_operand& Q, gl_epilogue e, long long I, int J, long long nq, float* partial, hipStream_t st);
 

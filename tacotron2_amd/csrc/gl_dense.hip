@@ -7,7 +7,7 @@
 // Which kernel, by sizes alone (the workspace query and the call must agree):
 //   up to 8 rows (forward): k_dense_few, one wave (or part of one) a column: W is read once, nothing else counts;
 //   16-bit types: the tiles of gl_mm16.h, on copies padded to whole chunks where a width is not a multiple of 8;
-//   float32 with enough work: the same tiles on three bfloat16 planes;
+//   float32 with enough work: the same tiles on planes of 16 bits;
 //   the rest, and operands whose rows start off 16 bytes against their widths: k_dense_any, element by element, on
 //   v_mfma_f32_32x32x16 or, for float32, v_mfma_f32_32x32x2_f32.
 // Sums are float32 everywhere.  Q is the matrix instruction's A operand: the accumulator's registers then run along j, the
@@ -308,7 +308,12 @@ __global__ void __launch_bounds__(256) k_dense_join(Epilogue e, long long I, int
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             float sum = s[v];
-            if (e.exact_p && !(fabsf(sum) < INFINITY)) {     // float32 through planes, not finite: once more from the operands
+            bool again = e.exact_p && !(fabsf(sum) < INFINITY);          // float32 through planes: once more from the operands
+            if (e.scale_p) {
+                const gl_scale p = {e.scale_p[i]}, q = {e.scale_q[j + v]};
+                again |= !gl_halves_give(ldexpf(sum, p.e() + q.e()), p, q, (float)e.exact_nq);
+            }
+            if (again) {
                 sum = 0.0f;
                 for (long long q = 0; q < e.exact_nq && sum == sum; ++q)
                     sum = fmaf(e.exact_p[i * e.exact_p_is + q * e.exact_p_qs], e.exact_q[(j + v) * e.exact_q_is + q * e.exact_q_qs], sum);
@@ -386,6 +391,73 @@ __global__ void __launch_bounds__(256) k_dense_pack(const T* __restrict__ in, lo
             *(v8*)(o + plane) = m;
             *(v8*)(o + 2 * plane) = l;
         }
+    }
+}
+
+// Rows of two float32 matrices, one after the other, into two planes of f16 each and their gl_scale; zeros up to `padded`
+// columns.  A wave a row, which it reads twice: for its largest value, and to convert it.
+struct Halves {
+    const float* in;
+    long long in_stride, rows;
+    gl_f16* out;
+    int* scale;
+};
+template <bool VEC>
+__global__ void __launch_bounds__(256) k_dense_halves(Halves a, Halves b, int cols, int padded) {
+    const int lane = threadIdx.x & 63;
+    for (long long at = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); at < a.rows + b.rows; at += (long long)gridDim.x * 4) {
+        const bool second = at >= a.rows;
+        const Halves h = second ? b : a;
+        const long long r = second ? at - a.rows : at;
+        const float* src = h.in + r * h.in_stride;
+        auto load = [&](int c, float (&v)[8]) {
+            if constexpr (VEC) {
+                const f32x4 lo = *(const f32x4*)(src + min(c, cols - 4)), hi = *(const f32x4*)(src + min(c + 4, cols - 4));
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    v[k] = c < cols ? lo[k] : 0.0f;
+                    v[4 + k] = c + 4 < cols ? hi[k] : 0.0f;
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const float t = src[min(c + k, cols - 1)];
+                    v[k] = c + k < cols ? t : 0.0f;
+                }
+            }
+        };
+        unsigned most = 0;                                   // of |x|, as bits: NaN above infinity above the rest
+#pragma unroll 2
+        for (int c = lane * 8; c < padded; c += 512) {
+            float v[8];
+            load(c, v);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) most = max(most, __builtin_bit_cast(unsigned, v[k]) & 0x7fffffffu);
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) most = max(most, (unsigned)__shfl_xor((int)most, o));
+        const bool wild = most >= 0x7f800000u;
+        const int e = wild || most == 0 ? 0 : 15 - __builtin_amdgcn_frexp_expf(__builtin_bit_cast(float, most));
+        bool small = false;
+#pragma unroll 2
+        for (int c = lane * 8; c < padded; c += 512) {
+            typedef typename vecn<gl_f16, 8>::type v8;
+            float v[8];
+            v8 hi, lo;
+            load(c, v);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float s = wild ? 0.0f : ldexpf(v[k], e);
+                small |= v[k] != 0.0f && fabsf(s) < 0x1p-13f;
+                hi[k] = (gl_f16)s;
+                lo[k] = (gl_f16)((s - (float)hi[k]) * 4096.0f);
+            }
+            gl_f16* o = h.out + r * padded + c;
+            *(v8*)o = hi;
+            *(v8*)(o + h.rows * padded) = lo;
+        }
+        small = __any(small);
+        if (lane == 0) h.scale[r] = gl_scale::of(e, small, wild).bits;
     }
 }
 
@@ -531,14 +603,16 @@ int any_product(const Operand& P, const Operand& Q, Epilogue e, long long I, int
 
 // Layers of fewer multiplications than this go as they are to k_dense_any (forward, where the tiles would need copies) and
 // k_dense_back_small.  Microseconds there / on the tiles:
-//   float32, widths on 16 bytes   forward 2000 x 1024 -> 1024 58 / 61, 6888 x 1024 -> 512 90 / 87
+//   float32, widths on 16 bytes   forward 2000 x 500 -> 700 33 / 34, 861 x 1024 -> 1024 40 / 35, 2000 x 1024 -> 1024 59 / 42
 //                                 backward 2000 x 1024 -> 1024 122 / 153, 6888 x 1024 -> 512 240 / 179
-//   float32, others               forward 2000 x 501 -> 701 53 / 51, backward 641 x 512 -> 1025 79 / 84, 2000 x 501 -> 701 104 / 98
+//   float32, others               forward 641 x 257 -> 513 19 / 25, 6888 x 81 -> 512 25 / 25, 2000 x 501 -> 701 54 / 38
+//                                 backward 641 x 512 -> 1025 79 / 84, 2000 x 501 -> 701 104 / 98
 //   16 bits forward               641 x 257 -> 513 18 / 18, 2000 x 501 -> 701 41 / 21
 //   16 bits backward              641 x 512 -> 512 29 / 38, 6888 x 80 -> 512 45 / 38
 double small_layer(int dtype, int inputs, int outputs, bool back) {
-    if (dtype == GL_F32) return inputs % 4 || outputs % 4 ? 1LL << 29 : 1LL << 31;
-    return back ? 3 << 26 : 1 << 27;
+    if (dtype != GL_F32) return back ? 3 << 26 : 1 << 27;
+    const bool odd = inputs % 4 || outputs % 4;
+    return back ? (odd ? 1LL << 29 : 1LL << 31) : odd ? 1 << 28 : 3 << 28;
 }
 bool is_small(long long rows, int inputs, int outputs, int dtype, bool back) {
     return (double)rows * inputs * outputs < small_layer(dtype, inputs, outputs, back);
@@ -548,6 +622,7 @@ bool copies(int dtype, int width) { return dtype == GL_F32 || width % 8 != 0; }
 long long copy_bytes(int dtype, long long rows, int cols) {
     return gl_align16(rows * pad_to(cols) * (dtype == GL_F32 ? 6LL : 2LL));
 }
+long long halves_bytes(long long rows, int cols) { return gl_align16(rows * pad_to(cols) * 4LL); }
 long long flag_bytes(int dtype, long long I, int J) { return dtype == GL_F32 ? gl_align16(gl_ceil_div(I, 64) * gl_ceil_div(J, 64) * 4) : 0; }
 // flags and parts of a product, whichever kernel takes it
 long long partial_bytes(int dtype, long long I, int J, long long nq, bool any_q, bool fast) {
@@ -569,12 +644,12 @@ int pack(Operand& o, bool across, long long stride, long long rows, int cols, vo
 }
 
 // The product on prepared operands (16-bit as they lie or copied, float32 in planes), else on the originals (P0, Q0).
-template <typename T, typename TO>
+template <typename T, typename TO, int SEG>
 int product(const Operand& P, const Operand& Q, const Operand& P0, const Operand& Q0, Epilogue e, long long I, int J, long long nq,
             float* partial, bool fast, hipStream_t st) {
     if constexpr (sizeof(T) == 2) {
         if (gl_mm16_takes(P, Q, e, I, J, nq, sizeof(TO))) return gl_mm16<T, TO, T, 1>(P, Q, e, I, J, nq, partial, st);
-    } else {
+    } else if constexpr (SEG > 1) {
         if (fast && gl_mm16_takes(P, Q, e, I, J, nq, sizeof(TO))) {
             e.exact_p = (const float*)P0.base;
             e.exact_q = (const float*)Q0.base;
@@ -584,9 +659,11 @@ int product(const Operand& P, const Operand& Q, const Operand& P0, const Operand
             e.exact_q_qs = Q0.qs;
             e.exact_nq = nq;
             e.flags = (int*)partial;
-            return gl_mm16<gl_bf16, float, float, 6>(P, Q, e, I, J, nq, partial + flag_bytes(GL_F32, I, J) / 4, st);
+            typedef typename std::conditional<SEG == 3, gl_f16, gl_bf16>::type Plane;
+            return gl_mm16<Plane, float, float, SEG>(P, Q, e, I, J, nq, partial + flag_bytes(GL_F32, I, J) / 4, st);
         }
     }
+    e.scale_p = nullptr;
     return any_product<T, TO>(P0, Q0, e, I, J, nq, partial, st);
 }
 
@@ -620,18 +697,22 @@ int check_workspace(const void* ws, long long have, long long need, const char* 
 // ---- forward ----
 constexpr int kFewRows = 8;
 
-// workspace: [copy of x] [copy of weight] [flags and parts]
+// workspace: [copy of x] [copy of weight] [their scales, where the copies are halves of float32] [flags and parts]
 struct FrontLayout {
     bool fast, copy;
-    long long x_bytes, w_bytes, partial;
-    long long total() const { return x_bytes + w_bytes + partial; }
+    long long x_bytes, w_bytes, scale_bytes, partial;
+    long long total() const { return x_bytes + w_bytes + scale_bytes + partial; }
 };
 FrontLayout front_layout(long long rows, int inputs, int outputs, int dtype) {
     FrontLayout l = {};
     if (rows <= kFewRows) return l;
     l.fast = !is_small(rows, inputs, outputs, dtype, false);
     l.copy = l.fast && copies(dtype, inputs);
-    if (l.copy) {
+    if (l.copy && dtype == GL_F32) {
+        l.x_bytes = halves_bytes(rows, inputs);
+        l.w_bytes = halves_bytes(outputs, inputs);
+        l.scale_bytes = gl_align16((rows + outputs) * 4);
+    } else if (l.copy) {
         l.x_bytes = copy_bytes(dtype, rows, inputs);
         l.w_bytes = copy_bytes(dtype, outputs, inputs);
     }
@@ -662,13 +743,31 @@ int forward(const void* x, long long x_stride, const void* w, long long w_stride
     if (rows <= kFewRows) return few<T, TO, kFewRows>(x, x_stride, w, w_stride, e, (int)rows, inputs, outputs, st);
     const Operand P0 = {x, x_stride, 1}, Q0 = {w, w_stride, 1};
     Operand P = P0, Q = Q0;
-    char* at = (char*)ws;
-    if (l.copy) {
+    char *at = (char*)ws, *w_copy = at + l.x_bytes, *scale = w_copy + l.w_bytes;
+    float* partial = (float*)(scale + l.scale_bytes);
+    if (!l.copy) return product<T, TO, 1>(P, Q, P0, Q0, e, rows, outputs, inputs, partial, l.fast, st);
+    if constexpr (sizeof(T) == 2) {
         int rc = pack<T>(P, false, x_stride, rows, inputs, at, st);
-        if (!rc) rc = pack<T>(Q, false, w_stride, outputs, inputs, at + l.x_bytes, st);
-        if (rc) return rc;
+        if (!rc) rc = pack<T>(Q, false, w_stride, outputs, inputs, w_copy, st);
+        return rc ? rc : product<T, TO, 1>(P, Q, P0, Q0, e, rows, outputs, inputs, partial, true, st);
+    } else {
+        const int padded = pad_to(inputs);
+        Epilogue f = e;
+        f.scale_p = (const int*)scale;
+        f.scale_q = f.scale_p + rows;
+        const Halves a = {(const float*)x, x_stride, rows, (gl_f16*)at, (int*)scale};
+        const Halves b = {(const float*)w, w_stride, outputs, (gl_f16*)w_copy, (int*)scale + rows};
+        const long long blocks = gl_ceil_div(rows + outputs, 4);
+        const dim3 grid((unsigned)(blocks < 4096 ? blocks : 4096));
+        if (wide_loads(P0, inputs, 4) && wide_loads(Q0, inputs, 4))
+            hipLaunchKernelGGL((k_dense_halves<true>), grid, dim3(256), 0, st, a, b, inputs, padded);
+        else
+            hipLaunchKernelGGL((k_dense_halves<false>), grid, dim3(256), 0, st, a, b, inputs, padded);
+        GL_HIP_CHECK(hipGetLastError());
+        P = {at, padded, 1, rows * padded, true};
+        Q = {w_copy, padded, 1, (long long)outputs * padded, true};
+        return product<T, TO, 3>(P, Q, P0, Q0, f, rows, outputs, inputs, partial, true, st);
     }
-    return product<T, TO>(P, Q, P0, Q0, e, rows, outputs, inputs, (float*)(at + l.x_bytes + l.w_bytes), l.fast, st);
 }
 
 // ---- backward ----
@@ -840,7 +939,7 @@ int backward(const void* dy, long long dy_stride, const void* x, long long x_str
         if (rc) return rc;
         e.y = dx;
         e.y_stride = dx_stride;
-        rc = product<T, T>({d, d_stride, 1, plane, padded}, Q, {d0, d0_stride, 1}, Q0, e, rows, inputs, outputs, partial, true, st);
+        rc = product<T, T, sizeof(T) == 4 ? 6 : 1>({d, d_stride, 1, plane, padded}, Q, {d0, d0_stride, 1}, Q0, e, rows, inputs, outputs, partial, true, st);
         if (rc) return rc;
     }
     if (dw) {
@@ -850,7 +949,7 @@ int backward(const void* dy, long long dy_stride, const void* x, long long x_str
         if (rc) return rc;
         e.y = dw;
         e.y_stride = dw_stride;
-        rc = product<T, T>({d, 1, d_stride, plane, padded}, Q, {d0, 1, d0_stride}, Q0, e, outputs, inputs, rows, partial, true, st);
+        rc = product<T, T, sizeof(T) == 4 ? 6 : 1>({d, 1, d_stride, plane, padded}, Q, {d0, 1, d0_stride}, Q0, e, outputs, inputs, rows, partial, true, st);
     }
     return rc;
 }
@@ -880,7 +979,7 @@ int gl_dense_flagged(const gl_epilogue& e, long long I, int J, long long nq, hip
     f.quads = quads<float>(e, J);
     const AnyArgs a = {{e.exact_p, e.exact_p_is, e.exact_p_qs}, {e.exact_q, e.exact_q_is, e.exact_q_qs}, {}, f, I, nq, nq, J,
                        (int)gl_ceil_div(J, kTile), (int)tiles, GL_ACT_NONE, e.exact_p_qs == 1, e.exact_q_qs == 1, nullptr, nullptr};
-    hipLaunchKernelGGL((k_dense_any<float, float, 1>), dim3((unsigned)(tiles < 512 ? tiles : 512)), dim3(256), 0, st, a, e.flags);
+    hipLaunchKernelGGL((k_dense_any<float, float, 1>), dim3((unsigned)(tiles < 8192 ? tiles : 8192)), dim3(256), 0, st, a, e.flags);
     GL_HIP_CHECK(hipGetLastError());
     return 0;
 }

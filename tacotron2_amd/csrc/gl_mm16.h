@@ -13,16 +13,18 @@
 // way); its 32-byte pieces are XORed with the row so that the 8 rows of half a wave spread over all banks.  The swizzle is
 // applied to the global address, since direct loads place consecutive lanes' chunks consecutively.
 //
-// float32 operands come as three planes of bfloat16, x = h + m + l with h = bf16(x), m = bf16(x - h), l = bf16(x - h - m):
-// 24 bits, exact up to the last half bit.  C is the sum of six products (SEG): hh, hm, mh, mm, hl, lh; what is left out (ml, lm,
-// ll) is below 2^-24 of |x| |y|, as one rounding of a product is.  A block with a sum that is not finite is not written but
-// flagged, and the float32 kernel computes it: an infinity times a zero plane would be NaN.
+// float32 operands come in planes, and C is a sum of SEG products of planes.  A block with a sum that the planes do not give
+// is not written but flagged, and the float32 kernel computes it.
+//   3: two planes of f16 per row (gl_scale), where a row of either side is one of the contraction: h l, l h, then, with the
+//      sums times 2^-12, h h.  Left out is l l 2^-24 <= 2^-24 |x| |y|: with both sides' rounding three roundings a product.
+//   6: three planes of bfloat16, x = h + m + l with h = bf16(x), m = bf16(x - h), l = bf16(x - h - m), which need no scale (an
+//      operand across the contraction has one per column): hh, hm, mh, mm, hl, lh; what is left out (ml, lm, ll) is below 2^-24
+//      of |x| |y|.  Sums that are not finite are flagged: an infinity times a zero plane would be NaN.
 //
 // v_mfma_f32_16x16x32: A = Q rows (columns j of C), B = P rows (rows i of C): a lane's four accumulator registers are four
 // consecutive j of one i.
 #pragma once
-#include "gl_internal.h"
-#include "gl_act.h"
+#include "gl_dense.h"
 
 namespace gl_mm {
 
@@ -64,9 +66,9 @@ __device__ __forceinline__ void barrier() {
     asm volatile("" ::: "memory");
 }
 
-// The planes of the six products of float32 operands, two bits each: hh, hm, mh, mm, hl, lh
-constexpr int kPlanesP = 0 | 0 << 2 | 1 << 4 | 1 << 6 | 0 << 8 | 2 << 10;
-constexpr int kPlanesQ = 0 | 1 << 2 | 0 << 4 | 1 << 6 | 2 << 8 | 0 << 10;
+// The planes of the products, two bits each
+template <int SEG> constexpr int kPlanesP = SEG == 3 ? 0 | 1 << 2 | 0 << 4 : 0 | 0 << 2 | 1 << 4 | 1 << 6 | 0 << 8 | 2 << 10;
+template <int SEG> constexpr int kPlanesQ = SEG == 3 ? 1 | 0 << 2 | 0 << 4 : 0 | 1 << 2 | 0 << 4 | 1 << 6 | 2 << 8 | 0 << 10;
 __device__ __forceinline__ int plane_of(int planes, int seg) { return planes >> (2 * seg) & 3; }
 
 constexpr int kFlags = 0x00027000;                           // raw 32-bit buffer: bounds-checked, no format conversion
@@ -79,7 +81,7 @@ template <int R, int BK, bool TR, int WAVES, bool TEXT>
 struct Stage {
     static constexpr int kLoads = (R * BK * 2 + 1024 * WAVES - 1) / (1024 * WAVES);   // 16-byte loads per lane and stage
     static constexpr int kBytes = kLoads * 1024 * WAVES;     // with whole loads of all waves: rows past R are zeros
-    static_assert(!TR || R % 32 == 0 && (R & (R - 1)) == 0, "pieces of 32 bytes are exchanged within a row");
+    static_assert(!TR || (R % 32 == 0 && (R & (R - 1)) == 0), "pieces of 32 bytes are exchanged within a row");
     static constexpr int kRowChunks = TR ? R / 8 : BK / 8;   // chunks per LDS row
     const char* base;            // first element of the tile at the current step
     const char* start;           // and at the first one
@@ -173,6 +175,7 @@ struct Out {
     long long part_stride;       // elements of y between the results of two parts of the contraction (bias, residual and z
                                  // are null then)
     int odd;                     // rows start off 4 bytes: elements are stored one by one (TAIL kernels)
+    const int *scale_p, *scale_q;    // SEG 3
 };
 
 template <typename T> struct bits;                          // what a buffer load or store of an element moves
@@ -323,6 +326,42 @@ __device__ __forceinline__ bool all_finite(int* flags, const f32x4 (&acc)[MI][NI
     return !bad;
 }
 
+// SEG 3: a wave's sums in the operands' own scale, plus the bias.  False: some of them are not to be had from planes (never
+// so for parts of the contraction, whose join decides); with flags, writes those of its 64 x 64 blocks.
+template <typename TB, int MI, int NI>
+__device__ __forceinline__ bool unscale(const Out& o, f32x4 (&acc)[MI][NI], long long i0, int j0, long long I, int J, float nq, int lane) {
+    static_assert(MI % 4 == 0 && NI == 4, "whole blocks of flags");
+    const int il = lane & 15, g4 = lane >> 4;
+    const int rows = max(0, (int)min(I - i0, (long long)16 * MI)), cols = max(0, min(J - j0, 16 * NI));
+    const __amdgpu_buffer_rsrc_t rp = __builtin_amdgcn_make_buffer_rsrc((void*)(o.scale_p + (rows ? i0 : 0)), 0, rows * 4, kFlags);
+    const __amdgpu_buffer_rsrc_t rq = __builtin_amdgcn_make_buffer_rsrc((void*)(o.scale_q + (cols ? j0 : 0)), 0, cols * 4, kFlags);
+    typename vec<TB, 4>::type bias[NI];
+    load_bias<TB, NI>(o, bias, j0, J, lane);
+    int qs[NI][4];
+#pragma unroll
+    for (int n = 0; n < NI; ++n)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) qs[n][r] = __builtin_amdgcn_raw_buffer_load_b32(rq, (16 * n + 4 * g4 + r) * 4, 0, 0);
+    bool good = true;
+#pragma unroll
+    for (int m = 0; m < MI; ++m) {
+        const gl_scale p = {(int)__builtin_amdgcn_raw_buffer_load_b32(rp, (16 * m + il) * 4, 0, 0)};
+#pragma unroll
+        for (int n = 0; n < NI; ++n)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const gl_scale q = {qs[n][r]};
+                good &= gl_halves_give(acc[m][n][r], p, q, nq);
+                acc[m][n][r] = ldexpf(acc[m][n][r], -(p.e() + q.e())) + gl_to_f32(bias[n][r]);
+            }
+    }
+    if (!o.flags) return true;
+    const bool bad = !__all(good);
+    const int per_row = (J + 63) / 64;
+    if (lane < MI / 4 && i0 + 64 * lane < I && j0 < J) o.flags[(i0 / 64 + lane) * per_row + j0 / 64] = bad;
+    return !bad;
+}
+
 // Writes a wave's block at (i0, j0): activation, residual and one rounding.  All loads come before the
 // results' stores: the memory counter runs in order, a load behind a store would wait for it.
 // EXTRA: there may be a residual or a preactivation.
@@ -373,6 +412,17 @@ __device__ __forceinline__ int epilogue(const Out& o, f32x4 (&acc)[MI][NI], long
     return put_block<TO, TAIL, LINES, MI, NI>((TO*)o.y + part * o.part_stride, o.y_stride, acc, i0, j0, I, J, lane, o.odd);
 }
 
+// the products h l + l h, which count 2^-12, before h h is added
+template <int MI, int NI>
+__device__ __forceinline__ void lower(f32x4 (&acc)[MI][NI]) {
+#pragma unroll
+    for (int m = 0; m < MI; ++m)
+#pragma unroll
+        for (int n = 0; n < NI; ++n)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[m][n][r] *= 0x1p-12f;
+}
+
 template <typename T, typename TO, typename TB, int SEG, int ACT, int BM, int BN, int WM, int WN, int BK, int ST, bool PT, bool QT, int WPE>
 __global__ void __launch_bounds__(64 * (BM / WM) * (BN / WN), WPE)
 k_mm16(Side P, Side Q, Out o, long long I, int J, long long nq, long long q_per_part, int tiles_j, int n_tiles) {
@@ -400,7 +450,9 @@ k_mm16(Side P, Side Q, Out o, long long I, int J, long long nq, long long q_per_
     SQ sq;
     sp.init(P, i0, q0, wave, lane);
     sq.init(Q, j0, q0, wave, lane);
-    const int steps = SEG * (int)((q1 - q0 + BK - 1) / BK);
+    sp.base += plane_of(kPlanesP<SEG>, 0) * P.plane * 2;
+    sq.base += plane_of(kPlanesQ<SEG>, 0) * Q.plane * 2;
+    const int once = (int)((q1 - q0 + BK - 1) / BK), steps = SEG * once;
     const int missing = (int)max(0LL, q1 - (nq - Q.missing));   // at the end of this part
     int krem = (int)(q1 - q0), seg = 0;
     auto load = [&](int slot) {
@@ -409,8 +461,8 @@ k_mm16(Side P, Side Q, Out o, long long I, int J, long long nq, long long q_per_
         krem -= BK;
         if (SEG > 1 && krem <= 0 && ++seg < SEG) {
             krem = (int)(q1 - q0);
-            sp.base = sp.start + plane_of(kPlanesP, seg) * P.plane * 2;
-            sq.base = sq.start + plane_of(kPlanesQ, seg) * Q.plane * 2;
+            sp.base = sp.start + plane_of(kPlanesP<SEG>, seg) * P.plane * 2;
+            sq.base = sq.start + plane_of(kPlanesQ<SEG>, seg) * Q.plane * 2;
         }
     };
 #pragma unroll
@@ -418,11 +470,12 @@ k_mm16(Side P, Side Q, Out o, long long I, int J, long long nq, long long q_per_
 
     f32x4 acc[MI][NI];
     typename vec<TB, 4>::type bias[NI];
-    load_bias<TB, NI>(o, bias, j0 + wj, J, lane);
+    load_bias<TB, NI>(o, bias, SEG == 3 ? J : j0 + wj, J, lane);
     start_sums<TB, MI, NI>(acc, bias);
 
     int slot = 0;
     for (int k = 0; k < steps; ++k) {
+        if (SEG == 3 && k == 2 * once) lower(acc);
         wait_loads((SP::kLoads + SQ::kLoads) * (ST - 2));
         barrier();
         load(slot == 0 ? ST - 1 : slot - 1);
@@ -444,7 +497,9 @@ k_mm16(Side P, Side Q, Out o, long long I, int J, long long nq, long long q_per_
     }
     wait_loads(0);                                           // nothing may be on its way into LDS when the wave ends
 
-    if constexpr (SEG > 1) {
+    if constexpr (SEG == 3) {
+        if (!unscale<TB, MI, NI>(o, acc, i0 + wi, j0 + wj, I, J, (float)nq, lane)) return;
+    } else if constexpr (SEG > 1) {
         if (o.flags && !all_finite<MI, NI>(o.flags, acc, i0 + wi, j0 + wj, I, J, lane)) return;
     }
     epilogue<T, TO, ACT, true, true, false, MI, NI>(o, acc, i0 + wi, j0 + wj, I, J, blockIdx.y, lane);
@@ -473,7 +528,7 @@ k_mm16_walk(Side P, Side Q, Out o, long long I, int J, long long nq, long long q
     const long long q0 = (long long)blockIdx.y * q_per_part;
     const int nk = (int)(nq - q0 < q_per_part ? nq - q0 : q_per_part);
     const int missing = (int)max(0LL, q0 + nk - (nq - Q.missing));           // of them on Q's side
-    const int steps = SEG * ((nk + BK - 1) / BK);
+    const int once = (nk + BK - 1) / BK, steps = SEG * once;
     const int pairs = max((RING + 1) / 2, (steps + 1) / 2);   // steps run in twos, at least RING of them: the
                                                                            // extra ones add zeros
     int tile = first + (blockIdx.x >> 3);
@@ -485,8 +540,8 @@ k_mm16_walk(Side P, Side Q, Out o, long long I, int J, long long nq, long long q
         krem -= BK;
         if (SEG > 1 && krem <= 0 && ++seg < SEG) {
             krem = nk;
-            sp.base = sp.start + plane_of(kPlanesP, seg) * P.plane * 2;
-            sq.base = sq.start + plane_of(kPlanesQ, seg) * Q.plane * 2;
+            sp.base = sp.start + plane_of(kPlanesP<SEG>, seg) * P.plane * 2;
+            sq.base = sq.start + plane_of(kPlanesQ<SEG>, seg) * Q.plane * 2;
         }
     };
     auto enter = [&](int t) {
@@ -494,6 +549,8 @@ k_mm16_walk(Side P, Side Q, Out o, long long I, int J, long long nq, long long q
         if (t < end) {
             sp.init(P, (long long)(t / tiles_j) * BM, q0, wave, lane);
             sq.init(Q, (long long)(t % tiles_j) * BN, q0, wave, lane);
+            sp.base += plane_of(kPlanesP<SEG>, 0) * P.plane * 2;
+            sq.base += plane_of(kPlanesQ<SEG>, 0) * Q.plane * 2;
         }
         krem = t < end ? nk : 0;                             // past the last tile: zeros
     };
@@ -509,7 +566,7 @@ k_mm16_walk(Side P, Side Q, Out o, long long I, int J, long long nq, long long q
     f32x4 acc[MI][NI];
     s16x8 a[2][NI], b[MI];
     typename vec<TB, 4>::type bias[NI];
-    load_bias<TB, NI>(o, bias, tile % tiles_j * BN + wj, J, lane);
+    load_bias<TB, NI>(o, bias, SEG == 3 ? J : tile % tiles_j * BN + wj, J, lane);
     // Stores of the last tile's results are newer than the first RING stages of this one: while those are waited for
     // (RING - 1 steps) they may stay outstanding; `old` is how many there are at least, rounded down to 16 or 32.
     int old = 0, grace = 0;
@@ -550,6 +607,7 @@ k_mm16_walk(Side P, Side Q, Out o, long long I, int J, long long nq, long long q
         start_sums<TB, MI, NI>(acc, bias);
 #pragma unroll 1
         for (int k = pairs; k > 0; --k) {
+            if (SEG == 3 && pairs - k == once) lower(acc);
             if (left == 0) enter(tile + walkers);
             step(a[0], a[1]);
             if (RING % 2 && left == 1) enter(tile + walkers);
@@ -558,16 +616,23 @@ k_mm16_walk(Side P, Side Q, Out o, long long I, int J, long long nq, long long q
         }
         left = 2 * pairs - RING;
         wait_loads(kLoads * (RING - 1));
-        if (tile + walkers < end) load_bias<TB, NI>(o, bias, (tile + walkers) % tiles_j * BN + wj, J, lane);
+        if constexpr (SEG != 3) {
+            if (tile + walkers < end) load_bias<TB, NI>(o, bias, (tile + walkers) % tiles_j * BN + wj, J, lane);
 #pragma unroll
-        for (int n = 0; n < NI; ++n) {                       // arrived before the stores below are issued
-            typedef unsigned uB __attribute__((ext_vector_type(sizeof(TB))));
-            uB t = __builtin_bit_cast(uB, bias[n]);
-            asm volatile("" : "+v"(t) : : "memory");
-            bias[n] = __builtin_bit_cast(typename vec<TB, 4>::type, t);
+            for (int n = 0; n < NI; ++n) {                   // arrived before the stores below are issued
+                typedef unsigned uB __attribute__((ext_vector_type(sizeof(TB))));
+                uB t = __builtin_bit_cast(uB, bias[n]);
+                asm volatile("" : "+v"(t) : : "memory");
+                bias[n] = __builtin_bit_cast(typename vec<TB, 4>::type, t);
+            }
         }
         grace = RING - 1;
-        if constexpr (SEG > 1) {
+        if constexpr (SEG == 3) {
+            if (!unscale<TB, MI, NI>(o, acc, (long long)(tile / tiles_j) * BM + wi, tile % tiles_j * BN + wj, I, J, (float)nq, lane)) {
+                old = 0;
+                continue;
+            }
+        } else if constexpr (SEG > 1) {
             if (o.flags && !all_finite<MI, NI>(o.flags, acc, (long long)(tile / tiles_j) * BM + wi, tile % tiles_j * BN + wj, I, J, lane)) {
                 old = 0;
                 continue;

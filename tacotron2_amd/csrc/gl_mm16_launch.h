@@ -69,7 +69,7 @@ template <typename T, typename TO, typename TB, int SEG, bool PT, bool QT>
 int one(const gl_operand& P, const gl_operand& Q, const gl_epilogue& e, long long I, int J, long long nq, const gl_mm_plan& p,
         float* partial, hipStream_t st) {
     if (p.parts > 1) {
-        const Out o = {nullptr, nullptr, 0, partial, J, nullptr, 0, GL_ACT_NONE, nullptr, I * J, 0};
+        const Out o = {nullptr, nullptr, 0, partial, J, nullptr, 0, GL_ACT_NONE, nullptr, I * J, 0, e.scale_p, e.scale_q};
         const int rc = p.kind == 2 ? walk<T, float, TB, SEG, GL_ACT_NONE, false, PT, QT>(P, Q, o, I, J, nq, p, st)
                      : p.kind == 1 ? tiles<T, float, TB, SEG, 128, 64, PT, QT>(P, Q, o, I, J, nq, p, st)
                                    : small<T, float, TB, SEG, PT, QT>(P, Q, o, I, J, nq, p, st);
@@ -78,8 +78,9 @@ int one(const gl_operand& P, const gl_operand& Q, const gl_epilogue& e, long lon
         j.partial = partial;
         return gl_dense_join<TB, TO>(j, I, J, p.parts, st);
     }
-    const Out o = {e.bias, e.residual, e.r_stride, e.y, e.y_stride, e.z, e.z_stride, e.act, e.flags, 0, sizeof(TO) == 2 && (e.y_stride % 2 || (uintptr_t)e.y % 4 || (e.z && (e.z_stride % 2 || (uintptr_t)e.z % 4)) ||
-                                                             (e.residual && (e.r_stride % 2 || (uintptr_t)e.residual % 4)))};
+    auto off4 = [](const void* q, long long stride) { return q && (stride % 2 || (uintptr_t)q % 4); };
+    const int odd = sizeof(TO) == 2 && (off4(e.y, e.y_stride) || off4(e.z, e.z_stride) || off4(e.residual, e.r_stride));
+    const Out o = {e.bias, e.residual, e.r_stride, e.y, e.y_stride, e.z, e.z_stride, e.act, e.flags, 0, odd, e.scale_p, e.scale_q};
     if (p.kind == 0) return small<T, TO, TB, SEG, PT, QT>(P, Q, o, I, J, nq, p, st);
     if (p.kind == 1) return tiles<T, TO, TB, SEG, 128, 64, PT, QT>(P, Q, o, I, J, nq, p, st);
     if constexpr (PT || QT) return walk<T, TO, TB, SEG, GL_ACT_NONE, false, PT, QT>(P, Q, o, I, J, nq, p, st);   // gradients: no epilogue
@@ -115,10 +116,13 @@ int gl_mm16(const gl_operand& P, const gl_operand& Q, gl_epilogue e, long long I
         f.y = (TO*)e.y + j;
         if (e.z) f.z = (TO*)e.z + j;
         if (e.exact_q) f.exact_q = e.exact_q + j * e.exact_q_is;
+        if (e.scale_q) f.scale_q = e.scale_q + j;
         const gl_mm_plan p = gl_mm_plan_for(I, n, pad, pt && qt);
-        const int rc = !pt && !qt ? gl_mm::one<T, TO, TB, SEG, false, false>(P, q, f, I, n, nq, p, partial, st)
-                     : !pt        ? gl_mm::one<T, TO, TB, SEG, false, true>(P, q, f, I, n, nq, p, partial, st)
-                                  : gl_mm::one<T, TO, TB, SEG, true, true>(P, q, f, I, n, nq, p, partial, st);
+        int rc;
+        if (SEG == 3 || (!pt && !qt)) rc = gl_mm::one<T, TO, TB, SEG, false, false>(P, q, f, I, n, nq, p, partial, st);
+        else if constexpr (SEG != 3)
+            rc = !pt ? gl_mm::one<T, TO, TB, SEG, false, true>(P, q, f, I, n, nq, p, partial, st)
+                     : gl_mm::one<T, TO, TB, SEG, true, true>(P, q, f, I, n, nq, p, partial, st);
         if (rc) return rc;
         if (SEG > 1 && p.parts == 1) {                       // the blocks that were left out, if any
             const int rf = gl_dense_flagged(f, I, n, nq, st);

@@ -311,6 +311,33 @@ def test_dense_full_precision_values_that_are_not_finite():
 
 
 @gpu
+@pytest.mark.parametrize("M,K,N", [(4400, 512, 2048), (64, 16384, 2064), (9000, 513, 600), (30000, 264, 1024)])
+def test_dense_full_precision_over_wide_ranges(M, K, N):
+    """Rows whose small values alone reach the result: a large one times zero, magnitudes over the range of float32."""
+    x, w, b = randn((M, K), F32, 1).cuda(), randn((N, K), F32, 2).cuda(), randn((N,), F32, 3).cuda()
+    r = randn((M, N), F32, 4).cuda()
+    w[:, 0] = 0.0
+    w[5] *= 2.0 ** torch.linspace(-80, 20, K, device="cuda").round()
+    w[N - 1], w[7] = 0.0, 1e-38
+    x[1] *= 1e-8
+    x[1, 0] = 1e10                                        # 60 powers of two above the rest, times zero
+    x[40] *= 2.0 ** torch.linspace(-60, 30, K, device="cuda").round()
+    x[41], x[42] = 0.0, torch.finfo(F32).smallest_normal * torch.rand(K, device="cuda")
+    x[M - 1] *= 1e30
+    z64, z_tol, y64, y_tol = dense64(x, w, None, None, None, F32)
+    # a product below the normal range is rounded (or flushed) there: one smallest normal number each at most
+    low = K * torch.finfo(F32).smallest_normal
+    close(inv.dense(x, w), z64.cpu(), z_tol.cpu() + low, "product")
+    z64, z_tol, y64, y_tol = dense64(x, w, b, "silu", r, F32)
+    keep = r.clone()
+    z = torch.empty_like(r)
+    got = inv.dense(x, w, b, activation="silu", residual=r, preactivation=z, out=r)
+    close(z, z64.cpu(), z_tol.cpu() + low, "preactivation")
+    close(got, y64.cpu(), y_tol.cpu() + 2 * low, "y")
+    assert torch.equal(got, inv.dense(x, w, b, activation="silu", residual=keep))
+
+
+@gpu
 def test_dense_backward_full_precision_values_that_are_not_finite():
     M, K, N = 16500, 512, 264                                                  # dweight: parts of the frames, joined
     x, w, dy = randn((M, K), F32, 1).cuda(), randn((N, K), F32, 2).cuda(), randn((M, N), F32, 3).cuda()
