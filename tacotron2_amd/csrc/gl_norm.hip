@@ -300,12 +300,11 @@ __global__ void __launch_bounds__(kMaxThreads) k_norm_slab(const T* x, long long
     for (int i = 0; i < kHeld; ++i) {
         const int t = p.r + i * p.RP;
         if (t >= Tn) continue;
-        vT o;
+        vT o = vT{};
+        if (t < live)
 #pragma unroll
-        for (int k = 0; k < V; ++k) {
-            const float u = fmaf(get<T, V>(held[i], k) - mean[k], ga[k], be[k]);
-            set<T, V>(o, k, t < live ? gl_act(u, ACT < 0 ? act : ACT) : 0.0f);
-        }
+            for (int k = 0; k < V; ++k)
+                set<T, V>(o, k, gl_act(fmaf(get<T, V>(held[i], k) - mean[k], ga[k], be[k]), ACT < 0 ? act : ACT));
         *(vT*)(yb + (long long)t * y_stride) = o;
     }
 }
@@ -452,13 +451,18 @@ __global__ void __launch_bounds__(kMaxThreads) k_norm_apply(const T* x, long lon
 
 // ---- gradients ----
 
-// du and xh of one vector
+// Of one element: d = x - mean and du; slope = rstd gamma.  Sums of du xh are those of du d, times rstd.
 template <typename T, int V, int ACT>
-__device__ __forceinline__ void du_xh(const typename vec_of<T, V>::type& x, const typename vec_of<T, V>::type& dy, int k, float mean,
-                                      float rstd, float ga, float be, int act, float& du, float& xh) {
-    xh = (get<T, V>(x, k) - mean) * rstd;
-    du = get<T, V>(dy, k) * gl_act_grad(fmaf(xh, ga, be), ACT < 0 ? act : ACT);
+__device__ __forceinline__ void du_d(const typename vec_of<T, V>::type& x, const typename vec_of<T, V>::type& dy, int k, float mean,
+                                     float slope, float be, int act, float& du, float& d) {
+    d = get<T, V>(x, k) - mean;
+    du = get<T, V>(dy, k) * gl_act_grad(fmaf(d, slope, be), ACT < 0 ? act : ACT);
 }
+// dx = rstd (du gamma - p - xh q) = du slope + d cq + cp
+struct Back {
+    float cp, cq;
+};
+__device__ __forceinline__ Back back_of(float rstd, float p, float q) { return {-rstd * p, -rstd * (rstd * q)}; }
 
 // One pass, as k_norm_slab.  sums [B][2][C]: sum du xh, sum du per channel of the utterance
 template <typename T, int V, int ACT, bool EVEN>
@@ -490,7 +494,7 @@ __global__ void __launch_bounds__(kBackThreads<T>) k_norm_back_slab(const T* dy,
     }
     float du[kHeld][V];                                      // in place of dy from here on: the activation's slope is
                                                              // worked out once
-    float ga[V], be[V], mean[V], rstd[V], a0[V], a1[V];
+    float ga[V], be[V], mean[V], rstd[V], slope[V], a0[V], a1[V];
 #pragma unroll
     for (int k = 0; k < V; ++k) a0[k] = a1[k] = 0.0f;
     if (p.on) {
@@ -506,20 +510,25 @@ __global__ void __launch_bounds__(kBackThreads<T>) k_norm_back_slab(const T* dy,
         } else {
             load_pairs<V>(stats + 2 * (long long)b * (C / n), c, n, mean, rstd);
         }
+#pragma unroll
+        for (int k = 0; k < V; ++k) slope[k] = rstd[k] * ga[k];
     }
 #pragma unroll
     for (int i = 0; i < kHeld; ++i)
         if (p.on && p.r + i * p.RP < live)
 #pragma unroll
             for (int k = 0; k < V; ++k) {
-                float xh;
-                du_xh<T, V, ACT>(hx[i], hd[i], k, mean[k], rstd[k], ga[k], be[k], act, du[i][k], xh);
-                a0[k] = fmaf(du[i][k], xh, a0[k]);
+                float d;
+                du_d<T, V, ACT>(hx[i], hd[i], k, mean[k], slope[k], be[k], act, du[i][k], d);
+                a0[k] = fmaf(du[i][k], d, a0[k]);
                 a1[k] += du[i][k];
             }
+    if (p.on)
+#pragma unroll
+        for (int k = 0; k < V; ++k) a0[k] *= rstd[k];
     const Lanes l = lanes_of<V>(p, n);
     const float scale = live ? 1.0f / (float)((long long)live * n) : 0.0f;
-    float gp[V], gq[V];
+    Back end[V];
     if constexpr (EVEN) {
         float vp = 0.0f, vq = 0.0f;
 #pragma unroll
@@ -537,10 +546,7 @@ __global__ void __launch_bounds__(kBackThreads<T>) k_norm_back_slab(const T* dy,
         vp = group_total(vp, p, l, red) * scale;
         vq = group_total(vq, p, l, red + blockDim.x) * scale;
 #pragma unroll
-        for (int k = 0; k < V; ++k) {
-            gp[k] = vp;
-            gq[k] = vq;
-        }
+        for (int k = 0; k < V; ++k) end[k] = back_of(rstd[k], vp, vq);
     } else {
         channel_sums<V>(a0, p, red, tot);
         channel_sums<V>(a1, p, red, tot + CB);
@@ -557,10 +563,7 @@ __global__ void __launch_bounds__(kBackThreads<T>) k_norm_back_slab(const T* dy,
         group_sums(p, n, pq + CB / n, [&](int k) { return tot[k]; });
         if (!p.on) return;
 #pragma unroll
-        for (int k = 0; k < V; ++k) {
-            gp[k] = pq[(p.col + k) / n] * scale;
-            gq[k] = pq[CB / n + (p.col + k) / n] * scale;
-        }
+        for (int k = 0; k < V; ++k) end[k] = back_of(rstd[k], pq[(p.col + k) / n] * scale, pq[CB / n + (p.col + k) / n] * scale);
     }
     T* ob = dx + (long long)b * Tn * dx_stride + c;
 #pragma unroll
@@ -570,10 +573,8 @@ __global__ void __launch_bounds__(kBackThreads<T>) k_norm_back_slab(const T* dy,
         vT o = vT{};
         if (t < live)
 #pragma unroll
-            for (int k = 0; k < V; ++k) {
-                const float xh = (get<T, V>(hx[i], k) - mean[k]) * rstd[k];
-                set<T, V>(o, k, rstd[k] * (du[i][k] * ga[k] - gp[k] - xh * gq[k]));
-            }
+            for (int k = 0; k < V; ++k)
+                set<T, V>(o, k, fmaf(du[i][k], slope[k], fmaf(get<T, V>(hx[i], k) - mean[k], end[k].cq, end[k].cp)));
         *(vT*)(ob + (long long)t * dx_stride) = o;
     }
 }
@@ -593,12 +594,14 @@ __global__ void __launch_bounds__(kMaxThreads) k_norm_back_chunk(const T* __rest
     const int b = blockIdx.y;
     const int live = live_frames(frames, b, Tn);
     const int t0 = blockIdx.x * rows, t1 = min(t0 + rows, live);
-    float ga[V], be[V], mean[V], rstd[V], a0[V], a1[V];
+    float slope[V], be[V], mean[V], rstd[V], a0[V], a1[V];
 #pragma unroll
     for (int k = 0; k < V; ++k) a0[k] = a1[k] = 0.0f;
     if (p.on) {
-        load_affine<T, V>(gamma, beta, p.col, ga, be);
+        load_affine<T, V>(gamma, beta, p.col, slope, be);
         load_pairs<V>(stats + 2 * (long long)b * (C / n), p.col, n, mean, rstd);
+#pragma unroll
+        for (int k = 0; k < V; ++k) slope[k] *= rstd[k];
         const T* xb = x + (long long)b * Tn * x_stride + p.col;
         const T* db = dy + (long long)b * Tn * dy_stride + p.col;
 #pragma unroll 4
@@ -607,12 +610,14 @@ __global__ void __launch_bounds__(kMaxThreads) k_norm_back_chunk(const T* __rest
             const vT vd = *(const vT*)(db + (long long)t * dy_stride);
 #pragma unroll
             for (int k = 0; k < V; ++k) {
-                float du, xh;
-                du_xh<T, V, ACT>(vx, vd, k, mean[k], rstd[k], ga[k], be[k], act, du, xh);
-                a0[k] = fmaf(du, xh, a0[k]);
+                float du, d;
+                du_d<T, V, ACT>(vx, vd, k, mean[k], slope[k], be[k], act, du, d);
+                a0[k] = fmaf(du, d, a0[k]);
                 a1[k] += du;
             }
         }
+#pragma unroll
+        for (int k = 0; k < V; ++k) a0[k] *= rstd[k];
     }
     float* o = parts + ((long long)b * gridDim.x + blockIdx.x) * 2 * C;
     const bool even = (p.TP & (p.TP - 1)) == 0;
@@ -665,9 +670,9 @@ __global__ void __launch_bounds__(kMaxThreads) k_norm_back_apply(const T* dy, lo
     const Place p = place<V>(C);
     const int b = blockIdx.y;
     const int live = live_frames(frames, b, Tn);
-    float ga[V], be[V], mean[V], rstd[V], gp[V], gq[V];
+    float slope[V], be[V], mean[V], rstd[V];
     if (p.on) {
-        load_affine<T, V>(gamma, beta, p.col, ga, be);
+        load_affine<T, V>(gamma, beta, p.col, slope, be);
         load_pairs<V>(stats + 2 * (long long)b * (C / n), p.col, n, mean, rstd);
     }
     float* pairs = lds + 2 * C;
@@ -696,7 +701,16 @@ __global__ void __launch_bounds__(kMaxThreads) k_norm_back_apply(const T* dy, lo
     }
     __syncthreads();
     if (!p.on) return;
-    load_pairs<V>(pairs, p.col, n, gp, gq);
+    Back end[V];
+    {
+        float gp[V], gq[V];
+        load_pairs<V>(pairs, p.col, n, gp, gq);
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            slope[k] *= rstd[k];
+            end[k] = back_of(rstd[k], gp[k], gq[k]);
+        }
+    }
     const T* xb = x + (long long)b * Tn * x_stride + p.col;
     const T* db = dy + (long long)b * Tn * dy_stride + p.col;
     T* ob = dx + (long long)b * Tn * dx_stride + p.col;
@@ -709,9 +723,9 @@ __global__ void __launch_bounds__(kMaxThreads) k_norm_back_apply(const T* dy, lo
             const vT vd = *(const vT*)(db + (long long)t * dy_stride);
 #pragma unroll
             for (int k = 0; k < V; ++k) {
-                float du, xh;
-                du_xh<T, V, ACT>(vx, vd, k, mean[k], rstd[k], ga[k], be[k], act, du, xh);
-                set<T, V>(o, k, rstd[k] * (du * ga[k] - gp[k] - xh * gq[k]));
+                float du, d;
+                du_d<T, V, ACT>(vx, vd, k, mean[k], slope[k], be[k], act, du, d);
+                set<T, V>(o, k, fmaf(du, slope[k], fmaf(d, end[k].cq, end[k].cp)));
             }
         }
         *(vT*)(ob + (long long)t * dx_stride) = o;
