@@ -243,6 +243,12 @@ __device__ __forceinline__ void any_tiles(const AnyArgs& a, long long first, lon
 // grid (workgroups, parts); workgroups walk over the tiles.  flags: only the tiles whose flag is set.
 template <typename T, typename TO, int V>
 __global__ void __launch_bounds__(256) k_dense_any(AnyArgs a, const int* __restrict__ flags) {
+    if (flags) {                                             // all of this workgroup's at once: there is hardly ever one
+        int set = 0;
+        for (long long tile = blockIdx.x + (long long)threadIdx.x * gridDim.x; tile < a.n_tiles; tile += 256LL * gridDim.x)
+            set |= flags[tile];
+        if (!__syncthreads_or(set)) return;
+    }
     any_tiles<T, TO, T, V, false>(a, blockIdx.x, gridDim.x, blockIdx.y, flags);
 }
 
@@ -979,7 +985,7 @@ int gl_dense_flagged(const gl_epilogue& e, long long I, int J, long long nq, hip
     f.quads = quads<float>(e, J);
     const AnyArgs a = {{e.exact_p, e.exact_p_is, e.exact_p_qs}, {e.exact_q, e.exact_q_is, e.exact_q_qs}, {}, f, I, nq, nq, J,
                        (int)gl_ceil_div(J, kTile), (int)tiles, GL_ACT_NONE, e.exact_p_qs == 1, e.exact_q_qs == 1, nullptr, nullptr};
-    hipLaunchKernelGGL((k_dense_any<float, float, 1>), dim3((unsigned)(tiles < 8192 ? tiles : 8192)), dim3(256), 0, st, a, e.flags);
+    hipLaunchKernelGGL((k_dense_any<float, float, 1>), dim3((unsigned)(tiles < 512 ? tiles : 512)), dim3(256), 0, st, a, e.flags);
     GL_HIP_CHECK(hipGetLastError());
     return 0;
 }
