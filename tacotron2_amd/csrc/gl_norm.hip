@@ -10,6 +10,8 @@
 // 256 MB cache behind the L2s where it fits.  Variances are sums of squared distances from a mean already known (of the slab
 // or the chunk, joined with the distances between the means), never a difference of large sums.  All sums run in a
 // fixed order.
+#include <initializer_list>
+
 #include "gl_internal.h"
 #include "gl_act.h"
 
@@ -38,6 +40,13 @@ template <typename T, int V>
 __device__ __forceinline__ void set(typename vec_of<T, V>::type& v, int k, float f) {
     if constexpr (V == 1) v = (T)f;
     else v[k] = (T)f;
+}
+
+// f(gl_int<the activation>): the kernel's own where it has one, else the argument's, chosen once around f's loop
+template <int ACT, typename F>
+__device__ __forceinline__ void act_for(int act, const F& f) {
+    if constexpr (ACT < 0) gl_with_act(act, f);
+    else f(gl_int<ACT>());
 }
 
 // Where a workgroup works: CB channels from c0 (whole groups), threads as rows x TP vectors.
@@ -296,17 +305,18 @@ __global__ void __launch_bounds__(kMaxThreads) k_norm_slab(const T* x, long long
     }
     if (!p.on) return;
     T* yb = y + (long long)b * Tn * y_stride + c;
+    act_for<ACT>(act, [&](auto a) {
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) {
-        const int t = p.r + i * p.RP;
-        if (t >= Tn) continue;
-        vT o = vT{};
-        if (t < live)
+        for (int i = 0; i < kHeld; ++i) {
+            const int t = p.r + i * p.RP;
+            if (t >= Tn) continue;
+            vT o = vT{};
+            if (t < live)
 #pragma unroll
-            for (int k = 0; k < V; ++k)
-                set<T, V>(o, k, gl_act(fmaf(get<T, V>(held[i], k) - mean[k], ga[k], be[k]), ACT < 0 ? act : ACT));
-        *(vT*)(yb + (long long)t * y_stride) = o;
-    }
+                for (int k = 0; k < V; ++k) set<T, V>(o, k, gl_act(fmaf(get<T, V>(held[i], k) - mean[k], ga[k], be[k]), decltype(a)::value));
+            *(vT*)(yb + (long long)t * y_stride) = o;
+        }
+    });
 }
 
 // Chunks of RP * kHeld frames, all channels: mean and sum of squared distances per group.  grid (chunks, B);
@@ -436,17 +446,18 @@ __global__ void __launch_bounds__(kMaxThreads) k_norm_apply(const T* x, long lon
     const T* xb = x + (long long)b * Tn * x_stride + p.col;
     T* yb = y + (long long)b * Tn * y_stride + p.col;
     const int step = gridDim.x * p.RP;
+    act_for<ACT>(act, [&](auto a) {
 #pragma unroll 4
-    for (int t = blockIdx.x * p.RP + p.r; t < Tn; t += step) {
-        vT o = vT{};
-        if (t < live) {
-            const vT in = *(const vT*)(xb + (long long)t * x_stride);
+        for (int t = blockIdx.x * p.RP + p.r; t < Tn; t += step) {
+            vT o = vT{};
+            if (t < live) {
+                const vT in = *(const vT*)(xb + (long long)t * x_stride);
 #pragma unroll
-            for (int k = 0; k < V; ++k)
-                set<T, V>(o, k, gl_act(fmaf(get<T, V>(in, k) - mean[k], ga[k], be[k]), ACT < 0 ? act : ACT));
+                for (int k = 0; k < V; ++k) set<T, V>(o, k, gl_act(fmaf(get<T, V>(in, k) - mean[k], ga[k], be[k]), decltype(a)::value));
+            }
+            *(vT*)(yb + (long long)t * y_stride) = o;
         }
-        *(vT*)(yb + (long long)t * y_stride) = o;
-    }
+    });
 }
 
 // ---- gradients ----
@@ -454,9 +465,9 @@ __global__ void __launch_bounds__(kMaxThreads) k_norm_apply(const T* x, long lon
 // Of one element: d = x - mean and du; slope = rstd gamma.  Sums of du xh are those of du d, times rstd.
 template <typename T, int V, int ACT>
 __device__ __forceinline__ void du_d(const typename vec_of<T, V>::type& x, const typename vec_of<T, V>::type& dy, int k, float mean,
-                                     float slope, float be, int act, float& du, float& d) {
+                                     float slope, float be, float& du, float& d) {
     d = get<T, V>(x, k) - mean;
-    du = get<T, V>(dy, k) * gl_act_grad(fmaf(d, slope, be), ACT < 0 ? act : ACT);
+    du = get<T, V>(dy, k) * gl_act_grad(fmaf(d, slope, be), ACT);
 }
 // dx = rstd (du gamma - p - xh q) = du slope + d cq + cp
 struct Back {
@@ -516,13 +527,15 @@ __global__ void __launch_bounds__(kBackThreads<T>) k_norm_back_slab(const T* dy,
 #pragma unroll
     for (int i = 0; i < kHeld; ++i)
         if (p.on && p.r + i * p.RP < live)
+            act_for<ACT>(act, [&](auto a) {
 #pragma unroll
-            for (int k = 0; k < V; ++k) {
-                float d;
-                du_d<T, V, ACT>(hx[i], hd[i], k, mean[k], slope[k], be[k], act, du[i][k], d);
-                a0[k] = fmaf(du[i][k], d, a0[k]);
-                a1[k] += du[i][k];
-            }
+                for (int k = 0; k < V; ++k) {
+                    float d;
+                    du_d<T, V, decltype(a)::value>(hx[i], hd[i], k, mean[k], slope[k], be[k], du[i][k], d);
+                    a0[k] = fmaf(du[i][k], d, a0[k]);
+                    a1[k] += du[i][k];
+                }
+            });
     if (p.on)
 #pragma unroll
         for (int k = 0; k < V; ++k) a0[k] *= rstd[k];
@@ -604,18 +617,20 @@ __global__ void __launch_bounds__(kMaxThreads) k_norm_back_chunk(const T* __rest
         for (int k = 0; k < V; ++k) slope[k] *= rstd[k];
         const T* xb = x + (long long)b * Tn * x_stride + p.col;
         const T* db = dy + (long long)b * Tn * dy_stride + p.col;
+        act_for<ACT>(act, [&](auto a) {
 #pragma unroll 4
-        for (int t = t0 + p.r; t < t1; t += p.RP) {
-            const vT vx = *(const vT*)(xb + (long long)t * x_stride);
-            const vT vd = *(const vT*)(db + (long long)t * dy_stride);
+            for (int t = t0 + p.r; t < t1; t += p.RP) {
+                const vT vx = *(const vT*)(xb + (long long)t * x_stride);
+                const vT vd = *(const vT*)(db + (long long)t * dy_stride);
 #pragma unroll
-            for (int k = 0; k < V; ++k) {
-                float du, d;
-                du_d<T, V, ACT>(vx, vd, k, mean[k], slope[k], be[k], act, du, d);
-                a0[k] = fmaf(du, d, a0[k]);
-                a1[k] += du;
+                for (int k = 0; k < V; ++k) {
+                    float du, d;
+                    du_d<T, V, decltype(a)::value>(vx, vd, k, mean[k], slope[k], be[k], du, d);
+                    a0[k] = fmaf(du, d, a0[k]);
+                    a1[k] += du;
+                }
             }
-        }
+        });
 #pragma unroll
         for (int k = 0; k < V; ++k) a0[k] *= rstd[k];
     }
@@ -715,21 +730,23 @@ __global__ void __launch_bounds__(kMaxThreads) k_norm_back_apply(const T* dy, lo
     const T* db = dy + (long long)b * Tn * dy_stride + p.col;
     T* ob = dx + (long long)b * Tn * dx_stride + p.col;
     const int step = gridDim.x * p.RP;
+    act_for<ACT>(act, [&](auto a) {
 #pragma unroll 2
-    for (int t = blockIdx.x * p.RP + p.r; t < Tn; t += step) {
-        vT o = vT{};
-        if (t < live) {
-            const vT vx = *(const vT*)(xb + (long long)t * x_stride);
-            const vT vd = *(const vT*)(db + (long long)t * dy_stride);
+        for (int t = blockIdx.x * p.RP + p.r; t < Tn; t += step) {
+            vT o = vT{};
+            if (t < live) {
+                const vT vx = *(const vT*)(xb + (long long)t * x_stride);
+                const vT vd = *(const vT*)(db + (long long)t * dy_stride);
 #pragma unroll
-            for (int k = 0; k < V; ++k) {
-                float du, d;
-                du_d<T, V, ACT>(vx, vd, k, mean[k], slope[k], be[k], act, du, d);
-                set<T, V>(o, k, fmaf(du, slope[k], fmaf(d, end[k].cq, end[k].cp)));
+                for (int k = 0; k < V; ++k) {
+                    float du, d;
+                    du_d<T, V, decltype(a)::value>(vx, vd, k, mean[k], slope[k], be[k], du, d);
+                    set<T, V>(o, k, fmaf(du, slope[k], fmaf(d, end[k].cq, end[k].cp)));
+                }
             }
+            *(vT*)(ob + (long long)t * dx_stride) = o;
         }
-        *(vT*)(ob + (long long)t * dx_stride) = o;
-    }
+    });
 }
 
 // ---- any size and alignment, element by element ----
@@ -877,9 +894,6 @@ int check_workspace(const void* ws, long long have, long long need, const char* 
 
 long long stats_bytes(int B, int groups) { return align16(8LL * B * groups); }
 
-// Channels a load moves: 16 bytes where rows and channels allow, else one.
-bool vector_ok(const void* p, long long stride, int size) { return (uintptr_t)p % 16 == 0 && stride * size % 16 == 0; }
-
 size_t lds_bytes(int threads, int V, int CB, int n, int totals) {
     return sizeof(float) * ((size_t)threads * (V > 1 ? V : 2) + (size_t)totals * CB + 2 * (size_t)(CB / n));
 }
@@ -945,27 +959,38 @@ bool even_blocks(const Cut& c, int C, int n, int V) {
     return n % V == 0 && pow2(n / V) && n / V <= 64 && pow2(c.blocks.CB / V) && pow2(last / V);
 }
 
-template <int ACT> struct act_tag { static constexpr int value = ACT; };
-// f(act_tag<the activation>) where the vector kernels fix it, f(act_tag<-1>) elsewhere
-template <int V, typename F>
+// f(gl_int<the activation>) where loads are of 16 bytes, f(gl_int<-1>) elsewhere: those kernels choose by themselves
+template <bool FIXED, typename F>
 int with_act(int act, F f) {
-    if constexpr (V == 1) return f(act_tag<-1>());
+    if constexpr (!FIXED) return f(gl_int<-1>());
     else
         switch (act) {
-            case GL_ACT_RELU: return f(act_tag<GL_ACT_RELU>());
-            case GL_ACT_SILU: return f(act_tag<GL_ACT_SILU>());
-            case GL_ACT_GELU: return f(act_tag<GL_ACT_GELU>());
-            case GL_ACT_TANH: return f(act_tag<GL_ACT_TANH>());
-            case GL_ACT_EXP: return f(act_tag<GL_ACT_EXP>());
-            default: return f(act_tag<GL_ACT_NONE>());
+            case GL_ACT_RELU: return f(gl_int<GL_ACT_RELU>());
+            case GL_ACT_SILU: return f(gl_int<GL_ACT_SILU>());
+            case GL_ACT_GELU: return f(gl_int<GL_ACT_GELU>());
+            case GL_ACT_TANH: return f(gl_int<GL_ACT_TANH>());
+            case GL_ACT_EXP: return f(gl_int<GL_ACT_EXP>());
+            default: return f(gl_int<GL_ACT_NONE>());
         }
+}
+// How many channels are moved at once: 16 bytes, or as much of that as divides the channels and the arrays' alignment.
+struct Array {
+    const void* p;
+    long long stride;
+};
+int channels_at_once(int C, int size, std::initializer_list<Array> arrays) {
+    int V = 16 / size;
+    for (const Array& a : arrays)
+        while (a.p && V > 1 && ((uintptr_t)a.p % (V * size) || a.stride % V)) V /= 2;
+    while (C % V) V /= 2;
+    return V;
 }
 
 // workspace: [statistics where the caller wants none] [parts of the chunks]
 long long parts_bytes(int B, int T, int C, int groups, int dtype) {
     const int size = dtype == GL_F32 ? 4 : 2;
     long long most = 0;
-    for (int V : {16 / size, 1}) {                           // alignment is not known to the query
+    for (int V = 16 / size; V; V /= 2) {                     // alignment is not known to the query
         if (C % V) continue;
         const Cut c = cut_for(B, T, C, groups, size, V, kMaxThreads, kRowBytes);
         if (c.kind == 1 && 8LL * B * groups * c.chunks > most) most = 8LL * B * groups * c.chunks;
@@ -975,7 +1000,7 @@ long long parts_bytes(int B, int T, int C, int groups, int dtype) {
 long long norm_bytes(int B, int T, int C, int groups, int dtype) {
     const int size = dtype == GL_F32 ? 4 : 2;
     bool slabs = B && T;
-    for (int V : {16 / size, 1})
+    for (int V = 16 / size; V; V /= 2)
         if (slabs && C % V == 0) slabs = cut_for(B, T, C, groups, size, V, kMaxThreads, kRowBytes).kind == 0;
     return slabs ? 0 : stats_bytes(B, groups) + (B && T ? parts_bytes(B, T, C, groups, dtype) : 0);
 }
@@ -1002,7 +1027,7 @@ int norm_fwd(const Norm& a, void* y, long long y_stride, float* stats, float* gi
     const T *x = (const T*)a.x, *ga = (const T*)a.gamma, *be = (const T*)a.beta;
     Cut c = a.T ? cut_for(a.B, a.T, a.C, a.groups, sizeof(T), V, kMaxThreads, kRowBytes) : Cut{2};
     if (c.kind == 0)
-        return with_act<V>(a.act, [&](auto act) -> int {
+        return with_act<V * sizeof(T) == 16>(a.act, [&](auto act) -> int {
             const bool even = even_blocks(c, a.C, n, V);
             auto kernel = even ? k_norm_slab<T, V, decltype(act)::value, true> : k_norm_slab<T, V, decltype(act)::value, false>;
             hipLaunchKernelGGL(kernel, dim3((unsigned)((c.blocks.total + 7) / 8 * 8)), dim3(c.threads), lds_bytes(c.threads, V, c.blocks.CB, n, 1), a.st, x, a.x_stride, ga, be, a.frames,
@@ -1016,7 +1041,7 @@ int norm_fwd(const Norm& a, void* y, long long y_stride, float* stats, float* gi
         GL_HIP_CHECK(hipGetLastError());
         hipLaunchKernelGGL(k_norm_join, dim3(a.groups, a.B), dim3(256), 0, a.st, parts, a.frames, stats, a.T, n, c.chunks, c.rows, eps);
         GL_HIP_CHECK(hipGetLastError());
-        return with_act<V>(a.act, [&](auto act) -> int {
+        return with_act<V * sizeof(T) == 16>(a.act, [&](auto act) -> int {
             hipLaunchKernelGGL((k_norm_apply<T, V, decltype(act)::value>),
                                dim3(apply_blocks(a.B, a.T, c.threads / (a.C / V)), a.B), dim3(c.threads), 0, a.st, x, a.x_stride,
                                ga, be, a.frames, stats, (T*)y, y_stride, a.T, a.C, n, a.act);
@@ -1041,7 +1066,7 @@ int norm_back(const Norm& a, const void* dy_, long long dy_stride, const float* 
     T* dx = (T*)dx_;
     const Cut c = cut_for(a.B, a.T, a.C, a.groups, sizeof(T), V, kBackThreads<T>, kBackRowBytes);
     if (c.kind == 0)
-        return with_act<V>(a.act, [&](auto act) -> int {
+        return with_act<V * sizeof(T) == 16>(a.act, [&](auto act) -> int {
             const bool even = even_blocks(c, a.C, n, V);
             auto kernel = even ? k_norm_back_slab<T, V, decltype(act)::value, true> : k_norm_back_slab<T, V, decltype(act)::value, false>;
             hipLaunchKernelGGL(kernel, dim3((unsigned)((c.blocks.total + 7) / 8 * 8)), dim3(c.threads), lds_bytes(c.threads, V, c.blocks.CB, n, 2), a.st, dy, dy_stride, x, a.x_stride,
@@ -1052,7 +1077,7 @@ int norm_back(const Norm& a, const void* dy_, long long dy_stride, const float* 
     if (c.kind == 1) {
         const int rows = back_rows(a.B, a.T), chunks = (int)ceil_div(a.T, rows);
         *done = a.B == 1;                                    // the join writes dgamma and dbeta
-        return with_act<V>(a.act, [&](auto act) -> int {
+        return with_act<V * sizeof(T) == 16>(a.act, [&](auto act) -> int {
             constexpr int ACT = decltype(act)::value;
             hipLaunchKernelGGL((k_norm_back_chunk<T, V, ACT>), dim3(chunks, a.B), dim3(c.threads),
                                lds_bytes(c.threads, V, a.C, n, 1), a.st, dy, dy_stride, x, a.x_stride, stats, ga, be, a.frames, parts,
@@ -1103,12 +1128,16 @@ int gl_group_norm(const void* x, long long x_stride, const void* gamma, const vo
     float* s = stats ? stats : (float*)workspace;
     float* parts = (float*)((char*)workspace + stats_bytes(B, groups));
     const Norm a = {x, x_stride, gamma, beta, frames, B, T, channels, groups, activation, (hipStream_t)stream};
-    const int size = dtype == GL_F32 ? 4 : 2, full = 16 / size;
-    const bool wide = channels % full == 0 && vector_ok(x, x_stride, size) && vector_ok(y, y_stride, size);
-#define GL_NORM(T_, V) norm_fwd<T_, V>(a, y, y_stride, s, stats, parts, eps)
-    if (dtype == GL_F32) return wide ? GL_NORM(float, 4) : GL_NORM(float, 1);
-    if (dtype == GL_BF16) return wide ? GL_NORM(gl_bf16, 8) : GL_NORM(gl_bf16, 1);
-    return wide ? GL_NORM(gl_f16, 8) : GL_NORM(gl_f16, 1);
+    const int V = channels_at_once(channels, dtype == GL_F32 ? 4 : 2, {{x, x_stride}, {y, y_stride}});
+#define GL_NORM(T_, V_) \
+    case V_: return norm_fwd<T_, V_>(a, y, y_stride, s, stats, parts, eps);
+#define GL_NORM16(T_) \
+    switch (V) { GL_NORM(T_, 8) GL_NORM(T_, 4) GL_NORM(T_, 2) GL_NORM(T_, 1) }
+    if (dtype == GL_BF16) GL_NORM16(gl_bf16)
+    else if (dtype == GL_F16) GL_NORM16(gl_f16)
+    else switch (V) { GL_NORM(float, 4) GL_NORM(float, 2) GL_NORM(float, 1) }
+    return 0;                                                // not reached
+#undef GL_NORM16
 #undef GL_NORM
 }
 
@@ -1137,13 +1166,15 @@ int gl_group_norm_backward(const void* dy, long long dy_stride, const void* x, l
         if (rc) return rc;
         float* parts = (float*)((char*)sums + align16(8LL * B * channels));
         const Norm a = {x, x_stride, gamma, beta, frames, B, T, channels, groups, activation, st};
-        const int size = dtype == GL_F32 ? 4 : 2, full = 16 / size;
-        const bool wide = channels % full == 0 && vector_ok(x, x_stride, size) && vector_ok(dy, dy_stride, size) &&
-                          (!dx || vector_ok(dx, dx_stride, size));
-#define GL_NORM(T_, V) norm_back<T_, V>(a, dy, dy_stride, stats, dx, dx_stride, pq, sums, parts, dgamma, dbeta, &done)
-        if (dtype == GL_F32) rc = wide ? GL_NORM(float, 4) : GL_NORM(float, 1);
-        else if (dtype == GL_BF16) rc = wide ? GL_NORM(gl_bf16, 8) : GL_NORM(gl_bf16, 1);
-        else rc = wide ? GL_NORM(gl_f16, 8) : GL_NORM(gl_f16, 1);
+        const int V = channels_at_once(channels, dtype == GL_F32 ? 4 : 2, {{x, x_stride}, {dy, dy_stride}, {dx, dx_stride}});
+#define GL_NORM(T_, V_)                                                                                                        \
+    case V_: rc = norm_back<T_, V_>(a, dy, dy_stride, stats, dx, dx_stride, pq, sums, parts, dgamma, dbeta, &done); break;
+#define GL_NORM16(T_) \
+    switch (V) { GL_NORM(T_, 8) GL_NORM(T_, 4) GL_NORM(T_, 2) GL_NORM(T_, 1) }
+        if (dtype == GL_BF16) GL_NORM16(gl_bf16)
+        else if (dtype == GL_F16) GL_NORM16(gl_f16)
+        else switch (V) { GL_NORM(float, 4) GL_NORM(float, 2) GL_NORM(float, 1) }
+#undef GL_NORM16
 #undef GL_NORM
         if (rc) return rc;
     }
