@@ -784,7 +784,9 @@ int rows_per_part(long long rows, int outputs) {
     return (int)(r < 16 ? 16 : r);
 }
 
-// One product of k_dense_back_small: parts for one workgroup a CU, of two steps at least, or for two, of eight.
+// One product of k_dense_back_small: parts for one workgroup a CU, of two steps at least, or for two, of eight; and no more
+// than balance a part's steps with the join, where eight parts cost what a step does (24 125 x 64 -> 64 bf16: dweight in 256
+// parts 44 us, in 78 32 us).
 struct SmallSplit {
     long long tiles, per;
     int parts;
@@ -796,7 +798,9 @@ SmallSplit small_split(long long I, int J, long long nq) {
         const long long fill = workgroups / s.tiles, most = nq / (steps * kBQ);
         return fill < most ? fill : most;
     };
-    const long long one = parts(kCUs, 2), two = parts(2 * kCUs, 8), most = one > two ? one : two;
+    const long long one = parts(kCUs, 2), two = parts(2 * kCUs, 8);
+    long long most = one > two ? one : two;
+    while (most > 1 && 4 * most * most > nq) --most;
     s.per = gl_ceil_div(gl_ceil_div(nq, most > 1 ? most : 1), kBQ) * kBQ;
     s.parts = (int)gl_ceil_div(nq, s.per);
     return s;

@@ -103,21 +103,22 @@ def _p(t):
 
 def _span(t):
     """Bytes [first, last) a tensor reaches."""
-    if t.numel() == 0:
-        return 0, 0
-    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
-    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+    n, first = t.numel(), t.data_ptr()
+    if n and not t.is_contiguous():
+        n = 1 + sum((k - 1) * s for k, s in zip(t.shape, t.stride()))
+    return first, first + n * t.element_size()
 
 
 def _apart(out, what, others, same=()):
     """Refuses an output whose memory an input still needs; `same`: inputs it may be, element for element."""
     a0, a1 = _span(out)
     for name, t in others:
-        if t is None or any(t is s for s in same) and t.data_ptr() == out.data_ptr() and t.stride() == out.stride() \
-                and t.dtype == out.dtype:
+        if t is None:
             continue
         b0, b1 = _span(t)
         if a0 < b1 and b0 < a1:
+            if b0 == a0 and any(t is s for s in same) and t.stride() == out.stride() and t.dtype == out.dtype:
+                continue
             raise ValueError(f"{what} overlaps {name}")
 
 
