@@ -412,7 +412,7 @@ __device__ __forceinline__ int epilogue(const Out& o, f32x4 (&acc)[MI][NI], long
     return put_block<TO, TAIL, LINES, MI, NI>((TO*)o.y + part * o.part_stride, o.y_stride, acc, i0, j0, I, J, lane, o.odd);
 }
 
-// the products h l + l h, which count 2^-12, before h h is added
+// SEG 3: the products h l + l h, which count 2^-12, before h h is added
 template <int MI, int NI>
 __device__ __forceinline__ void lower(f32x4 (&acc)[MI][NI]) {
 #pragma unroll
@@ -423,6 +423,9 @@ __device__ __forceinline__ void lower(f32x4 (&acc)[MI][NI]) {
             for (int r = 0; r < 4; ++r) acc[m][n][r] *= 0x1p-12f;
 }
 
+// A tile a workgroup, for products too small for the walk below: two stages of 64 contraction indexes, two workgroups a CU
+// that cover each other's waits.  Bound by LDS reads (a wave of 64 x 64 reads 8 KiB for 16 matrix instructions): float32 as three
+// products of 6888 x 1024 x 1024 58 to 66 us (43 GF, 700 TF), gradients as six of 13 776 x 512 x 512 48 to 79 us.
 template <typename T, typename TO, typename TB, int SEG, int ACT, int BM, int BN, int WM, int WN, int BK, int ST, bool PT, bool QT, int WPE>
 __global__ void __launch_bounds__(64 * (BM / WM) * (BN / WN), WPE)
 k_mm16(Side P, Side Q, Out o, long long I, int J, long long nq, long long q_per_part, int tiles_j, int n_tiles) {
@@ -509,6 +512,12 @@ k_mm16(Side P, Side Q, Out o, long long I, int J, long long nq, long long q_per_
 // tile's first stages while a tile's results are written.  A step's fragments are read, and the loads of the step RING
 // ahead started, between the products of the step before.
 // A contraction that one side is contiguous in is a multiple of 32 here, J a multiple of BN.
+// 256 x 256 tiles of 8 waves: a wave of 128 x 64 needs 12 KiB of LDS reads for 32 matrix instructions, which leaves room under
+// the LDS rate; 4 stages, one barrier a step.  Two workgroups a CU on 256 x 128 tiles, to cover the epilogue, read half again
+// as much from the L2s: 150 us where this one takes 124, and 181 with gelu where this one takes 179.
+// Measured, bf16: 55 104 x 512 x 2048 124 us (930 TF; 1200 without results), with gelu 155 to 175 (two transcendental
+// and eleven other operations a result, which no product runs under: the wave of both SIMD slots is in its epilogue then);
+// x 1025 exp to float32 89 us for the first 1024; gradients: dx 55 104 x 2048 x 512 115 us (1000 TF), dweight in 16 parts 114 to 124.
 template <typename T, typename TO, typename TB, int SEG, int ACT, bool EXTRA, bool LINES, int BM, int BN, int WM, int WN, int RING, int WGS, bool PT, bool QT>
 __global__ void __launch_bounds__(64 * (BM / WM) * (BN / WN), WGS * (BM / WM) * (BN / WN) / 4)
 k_mm16_walk(Side P, Side Q, Out o, long long I, int J, long long nq, long long q_per_part, int tiles_j, int n_tiles) {

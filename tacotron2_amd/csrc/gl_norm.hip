@@ -202,7 +202,9 @@ __device__ __forceinline__ void channel_totals(float (&v)[V], const Place& p, fl
     __syncthreads();
 }
 
-// One pass: statistics and result of CB channels of utterance b.  grid (blocks of channels x B), see block_of().
+// One pass: statistics and result of CB channels of utterance b.  grid (blocks of channels x B), see block_of().  Bound by
+// memory and the activation's arithmetic in turn (a workgroup loads, sums, then writes; a CU holds few of them): 64 ragged
+// utterances of 861 x 512 bf16 silu 25 us (94 MB, 3.7 TB/s); one utterance of 641 x 512 7.7 us.
 // Neighbouring blocks share cache lines where CB channels are less than 128 bytes: they go to one XCD (ids 8 apart).
 struct Blocks {
     int per_b, total;                    // blocks of channels per utterance, and in all
@@ -320,7 +322,8 @@ __global__ void __launch_bounds__(kMaxThreads) k_norm_slab(const T* x, long long
 }
 
 // Chunks of RP * kHeld frames, all channels: mean and sum of squared distances per group.  grid (chunks, B);
-// parts [B][groups][chunks][2]
+// parts [B][groups][chunks][2].  51 680 x 256 float32: 12.5 us (4.2 TB/s), the join below 3.8, k_norm_apply 18 (5.9 TB/s, its
+// input from the cache).
 template <typename T, int V>
 __global__ void __launch_bounds__(kMaxThreads) k_norm_chunk(const T* __restrict__ x, long long x_stride, const int* __restrict__ frames,
                                                     float* __restrict__ parts, int Tn, int C, int n) {
@@ -475,7 +478,9 @@ struct Back {
 };
 __device__ __forceinline__ Back back_of(float rstd, float p, float q) { return {-rstd * p, -rstd * (rstd * q)}; }
 
-// One pass, as k_norm_slab.  sums [B][2][C]: sum du xh, sum du per channel of the utterance
+// One pass, as k_norm_slab.  sums [B][2][C]: sum du xh, sum du per channel of the utterance.  64 ragged utterances of 861 x 512
+// bf16 silu 43 us (131 MB, 3.0 TB/s): 157 registers leave three workgroups a CU, whose loads, sums and stores overlap little.  Four
+// vectors a thread instead of eight, with more waves: 51 us; 64-byte rows in workgroups of 512: 47.
 template <typename T, int V, int ACT, bool EVEN>
 __global__ void __launch_bounds__(kBackThreads<T>) k_norm_back_slab(const T* dy, long long dy_stride, const T* __restrict__ x,
                                                                 long long x_stride, const float* __restrict__ stats,
@@ -592,7 +597,8 @@ __global__ void __launch_bounds__(kBackThreads<T>) k_norm_back_slab(const T* dy,
     }
 }
 
-// grid (chunks, B): per channel sums of a run of `rows` frames to parts [B][chunks][2][C]
+// grid (chunks, B): per channel sums of a run of `rows` frames to parts [B][chunks][2][C].  51 680 x 256 f16 silu 15 us (53 MB,
+// 3.5 TB/s), its join 3.9, k_norm_back_apply 18 (79 MB, 4.5 TB/s).
 template <typename T, int V, int ACT>
 __global__ void __launch_bounds__(kMaxThreads) k_norm_back_chunk(const T* __restrict__ dy, long long dy_stride, const T* __restrict__ x,
                                                          long long x_stride, const float* __restrict__ stats,
@@ -749,30 +755,37 @@ __global__ void __launch_bounds__(kMaxThreads) k_norm_back_apply(const T* dy, lo
     });
 }
 
-// ---- any size and alignment, element by element ----
+// ---- rows that no workgroup spans (more than 1024 vectors, or channels of 64 KiB of sums), element by element: 8 x 861 x 2050
+// float32 in 2 groups 89 us (44 for the chunks, 41 to apply; 113 MB), its gradients 78 ----
 
-// grid (groups, B): mean first, then the squared distances from it (no cancellation whatever the level of x)
+// grid (groups, B, chunks of `rows` frames): as k_norm_chunk
 template <typename T>
-__global__ void __launch_bounds__(256) k_norm_plain_stats(const T* __restrict__ x, long long stride, const int* __restrict__ frames,
-                                                    float* __restrict__ stats, int Tn, int n, float eps) {
+__global__ void __launch_bounds__(256) k_norm_plain_chunk(const T* __restrict__ x, long long stride, const int* __restrict__ frames,
+                                                    float* __restrict__ parts, int Tn, int n, int rows) {
     __shared__ float s[4];
-    const int g = blockIdx.x, b = blockIdx.y;
-    const int live = live_frames(frames, b, Tn);
-    const long long count = (long long)live * n;
-    const T* base = x + (long long)b * Tn * stride + g * n;
+    const int g = blockIdx.x, b = blockIdx.y, k = blockIdx.z;
+    const int t0 = k * rows, here = max(0, min(rows, live_frames(frames, b, Tn) - t0));
+    const T* base = x + ((long long)b * Tn + t0) * stride + (long long)g * n;
+    // 256 threads on `across` channels of 256 / across frames at a time
+    const int across = min(n, 256), c0 = threadIdx.x % across, r0 = threadIdx.x / across, step = 256 / across;
+    const float inv = here ? 1.0f / ((float)here * (float)n) : 0.0f;
     float sum = 0.0f;
-    for (long long e = threadIdx.x; e < count; e += 256) sum += gl_to_f32(base[e / n * stride + e % n]);
-    const float mean = count ? block_sum(sum, s) / (float)count : 0.0f;
+    if (r0 < step)
+        for (int t = r0; t < here; t += step)
+            for (int c = c0; c < n; c += across) sum += gl_to_f32(base[t * stride + c]);
+    const float mean = block_sum(sum, s) * inv;
     float m2 = 0.0f;
-    for (long long e = threadIdx.x; e < count; e += 256) {
-        const float d = gl_to_f32(base[e / n * stride + e % n]) - mean;
-        m2 += d * d;
-    }
+    if (r0 < step)
+        for (int t = r0; t < here; t += step)
+            for (int c = c0; c < n; c += across) {
+                const float d = gl_to_f32(base[t * stride + c]) - mean;
+                m2 = fmaf(d, d, m2);
+            }
     m2 = block_sum(m2, s);
     if (threadIdx.x == 0) {
-        float* o = stats + 2 * ((long long)b * gridDim.x + g);
+        float* o = parts + 2 * (((long long)b * gridDim.x + g) * gridDim.z + k);
         o[0] = mean;
-        o[1] = count ? 1.0f / sqrtf(m2 / (float)count + eps) : 0.0f;
+        o[1] = m2;
     }
 }
 
@@ -798,42 +811,53 @@ __global__ void __launch_bounds__(256) k_norm_plain_apply(const T* x, long long 
     }
 }
 
-// grid (groups, B): per channel sums over the live frames (parts [B][2][C]: sum du xh, sum du) and the group's p, q
+// grid (blocks of 256 channels, B, chunks): as k_norm_back_chunk, a thread a channel
 template <typename T>
-__global__ void __launch_bounds__(256) k_norm_plain_back_sums(const T* __restrict__ dy, long long dy_stride, const T* __restrict__ x,
+__global__ void __launch_bounds__(256) k_norm_plain_back_chunk(const T* __restrict__ dy, long long dy_stride, const T* __restrict__ x,
                                                         long long x_stride, const float* __restrict__ stats,
                                                         const T* __restrict__ gamma, const T* __restrict__ beta,
-                                                        const int* __restrict__ frames, float* __restrict__ parts,
-                                                        float* __restrict__ pq, int Tn, int C, int n, int act) {
-    __shared__ float s[4];
-    const int g = blockIdx.x, b = blockIdx.y;
-    const int live = live_frames(frames, b, Tn);
-    const float mean = stats[2 * ((long long)b * gridDim.x + g)], rstd = stats[2 * ((long long)b * gridDim.x + g) + 1];
-    float p = 0.0f, q = 0.0f;
-    for (int c = g * n; c < (g + 1) * n; ++c) {
-        const float ga = gamma ? gl_to_f32(gamma[c]) : 1.0f, be = beta ? gl_to_f32(beta[c]) : 0.0f;
-        float a0 = 0.0f, a1 = 0.0f;
-        for (int t = threadIdx.x; t < live; t += 256) {
-            const long long row = (long long)b * Tn + t;
-            const float xh = (gl_to_f32(x[row * x_stride + c]) - mean) * rstd;
-            const float du = gl_to_f32(dy[row * dy_stride + c]) * gl_act_grad(xh * ga + be, act);
-            a0 += du * xh;
-            a1 += du;
-        }
-        a0 = block_sum(a0, s);
-        a1 = block_sum(a1, s);
-        if (threadIdx.x == 0) {
-            parts[((long long)b * 2 + 0) * C + c] = a0;
-            parts[((long long)b * 2 + 1) * C + c] = a1;
-        }
-        p += a1 * ga;
-        q += a0 * ga;
+                                                        const int* __restrict__ frames, float* __restrict__ parts, int Tn, int C,
+                                                        int n, int rows, int act) {
+    const int c = blockIdx.x * 256 + threadIdx.x, b = blockIdx.y, k = blockIdx.z;
+    if (c >= C) return;
+    const int t0 = k * rows, here = max(0, min(rows, live_frames(frames, b, Tn) - t0));
+    const float* st = stats + 2 * ((long long)b * (C / n) + c / n);
+    const float mean = st[0], rstd = st[1];
+    const float slope = rstd * (gamma ? gl_to_f32(gamma[c]) : 1.0f), be = beta ? gl_to_f32(beta[c]) : 0.0f;
+    const T* xb = x + ((long long)b * Tn + t0) * x_stride + c;
+    const T* db = dy + ((long long)b * Tn + t0) * dy_stride + c;
+    float a0 = 0.0f, a1 = 0.0f;
+#pragma unroll 4
+    for (int t = 0; t < here; ++t) {
+        const float d = gl_to_f32(xb[t * x_stride]) - mean;
+        const float du = gl_to_f32(db[t * dy_stride]) * gl_act_grad(fmaf(d, slope, be), act);
+        a0 = fmaf(du, d, a0);
+        a1 += du;
     }
+    float* o = parts + ((long long)b * gridDim.z + k) * 2 * C;
+    o[c] = a0 * rstd;
+    o[C + c] = a1;
+}
+
+// grid (groups, B): p and q of a group from the sums [B][2][C]
+template <typename T>
+__global__ void __launch_bounds__(256) k_norm_plain_back_pq(const float* __restrict__ sums, const T* __restrict__ gamma,
+                                                      const int* __restrict__ frames, float* __restrict__ pq, int Tn, int C, int n) {
+    __shared__ float s[4];
+    const int g = blockIdx.x, b = blockIdx.y, live = live_frames(frames, b, Tn);
+    float p = 0.0f, q = 0.0f;
+    for (int c = g * n + threadIdx.x; c < (g + 1) * n; c += 256) {
+        const float ga = gamma ? gl_to_f32(gamma[c]) : 1.0f;
+        q = fmaf(sums[((long long)b * 2 + 0) * C + c], ga, q);
+        p = fmaf(sums[((long long)b * 2 + 1) * C + c], ga, p);
+    }
+    p = block_sum(p, s);
+    q = block_sum(q, s);
     if (threadIdx.x == 0) {
-        const float count = (float)((long long)live * n);
+        const float inv = live ? 1.0f / ((float)live * (float)n) : 0.0f;
         float* o = pq + 2 * ((long long)b * gridDim.x + g);
-        o[0] = live ? p / count : 0.0f;
-        o[1] = live ? q / count : 0.0f;
+        o[0] = p * inv;
+        o[1] = q * inv;
     }
 }
 
@@ -929,6 +953,10 @@ Cut cut_for(int B, int T, int C, int groups, int size, int V, int most, int row_
     }
     if (C / V > kMaxThreads || lds_bytes(kMaxThreads, V, C, n, 1) > kMaxLds) {
         c.kind = 2;
+        const long long chunks = 1024 / ((long long)B * groups);
+        c.rows = (int)ceil_div(T, chunks < 1 ? 1 : chunks);
+        if (c.rows < 1) c.rows = 1;
+        c.chunks = (int)ceil_div(T, c.rows);
         return c;
     }
     c.kind = 1;
@@ -993,7 +1021,7 @@ long long parts_bytes(int B, int T, int C, int groups, int dtype) {
     for (int V = 16 / size; V; V /= 2) {                     // alignment is not known to the query
         if (C % V) continue;
         const Cut c = cut_for(B, T, C, groups, size, V, kMaxThreads, kRowBytes);
-        if (c.kind == 1 && 8LL * B * groups * c.chunks > most) most = 8LL * B * groups * c.chunks;
+        if (c.kind && 8LL * B * groups * c.chunks > most) most = 8LL * B * groups * c.chunks;
     }
     return align16(most);
 }
@@ -1049,7 +1077,12 @@ int norm_fwd(const Norm& a, void* y, long long y_stride, float* stats, float* gi
             return 0;
         });
     }
-    hipLaunchKernelGGL((k_norm_plain_stats<T>), dim3(a.groups, a.B), dim3(256), 0, a.st, x, a.x_stride, a.frames, stats, a.T, n, eps);
+    if (c.chunks) {
+        hipLaunchKernelGGL((k_norm_plain_chunk<T>), dim3(a.groups, a.B, c.chunks), dim3(256), 0, a.st, x, a.x_stride, a.frames, parts, a.T,
+                           n, c.rows);
+        GL_HIP_CHECK(hipGetLastError());
+    }
+    hipLaunchKernelGGL(k_norm_join, dim3(a.groups, a.B), dim3(256), 0, a.st, parts, a.frames, stats, a.T, n, c.chunks, c.rows, eps);
     GL_HIP_CHECK(hipGetLastError());
     if (!a.T) return 0;
     hipLaunchKernelGGL((k_norm_plain_apply<T>), dim3(plain_blocks(a.B, a.T, a.C), a.B), dim3(256), 0, a.st, x, a.x_stride, ga, be,
@@ -1094,10 +1127,17 @@ int norm_back(const Norm& a, const void* dy_, long long dy_stride, const float* 
             return 0;
         });
     }
-    hipLaunchKernelGGL((k_norm_plain_back_sums<T>), dim3(a.groups, a.B), dim3(256), 0, a.st, dy, dy_stride, x, a.x_stride, stats, ga,
-                       be, a.frames, sums, pq, a.T, a.C, n, a.act);
+    const int rows = back_rows(a.B, a.T), chunks = (int)ceil_div(a.T, rows);
+    *done = a.B == 1;
+    hipLaunchKernelGGL((k_norm_plain_back_chunk<T>), dim3((unsigned)ceil_div(a.C, 256), a.B, chunks), dim3(256), 0, a.st, dy, dy_stride, x,
+                       a.x_stride, stats, ga, be, a.frames, parts, a.T, a.C, n, rows, a.act);
+    GL_HIP_CHECK(hipGetLastError());
+    hipLaunchKernelGGL((k_norm_back_join<T>), dim3((unsigned)ceil_div(2 * a.C, 16), a.B), dim3(1024), 0, a.st, parts, sums,
+                       (T*)dgamma, (T*)dbeta, a.C, chunks, *done);
     GL_HIP_CHECK(hipGetLastError());
     if (!dx) return 0;
+    hipLaunchKernelGGL((k_norm_plain_back_pq<T>), dim3(a.groups, a.B), dim3(256), 0, a.st, sums, ga, a.frames, pq, a.T, a.C, n);
+    GL_HIP_CHECK(hipGetLastError());
     hipLaunchKernelGGL((k_norm_plain_back_apply<T>), dim3(plain_blocks(a.B, a.T, a.C), a.B), dim3(256), 0, a.st, dy, dy_stride, x,
                        a.x_stride, stats, pq, ga, be, a.frames, dx, dx_stride, a.T, a.C, n, a.act);
     GL_HIP_CHECK(hipGetLastError());

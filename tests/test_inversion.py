@@ -415,7 +415,7 @@ def norm64(x, G, ga, be, eps, name, ends):
 NORM_SIZES = [(1, 1, 1, 1), (1, 1, 32, 32), (1, 1, 512, 32), (2, 2, 6, 2), (3, 5, 35, 5), (1, 641, 512, 32), (4, 33, 96, 4),
               (2, 100, 80, 1), (3, 17, 1025, 1), (2, 300, 24, 8), (1, 2049, 16, 16), (5, 64, 256, 8), (2, 7, 2048, 2),
               (1, 9000, 40, 2), (8, 257, 512, 32), (1, 5000, 512, 1), (2, 900, 500, 5), (2, 70, 36, 4), (3, 50, 26, 2), (1, 3000, 250, 2),
-              (3, 40, 4, 4), (2, 1200, 1022, 1)]
+              (3, 40, 4, 4), (2, 1200, 1022, 1), (2, 300, 2050, 2), (1, 90, 4098, 2049), (5, 40, 1027, 13)]
 
 
 def ends_of(B, T, ragged):
