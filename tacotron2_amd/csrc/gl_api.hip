@@ -87,7 +87,7 @@ int gl_plan_alloc(gl_plan* p, void** ptr, size_t bytes) {
 
 extern "C" {
 
-int gl_version(void) { return 300; }
+int gl_version(void) { return 310; }
 
 const char* gl_last_error(void) { return g_err; }
 
