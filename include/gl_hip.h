@@ -286,7 +286,8 @@ int gl_pcm16_encode(gl_plan* plan, const float* x, long long row_stride, long lo
  *   dtype of x, weight, bias and gradients: GL_F32, GL_BF16 or GL_F16; sums are 32-bit.
  *   out_dtype of y, residual, preactivation and dy: dtype, or GL_F32.
  *   Rows are frames; row strides are in elements, the elements of a row are contiguous.  A row stride may exceed
- *   the row; elements between rows are neither read into results nor written.                                   */
+ *   the row; elements between rows are neither read into results nor written.  Results and workspace overlap no
+ *   other argument, except where it says "may be".                                                               */
 enum gl_dtype { GL_F32 = 0, GL_BF16 = 1, GL_F16 = 2 };
 enum gl_activation { GL_ACT_NONE = 0, GL_ACT_RELU = 1, GL_ACT_SILU = 2, GL_ACT_GELU = 3, GL_ACT_TANH = 4, GL_ACT_EXP = 5 };
 

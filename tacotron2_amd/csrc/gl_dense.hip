@@ -1063,7 +1063,7 @@ bool gl_mm16_takes(const gl_operand& P, const gl_operand& Q, const gl_epilogue& 
     };
     if (P.across() && !Q.across()) return false;
     return side(P, I) && side(Q, J) && out(e.y, e.y_stride) && out(e.z, e.z_stride) && out(e.residual, e.r_stride) && nq < (1LL << 31) - 64 &&
-           gl_ceil_div(I, 64) * gl_ceil_div(J, 64) < (1LL << 31) - 8;
+           gl_ceil_div(I, 64) * gl_ceil_div(J, 64) < (1LL << 24) - 8;   // workgroups of 256 threads in a launch
 }
 
 extern "C" {

@@ -53,7 +53,7 @@ __device__ __forceinline__ f32x4 mfma16(s16x8 a, s16x8 b, f32x4 c) {
 __device__ __forceinline__ void wait_loads(int n) {          // at most n vector memory operations outstanding
     switch (n) {
 #define GL_WAIT(k) case k: asm volatile("s_waitcnt vmcnt(" #k ")" ::: "memory"); break;
-        GL_WAIT(0) GL_WAIT(2) GL_WAIT(3) GL_WAIT(4) GL_WAIT(5) GL_WAIT(6) GL_WAIT(8) GL_WAIT(10) GL_WAIT(12) GL_WAIT(16) GL_WAIT(18) GL_WAIT(22) GL_WAIT(24) GL_WAIT(28) GL_WAIT(38) GL_WAIT(40) GL_WAIT(44)
+        GL_WAIT(8) GL_WAIT(12) GL_WAIT(24) GL_WAIT(40)
 #undef GL_WAIT
         default: asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
@@ -508,7 +508,7 @@ k_mm16(Side P, Side Q, Out o, long long I, int J, long long nq, long long q_per_
     epilogue<T, TO, ACT, true, true, false, MI, NI>(o, acc, i0 + wi, j0 + wj, I, J, blockIdx.y, lane);
 }
 
-// The same product for many tiles.  Persistent: WGS workgroups a CU walk over the tiles, the ring running on into the next
+// The same product for many tiles.  Persistent: one workgroup a CU walks over the tiles, the ring running on into the next
 // tile's first stages while a tile's results are written.  A step's fragments are read, and the loads of the step RING
 // ahead started, between the products of the step before.
 // A contraction that one side is contiguous in is a multiple of 32 here, J a multiple of BN.
@@ -518,8 +518,8 @@ k_mm16(Side P, Side Q, Out o, long long I, int J, long long nq, long long q_per_
 // Measured, bf16: 55 104 x 512 x 2048 124 us (930 TF; 1200 without results), with gelu 155 to 175 (two transcendental
 // and eleven other operations a result, which no product runs under: the wave of both SIMD slots is in its epilogue then);
 // x 1025 exp to float32 89 us for the first 1024; gradients: dx 55 104 x 2048 x 512 115 us (1000 TF), dweight in 16 parts 114 to 124.
-template <typename T, typename TO, typename TB, int SEG, int ACT, bool EXTRA, bool LINES, int BM, int BN, int WM, int WN, int RING, int WGS, bool PT, bool QT>
-__global__ void __launch_bounds__(64 * (BM / WM) * (BN / WN), WGS * (BM / WM) * (BN / WN) / 4)
+template <typename T, typename TO, typename TB, int SEG, int ACT, bool EXTRA, bool LINES, int BM, int BN, int WM, int WN, int RING, bool PT, bool QT>
+__global__ void __launch_bounds__(64 * (BM / WM) * (BN / WN), (BM / WM) * (BN / WN) / 4)
 k_mm16_walk(Side P, Side Q, Out o, long long I, int J, long long nq, long long q_per_part, int tiles_j, int n_tiles) {
     constexpr int BK = 32, WAVES = (BM / WM) * (BN / WN);
     typedef Stage<BM, BK, PT, WAVES, PT || QT> SP;
@@ -538,8 +538,8 @@ k_mm16_walk(Side P, Side Q, Out o, long long I, int J, long long nq, long long q
     const int nk = (int)(nq - q0 < q_per_part ? nq - q0 : q_per_part);
     const int missing = (int)max(0LL, q0 + nk - (nq - Q.missing));           // of them on Q's side
     const int once = (nk + BK - 1) / BK, steps = SEG * once;
-    const int pairs = max((RING + 1) / 2, (steps + 1) / 2);   // steps run in twos, at least RING of them: the
-                                                                           // extra ones add zeros
+    const int pairs = max(RING / 2, (steps + 1) / 2);        // steps run in twos, at least RING of them: the extra ones add zeros
+    static_assert(RING % 2 == 0, "a tile's first load is a pair's first");
     int tile = first + (blockIdx.x >> 3);
     if (tile >= end) return;
     SP sp;
@@ -619,7 +619,6 @@ k_mm16_walk(Side P, Side Q, Out o, long long I, int J, long long nq, long long q
             if (SEG == 3 && pairs - k == once) lower(acc);
             if (left == 0) enter(tile + walkers);
             step(a[0], a[1]);
-            if (RING % 2 && left == 1) enter(tile + walkers);
             left -= 2;
             step(a[1], a[0]);
         }

@@ -25,7 +25,7 @@ int walk_as(const gl_operand& P, const gl_operand& Q, const Out& o, long long I,
     long long walkers = 256 / p.parts / 8 * 8;               // one workgroup a CU in all, whole rounds of the 8 XCDs
     if (walkers > (tiles + 7) / 8 * 8) walkers = (tiles + 7) / 8 * 8;
     if (walkers < 8) walkers = 8;
-    hipLaunchKernelGGL((k_mm16_walk<T, TO, TB, SEG, ACT, EXTRA, LINES, BM, 256, BM / 2, 64, 4, 1, PT, QT>), dim3((unsigned)walkers, p.parts), dim3(512),
+    hipLaunchKernelGGL((k_mm16_walk<T, TO, TB, SEG, ACT, EXTRA, LINES, BM, 256, BM / 2, 64, 4, PT, QT>), dim3((unsigned)walkers, p.parts), dim3(512),
                        0, st, side(P, I, nq, pad), side(Q, J, nq, pad), o, I, J, pad, p.per, tiles_j, (int)tiles);
     GL_HIP_CHECK(hipGetLastError());
     return 0;

@@ -948,8 +948,12 @@ Cut cut_for(int B, int T, int C, int groups, int size, int V, int most, int row_
         c.kind = 0;
         c.threads = threads_for(n * k / V, T, most);
         c.blocks = {(int)ceil_div(groups, k), 0, n * k, C};
-        c.blocks.total = B * c.blocks.per_b;
-        return c;
+        const long long total = (long long)B * c.blocks.per_b;
+        if (total * c.threads < 0xff000000LL) {              // what one launch can have
+            c.blocks.total = (int)total;
+            return c;
+        }
+        c = {};
     }
     if (C / V > kMaxThreads || lds_bytes(kMaxThreads, V, C, n, 1) > kMaxLds) {
         c.kind = 2;

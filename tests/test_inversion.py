@@ -374,6 +374,27 @@ def test_dense_backward_narrow(M, K, N, apart, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("M,K,N", [(9000, 520, 600), (20000, 257, 512), (33000, 130, 257)])
+def test_dense_many_rows_off_their_alignment(M, K, N, dtype):
+    """Sizes of the large tiles whose operands start one element off: copied where a copy helps, else element by element."""
+    def off(t):
+        flat = torch.full((t.numel() + 1,), float("nan"), dtype=dtype, device="cuda")
+        flat[1:] = t.flatten()
+        return flat[1:].view(t.shape)
+
+    x, w = randn((M, K), dtype, 1).cuda(), randn((N, K), dtype, 2, K ** -0.5).cuda()
+    z, dy = randn((M, N), dtype, 3).cuda(), randn((M, N), dtype, 4).cuda()
+    _, _, y64, y_tol = dense64(x, w, None, "silu", None, dtype)
+    out = off(torch.zeros(M, N, dtype=dtype, device="cuda"))
+    close(inv.dense(off(x), off(w), activation="silu", out=out), y64.cpu(), y_tol.cpu(), "y")
+    want = dense_back64(dy, x, w, z, "silu", dtype)
+    got = inv.dense_backward(off(dy), off(x), off(w), off(z), activation="silu")
+    for g, (v, t), what in zip(got, want, ("dx", "dweight", "dbias")):
+        close(g, v.cpu(), t.cpu(), what)
+
+
+@gpu
 def test_dense_without_rows():
     w, b = torch.randn(6, 5, device="cuda"), torch.randn(6, device="cuda")
     x = torch.empty((2, 0, 5), device="cuda")
@@ -665,6 +686,53 @@ def test_captured_step_replays(dtype):
         assert all(torch.equal(a, c) for a, c in zip(outs, want)), f"replay {k}"
     g.close()
     plan.close()
+
+
+@gpu
+@pytest.mark.parametrize("M,K,N,T", [(600, 80, 96, 300), (4400, 512, 2048, 2200)])
+def test_two_graphs_replay_side_by_side(M, K, N, T):
+    """Each with its own workspaces, on two streams at once, the inputs changing in between."""
+    from tacotron2_amd.plan import Plan
+    plans = [Plan(64, 16, 4, 4) for _ in range(2)]
+    sets, graphs = [], []
+    for k, plan in enumerate(plans):
+        x, w, dy, z = (t.cuda() for t in (randn((M, K), F32, k), randn((N, K), F32, 2 + k), randn((M, N), F32, 4 + k), randn((M, N), F32, 6 + k)))
+        y, h, st = torch.zeros_like(dy), torch.zeros_like(dy).view(2, T, N), torch.zeros(2, 4, 2, device="cuda")
+        dx, dw, db, dh = torch.zeros_like(x), torch.zeros_like(w), torch.zeros(N, device="cuda"), torch.zeros_like(h)
+        space = [torch.empty(max(1, n), dtype=torch.uint8, device="cuda") for n in (
+            inv.dense_workspace(M, K, N), inv.dense_backward_workspace(M, K, N, F32, None, "silu"),
+            inv.group_norm_workspace(2, T, N, 4), inv.group_norm_backward_workspace(2, T, N, 4))]
+
+        def step(x=x, w=w, dy=dy, z=z, y=y, h=h, st=st, dx=dx, dw=dw, db=db, dh=dh, space=space):
+            inv.dense(x, w, activation="silu", out=y, workspace=space[0])
+            inv.dense_backward(dy, x, w, z, activation="silu", dx=dx, dweight=dw, dbias=db, workspace=space[1])
+            inv.group_norm(y.view(2, T, N), 4, out=h, stats=st, workspace=space[2])
+            inv.group_norm_backward(dy.view(2, T, N), y.view(2, T, N), 4, st, dx=dh, workspace=space[3])
+
+        with plan.capture() as g:
+            step()
+        sets.append((step, (x, w, dy, z), (y, h, st, dx, dw, db, dh)))
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for turn in range(3):
+        want = []
+        for step, inputs, outs in sets:
+            for t in inputs:
+                t.mul_(0.5).add_(0.01 * turn)
+            step()
+            want.append([t.clone() for t in outs])
+            for t in outs:
+                t.fill_(float("nan"))
+        torch.cuda.synchronize()
+        for g, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                g.launch()
+        torch.cuda.synchronize()
+        for (_, _, outs), w in zip(sets, want):
+            assert all(torch.equal(a, b) for a, b in zip(outs, w)), f"turn {turn}"
+    for g, plan in zip(graphs, plans):
+        g.close()
+        plan.close()
 
 
 @gpu
