@@ -18,6 +18,7 @@ refuses to run under a stream capture: autograd's own bookkeeping for leaves tha
 the process there; capture the explicit forward and backward calls instead.
 """
 import contextlib
+import ctypes
 import functools
 
 import torch
@@ -25,12 +26,18 @@ import torch
 from . import _lib
 from .plan import _require_gpu, raw_capture_active
 
+try:
+    from . import _calls                 # the plain case of the calls below, compiled; they say None to any other
+except ImportError:                      # not built: all cases take the way through this file
+    _calls = None
+
 ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "silu": 2, "gelu": 3, "tanh": 4, "exp": 5}
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
 # -- argument plumbing -----------------------------------------------------------------------------------------
-# Small calls are bound by this file, so its checks are few attribute reads each.
+# Small calls are bound by the host: the plain case goes through _calls; for the others the checks here are few attribute
+# reads each.
 def _activation(name):
     try:
         return ACTIVATIONS[name]
@@ -170,6 +177,23 @@ def _stream(device):
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
+_bound = False
+
+
+def _plain():
+    """_calls with the library's addresses, or None where it may not be used: inside Plan.capture() nothing is allocated."""
+    global _bound
+    if _calls is None or raw_capture_active():
+        return None
+    if not _bound:
+        lib = _lib.lib()
+        _calls.bind(torch._C._cuda_getCurrentRawStream, *(ctypes.cast(getattr(lib, f"gl_{name}{query}"), ctypes.c_void_p).value
+                                                          for name in ("dense", "dense_backward", "group_norm", "group_norm_backward")
+                                                          for query in ("_workspace", "")))
+        _bound = True
+    return _calls
+
+
 def _needs_grad(*tensors):
     if torch.is_grad_enabled():
         for t in tensors:
@@ -257,7 +281,10 @@ class _Dense(torch.autograd.Function):
     def forward(ctx, x, weight, bias, residual, act, out_dtype):
         shape, out_dtype, device = _dense_args(x, weight, bias, residual, out_dtype)
         z = torch.empty(shape, dtype=out_dtype, device=device) if act else None
-        y = _dense(x, weight, bias, act, residual, out_dtype, None, z, None)
+        calls = _plain()
+        y = None if calls is None else calls.dense(x, weight, bias, residual, z, out_dtype, act)
+        if y is None:
+            y = _dense(x, weight, bias, act, residual, out_dtype, None, z, None)
         ctx.act = act
         ctx.save_for_backward(x, weight, z)
         return y
@@ -281,6 +308,12 @@ def dense(x, weight, bias=None, *, activation=None, residual=None, out_dtype=Non
     receives the sum with the bias, which :func:`dense_backward` needs unless activation is None.  Differentiable in x,
     weight, bias and residual (without out= and preactivation=)."""
     act = _activation(activation)
+    if out is None and workspace is None:
+        calls = _plain()
+        if calls is not None:
+            y = calls.dense(x, weight, bias, residual, preactivation, out_dtype, act)
+            if y is not None:
+                return y
     if _needs_grad(x, weight, bias, residual):
         if out is not None or preactivation is not None:
             raise ValueError("out= and preactivation= belong to the form without gradients: use torch.no_grad()")
@@ -297,6 +330,12 @@ def _apart_from_all(outs, made, inputs, same=()):
 
 
 def _dense_backward(dy, x, weight, z, act, need, outs, workspace):
+    if workspace is None and outs[0] is None and outs[1] is None and outs[2] is None:
+        calls = _plain()
+        if calls is not None:
+            grads = calls.dense_backward(dy, x, weight, z, act, bool(need[0]), bool(need[1]), bool(need[2]))
+            if grads is not None:
+                return grads
     _tensor(x, "x")
     if x.dim() < 1 or not isinstance(weight, torch.Tensor) or weight.dim() != 2:
         raise ValueError("x must be (..., inputs) and weight (outputs, inputs)")
@@ -426,7 +465,10 @@ class _GroupNorm(torch.autograd.Function):
     def forward(ctx, x, weight, bias, groups, eps, act, lengths):
         groups, B, T, C, lens = _norm_args(x, groups, weight, bias, lengths)
         stats = torch.empty((B, groups, 2), dtype=torch.float32, device=x.device)
-        y = _group_norm(x, groups, weight, bias, eps, act, lens, None, stats, None)
+        calls = _plain()
+        y = None if calls is None else calls.group_norm(x, weight, bias, lens, stats, groups, act, eps)
+        if y is None:
+            y = _group_norm(x, groups, weight, bias, eps, act, lens, None, stats, None)
         ctx.groups, ctx.act = groups, act
         ctx.save_for_backward(x, weight, bias, stats, lens)
         return y
@@ -450,6 +492,12 @@ def group_norm(x, groups, weight=None, bias=None, *, eps=1e-5, activation=None, 
     receives mean and 1 / sqrt(var + eps) for :func:`group_norm_backward`.  Differentiable in x, weight and bias
     (without out= and stats=)."""
     act = _activation(activation)
+    if out is None and workspace is None:
+        calls = _plain()
+        if calls is not None:
+            y = calls.group_norm(x, weight, bias, lengths, stats, int(groups), act, eps)
+            if y is not None:
+                return y
     if _needs_grad(x, weight, bias):
         if out is not None or stats is not None:
             raise ValueError("out= and stats= belong to the form without gradients: use torch.no_grad()")
@@ -459,6 +507,13 @@ def group_norm(x, groups, weight=None, bias=None, *, eps=1e-5, activation=None, 
 
 
 def _group_norm_backward(dy, x, groups, stats, weight, bias, act, lengths, need, outs, workspace):
+    if workspace is None and outs[0] is None and outs[1] is None and outs[2] is None:
+        calls = _plain()
+        if calls is not None:
+            grads = calls.group_norm_backward(dy, x, stats, weight, bias, lengths, int(groups), act, bool(need[0]), bool(need[1]),
+                                              bool(need[2]))
+            if grads is not None:
+                return grads
     groups, B, T, C, lens = _norm_args(x, groups, weight, bias, lengths)
     device, dtype = x.device, x.dtype
     _tensor(dy, "dy", device, dtype, x.shape)

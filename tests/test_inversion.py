@@ -628,6 +628,50 @@ def test_autograd_broadcast_and_shared_inputs():
 
 # -- streams and graphs ------------------------------------------------------------------------------------------
 @gpu
+def test_plain_calls_and_the_others_agree(monkeypatch):
+    """The compiled way of the plain case and the way through Python: equal bits, and only the plain case is taken."""
+    calls = inv._plain()
+    assert calls is not None
+    x, w, b, r = (randn(s, BF16, k).cuda() for k, s in enumerate(((2, 70, 64), (96, 64), (96,), (2, 70, 96))))
+    z, dy = torch.empty(2, 70, 96, dtype=BF16, device="cuda"), randn((2, 70, 96), BF16, 9).cuda()
+    ga, lens, stats = randn((64,), BF16, 5).cuda(), torch.tensor([70, 13], dtype=torch.int32, device="cuda"), torch.empty(2, 8, 2, device="cuda")
+
+    def run():
+        out = [inv.dense(x, w, b, activation="silu", residual=r, preactivation=z), z.clone(), inv.dense(x[0, 0], w, out_dtype=F32),
+               *inv.dense_backward(dy, x, w, z, activation="silu"), *inv.dense_backward(dy, x, w, needs=(False, True, True)),
+               inv.group_norm(x, 8, ga, activation="gelu", lengths=lens, stats=stats), stats.clone(), inv.group_norm(x[0], 4),
+               *inv.group_norm_backward(x, x, 8, stats, ga, ga, lengths=lens), *inv.group_norm_backward(x, x, 8, stats, ga, lengths=[70, 13])]
+        leaf = x.clone().requires_grad_()
+        inv.group_norm(inv.dense(leaf, w, b, activation="tanh"), 8).float().square().sum().backward()
+        return out + [leaf.grad]
+
+    got = run()
+    with monkeypatch.context() as m:
+        m.setattr(inv, "_calls", None)
+        want = run()
+    assert len(got) == len(want)
+    for a, c in zip(got, want):
+        assert (a is None and c is None) or (a.dtype == c.dtype and a.shape == c.shape and torch.equal(a, c))
+    assert torch.equal(calls.dense(x, w, b, None, None, None, 2), inv.dense(x, w, b, activation="silu"))
+    bad = x.transpose(0, 1)
+    for args in ((bad, w, None, None, None, None, 0), (x.cpu(), w, None, None, None, None, 0), (x, w.half(), None, None, None, None, 0),
+                 (x, w, b[:5], None, None, None, 0), (x, w, b, None, r[0], None, 0), (x, w, b, r, r, None, 0),
+                 (x, w, [1.0], None, None, None, 0), (x, w, b, None, None, F16, 0), (x, w, b, None, None, "f32", 0),
+                 (None, w, b, None, None, None, 0), (x.clone().requires_grad_(), w, b, None, None, None, 0), (x[:0], w, b, None, None, None, 0),
+                 (x, w, b, None, None, None, 9), (x, w[0], None, None, None, None, 0), (x, w, b)):
+        assert calls.dense(*args) is None
+    with pytest.raises(TypeError):
+        calls.dense(x, w, b, None, None, None, "silu")
+    for args in ((x, None, None, [1, 2], None, 8, 0, 1e-5), (x, None, None, None, stats[:1], 8, 0, 1e-5), (x, None, None, None, None, 7, 0, 1e-5),
+                 (x, None, None, None, None, 8, 0, -1.0), (x, None, None, None, None, 8, 0, float("nan")), (x[0, 0], None, None, None, None, 8, 0, 1.0),
+                 (x, None, None, lens.long(), None, 8, 0, 1e-5), (x, None, None, lens[:1], None, 8, 0, 1e-5)):
+        assert calls.group_norm(*args) is None
+    assert calls.dense_backward(dy, x, w, None, 2, True, True, True) is None                   # no preactivation
+    assert calls.dense_backward(dy, x, w, None, 0, False, False, False) is None
+    assert calls.group_norm_backward(x, x, stats[:, :4], None, None, None, 8, 0, True, True, True) is None
+
+
+@gpu
 def test_another_stream():
     x, w = torch.randn(700, 256, device="cuda"), torch.randn(192, 256, device="cuda")
     ga = torch.randn(192, device="cuda")
