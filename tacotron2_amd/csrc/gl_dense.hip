@@ -337,11 +337,11 @@ __global__ void __launch_bounds__(256) k_dense_join(Epilogue e, long long I, int
 // Up to ROWS frames: L lanes a column (as many as 16-byte pieces of its weights, to 64), 64 / L columns a wave.  W streams
 // through once and bounds it: 1 x 2048 -> 8192 bf16 6.1 us (5.5 TB/s, W in the cache behind the L2s); from about four rows on the
 // multiplications do (8 rows 20 us).  1 x 512 -> 1025 3.3 us, a launch.
-template <typename T, typename TO, int ROWS, bool VEC>
+template <typename T, typename TO, int ROWS, int V>
 __global__ void __launch_bounds__(256) k_dense_few(const T* __restrict__ x, long long x_stride, const T* __restrict__ w,
                                                    long long w_stride, Epilogue e, int rows, int K, int N, int L) {
-    constexpr int V = VEC ? 16 / sizeof(T) : 1;
     typedef typename vecn<T, V>::type vT;
+    constexpr int kAtOnce = V * sizeof(T) >= 8 ? 2 : 4;      // pieces a lane has on the way
     const int lane = threadIdx.x & 63, l = lane & (L - 1);
     const int n = (blockIdx.x * 4 + (threadIdx.x >> 6)) * (64 / L) + lane / L;
     float acc[ROWS];
@@ -349,7 +349,7 @@ __global__ void __launch_bounds__(256) k_dense_few(const T* __restrict__ x, long
     for (int m = 0; m < ROWS; ++m) acc[m] = 0.0f;
     if (n < N) {
         const T* wn = w + n * w_stride;
-#pragma unroll 2
+#pragma unroll kAtOnce
         for (int k = l * V; k < K; k += L * V) {
             const vT wv = *(const vT*)(wn + k);
 #pragma unroll
@@ -738,16 +738,16 @@ FrontLayout front_layout(long long rows, int inputs, int outputs, int dtype) {
 
 template <typename T, typename TO, int ROWS>
 int few(const void* x, long long x_stride, const void* w, long long w_stride, const Epilogue& e, int rows, int K, int N, hipStream_t st) {
-    const int V = 16 / sizeof(T);
-    const bool vec = K % V == 0 && (uintptr_t)x % 16 == 0 && (uintptr_t)w % 16 == 0 && x_stride % V == 0 && w_stride % V == 0;
-    const int pieces = vec ? K / V : K;
+    int V = 16 / sizeof(T);              // elements at once: what the widths and the arrays' alignment allow
+    auto fits = [&](const void* p, long long stride) { return K % V == 0 && stride % V == 0 && (uintptr_t)p % (V * sizeof(T)) == 0; };
+    while (!fits(x, x_stride) || !fits(w, w_stride)) V /= 2;
+    const int pieces = K / V;
     int L = kFewRows;                    // a lane for every row's result at least
     while (L < 64 && L < pieces) L *= 2;
     const unsigned grid = (unsigned)gl_ceil_div(N, 4 * (64 / L));
-    if (vec) hipLaunchKernelGGL((k_dense_few<T, TO, ROWS, true>), dim3(grid), dim3(256), 0, st, (const T*)x, x_stride, (const T*)w,
-                                w_stride, e, rows, K, N, L);
-    else hipLaunchKernelGGL((k_dense_few<T, TO, ROWS, false>), dim3(grid), dim3(256), 0, st, (const T*)x, x_stride, (const T*)w,
-                            w_stride, e, rows, K, N, L);
+    auto kernel = V == 1 ? k_dense_few<T, TO, ROWS, 1> : V == 2 ? k_dense_few<T, TO, ROWS, 2>
+                : V == 4 ? k_dense_few<T, TO, ROWS, 4> : k_dense_few<T, TO, ROWS, 16 / sizeof(T)>;
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), 0, st, (const T*)x, x_stride, (const T*)w, w_stride, e, rows, K, N, L);
     GL_HIP_CHECK(hipGetLastError());
     return 0;
 }
