@@ -354,8 +354,7 @@ __global__ void __launch_bounds__(256) k_dense_few(const T* __restrict__ x, long
             const vT wv = *(const vT*)(wn + k);
 #pragma unroll
             for (int m = 0; m < ROWS; ++m) {
-                if (m >= rows) break;                        // uniform
-                const vT xv = *(const vT*)(x + m * x_stride + k);
+                const vT xv = *(const vT*)(x + min(m, rows - 1) * x_stride + k);     // rows past the last: once more, unused
 #pragma unroll
                 for (int v = 0; v < V; ++v) acc[m] = fmaf(gl_to_f32(xv[v]), gl_to_f32(wv[v]), acc[m]);
             }
@@ -756,6 +755,8 @@ template <typename T, typename TO>
 int forward(const void* x, long long x_stride, const void* w, long long w_stride, const Epilogue& e, long long rows,
             int inputs, int outputs, const FrontLayout& l, void* ws, hipStream_t st) {
     if (rows == 1) return few<T, TO, 1>(x, x_stride, w, w_stride, e, 1, inputs, outputs, st);
+    if (rows == 2) return few<T, TO, 2>(x, x_stride, w, w_stride, e, 2, inputs, outputs, st);
+    if (rows <= 4) return few<T, TO, 4>(x, x_stride, w, w_stride, e, (int)rows, inputs, outputs, st);
     if (rows <= kFewRows) return few<T, TO, kFewRows>(x, x_stride, w, w_stride, e, (int)rows, inputs, outputs, st);
     const Operand P0 = {x, x_stride, 1}, Q0 = {w, w_stride, 1};
     Operand P = P0, Q = Q0;
