@@ -335,8 +335,8 @@ __global__ void __launch_bounds__(256) k_dense_join(Epilogue e, long long I, int
 }
 
 // Up to ROWS frames: L lanes a column (as many as 16-byte pieces of its weights, to 64), 64 / L columns a wave.  W streams
-// through once and bounds it: 1 x 2048 -> 8192 bf16 6.1 us (5.5 TB/s, W in the cache behind the L2s); from about four rows on the
-// multiplications do (8 rows 20 us).  1 x 512 -> 1025 3.3 us, a launch.
+// through once and bounds it: 1 x 2048 -> 8192 bf16 5.4 us (6.2 TB/s, W in the cache behind the L2s); 8 rows, whose x no longer
+// stays in the L1, 19 us.  1 x 512 -> 1025 3.3 us, a launch.
 template <typename T, typename TO, int ROWS, int V>
 __global__ void __launch_bounds__(256) k_dense_few(const T* __restrict__ x, long long x_stride, const T* __restrict__ w,
                                                    long long w_stride, Epilogue e, int rows, int K, int N, int L) {
@@ -360,13 +360,21 @@ __global__ void __launch_bounds__(256) k_dense_few(const T* __restrict__ x, long
             }
         }
     }
+    // over the L lanes: first each half takes half of the rows over, until a lane has one, then that row's sum alone
+    int m = 0, o = L / 2;
 #pragma unroll
-    for (int m = 0; m < ROWS; ++m)
-        for (int o = L / 2; o > 0; o >>= 1) acc[m] += __shfl_xor(acc[m], o);
-    if (n >= N) return;
+    for (int half = ROWS / 2; half > 0; half /= 2, o >>= 1) {
+        const bool up = l & o;
 #pragma unroll
-    for (int m = 0; m < ROWS; ++m)
-        if (m < rows && l == m) gl_finish<T, TO>(e, m, n, acc[m]);
+        for (int k = 0; k < half; ++k) {
+            const float got = __shfl_xor(up ? acc[k] : acc[k + half], o);
+            acc[k] = (up ? acc[k + half] : acc[k]) + got;
+        }
+        if (up) m += half;
+    }
+    const int same = max(2 * o, 1) - 1;                      // lanes that differ in these bits have the same row
+    for (; o > 0; o >>= 1) acc[0] += __shfl_xor(acc[0], o);
+    if (n < N && m < rows && (l & same) == 0) gl_finish<T, TO>(e, m, n, acc[0]);
 }
 
 // Copies a matrix into rows of whole chunks: zeros up to `padded` columns.  PLANES 3: float32 into three bfloat16 planes.  Rows

@@ -85,7 +85,7 @@ def dense64(x, w, b, name, r, out_dtype):
     return z, off + u(out_dtype) * z.abs() + tiny(out_dtype), y, y_off + u(out_dtype) * (y.abs() + y_off) + tiny(out_dtype)
 
 
-DENSE_SIZES = [(1, 1, 1), (1, 512, 1025), (2, 80, 513), (3, 7, 33), (8, 1024, 1024), (16, 96, 250), (7, 828, 188), (4, 1910, 130), (3, 1911, 70), (17, 31, 65), (33, 64, 64),
+DENSE_SIZES = [(1, 1, 1), (1, 512, 1025), (2, 80, 513), (3, 7, 33), (8, 1024, 1024), (16, 96, 250), (7, 828, 188), (4, 1910, 130), (3, 1911, 70), (8, 40, 33), (5, 64, 70), (6, 9, 20), (2, 8, 9), (17, 31, 65), (33, 64, 64),
                (64, 64, 64), (65, 128, 200), (128, 256, 256), (129, 513, 96), (257, 264, 520), (641, 80, 512), (300, 1024, 256),
                (1100, 72, 1025), (2600, 136, 328)]
 
