@@ -86,6 +86,14 @@ __device__ __forceinline__ void any_tiles(const AnyArgs& a, long long first, lon
     auto deposit = [&](T* dst, bool along, const T (&v)[8]) {
         int r, q;
         spot(along, r, q);
+        if (k16 && along) {                                  // uniform; a row's eight lie on 16 bytes
+            typedef typename vecn<T, 8>::type v8;
+            v8 t;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) t[k] = v[k];
+            *(v8*)(dst + r * kPitch + q) = t;
+            return;
+        }
         const int across = along ? 1 : kPitch;
 #pragma unroll
         for (int k = 0; k < 8; ++k) dst[r * kPitch + q + k * across] = v[k];
