@@ -490,14 +490,15 @@ __global__ void __launch_bounds__(256) k_dense_halves(Halves a, Halves b, int co
     }
 }
 
-// dz = dy act'(z), rounded for the products that read it (to T, or into three planes), zeros up to dz_stride columns, and
-// column sums of the unrounded dz over this workgroup's frames.  grid (blocks of 64 V columns, parts of the frames); thread =
+// dz = dy act'(z), rounded for the products that read it (to T, which is what the matrix instructions take: half a step a term;
+// or into three planes beside `exact`), zeros up to dz_stride columns, and column sums of the unrounded dz over this
+// workgroup's frames.  grid (blocks of 64 V columns, parts of the frames); thread =
 // (V columns, one of 4 frame lanes).  dz is a pass of its own, since both products read it and one of them transposed; it is
 // bound by memory: 55 104 x 2048 bf16 gelu 129 us (677 MB, 5.2 TB/s).
 template <typename T, typename TO, int V, int PLANES>
 __global__ void __launch_bounds__(256) k_dense_dz(const TO* __restrict__ dy, long long dy_stride, const TO* __restrict__ z,
                                                   long long z_stride, void* __restrict__ dz_, long long dz_stride, long long plane,
-                                                  float* __restrict__ parts, long long rows, int N, int rows_per_part, int act) {
+                                                  float* __restrict__ exact, float* __restrict__ parts, long long rows, int N, int rows_per_part, int act) {
     typedef typename vecn<TO, V>::type vI;
     __shared__ float s[4][64 * V];
     const int c = threadIdx.x & 63, r = threadIdx.x >> 6;
@@ -545,6 +546,12 @@ __global__ void __launch_bounds__(256) k_dense_dz(const TO* __restrict__ dy, lon
                 *(typename vecn<gl_bf16, V>::type*)o = h;
                 *(typename vecn<gl_bf16, V>::type*)(o + plane) = m;
                 *(typename vecn<gl_bf16, V>::type*)(o + 2 * plane) = l;
+                if (exact) {
+                    typename vecn<float, V>::type f;
+#pragma unroll
+                    for (int v = 0; v < V; ++v) f[v] = d[v];
+                    *(typename vecn<float, V>::type*)(exact + i * dz_stride + n) = f;
+                }
             }
         }
     };
@@ -872,23 +879,23 @@ BackLayout back_layout(long long rows, int inputs, int outputs, int dtype, int o
 }
 
 template <typename T, typename TO, int V, int PLANES>
-int dz_launch(const void* dy, long long dy_stride, const void* z, long long z_stride, void* dz, long long dz_stride, float* parts,
+int dz_launch(const void* dy, long long dy_stride, const void* z, long long z_stride, void* dz, long long dz_stride, float* exact, float* parts,
               long long rows, int outputs, int act, hipStream_t st) {
     const int rpp = rows_per_part(rows, outputs);
     hipLaunchKernelGGL((k_dense_dz<T, TO, V, PLANES>), dim3((unsigned)gl_ceil_div(dz ? dz_stride : outputs, 64 * V),
                        (unsigned)gl_ceil_div(rows, rpp)), dim3(256), 0, st, (const TO*)dy, dy_stride, (const TO*)z, z_stride, dz,
-                       dz_stride, rows * dz_stride, parts, rows, outputs, rpp, act);
+                       dz_stride, rows * dz_stride, exact, parts, rows, outputs, rpp, act);
     GL_HIP_CHECK(hipGetLastError());
     return 0;
 }
 template <typename T, typename TO, int PLANES>
-int dz_pass(const void* dy, long long dy_stride, const void* z, long long z_stride, void* dz, long long dz_stride, float* parts,
+int dz_pass(const void* dy, long long dy_stride, const void* z, long long z_stride, void* dz, long long dz_stride, float* exact, float* parts,
             long long rows, int outputs, int act, hipStream_t st) {
     constexpr int V = 16 / sizeof(TO);   // 16 bytes at a time where rows and columns allow
     auto wide = [&](const void* p, long long stride) { return (uintptr_t)p % 16 == 0 && stride % V == 0; };
     if (outputs % V == 0 && wide(dy, dy_stride) && (act == GL_ACT_NONE || wide(z, z_stride)))
-        return dz_launch<T, TO, V, PLANES>(dy, dy_stride, z, z_stride, dz, dz_stride, parts, rows, outputs, act, st);
-    return dz_launch<T, TO, 1, PLANES>(dy, dy_stride, z, z_stride, dz, dz_stride, parts, rows, outputs, act, st);
+        return dz_launch<T, TO, V, PLANES>(dy, dy_stride, z, z_stride, dz, dz_stride, exact, parts, rows, outputs, act, st);
+    return dz_launch<T, TO, 1, PLANES>(dy, dy_stride, z, z_stride, dz, dz_stride, exact, parts, rows, outputs, act, st);
 }
 
 template <typename T, typename TO>
@@ -949,12 +956,7 @@ int backward(const void* dy, long long dy_stride, const void* x, long long x_str
     int rc = 0;
     if (dz || db) {
         float* sums = db ? parts : nullptr;
-        if constexpr (sizeof(T) == 4) {
-            rc = dz_pass<T, TO, 3>(dy, dy_stride, z, z_stride, dz, l.dz_stride, sums, rows, outputs, act, st);
-            if (!rc && dz32) rc = dz_pass<T, TO, 1>(dy, dy_stride, z, z_stride, dz32, l.dz_stride, nullptr, rows, outputs, act, st);
-        } else {
-            rc = dz_pass<T, TO, 1>(dy, dy_stride, z, z_stride, dz, l.dz_stride, sums, rows, outputs, act, st);
-        }
+        rc = dz_pass<T, TO, sizeof(T) == 4 ? 3 : 1>(dy, dy_stride, z, z_stride, dz, l.dz_stride, dz32, sums, rows, outputs, act, st);
         if (rc) return rc;
     }
     if (db) {
