@@ -385,17 +385,25 @@ __global__ void __launch_bounds__(256) k_dense_few(const T* __restrict__ x, long
     if (n < N && m < rows && (l & same) == 0) gl_finish<T, TO>(e, m, n, acc[0]);
 }
 
-// Copies a matrix into rows of whole chunks: zeros up to `padded` columns.  PLANES 3: float32 into three bfloat16 planes.  Rows
-// may start anywhere, so elements are read one by one: 55 104 x 513 bf16 30 us (3.8 TB/s).
+// Copies two matrices of as many columns, one after the other, into rows of whole chunks: zeros up to `padded` columns.
+// PLANES 3: float32 into three bfloat16 planes.  Rows may start anywhere, so elements are read one by one: 55 104 x 513 bf16 30 us
+// (3.8 TB/s).
+struct Packed {
+    const void* in;
+    long long in_stride, rows;
+    void* out;
+};
 template <typename T, int PLANES>
-__global__ void __launch_bounds__(256) k_dense_pack(const T* __restrict__ in, long long in_stride, void* __restrict__ out, long long rows,
-                                                    int cols, int padded, long long plane) {
+__global__ void __launch_bounds__(256) k_dense_pack(Packed first, Packed second, int cols, int padded) {
     const int per_row = padded / 8;
-    const long long n = rows * per_row;
+    const long long n = (first.rows + second.rows) * per_row;
     for (long long at = (long long)blockIdx.x * 256 + threadIdx.x; at < n; at += (long long)gridDim.x * 256) {
-        const long long r = at / per_row;
-        const int c = (int)(at - r * per_row) * 8;
-        const T* src = in + r * in_stride + c;
+        const long long row = at / per_row;
+        const int c = (int)(at - row * per_row) * 8;
+        const bool other = row >= first.rows;
+        const long long r = other ? row - first.rows : row, plane = (other ? second.rows : first.rows) * padded;
+        const T* src = (const T*)(other ? second.in : first.in) + r * (other ? second.in_stride : first.in_stride) + c;
+        void* out = other ? second.out : first.out;
         T v[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[k] = c + k < cols ? src[k] : (T)0.0f;
@@ -669,16 +677,19 @@ long long partial_bytes(int dtype, long long I, int J, long long nq, bool any_q,
     return (any > mm ? any : mm) + (fast ? flag_bytes(dtype, I, J) : 0);
 }
 
-// Copies `rows` x `cols` of o to `out` and points o at the copy.
+// Copies of `cols` columns of a and, where it has rows, b.
 template <typename T>
-int pack(Operand& o, bool across, long long stride, long long rows, int cols, void* out, hipStream_t st) {
+int pack(const Packed& a, const Packed& b, int cols, hipStream_t st) {
     const int padded = pad_to(cols);
-    const long long plane = rows * padded, blocks = gl_ceil_div(rows * (padded / 8), 256);
-    hipLaunchKernelGGL((k_dense_pack<T, sizeof(T) == 4 ? 3 : 1>), dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, st,
-                       (const T*)o.base, stride, out, rows, cols, padded, plane);
+    const long long blocks = gl_ceil_div((a.rows + b.rows) * (padded / 8), 256);
+    hipLaunchKernelGGL((k_dense_pack<T, sizeof(T) == 4 ? 3 : 1>), dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, st, a, b, cols, padded);
     GL_HIP_CHECK(hipGetLastError());
-    o = across ? Operand{out, 1, padded, plane, true} : Operand{out, padded, 1, plane, true};
     return 0;
+}
+// The operand that a copy is: of `rows` rows of `cols` columns, which lie across or along the contraction
+Operand copied(const Packed& a, int cols, bool across) {
+    const int padded = pad_to(cols);
+    return across ? Operand{a.out, 1, padded, a.rows * padded, true} : Operand{a.out, padded, 1, a.rows * padded, true};
 }
 
 // The product on prepared operands (16-bit as they lie or copied, float32 in planes), else on the originals (P0, Q0).
@@ -787,8 +798,10 @@ int forward(const void* x, long long x_stride, const void* w, long long w_stride
     float* partial = (float*)(scale + l.scale_bytes);
     if (!l.copy) return product<T, TO, 1>(P, Q, P0, Q0, e, rows, outputs, inputs, partial, l.fast, st);
     if constexpr (sizeof(T) == 2) {
-        int rc = pack<T>(P, false, x_stride, rows, inputs, at, st);
-        if (!rc) rc = pack<T>(Q, false, w_stride, outputs, inputs, w_copy, st);
+        const Packed a = {x, x_stride, rows, at}, b = {w, w_stride, outputs, w_copy};
+        const int rc = pack<T>(a, b, inputs, st);
+        P = copied(a, inputs, false);
+        Q = copied(b, inputs, false);
         return rc ? rc : product<T, TO, 1>(P, Q, P0, Q0, e, rows, outputs, inputs, partial, true, st);
     } else {
         const int padded = pad_to(inputs);
@@ -970,25 +983,23 @@ int backward(const void* dy, long long dy_stride, const void* x, long long x_str
     const bool padded = dz != nullptr;
     const void* d0 = !l.planes ? d : dz32 ? (const void*)dz32 : dy;
     const long long d0_stride = !l.planes ? d_stride : dz32 ? l.dz_stride : dy_stride;
+    const Packed wp = {w, w_stride, dx ? outputs : 0, w_copy}, xp = {x, x_stride, dw ? rows : 0, x_copy};
+    if (l.copy && products) rc = pack<T>(wp, xp, inputs, st);
+    if (rc) return rc;
+    constexpr int SEG = sizeof(T) == 4 ? 6 : 1;
     Epilogue e = {};
     if (dx) {
-        const Operand Q0 = {w, 1, w_stride};
-        Operand Q = Q0;
-        if (l.copy) rc = pack<T>(Q, true, w_stride, outputs, inputs, w_copy, st);
-        if (rc) return rc;
+        const Operand Q0 = {w, 1, w_stride}, Q = l.copy ? copied(wp, inputs, true) : Q0;
         e.y = dx;
         e.y_stride = dx_stride;
-        rc = product<T, T, sizeof(T) == 4 ? 6 : 1>({d, d_stride, 1, plane, padded}, Q, {d0, d0_stride, 1}, Q0, e, rows, inputs, outputs, partial, true, st);
+        rc = product<T, T, SEG>({d, d_stride, 1, plane, padded}, Q, {d0, d0_stride, 1}, Q0, e, rows, inputs, outputs, partial, true, st);
         if (rc) return rc;
     }
     if (dw) {
-        const Operand Q0 = {x, 1, x_stride};
-        Operand Q = Q0;
-        if (l.copy) rc = pack<T>(Q, true, x_stride, rows, inputs, x_copy, st);
-        if (rc) return rc;
+        const Operand Q0 = {x, 1, x_stride}, Q = l.copy ? copied(xp, inputs, true) : Q0;
         e.y = dw;
         e.y_stride = dw_stride;
-        rc = product<T, T, sizeof(T) == 4 ? 6 : 1>({d, 1, d_stride, plane, padded}, Q, {d0, 1, d0_stride}, Q0, e, outputs, inputs, rows, partial, true, st);
+        rc = product<T, T, SEG>({d, 1, d_stride, plane, padded}, Q, {d0, 1, d0_stride}, Q0, e, outputs, inputs, rows, partial, true, st);
     }
     return rc;
 }
