@@ -648,17 +648,19 @@ int any_product(const Operand& P, const Operand& Q, Epilogue e, long long I, int
 }
 
 // Layers of fewer multiplications than this go as they are to k_dense_any (forward, where the tiles would need copies) and
-// k_dense_back_small.  Microseconds there / on the tiles:
-//   float32, widths on 16 bytes   forward 2000 x 500 -> 700 33 / 34, 861 x 1024 -> 1024 40 / 35, 2000 x 1024 -> 1024 59 / 42
-//                                 backward 2000 x 1024 -> 1024 122 / 153, 6888 x 1024 -> 512 240 / 179
-//   float32, others               forward 641 x 257 -> 513 19 / 25, 6888 x 81 -> 512 25 / 25, 2000 x 501 -> 701 54 / 38
-//                                 backward 641 x 512 -> 1025 79 / 84, 2000 x 501 -> 701 104 / 98
-//   16 bits forward               641 x 257 -> 513 18 / 18, 2000 x 501 -> 701 41 / 21
-//   16 bits backward              641 x 512 -> 512 29 / 38, 6888 x 80 -> 512 45 / 38
+// k_dense_back_small.  `odd`: widths off the 16 bytes that those load at once.  Microseconds a call there / on the tiles:
+//   float32   forward   2000 x 512 -> 512 23 / 29, 2000 x 500 -> 700 34 / 34, 861 x 1024 -> 1024 41 / 36
+//             odd       641 x 257 -> 513 18 / 24, 6888 x 81 -> 512 25 / 23, 2000 x 501 -> 701 54 / 37
+//             backward  861 x 1024 -> 1024 73 / 90, 2000 x 1024 -> 1024 137 / 132, 6888 x 1024 -> 512 229 / 165
+//             odd       641 x 257 -> 513 33 / 66, 6888 x 81 -> 512 101 / 75, 641 x 512 -> 1025 82 / 72
+//   16 bits   odd       4000 x 17 -> 33 6.5 / 7.8, 641 x 81 -> 100 8.1 / 8.1, 61 x 948 -> 144 13.4 / 11.5, 641 x 257 -> 513 17 / 10
+//             backward  861 x 512 -> 512 22 / 28, 6888 x 80 -> 512 40 / 35, 2000 x 512 -> 512 39 / 34
+//             odd       641 x 129 -> 300 18 / 22, 2000 x 129 -> 300 25 / 25, 300 x 1001 -> 300 26 / 21
 double small_layer(int dtype, int inputs, int outputs, bool back) {
-    if (dtype != GL_F32) return back ? 3 << 26 : 1 << 27;
-    const bool odd = inputs % 4 || outputs % 4;
-    return back ? (odd ? 1LL << 29 : 1LL << 31) : odd ? 1 << 28 : 3 << 28;
+    const int whole = dtype == GL_F32 ? 4 : 8;
+    const bool odd = inputs % whole || (back && outputs % whole);
+    if (dtype == GL_F32) return back ? (odd ? 3 << 26 : 3LL << 29) : odd ? 1 << 28 : 3 << 28;
+    return back ? (odd ? 3 << 24 : 1 << 28) : 1 << 22;
 }
 bool is_small(long long rows, int inputs, int outputs, int dtype, bool back) {
     return (double)rows * inputs * outputs < small_layer(dtype, inputs, outputs, back);
