@@ -6,7 +6,7 @@
 struct gl_operand {              // element (i, q) at base[i * is + q * qs], one of is, qs is 1
     const void* base;
     long long is, qs;
-    long long plane = 0;         // elements between the three planes of a float32 operand
+    long long plane = 0;         // elements between the planes of an operand that has several
     bool padded = false;         // this library's own copy: zeros up to whole multiples of 32 in the contiguous direction
     bool across() const { return is == 1 && qs != 1; }       // contiguous across the contraction
 };
@@ -46,6 +46,19 @@ __device__ __forceinline__ bool gl_halves_give(float sum, gl_scale p, gl_scale q
     return !both.wild() && !(both.small() && fabsf(sum) < 6.0f * nq);
 }
 
+// A float32 value in two planes of a 16-bit type: v = high + low kSplitStep.  bfloat16 has the range for low to be what high leaves:
+// off by 2^-18 |v|.  float16: what high leaves, 2^24 up, so that values far below high's range stay: off by 2^-23 |v| or 2^-49 where
+// |v| < 8; above, where 2^24 times the rest may not fit, by half a step of float16.  Infinities, NaN and what rounds to infinity
+// stay in high alone.
+template <typename T> constexpr float kSplitStep = __is_same(T, gl_f16) ? 0x1p-24f : 1.0f;
+template <typename T>
+__device__ __forceinline__ void gl_split(float v, T& high, T& low) {
+    high = (T)v;
+    float rest = v - (float)high;                            // exact where it is finite
+    if constexpr (__is_same(T, gl_f16)) rest = __builtin_amdgcn_fmed3f(rest * 0x1p24f, -65504.0f, 65504.0f);
+    low = (T)(fabsf((float)high) < INFINITY ? rest : 0.0f);
+}
+
 static inline long long gl_ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 static inline long long gl_align16(long long b) { return (b + 15) / 16 * 16; }
 
@@ -64,7 +77,8 @@ long long gl_mm_partial_bytes(long long I, int J, long long nq, bool any_q);
 
 // Whether the fast kernels take the operands as they lie, else the strided kernel does.
 bool gl_mm16_takes(const gl_operand& P, const gl_operand& Q, const gl_epilogue& e, long long I, int J, long long nq, int out_size);
-// T: gl_bf16 / gl_f16; TO: T or float; TB: type of the bias; SEG 6 (gl_bf16), 3 (gl_f16): planes of float32 operands, else 1
+// T: gl_bf16 / gl_f16; TO: T or float; TB: type of the bias; SEG: products of planes that make C (gl_mm16.h), 6 or 3 for float32
+// operands, 2 where P has two planes (gl_split), else 1
 template <typename T, typename TO, typename TB, int SEG>
 int gl_mm16(const gl_operand& P, const gl_operand& Q, gl_epilogue e, long long I, int J, long long nq, float* partial, hipStream_t st);
 

@@ -30,8 +30,8 @@ constexpr int kBQ = 32;          // contraction indexes staged per step
 constexpr long long kMostBlocks = 1 << 23;   // of 256 threads: a launch has less than 2^32
 constexpr int kCUs = 256;        // compute units of an MI355X: the work split must not depend on the moment
 
-// A product of k_dense_any.  With DZ, P is dy and Z the preactivation: the first factor is dz = dy act'(z), rounded to T, and
-// `sums` ([parts][I]) or, without parts, `db` gets the unrounded dz's sums over q, from the tiles at j = 0.
+// A product of k_dense_any.  With DZ, P is dy and Z the preactivation: the first factor is dz = dy act'(z), rounded to T or split
+// into two planes, and `sums` ([parts][I]) or, without parts, `db` gets the unrounded dz's sums over q, from the tiles at j = 0.
 struct AnyArgs {
     Operand P, Q, Z;             // base null: zeros
     Epilogue e;
@@ -44,15 +44,16 @@ struct AnyArgs {
 
 // Any size, stride and alignment.  A thread stages eight consecutive elements of each side, two steps ahead of the
 // products.  V: 1, or 16 bytes of T: loads are 16 bytes wide (the sides' pointers, strides and sizes allow it).
-// T: what is multiplied, TY: what is written, TD: what dy and z are.
+// T: what is multiplied, TY: what is written, TD: what dy and z are.  TWO: the first factor is in two planes (gl_split).
 // Bound by latency where it is small, by the LDS traffic of 4-byte elements where it is not: 641 x 80 -> 512 float32 8.3 us,
 // 2000 x 500 -> 700 float32 32 us (43 TF).
-template <typename T, typename TY, typename TD, int V, bool DZ>
+template <typename T, typename TY, typename TD, int V, bool DZ, bool TWO>
 __device__ __forceinline__ void any_tiles(const AnyArgs& a, long long first, long long step, int part, const int* __restrict__ flags) {
     constexpr bool k16 = sizeof(T) == 2;
     constexpr int kPitch = k16 ? kBQ + 8 : kBQ + 1;
     __shared__ __attribute__((aligned(16))) T Ps[kTile * kPitch];
     __shared__ __attribute__((aligned(16))) T Qs[kTile * kPitch];
+    __shared__ __attribute__((aligned(16))) T Ls[TWO ? kTile * kPitch : 8];      // P's lower plane
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 31, lk = lane >> 5;
     const long long q_begin = (long long)part * a.q_per_part;
     const long long q_end = q_begin + a.q_per_part < a.nq ? q_begin + a.q_per_part : a.nq;
@@ -102,9 +103,9 @@ __device__ __forceinline__ void any_tiles(const AnyArgs& a, long long first, lon
         if (flags && !flags[tile]) continue;                 // uniform over the workgroup
         const long long i0 = tile / a.tiles_j * kTile;
         const int j0 = (int)(tile % a.tiles_j) * kTile;
-        f32x16 acc;
+        f32x16 acc, low;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) acc[r] = 0.0f;
+        for (int r = 0; r < 16; ++r) acc[r] = low[r] = 0.0f;
         float bias[16];                                      // arrives under the products
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
@@ -116,6 +117,8 @@ __device__ __forceinline__ void any_tiles(const AnyArgs& a, long long first, lon
             T q[8];
             int p_have, q_have;
         };
+        Operand below = a.P;                                 // the lower plane, where there is one in memory
+        if (TWO && !DZ) below.base = (const T*)a.P.base + a.P.plane;
         float sum[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) sum[k] = 0.0f;
@@ -123,11 +126,12 @@ __device__ __forceinline__ void any_tiles(const AnyArgs& a, long long first, lon
             if (q0 >= q_end) return;                         // uniform, as all conditions outside of fetch
             t.p_have = fetch(t.p, a.P, a.p_along, i0, a.I, q0);
             if (DZ && a.act != GL_ACT_NONE) fetch(t.z, a.Z, a.p_along, i0, a.I, q0);
+            if (TWO && !DZ) fetch(t.z, below, a.p_along, i0, a.I, q0);
             t.q_have = a.Q.base ? fetch(t.q, a.Q, a.q_along, j0, a.J, q0) : 0;
         };
         auto multiply = [&](Staged& t, long long q0) {
             if (q0 >= q_end) return;
-            T pt[8];
+            T pt[8], pl[8];
             if constexpr (DZ) {
                 float d[8];
                 gl_with_act(a.act, [&](auto act) {
@@ -141,16 +145,21 @@ __device__ __forceinline__ void any_tiles(const AnyArgs& a, long long first, lon
                 for (int k = 0; k < 8; ++k) {
                     d[k] = k < t.p_have ? d[k] : 0.0f;
                     sum[k] += d[k];
-                    pt[k] = (T)d[k];
+                    if constexpr (TWO) gl_split(d[k], pt[k], pl[k]);
+                    else pt[k] = (T)d[k];
                 }
             } else {
 #pragma unroll
-                for (int k = 0; k < 8; ++k) pt[k] = k < t.p_have ? t.p[k] : (T)0.0f;
+                for (int k = 0; k < 8; ++k) {
+                    pt[k] = k < t.p_have ? t.p[k] : (T)0.0f;
+                    if constexpr (TWO) pl[k] = k < t.p_have ? t.z[k] : (T)0.0f;
+                }
             }
 #pragma unroll
             for (int k = 0; k < 8; ++k) t.q[k] = k < t.q_have ? t.q[k] : (T)0.0f;
             __syncthreads();
             deposit(Ps, a.p_along, pt);
+            if constexpr (TWO) deposit(Ls, a.p_along, pl);
             deposit(Qs, a.q_along, t.q);
             __syncthreads();
             load(t, q0 + 2 * kBQ);
@@ -159,11 +168,13 @@ __device__ __forceinline__ void any_tiles(const AnyArgs& a, long long first, lon
 #pragma unroll
                 for (int s = 0; s < kBQ; s += 16) {
                     const v8 x = *(const v8*)(Qs + (wj + li) * kPitch + s + 8 * lk);
-                    const v8 y = *(const v8*)(Ps + (wi + li) * kPitch + s + 8 * lk);
-                    if constexpr (__is_same(T, gl_bf16))
-                        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, acc, 0, 0, 0);
-                    else
-                        acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, y, acc, 0, 0, 0);
+                    auto product = [&](const T* side, f32x16 c) -> f32x16 {
+                        const v8 y = *(const v8*)(side + (wi + li) * kPitch + s + 8 * lk);
+                        if constexpr (__is_same(T, gl_bf16)) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, c, 0, 0, 0);
+                        else return __builtin_amdgcn_mfma_f32_32x32x16_f16(x, y, c, 0, 0, 0);
+                    };
+                    acc = product(Ps, acc);
+                    if constexpr (TWO) low = product(Ls, low);
                 }
             } else {
 #pragma unroll
@@ -179,6 +190,9 @@ __device__ __forceinline__ void any_tiles(const AnyArgs& a, long long first, lon
             multiply(even, q0);
             multiply(odd, q0 + kBQ);
         }
+        if constexpr (TWO)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[r] = fmaf(low[r], kSplitStep<T>, acc[r]);
         if constexpr (DZ) {
             if ((a.sums || a.db) && j0 == 0) {               // not p_along: thread = (8 rows, one of 32 indexes)
                 __shared__ float red[4][kTile];
@@ -252,7 +266,7 @@ __device__ __forceinline__ void any_tiles(const AnyArgs& a, long long first, lon
 }
 
 // grid (workgroups, parts); workgroups walk over the tiles.  flags: only the tiles whose flag is set.
-template <typename T, typename TO, int V>
+template <typename T, typename TO, int V, bool TWO>
 __global__ void __launch_bounds__(256) k_dense_any(AnyArgs a, const int* __restrict__ flags) {
     if (flags) {                                             // all of this workgroup's at once: there is hardly ever one
         int set = 0;
@@ -260,18 +274,18 @@ __global__ void __launch_bounds__(256) k_dense_any(AnyArgs a, const int* __restr
             set |= flags[tile];
         if (!__syncthreads_or(set)) return;
     }
-    any_tiles<T, TO, T, V, false>(a, blockIdx.x, gridDim.x, blockIdx.y, flags);
+    any_tiles<T, TO, T, V, false, TWO>(a, blockIdx.x, gridDim.x, blockIdx.y, flags);
 }
 
 // The gradients of a small layer in one launch: tiles (times parts) of dx, then of dweight, whose first ones sum dz for dbias.
 // dz is worked out from dy and z by every tile that reads it.  641 x 80 -> 512 float32: 11.6 us and 5.8 for the join, where a pass
 // for dz, its sums, two products and their joins took 35 us.
-template <typename T, typename TO, int V>
+template <typename T, typename TO, int V, bool TWO>
 __global__ void __launch_bounds__(256) k_dense_back_small(AnyArgs x, AnyArgs w, int x_blocks) {
     const bool second = (int)blockIdx.x >= x_blocks;
     const AnyArgs a = second ? w : x;
     const int block = blockIdx.x - (second ? x_blocks : 0), part = block / a.n_tiles;
-    any_tiles<T, T, TO, V, true>(a, block - part * a.n_tiles, a.n_tiles, part, nullptr);
+    any_tiles<T, T, TO, V, true, TWO>(a, block - part * a.n_tiles, a.n_tiles, part, nullptr);
 }
 
 // Its join: elements of dx, then of dweight (where there are parts of them), then of dbias.  V divides `inputs`.
@@ -498,9 +512,8 @@ __global__ void __launch_bounds__(256) k_dense_halves(Halves a, Halves b, int co
     }
 }
 
-// dz = dy act'(z), rounded for the products that read it (to T, which is what the matrix instructions take: half a step a term;
-// or into three planes beside `exact`), zeros up to dz_stride columns, and column sums of the unrounded dz over this
-// workgroup's frames.  grid (blocks of 64 V columns, parts of the frames); thread =
+// dz = dy act'(z), as the products read it (splits_dz() says which): rounded to T, in two planes of T, or, float32, in three of
+// bfloat16 beside `exact`; zeros up to dz_stride columns, and column sums of the unrounded dz over this workgroup's frames.  grid (blocks of 64 V columns, parts of the frames); thread =
 // (V columns, one of 4 frame lanes).  dz is a pass of its own, since both products read it and one of them transposed; it is
 // bound by memory: 55 104 x 2048 bf16 gelu 129 us (677 MB, 5.2 TB/s).
 template <typename T, typename TO, int V, int PLANES>
@@ -541,6 +554,18 @@ __global__ void __launch_bounds__(256) k_dense_dz(const TO* __restrict__ dy, lon
 #pragma unroll
                 for (int v = 0; v < V; ++v) o[v] = (T)d[v];
                 *(typename vecn<T, V>::type*)((T*)dz_ + i * dz_stride + n) = o;
+            } else if constexpr (PLANES == 2) {
+                typename vecn<T, V>::type h, l;
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    T high, below;
+                    gl_split(d[v], high, below);
+                    h[v] = high;
+                    l[v] = below;
+                }
+                T* o = (T*)dz_ + i * dz_stride + n;
+                *(typename vecn<T, V>::type*)o = h;
+                *(typename vecn<T, V>::type*)(o + plane) = l;
             } else {
                 typename vecn<gl_bf16, V>::type h, m, l;
 #pragma unroll
@@ -627,7 +652,7 @@ bool quads(const Epilogue& e, int J) {
     return J % 4 == 0 && whole(e.y, e.y_stride) && whole(e.z, e.z_stride) && whole(e.residual, e.r_stride);
 }
 
-template <typename T, typename TO>
+template <typename T, typename TO, bool TWO>
 int any_product(const Operand& P, const Operand& Q, Epilogue e, long long I, int J, long long nq, float* partial, hipStream_t st) {
     const int splits = n_splits(I, J, nq);
     const long long per = gl_ceil_div(gl_ceil_div(nq, splits), kBQ) * kBQ;
@@ -638,7 +663,7 @@ int any_product(const Operand& P, const Operand& Q, Epilogue e, long long I, int
     e.exact_p = nullptr;
     e.quads = quads<TO>(e, J);
     const bool wide = wide_loads(P, P.qs == 1 ? nq : I, sizeof(T)) && wide_loads(Q, Q.qs == 1 ? nq : J, sizeof(T));
-    auto kernel = wide ? k_dense_any<T, TO, 16 / sizeof(T)> : k_dense_any<T, TO, 1>;
+    auto kernel = wide ? k_dense_any<T, TO, 16 / sizeof(T), TWO> : k_dense_any<T, TO, 1, TWO>;
     const AnyArgs a = {P, Q, {}, e, I, nq, per, J, (int)gl_ceil_div(J, kTile), (int)tiles, GL_ACT_NONE, P.qs == 1,
                        Q.qs == 1, nullptr, nullptr};
     hipLaunchKernelGGL(kernel, dim3((unsigned)(tiles < kMostBlocks ? tiles : kMostBlocks), (unsigned)used), dim3(256), 0, st, a,
@@ -699,7 +724,7 @@ template <typename T, typename TO, int SEG>
 int product(const Operand& P, const Operand& Q, const Operand& P0, const Operand& Q0, Epilogue e, long long I, int J, long long nq,
             float* partial, bool fast, hipStream_t st) {
     if constexpr (sizeof(T) == 2) {
-        if (gl_mm16_takes(P, Q, e, I, J, nq, sizeof(TO))) return gl_mm16<T, TO, T, 1>(P, Q, e, I, J, nq, partial, st);
+        if (gl_mm16_takes(P, Q, e, I, J, nq, sizeof(TO))) return gl_mm16<T, TO, T, SEG>(P, Q, e, I, J, nq, partial, st);
     } else if constexpr (SEG > 1) {
         if (fast && gl_mm16_takes(P, Q, e, I, J, nq, sizeof(TO))) {
             e.exact_p = (const float*)P0.base;
@@ -715,7 +740,7 @@ int product(const Operand& P, const Operand& Q, const Operand& P0, const Operand
         }
     }
     e.scale_p = nullptr;
-    return any_product<T, TO>(P0, Q0, e, I, J, nq, partial, st);
+    return any_product<T, TO, SEG == 2>(P0, Q0, e, I, J, nq, partial, st);
 }
 
 int check_types(int dtype, int out_dtype, int act, const char* who) {
@@ -855,17 +880,28 @@ SmallSplit small_split(long long I, int J, long long nq) {
     return s;
 }
 
+// Whether 16-bit products take dz in two planes.  bfloat16 with a dy of its own type: once rounded (half a step a term, what dy
+// itself has lost already: the gradients' error against 64 bits is 0.0023 of them where their own rounding makes 0.0017, and
+// 55 104 x 512 -> 2048 gelu takes 374 us where two planes take 614).  A caller who keeps dy and z in float32 keeps dz to 2^-18
+// of it (676 us, rounded once 463).  float16: dz falls below the type's
+// range where dy does not (a mean over a batch's magnitudes has gradients of 2e-8, and act' makes them smaller), and sums over
+// frames bring it back: two planes reach 2^-48.  dy itself serves without an activation, where it is of the products' type.
+bool splits_dz(int dtype, int out_dtype, int act) {
+    return dtype != GL_F32 && (out_dtype == GL_F32 || (dtype == GL_F16 && act != GL_ACT_NONE));
+}
+
 // workspace of a small layer: [parts of dx] [parts of dweight] [parts of dbias]; else
 // [dz (unless dy serves), or its planes] [with planes: dz itself, for sums that are not finite] [copy of x]
 // [copy of weight] [column-sum parts] [flags and parts of dx and dweight, one after the other on the stream: the larger]
 struct BackLayout {
-    bool small, own_dz, copy, planes;
+    bool small, own_dz, copy, planes, two;
     SmallSplit x, w;
     long long dz_stride, dz_bytes, dz32_bytes, x_bytes, w_bytes, parts_bytes, partial;
     long long total() const { return dz_bytes + dz32_bytes + x_bytes + w_bytes + parts_bytes + partial; }
 };
 BackLayout back_layout(long long rows, int inputs, int outputs, int dtype, int out_dtype, int act) {
     BackLayout l = {};
+    l.two = splits_dz(dtype, out_dtype, act);
     l.small = is_small(rows, inputs, outputs, dtype, true);
     if (l.small) {
         l.x = small_split(rows, inputs, outputs);
@@ -879,7 +915,7 @@ BackLayout back_layout(long long rows, int inputs, int outputs, int dtype, int o
     // dy itself serves where nothing is to be multiplied, converted or padded
     l.own_dz = act != GL_ACT_NONE || dtype != out_dtype || (dtype != GL_F32 && outputs % 32) || l.planes;
     l.dz_stride = pad_to(outputs);
-    if (l.own_dz) l.dz_bytes = gl_align16(rows * l.dz_stride * (l.planes ? 6 : 2));
+    if (l.own_dz) l.dz_bytes = gl_align16(rows * l.dz_stride * (l.planes ? 6 : l.two ? 4 : 2));
     if (l.planes && act != GL_ACT_NONE) l.dz32_bytes = gl_align16(rows * l.dz_stride * 4);
     l.copy = copies(dtype, inputs);
     if (l.copy) {
@@ -913,7 +949,7 @@ int dz_pass(const void* dy, long long dy_stride, const void* z, long long z_stri
     return dz_launch<T, TO, 1, PLANES>(dy, dy_stride, z, z_stride, dz, dz_stride, exact, parts, rows, outputs, act, st);
 }
 
-template <typename T, typename TO>
+template <typename T, typename TO, bool TWO>
 int backward_small(const void* dy, long long dy_stride, const void* x, long long x_stride, const void* w, long long w_stride,
                    const void* z, long long z_stride, void* dx, long long dx_stride, void* dw, long long dw_stride, void* db,
                    long long rows, int inputs, int outputs, int act, const BackLayout& l, void* ws, hipStream_t st) {
@@ -940,7 +976,7 @@ int backward_small(const void* dy, long long dy_stride, const void* x, long long
     const long long x_blocks = dx ? l.x.tiles * l.x.parts : 0, w_blocks = dw || db ? (long long)b.n_tiles * l.w.parts : 0;
     const bool v = wide_loads(a.P, outputs, sizeof(TO)) && (act == GL_ACT_NONE || wide_loads(a.Z, outputs, sizeof(TO))) &&
                    (!dx || wide_loads(a.Q, inputs, sizeof(T))) && (!dw || wide_loads(b.Q, inputs, sizeof(T)));
-    auto kernel = v ? k_dense_back_small<T, TO, 16 / sizeof(T)> : k_dense_back_small<T, TO, 1>;
+    auto kernel = v ? k_dense_back_small<T, TO, 16 / sizeof(T), TWO> : k_dense_back_small<T, TO, 1, TWO>;
     hipLaunchKernelGGL(kernel, dim3((unsigned)(x_blocks + w_blocks)), dim3(256), 0, st, a, b, (int)x_blocks);
     GL_HIP_CHECK(hipGetLastError());
     BackJoin j = {a.e.partial, b.e.partial, b.sums, l.x.parts, l.w.parts, a.e.partial ? rows * inputs : 0,
@@ -956,7 +992,7 @@ int backward_small(const void* dy, long long dy_stride, const void* x, long long
     return 0;
 }
 
-template <typename T, typename TO>
+template <typename T, typename TO, bool TWO>
 int backward(const void* dy, long long dy_stride, const void* x, long long x_stride, const void* w, long long w_stride,
              const void* z, long long z_stride, void* dx, long long dx_stride, void* dw, long long dw_stride, void* db,
              long long rows, int inputs, int outputs, int act, const BackLayout& l, void* ws, hipStream_t st) {
@@ -971,7 +1007,7 @@ int backward(const void* dy, long long dy_stride, const void* x, long long x_str
     int rc = 0;
     if (dz || db) {
         float* sums = db ? parts : nullptr;
-        rc = dz_pass<T, TO, sizeof(T) == 4 ? 3 : 1>(dy, dy_stride, z, z_stride, dz, l.dz_stride, dz32, sums, rows, outputs, act, st);
+        rc = dz_pass<T, TO, sizeof(T) == 4 ? 3 : TWO ? 2 : 1>(dy, dy_stride, z, z_stride, dz, l.dz_stride, dz32, sums, rows, outputs, act, st);
         if (rc) return rc;
     }
     if (db) {
@@ -988,20 +1024,20 @@ int backward(const void* dy, long long dy_stride, const void* x, long long x_str
     const Packed wp = {w, w_stride, dx ? outputs : 0, w_copy}, xp = {x, x_stride, dw ? rows : 0, x_copy};
     if (l.copy && products) rc = pack<T>(wp, xp, inputs, st);
     if (rc) return rc;
-    constexpr int SEG = sizeof(T) == 4 ? 6 : 1;
+    constexpr int SEG = sizeof(T) == 4 ? 6 : TWO ? 2 : 1;
     Epilogue e = {};
     if (dx) {
         const Operand Q0 = {w, 1, w_stride}, Q = l.copy ? copied(wp, inputs, true) : Q0;
         e.y = dx;
         e.y_stride = dx_stride;
-        rc = product<T, T, SEG>({d, d_stride, 1, plane, padded}, Q, {d0, d0_stride, 1}, Q0, e, rows, inputs, outputs, partial, true, st);
+        rc = product<T, T, SEG>({d, d_stride, 1, plane, padded}, Q, {d0, d0_stride, 1, plane}, Q0, e, rows, inputs, outputs, partial, true, st);
         if (rc) return rc;
     }
     if (dw) {
         const Operand Q0 = {x, 1, x_stride}, Q = l.copy ? copied(xp, inputs, true) : Q0;
         e.y = dw;
         e.y_stride = dw_stride;
-        rc = product<T, T, SEG>({d, 1, d_stride, plane, padded}, Q, {d0, 1, d0_stride}, Q0, e, outputs, inputs, rows, partial, true, st);
+        rc = product<T, T, SEG>({d, 1, d_stride, plane, padded}, Q, {d0, 1, d0_stride, plane}, Q0, e, outputs, inputs, rows, partial, true, st);
     }
     return rc;
 }
@@ -1031,7 +1067,7 @@ int gl_dense_flagged(const gl_epilogue& e, long long I, int J, long long nq, hip
     f.quads = quads<float>(e, J);
     const AnyArgs a = {{e.exact_p, e.exact_p_is, e.exact_p_qs}, {e.exact_q, e.exact_q_is, e.exact_q_qs}, {}, f, I, nq, nq, J,
                        (int)gl_ceil_div(J, kTile), (int)tiles, GL_ACT_NONE, e.exact_p_qs == 1, e.exact_q_qs == 1, nullptr, nullptr};
-    hipLaunchKernelGGL((k_dense_any<float, float, 1>), dim3((unsigned)(tiles < 512 ? tiles : 512)), dim3(256), 0, st, a, e.flags);
+    hipLaunchKernelGGL((k_dense_any<float, float, 1, false>), dim3((unsigned)(tiles < 512 ? tiles : 512)), dim3(256), 0, st, a, e.flags);
     GL_HIP_CHECK(hipGetLastError());
     return 0;
 }
@@ -1180,12 +1216,13 @@ int gl_dense_backward(const void* dy, long long dy_stride, const void* x, long l
     const BackLayout l = back_layout(rows, inputs, outputs, dtype, out_dtype, activation);
     if (!rc) rc = check_workspace(workspace, workspace_bytes, l.total(), "gl_dense_backward");
     if (rc) return rc;
-#define GL_BACK(T, TO)                                                                                                    \
-    (l.small ? backward_small<T, TO> : backward<T, TO>)(dy, dy_stride, x, x_stride, weight, w_stride, preactivation,      \
+#define GL_BACK(T, TO, TWO)                                                                                               \
+    (l.small ? backward_small<T, TO, TWO> : backward<T, TO, TWO>)(dy, dy_stride, x, x_stride, weight, w_stride, preactivation,      \
         z_stride, dx, dx_stride, dweight, dw_stride, dbias, rows, inputs, outputs, activation, l, workspace, st)
-    if (dtype == GL_F32) return GL_BACK(float, float);
-    if (dtype == GL_BF16) return out_dtype == GL_F32 ? GL_BACK(gl_bf16, float) : GL_BACK(gl_bf16, gl_bf16);
-    return out_dtype == GL_F32 ? GL_BACK(gl_f16, float) : GL_BACK(gl_f16, gl_f16);
+    if (dtype == GL_F32) return GL_BACK(float, float, false);
+    if (dtype == GL_BF16) return l.two ? GL_BACK(gl_bf16, float, true) : GL_BACK(gl_bf16, gl_bf16, false);
+    if (out_dtype == GL_F32) return GL_BACK(gl_f16, float, true);
+    return l.two ? GL_BACK(gl_f16, gl_f16, true) : GL_BACK(gl_f16, gl_f16, false);
 #undef GL_BACK
 }
 

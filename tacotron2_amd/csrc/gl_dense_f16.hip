@@ -3,3 +3,4 @@
 
 template int gl_mm16<gl_f16, gl_f16, gl_f16, 1>(const gl_operand&, const gl_operand&, gl_epilogue, long long, int, long long, float*, hipStream_t);
 template int gl_mm16<gl_f16, float, gl_f16, 1>(const gl_operand&, const gl_operand&, gl_epilogue, long long, int, long long, float*, hipStream_t);
+template int gl_mm16<gl_f16, gl_f16, gl_f16, 2>(const gl_operand&, const gl_operand&, gl_epilogue, long long, int, long long, float*, hipStream_t);

@@ -13,8 +13,9 @@
 // way); its 32-byte pieces are XORed with the row so that the 8 rows of half a wave spread over all banks.  The swizzle is
 // applied to the global address, since direct loads place consecutive lanes' chunks consecutively.
 //
-// float32 operands come in planes, and C is a sum of SEG products of planes.  A block with a sum that the planes do not give
-// is not written but flagged, and the float32 kernel computes it.
+// Operands of more bits come in planes, and C is a sum of SEG products of planes.
+//   2: P in two planes of Q's own type (gl_split): low x Q first, times kSplitStep, then high x Q.
+// float32 operands: a block with a sum that the planes do not give is not written but flagged, and the float32 kernel computes it.
 //   3: two planes of f16 per row (gl_scale), where a row of either side is one of the contraction: h l, l h, then, with the
 //      sums times 2^-12, h h.  Left out is l l 2^-24 <= 2^-24 |x| |y|: with both sides' rounding three roundings a product.
 //   6: three planes of bfloat16, x = h + m + l with h = bf16(x), m = bf16(x - h), l = bf16(x - h - m), which need no scale (an
@@ -67,8 +68,8 @@ __device__ __forceinline__ void barrier() {
 }
 
 // The planes of the products, two bits each
-template <int SEG> constexpr int kPlanesP = SEG == 3 ? 0 | 1 << 2 | 0 << 4 : 0 | 0 << 2 | 1 << 4 | 1 << 6 | 0 << 8 | 2 << 10;
-template <int SEG> constexpr int kPlanesQ = SEG == 3 ? 1 | 0 << 2 | 0 << 4 : 0 | 1 << 2 | 0 << 4 | 1 << 6 | 2 << 8 | 0 << 10;
+template <int SEG> constexpr int kPlanesP = SEG == 2 ? 1 | 0 << 2 : SEG == 3 ? 0 | 1 << 2 | 0 << 4 : 0 | 0 << 2 | 1 << 4 | 1 << 6 | 0 << 8 | 2 << 10;
+template <int SEG> constexpr int kPlanesQ = SEG == 2 ? 0 : SEG == 3 ? 1 | 0 << 2 | 0 << 4 : 0 | 1 << 2 | 0 << 4 | 1 << 6 | 2 << 8 | 0 << 10;
 __device__ __forceinline__ int plane_of(int planes, int seg) { return planes >> (2 * seg) & 3; }
 
 constexpr int kFlags = 0x00027000;                           // raw 32-bit buffer: bounds-checked, no format conversion
@@ -171,7 +172,7 @@ struct Out {
     void* z;                     // of TO or null
     long long z_stride;
     int act;                     // where the kernel does not fix it
-    int* flags;                  // SEG > 1: per 64 x 64 block of C, whether it is left to the float32 kernel; or null
+    int* flags;                  // float32 operands: per 64 x 64 block of C, whether it is left to the float32 kernel; or null
     long long part_stride;       // elements of y between the results of two parts of the contraction (bias, residual and z
                                  // are null then)
     int odd;                     // rows start off 4 bytes: elements are stored one by one (TAIL kernels)
@@ -412,15 +413,16 @@ __device__ __forceinline__ int epilogue(const Out& o, f32x4 (&acc)[MI][NI], long
     return put_block<TO, TAIL, LINES, MI, NI>((TO*)o.y + part * o.part_stride, o.y_stride, acc, i0, j0, I, J, lane, o.odd);
 }
 
-// SEG 3: the products h l + l h, which count 2^-12, before h h is added
+// The sums of the lower planes, which count `step`, before the highest ones' are added: SEG 3, h l + l h, 2^-12; SEG 2, kSplitStep
+template <int SEG, typename T> constexpr float kLower = SEG == 3 ? 0x1p-12f : SEG == 2 ? kSplitStep<T> : 1.0f;
 template <int MI, int NI>
-__device__ __forceinline__ void lower(f32x4 (&acc)[MI][NI]) {
+__device__ __forceinline__ void lower(f32x4 (&acc)[MI][NI], float step) {
 #pragma unroll
     for (int m = 0; m < MI; ++m)
 #pragma unroll
         for (int n = 0; n < NI; ++n)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) acc[m][n][r] *= 0x1p-12f;
+            for (int r = 0; r < 4; ++r) acc[m][n][r] *= step;
 }
 
 // A tile a workgroup, for products too small for the walk below: two stages of 64 contraction indexes, two workgroups a CU
@@ -478,7 +480,7 @@ k_mm16(Side P, Side Q, Out o, long long I, int J, long long nq, long long q_per_
 
     int slot = 0;
     for (int k = 0; k < steps; ++k) {
-        if (SEG == 3 && k == 2 * once) lower(acc);
+        if (kLower<SEG, T> != 1.0f && k == (SEG - 1) * once) lower(acc, kLower<SEG, T>);
         wait_loads((SP::kLoads + SQ::kLoads) * (ST - 2));
         barrier();
         load(slot == 0 ? ST - 1 : slot - 1);
@@ -502,7 +504,7 @@ k_mm16(Side P, Side Q, Out o, long long I, int J, long long nq, long long q_per_
 
     if constexpr (SEG == 3) {
         if (!unscale<TB, MI, NI>(o, acc, i0 + wi, j0 + wj, I, J, (float)nq, lane)) return;
-    } else if constexpr (SEG > 1) {
+    } else if constexpr (SEG > 2) {
         if (o.flags && !all_finite<MI, NI>(o.flags, acc, i0 + wi, j0 + wj, I, J, lane)) return;
     }
     epilogue<T, TO, ACT, true, true, false, MI, NI>(o, acc, i0 + wi, j0 + wj, I, J, blockIdx.y, lane);
@@ -616,10 +618,12 @@ k_mm16_walk(Side P, Side Q, Out o, long long I, int J, long long nq, long long q
         start_sums<TB, MI, NI>(acc, bias);
 #pragma unroll 1
         for (int k = pairs; k > 0; --k) {
-            if (SEG == 3 && pairs - k == once) lower(acc);
+            const int at = 2 * (pairs - k), from = (SEG - 1) * once;
+            if (kLower<SEG, T> != 1.0f && at == from) lower(acc, kLower<SEG, T>);
             if (left == 0) enter(tile + walkers);
             step(a[0], a[1]);
             left -= 2;
+            if (kLower<SEG, T> != 1.0f && SEG == 2 && at + 1 == from) lower(acc, kLower<SEG, T>);
             step(a[1], a[0]);
         }
         left = 2 * pairs - RING;
@@ -640,7 +644,7 @@ k_mm16_walk(Side P, Side Q, Out o, long long I, int J, long long nq, long long q
                 old = 0;
                 continue;
             }
-        } else if constexpr (SEG > 1) {
+        } else if constexpr (SEG > 2) {
             if (o.flags && !all_finite<MI, NI>(o.flags, acc, (long long)(tile / tiles_j) * BM + wi, tile % tiles_j * BN + wj, I, J, lane)) {
                 old = 0;
                 continue;

@@ -35,7 +35,7 @@ template <typename T, typename TO, typename TB, int SEG, int ACT, bool EXTRA, bo
 int walk(const gl_operand& P, const gl_operand& Q, const Out& o, long long I, int J, long long nq, const gl_mm_plan& p, hipStream_t st) {
     auto on_lines = [](const void* q, long long stride) { return !q || ((uintptr_t)q % 128 == 0 && stride * (long long)sizeof(TO) % 128 == 0); };
     const bool lines = p.parts == 1 && on_lines(o.y, o.y_stride) && on_lines(o.z, o.z_stride);
-    if constexpr (!PT && SEG == 1) {
+    if constexpr (!PT && SEG <= 2) {
         // Tiles of 224 rows where the chip's rounds of them are shorter than of 256: 55 104 x 512 (of 2048) are 1.7 rounds of 256,
         // 136 us, and 1.9 of 224, 123 us.  Not for rows read transposed (whole powers of two) or flagged in blocks of 64.
         auto rounds = [&](int rows) { return gl_ceil_div(gl_ceil_div(I, rows) * (J / 256), 256) * rows; };
@@ -61,7 +61,7 @@ int tiles(const gl_operand& P, const gl_operand& Q, const Out& o, long long I, i
 // 64 x 64 tiles: their waves are smaller than a block of flags, so float32 planes take 128 x 128 instead
 template <typename T, typename TO, typename TB, int SEG, bool PT, bool QT>
 int small(const gl_operand& P, const gl_operand& Q, const Out& o, long long I, int J, long long nq, const gl_mm_plan& p, hipStream_t st) {
-    if constexpr (SEG > 1) return tiles<T, TO, TB, SEG, 128, 64, PT, QT>(P, Q, o, I, J, nq, p, st);
+    if constexpr (SEG > 2) return tiles<T, TO, TB, SEG, 128, 64, PT, QT>(P, Q, o, I, J, nq, p, st);
     else return tiles<T, TO, TB, SEG, 64, 32, PT, QT>(P, Q, o, I, J, nq, p, st);
 }
 
@@ -118,13 +118,18 @@ int gl_mm16(const gl_operand& P, const gl_operand& Q, gl_epilogue e, long long I
         if (e.exact_q) f.exact_q = e.exact_q + j * e.exact_q_is;
         if (e.scale_q) f.scale_q = e.scale_q + j;
         const gl_mm_plan p = gl_mm_plan_for(I, n, pad, pt && qt);
-        int rc;
-        if (SEG == 3 || (!pt && !qt)) rc = gl_mm::one<T, TO, TB, SEG, false, false>(P, q, f, I, n, nq, p, partial, st);
-        else if constexpr (SEG != 3)
-            rc = !pt ? gl_mm::one<T, TO, TB, SEG, false, true>(P, q, f, I, n, nq, p, partial, st)
+        int rc = 0;
+        bool along = SEG == 3;                               // both sides contiguous in the contraction: no gradients
+        if constexpr (SEG != 2) {
+            along |= !pt && !qt;
+            if (along) rc = gl_mm::one<T, TO, TB, SEG, false, false>(P, q, f, I, n, nq, p, partial, st);
+        }
+        if constexpr (SEG != 3) {
+            if (!along) rc = !pt ? gl_mm::one<T, TO, TB, SEG, false, true>(P, q, f, I, n, nq, p, partial, st)
                      : gl_mm::one<T, TO, TB, SEG, true, true>(P, q, f, I, n, nq, p, partial, st);
+        }
         if (rc) return rc;
-        if (SEG > 1 && p.parts == 1) {                       // the blocks that were left out, if any
+        if (SEG > 2 && p.parts == 1) {                       // the blocks that were left out, if any
             const int rf = gl_dense_flagged(f, I, n, nq, st);
             if (rf) return rf;
         }
