@@ -6,6 +6,7 @@ typedef _Float16 gl_f16;
 typedef __bf16 gl_bf16;
 
 template <int N> struct gl_int { static constexpr int value = N; };
+template <typename T> constexpr bool gl_fine = __is_same(T, float);
 
 __device__ __forceinline__ float gl_to_f32(float v) { return v; }
 __device__ __forceinline__ float gl_to_f32(gl_bf16 v) { return (float)v; }
@@ -22,26 +23,49 @@ __device__ __forceinline__ float gl_exp(float z) {
 __device__ __forceinline__ float gl_sigmoid(float z) {
     return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504088896341f));
 }
-// Phi(-a) = t p exp(-a^2 / 2) for a >= 0: Abramowitz and Stegun 7.1.26, erfc(x) = t (a1 + t (a2 + ...)) exp(-x^2),
-// t = 1 / (1 + p x), with x = a / sqrt 2; |error of erf| <= 1.5e-7.
-__device__ __forceinline__ float gl_phi_poly(float a, float& t) {
-    t = __builtin_amdgcn_rcpf(fmaf(a, 0.3275911f * 0.70710678118654752f, 1.0f));
-    float p = fmaf(t, 1.061405429f * 0.5f, -1.453152027f * 0.5f);
-    p = fmaf(p, t, 1.421413741f * 0.5f);
-    p = fmaf(p, t, -0.284496736f * 0.5f);
-    return fmaf(p, t, 0.254829592f * 0.5f);
+// FINE, here and below: for float32 results.  The rest is for 16-bit ones, next to whose half step (2^-12 and more) it errs little.
+
+// Phi(-a) / exp(-a^2 / 2) for a >= 0, in the form of Hastings' approximations: t P(t), t = 1 / (1 + c a).  c and P are fitted by
+// weighted least squares (Lawson's weights) for the smallest relative error over a <= 14.6, where the result leaves float32's
+// range: 2^-24.9.  Eight terms would leave 2^-22.5, five 2^-14.9, which shows in float16.
+__device__ __forceinline__ float gl_phi_ratio(float a) {
+    const float t = __builtin_amdgcn_rcpf(fmaf(a, 0.35f, 1.0f));
+    float p = fmaf(t, -2.915946483e-02f, 1.440387674e-01f);
+    p = fmaf(p, t, -2.558555896e-01f);
+    p = fmaf(p, t, 1.593390985e-01f);
+    p = fmaf(p, t, -2.322604228e-02f);
+    p = fmaf(p, t, 1.055584544e-01f);
+    p = fmaf(p, t, 1.198197353e-01f);
+    p = fmaf(p, t, 1.398637337e-01f);
+    p = fmaf(p, t, 1.396212914e-01f);
+    return t * p;
+}
+// exp(-a^2 / 2).  FINE: with what a^2 and its product with log2(e) / 2 lose; a is cut off where the result has long been zero.
+template <bool FINE>
+__device__ __forceinline__ float gl_gauss(float a) {
+    if constexpr (!FINE) return __builtin_amdgcn_exp2f(a * a * -0.72134752044448170f);
+    else {
+#pragma clang fp contract(off)
+        constexpr float k = -0.72134752044448170f;           // -log2(e) / 2, and what float32 leaves of it
+        constexpr float k_rest = (float)(-0.72134752044448170 - (double)k);
+        a = __builtin_amdgcn_fmed3f(a, 0.0f, 16.0f);
+        const float s = a * a, t = s * k;
+        const float rest = fmaf(fmaf(a, a, -s), k, fmaf(s, k_rest, fmaf(s, k, -t)));
+        const float e = __builtin_amdgcn_exp2f(t);
+        return fmaf(e, rest * 0.69314718055994531f, e);
+    }
 }
 
 // act(z).  Every branch on `act` is uniform: a kernel argument or a template constant.  For many values at once take
 // gl_with_act around the loop: a branch a value scatters the code that runs over all activations of all values.
+template <bool FINE>
 __device__ __forceinline__ float gl_act(float z, int act) {
     switch (act) {
         case GL_ACT_RELU: return z < 0.0f ? 0.0f : z;                  // NaN stays NaN
         case GL_ACT_SILU: return z * gl_sigmoid(z);
-        case GL_ACT_GELU: {                                            // z Phi(z) = z / 2 + |z| (1 / 2 - Phi(-|z|))
-            float t;
-            const float p = gl_phi_poly(fabsf(z), t), e = __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f);
-            return fmaf(fabsf(z), fmaf(-(t * p), e, 0.5f), 0.5f * z);
+        case GL_ACT_GELU: {                                            // z Phi(z), Phi(z) = 1 - Phi(-z): no tail is a difference
+            const float h = gl_phi_ratio(fabsf(z)) * gl_gauss<FINE>(fabsf(z));
+            return z * (z > 0.0f ? 1.0f - h : h);
         }
         case GL_ACT_TANH: {
             // (1 - e) / (1 + e) with e = exp(-2 |z|); near zero the series z - z^3/3 + 2 z^5/15 - 17 z^7/315
@@ -56,7 +80,8 @@ __device__ __forceinline__ float gl_act(float z, int act) {
     }
 }
 
-// act'(z)
+// act'(z).  FINE: of float32 gradients
+template <bool FINE>
 __device__ __forceinline__ float gl_act_grad(float z, int act) {
     switch (act) {
         case GL_ACT_RELU: return z > 0.0f ? 1.0f : (z != z ? z : 0.0f);
@@ -65,9 +90,7 @@ __device__ __forceinline__ float gl_act_grad(float z, int act) {
             return fmaf(z * s, 1.0f - s, s);
         }
         case GL_ACT_GELU: {                                            // Phi(z) + z phi(z)
-            const float a = fabsf(z), e = __builtin_amdgcn_exp2f(a * a * -0.72134752044448170f);
-            float t;
-            const float p = gl_phi_poly(a, t), h = t * p * e;
+            const float a = fabsf(z), e = gl_gauss<FINE>(a), h = gl_phi_ratio(a) * e;
             return fmaf(z * e, 0.39894228040143268f, z < 0.0f ? h : 1.0f - h);
         }
         case GL_ACT_TANH: {                                            // 4 e / (1 + e)^2 with e = exp(-2 |z|)
