@@ -12,18 +12,29 @@ __device__ __forceinline__ float gl_to_f32(float v) { return v; }
 __device__ __forceinline__ float gl_to_f32(gl_bf16 v) { return (float)v; }
 __device__ __forceinline__ float gl_to_f32(gl_f16 v) { return (float)v; }
 
-// exp(z) = 2^(z log2 e).  The product's rounding moves the result by |z| 2^-24 of it, as half a step of z itself does: a sum z
-// is not known better than that, so it is not carried further.
+// FINE, here and below: for float32 results.  The rest is for 16-bit ones, next to whose half step (2^-12 and more) it errs little.
+
+// exp(z) = 2^(z log2 e).  The product's rounding moves the result by up to |z| 2^-24 of it; FINE takes what it lost along.
+template <bool FINE>
 __device__ __forceinline__ float gl_exp(float z) {
-    const float t = z * 1.44269504088896341f;
+    constexpr float k = 1.44269504088896341f;
+    float t = z * k;
+    if constexpr (FINE) asm("" : "+v"(t));                   // the rounded product itself: never one operation with what is added below
     const bool low = t < -120.0f;                            // subnormal results: 2^64 up, then down with one rounding
-    return __builtin_amdgcn_exp2f(t + (low ? 64.0f : 0.0f)) * (low ? 0x1p-64f : 1.0f);
+    float e = __builtin_amdgcn_exp2f(t + (low ? 64.0f : 0.0f));
+    if constexpr (FINE) {
+        constexpr float k_rest = (float)(1.44269504088896341 - (double)k);
+        const float rest = fmaf(z, k_rest, fmaf(z, k, -t));
+        e = fabsf(t + 16.0f) < 144.0f ? fmaf(e, rest * 0.69314718055994531f, e) : e;        // not where e is infinite, or z
+    }
+    return e * (low ? 0x1p-64f : 1.0f);
 }
 
+template <bool FINE>
 __device__ __forceinline__ float gl_sigmoid(float z) {
-    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504088896341f));
+    if constexpr (FINE) return __builtin_amdgcn_rcpf(1.0f + gl_exp<true>(-z));
+    else return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504088896341f));
 }
-// FINE, here and below: for float32 results.  The rest is for 16-bit ones, next to whose half step (2^-12 and more) it errs little.
 
 // Phi(-a) / exp(-a^2 / 2) for a >= 0, in the form of Hastings' approximations: t P(t), t = 1 / (1 + c a).  c and P are fitted by
 // weighted least squares (Lawson's weights) for the smallest relative error over a <= 14.6, where the result leaves float32's
@@ -45,7 +56,6 @@ template <bool FINE>
 __device__ __forceinline__ float gl_gauss(float a) {
     if constexpr (!FINE) return __builtin_amdgcn_exp2f(a * a * -0.72134752044448170f);
     else {
-#pragma clang fp contract(off)
         constexpr float k = -0.72134752044448170f;           // -log2(e) / 2, and what float32 leaves of it
         constexpr float k_rest = (float)(-0.72134752044448170 - (double)k);
         a = __builtin_amdgcn_fmed3f(a, 0.0f, 16.0f);
@@ -62,7 +72,7 @@ template <bool FINE>
 __device__ __forceinline__ float gl_act(float z, int act) {
     switch (act) {
         case GL_ACT_RELU: return z < 0.0f ? 0.0f : z;                  // NaN stays NaN
-        case GL_ACT_SILU: return z * gl_sigmoid(z);
+        case GL_ACT_SILU: return z * gl_sigmoid<FINE>(z);
         case GL_ACT_GELU: {                                            // z Phi(z), Phi(z) = 1 - Phi(-z): no tail is a difference
             const float h = gl_phi_ratio(fabsf(z)) * gl_gauss<FINE>(fabsf(z));
             return z * (z > 0.0f ? 1.0f - h : h);
@@ -75,7 +85,7 @@ __device__ __forceinline__ float gl_act(float z, int act) {
             const float near = fmaf(z * q, fmaf(q, fmaf(q, -0.0539682540f, 0.133333333f), -0.333333333f), z);
             return a < 0.25f ? near : far;
         }
-        case GL_ACT_EXP: return gl_exp(z);
+        case GL_ACT_EXP: return gl_exp<FINE>(z);
         default: return z;
     }
 }
@@ -86,7 +96,11 @@ __device__ __forceinline__ float gl_act_grad(float z, int act) {
     switch (act) {
         case GL_ACT_RELU: return z > 0.0f ? 1.0f : (z != z ? z : 0.0f);
         case GL_ACT_SILU: {
-            const float s = gl_sigmoid(z);
+            if constexpr (FINE) {                                      // s(z) and 1 - s(z) from exp(-|z|) <= 1, neither a difference
+                const float e = gl_exp<true>(-fabsf(z)), r = __builtin_amdgcn_rcpf(1.0f + e), s = z < 0.0f ? e * r : r;
+                return fmaf(z * s, z < 0.0f ? r : e * r, s);
+            }
+            const float s = gl_sigmoid<false>(z);
             return fmaf(z * s, 1.0f - s, s);
         }
         case GL_ACT_GELU: {                                            // Phi(z) + z phi(z)
@@ -98,7 +112,7 @@ __device__ __forceinline__ float gl_act_grad(float z, int act) {
             const float r = __builtin_amdgcn_rcpf(1.0f + e);
             return 4.0f * e * r * r;
         }
-        case GL_ACT_EXP: return gl_exp(z);
+        case GL_ACT_EXP: return gl_exp<FINE>(z);
         default: return 1.0f;
     }
 }

@@ -70,3 +70,39 @@ def test_gelu_slope_in_float32():
     parts = (0.5 * torch.special.erfc(-d / math.sqrt(2))) + (d * torch.exp(-d * d / 2)).abs() / math.sqrt(2 * math.pi)
     got = slopes(z, "gelu")
     assert ((got - slope64(d, "gelu")).abs() <= 2.0 ** -19.8 * parts + 2.0 ** -126).all()
+
+
+# -- exp, and silu through it ------------------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("way", [through, through_norm])
+def test_exp_and_silu_keep_float32_over_their_range(way):
+    """exp: exp2 two half steps, the correction one, the subnormal range's last product one, and one for the argument's own rest.
+    silu: that, 1 + e one, its reciprocal two, z one."""
+    z = torch.cat([torch.linspace(-87, 88.5, 3001), torch.linspace(-2, 2, 1001)])
+    d = z.double()
+    close(way(z, "exp"), torch.exp(d), 5 * 2.0 ** -24, 2.0 ** -126, "exp")
+    close(way(z, "silu"), d * torch.sigmoid(d), 9 * 2.0 ** -24, 2.0 ** -126 * 88, "silu")
+
+
+@gpu
+def test_exp_at_its_ends():
+    inf = float("inf")
+    z = torch.tensor([89.0, 200.0, 3e38, inf, -104.5, -200.0, -3e38, -inf, float("nan"), -100.0, 88.72, -87.4])
+    y = through(z, "exp")
+    assert (y[:4] == inf).all() and not y[4:8].any() and y[8].isnan()
+    assert ((y[9:] - torch.exp(z[9:].double())).abs() <= 2.0 ** -21 * y[9:] + 2.0 ** -149).all()
+    s = through(torch.tensor([inf, 3e38, -3e38, -200.0, float("nan")]), "silu")
+    assert s[0] == inf and s[1] == z[2].double()
+    assert not s[2:4].any() and s[4].isnan()
+
+
+@gpu
+def test_slopes_of_exp_and_silu_in_float32():
+    """exp as above.  silu: s and 1 - s six half steps each, their product with z two more, the sum one: of the larger part."""
+    z = torch.cat([torch.linspace(-80, 80, 2001), torch.linspace(-2, 2, 1001)])
+    d = z.double()
+    close(slopes(z, "exp"), torch.exp(d), 5 * 2.0 ** -24, 2.0 ** -126, "exp'")
+    s, o = torch.sigmoid(d), torch.sigmoid(-d)
+    assert ((slopes(z, "silu") - (s + d * s * o)).abs() <= 16 * 2.0 ** -24 * (s + (d * s * o).abs()) + 2.0 ** -126 * 80).all()
+    ends = slopes(torch.tensor([200.0, 3e38, -200.0, -3e38]), "silu")
+    assert torch.equal(ends.abs(), torch.tensor([1.0, 1.0, 0.0, 0.0]).double())
