@@ -106,3 +106,24 @@ def test_slopes_of_exp_and_silu_in_float32():
     assert ((slopes(z, "silu") - (s + d * s * o)).abs() <= 16 * 2.0 ** -24 * (s + (d * s * o).abs()) + 2.0 ** -126 * 80).all()
     ends = slopes(torch.tensor([200.0, 3e38, -200.0, -3e38]), "silu")
     assert torch.equal(ends.abs(), torch.tensor([1.0, 1.0, 0.0, 0.0]).double())
+
+
+# -- tanh --------------------------------------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("way", [through, through_norm])
+def test_tanh_keeps_float32_around_the_end_of_its_series(way):
+    """Near zero: z^2 and z^3 a half step each, of which at most 0.12 counts, five more in P, the sum one: 2 half steps.  Beyond 0.6:
+    e <= 0.31, five half steps of it moved onto 1 - e >= 0.69 (three), 1 - e and 1 + e one each, the reciprocal two, one: 8."""
+    z = torch.cat([torch.linspace(-1, 1, 4001), torch.linspace(-12, 12, 1001), torch.tensor([1e-6, -1e-30, 0.0, 50.0, -3e38])])
+    close(way(z, "tanh"), torch.tanh(z.double()), 8 * 2.0 ** -24, 2.0 ** -149, "tanh")
+    near = z[z.abs() < 0.59]
+    close(way(near, "tanh"), torch.tanh(near.double()), 2 * 2.0 ** -24, 2.0 ** -149, "tanh near zero")
+    ends = through(torch.tensor([float("inf"), -float("inf"), float("nan")]), "tanh")
+    assert ends[0] == 1 and ends[1] == -1 and ends[2].isnan()
+
+
+@gpu
+def test_slope_of_tanh_in_float32():
+    """4 e / (1 + e)^2: e five half steps, (1 + e) one, its reciprocal two, both twice, three products: 14."""
+    z = torch.cat([torch.linspace(-40, 40, 2001), torch.linspace(-1, 1, 1001)])
+    close(slopes(z, "tanh"), torch.cosh(z.double()) ** -2, 14 * 2.0 ** -24, 2.0 ** -126, "tanh'")
