@@ -11,6 +11,7 @@
 #include <c10/core/GradMode.h>
 #include <c10/core/impl/VirtualGuardImpl.h>
 #include <torch/csrc/Dtype.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "../../include/gl_hip.h"
@@ -90,15 +91,16 @@ bool stream_of(c10::Device device, void** stream) {
     return !PyErr_Occurred();
 }
 
-// f() with C++ exceptions as Python errors; f returns a new reference, or null for "not here"
+// f() with C++ exceptions as the Python errors that torch makes of them (torch.OutOfMemoryError among them); f returns a new
+// reference, or null for "not here"
 template <typename F>
 PyObject* guarded(F f) {
     try {
         PyObject* r = f();
         if (r || PyErr_Occurred()) return r;
         Py_RETURN_NONE;
-    } catch (const std::exception& e) {
-        PyErr_SetString(PyExc_RuntimeError, e.what());
+    } catch (...) {
+        torch::translate_exception_to_python(std::current_exception());
         return nullptr;
     }
 }
