@@ -288,6 +288,7 @@ int gl_pcm16_encode(gl_plan* plan, const float* x, long long row_stride, long lo
  *   Rows are frames; row strides are in elements, the elements of a row are contiguous.  A row stride may exceed
  *   the row; elements between rows are neither read into results nor written.  Results and workspace overlap no
  *   other argument, except where it says "may be".
+ *   Pointers are on whole multiples of their elements' size (GL_ERR_INVALID else).
  *   Limits (GL_ERR_INVALID beyond): rows < 2^31, T <= 2^30, B <= 65535, widths and channels <= 2^20, strides <= 2^31. */
 enum gl_dtype { GL_F32 = 0, GL_BF16 = 1, GL_F16 = 2 };
 enum gl_activation { GL_ACT_NONE = 0, GL_ACT_RELU = 1, GL_ACT_SILU = 2, GL_ACT_GELU = 3, GL_ACT_TANH = 4, GL_ACT_EXP = 5 };

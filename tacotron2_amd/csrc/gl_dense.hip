@@ -13,6 +13,7 @@
 //   v_mfma_f32_32x32x16 or, for float32, v_mfma_f32_32x32x2_f32.
 // Sums are float32 everywhere.  Q is the matrix instruction's A operand: the accumulator's registers then run along j, the
 // contiguous direction of C.
+#include <initializer_list>
 #include <type_traits>
 
 #include "gl_dense.h"
@@ -762,6 +763,12 @@ int check_stride(long long stride, int cols, const char* what, const char* who) 
         return gl_set_error(GL_ERR_INVALID, "%s: %s row stride %lld outside [%d, 2^31]", who, what, stride, cols);
     return 0;
 }
+// Elements start on whole multiples of their own size.
+int check_elements(std::initializer_list<const void*> arrays, int dtype, const char* who) {
+    for (const void* p : arrays)
+        if ((uintptr_t)p % (dtype == GL_F32 ? 4 : 2)) return gl_set_error(GL_ERR_INVALID, "%s: %p is not on its elements' size", who, p);
+    return 0;
+}
 int check_workspace(const void* ws, long long have, long long need, const char* who) {
     if (need == 0) return 0;
     if (!ws || have < need)
@@ -800,7 +807,7 @@ template <typename T, typename TO, int ROWS>
 int few(const void* x, long long x_stride, const void* w, long long w_stride, const Epilogue& e, int rows, int K, int N, hipStream_t st) {
     int V = 16 / sizeof(T);              // elements at once: what the widths and the arrays' alignment allow
     auto fits = [&](const void* p, long long stride) { return K % V == 0 && stride % V == 0 && (uintptr_t)p % (V * sizeof(T)) == 0; };
-    while (!fits(x, x_stride) || !fits(w, w_stride)) V /= 2;
+    while (V > 1 && (!fits(x, x_stride) || !fits(w, w_stride))) V /= 2;
     const int pieces = K / V;
     int L = kFewRows;                    // a lane for every row's result at least
     while (L < 64 && L < pieces) L *= 2;
@@ -1155,6 +1162,8 @@ int gl_dense(const void* x, long long x_stride, const void* weight, long long w_
     if (!rc) rc = check_stride(y_stride, outputs, "y", "gl_dense");
     if (!rc && residual) rc = check_stride(r_stride, outputs, "residual", "gl_dense");
     if (!rc && preactivation) rc = check_stride(z_stride, outputs, "preactivation", "gl_dense");
+    if (!rc) rc = check_elements({x, weight, bias}, dtype, "gl_dense");
+    if (!rc) rc = check_elements({residual, y, preactivation}, out_dtype, "gl_dense");
     const FrontLayout l = front_layout(rows, inputs, outputs, dtype);
     if (!rc) rc = check_workspace(workspace, workspace_bytes, l.total(), "gl_dense");
     if (rc) return rc;
@@ -1190,6 +1199,8 @@ int gl_dense_backward(const void* dy, long long dy_stride, const void* x, long l
     int rc = check_types(dtype, out_dtype, activation, "gl_dense_backward");
     if (!rc) rc = check_sizes(rows, inputs, outputs, "gl_dense_backward");
     if (!rc && dweight) rc = check_stride(dw_stride, inputs, "dweight", "gl_dense_backward");
+    if (!rc) rc = check_elements({x, weight, dx, dweight, dbias}, dtype, "gl_dense_backward");
+    if (!rc) rc = check_elements({dy, preactivation}, out_dtype, "gl_dense_backward");
     if (rc) return rc;
     const hipStream_t st = (hipStream_t)stream;
     if (rows == 0) {                                         // empty sums

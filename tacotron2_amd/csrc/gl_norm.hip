@@ -908,6 +908,12 @@ int check_stride(long long stride, int cols, const char* what, const char* who) 
         return gl_set_error(GL_ERR_INVALID, "%s: %s row stride %lld outside [%d, 2^31]", who, what, stride, cols);
     return 0;
 }
+// Elements start on whole multiples of their own size.
+int check_elements(std::initializer_list<const void*> arrays, int size, const char* who) {
+    for (const void* p : arrays)
+        if ((uintptr_t)p % size) return gl_set_error(GL_ERR_INVALID, "%s: %p is not on its elements' size", who, p);
+    return 0;
+}
 int check_workspace(const void* ws, long long have, long long need, const char* who) {
     if (need == 0) return 0;
     if (!ws || have < need)
@@ -1166,6 +1172,8 @@ int gl_group_norm(const void* x, long long x_stride, const void* gamma, const vo
     if (T > 0 && (!x || !y)) return gl_set_error(GL_ERR_INVALID, "gl_group_norm: NULL buffer");
     rc = check_stride(x_stride, channels, "x", "gl_group_norm");
     if (!rc) rc = check_stride(y_stride, channels, "y", "gl_group_norm");
+    if (!rc) rc = check_elements({x, gamma, beta, y}, dtype == GL_F32 ? 4 : 2, "gl_group_norm");
+    if (!rc) rc = check_elements({frames, stats}, 4, "gl_group_norm");
     if (!rc) rc = check_workspace(workspace, workspace_bytes, norm_bytes(B, T, channels, groups, dtype), "gl_group_norm");
     if (rc) return rc;
     if (T == 0 && !stats) return 0;
@@ -1195,6 +1203,8 @@ int gl_group_norm_backward(const void* dy, long long dy_stride, const void* x, l
                            void* dgamma, void* dbeta, int B, int T, int channels, int groups, int dtype,
                            int activation, void* workspace, long long workspace_bytes, void* stream) {
     int rc = check_norm(B, T, channels, groups, dtype, activation, "gl_group_norm_backward");
+    if (!rc) rc = check_elements({dy, x, gamma, beta, dx, dgamma, dbeta}, dtype == GL_F32 ? 4 : 2, "gl_group_norm_backward");
+    if (!rc) rc = check_elements({frames, stats}, 4, "gl_group_norm_backward");
     if (rc) return rc;
     const hipStream_t st = (hipStream_t)stream;
     float* pq = (float*)workspace;
