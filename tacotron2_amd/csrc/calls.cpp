@@ -13,6 +13,7 @@
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include "../../include/gl_hip.h"
 
@@ -39,7 +40,7 @@ struct Arg {
     bool other = false;
     explicit Arg(PyObject* o) {
         if (o == Py_None) return;
-        if (!THPVariable_CheckExact(o)) other = true;
+        if (!THPVariable_CheckExact(o) || THPVariable_Unpack(o)._fw_grad(0).defined()) other = true;     // with a tangent: refused
         else t = &THPVariable_Unpack(o);
     }
     explicit operator bool() const { return t; }
@@ -54,6 +55,7 @@ struct Arg {
 
 // A first argument that leads: float type, contiguous, on the current device
 bool leads(const Arg& x) {
+    if (torch::jit::tracer::isTracing()) return false;       // refused
     if (!x || x->layout() != at::kStrided || !x->is_cuda() || x->dim() < 1 || x->numel() == 0 || !x->is_contiguous()) return false;
     if (type_of(x->scalar_type()) < 0) return false;
     return c10::impl::VirtualGuardImpl(c10::DeviceType::CUDA).getDevice() == x->device();

@@ -15,13 +15,15 @@ with a row stride (``h[..., :512]``); anything that is not one row stride over c
 ``Plan.capture()`` nothing may be allocated: pass ``out=`` and ``workspace=`` (a uint8 tensor of at least
 :func:`dense_workspace` / ... bytes, not used by anything that may run at the same time).  The differentiable form
 refuses to run under a stream capture: autograd's own bookkeeping for leaves that already live in an eager graph ends
-the process there; capture the explicit forward and backward calls instead.
+the process there; capture the explicit forward and backward calls instead.  Tangents (forward-mode derivatives) and
+torch.jit.trace are refused.
 """
 import contextlib
 import ctypes
 import functools
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .plan import _require_gpu, raw_capture_active
@@ -202,6 +204,16 @@ def _needs_grad(*tensors):
     return False
 
 
+def _plain_call(what, *tensors):
+    """Refuses what would lose a derivative or the call itself without a word: tangents, and torch.jit.trace."""
+    if torch._C._get_tracing_state() is not None:
+        raise RuntimeError(f"{what}() cannot be traced: torch.jit.trace would record its empty result alone")
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{what}() has no forward-mode derivative: an argument carries a tangent")
+
+
 def _eager_only(device, what):
     with _on(device):
         capturing = torch.cuda.is_current_stream_capturing()
@@ -314,6 +326,7 @@ def dense(x, weight, bias=None, *, activation=None, residual=None, out_dtype=Non
             y = calls.dense(x, weight, bias, residual, preactivation, out_dtype, act)
             if y is not None:
                 return y
+    _plain_call("dense", x, weight, bias, residual)
     if _needs_grad(x, weight, bias, residual):
         if out is not None or preactivation is not None:
             raise ValueError("out= and preactivation= belong to the form without gradients: use torch.no_grad()")
@@ -336,6 +349,7 @@ def _dense_backward(dy, x, weight, z, act, need, outs, workspace):
             grads = calls.dense_backward(dy, x, weight, z, act, bool(need[0]), bool(need[1]), bool(need[2]))
             if grads is not None:
                 return grads
+    _plain_call("dense_backward", dy, x, weight, z)
     _tensor(x, "x")
     if x.dim() < 1 or not isinstance(weight, torch.Tensor) or weight.dim() != 2:
         raise ValueError("x must be (..., inputs) and weight (outputs, inputs)")
@@ -500,6 +514,7 @@ def group_norm(x, groups, weight=None, bias=None, *, eps=1e-5, activation=None, 
             y = calls.group_norm(x, weight, bias, lengths, stats, int(groups), act, eps)
             if y is not None:
                 return y
+    _plain_call("group_norm", x, weight, bias)
     if _needs_grad(x, weight, bias):
         if out is not None or stats is not None:
             raise ValueError("out= and stats= belong to the form without gradients: use torch.no_grad()")
@@ -516,6 +531,7 @@ def _group_norm_backward(dy, x, groups, stats, weight, bias, act, lengths, need,
                                               bool(need[2]))
             if grads is not None:
                 return grads
+    _plain_call("group_norm_backward", dy, x, stats, weight, bias)
     groups, B, T, C, lens = _norm_args(x, groups, weight, bias, lengths)
     device, dtype = x.device, x.dtype
     _tensor(dy, "dy", device, dtype, x.shape)

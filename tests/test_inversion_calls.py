@@ -3,6 +3,7 @@ import ctypes
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from tacotron2_amd import _lib
 from tacotron2_amd import inversion as inv
@@ -25,6 +26,52 @@ def test_a_result_past_the_memory_raises_torchs_own_error(way):
     with pytest.raises(torch.OutOfMemoryError):
         inv.dense(x, w)
     assert torch.equal(inv.dense(x[:2], w[:3]), torch.zeros(2, 3, device="cuda"))
+
+
+def arguments(device):
+    """(call, its tensors) of the four operators."""
+    x, w, b = (torch.randn(s, device=device) for s in ((3, 4), (6, 4), (6,)))
+    y, st, g = torch.randn(3, 6, device=device), torch.ones(1, 2, 2, device=device), torch.ones(4, device=device)
+    return [(lambda x, w, b, r: inv.dense(x, w, b, residual=r), [x, w, b, y]), (lambda x, w, b: inv.group_norm(x, 2, w, b), [x, g, g.clone()]),
+            (lambda dy, x, w, z: inv.dense_backward(dy, x, w, z, activation="silu"), [y, x, w, y.clone()]),
+            (lambda dy, x, st, w, b: inv.group_norm_backward(dy, x, 2, st, w, b), [x.clone(), x, st, g, g.clone()])]
+
+
+def refuses_tangents(device):
+    for call, tensors in arguments(device):
+        for k, t in enumerate(tensors):
+            with forward_ad.dual_level():
+                dual = forward_ad.make_dual(t, torch.ones_like(t))
+                with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                    call(*tensors[:k], dual, *tensors[k + 1:])
+                with torch.no_grad(), pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                    call(*tensors[:k], dual, *tensors[k + 1:])
+
+
+def refuses_traces(device):
+    for call, tensors in arguments(device):
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            torch.jit.trace(call, tuple(tensors), check_trace=False)
+
+
+def test_tangents_and_traces_are_refused_without_a_gpu(way):
+    refuses_tangents("cpu")
+    refuses_traces("cpu")
+
+
+@gpu
+def test_tangents_and_traces_are_refused(way):
+    refuses_tangents("cuda")
+    refuses_traces("cuda")
+    for call, tensors in arguments("cuda"):
+        with forward_ad.dual_level():                        # a level alone, without a tangent, changes nothing
+            inside = call(*tensors)
+        outside = call(*tensors)
+        for a, b in zip(inside if isinstance(inside, tuple) else (inside,), outside if isinstance(outside, tuple) else (outside,)):
+            assert torch.equal(a, b)
+    net = inv.MelInversion(n_mels=8, n_bins=9, channels=16, hidden=16, blocks=1, groups=4, device="cuda")
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        torch.jit.trace(net, torch.zeros(1, 5, 8, device="cuda"), check_trace=False)
 
 
 def test_pointers_off_their_elements_are_refused():
