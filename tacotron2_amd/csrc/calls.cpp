@@ -76,6 +76,11 @@ bool apart(const at::Tensor& out, std::initializer_list<const Arg*> args) {
     return true;
 }
 
+// What a call writes into a tensor of the caller's counts as a change of it: autograd then finds gradients that would be stale
+void written(const Arg& a) {
+    if (a && !a->is_inference()) a->unsafeGetTensorImpl()->bump_version();
+}
+
 at::Tensor scratch(long long bytes, const at::Tensor& like) {
     return bytes > 0 ? at::empty({bytes}, like.options().dtype(at::kByte)) : at::Tensor();
 }
@@ -165,7 +170,9 @@ PyObject* dense(PyObject*, PyObject* const* o, Py_ssize_t n) {
         rc = dense_call(x.p(), K, w.p(), K, b.p(), r.p(), N, y.data_ptr(), N, z.p(), N, rows, (int)K, (int)N, type_of(type), type_of(to),
                         (int)act, pointer(ws), bytes, stream);
         Py_END_ALLOW_THREADS
-        return rc ? nullptr : wrap(y);
+        if (rc) return nullptr;
+        written(z);
+        return wrap(y);
     });
 }
 
@@ -241,7 +248,9 @@ PyObject* group_norm(PyObject*, PyObject* const* o, Py_ssize_t n) {
         rc = group_norm_call(x.p(), f.C, w.p(), b.p(), (const int*)lens.p(), y.data_ptr(), f.C, (float*)stats.p(), (int)f.B, (int)f.T, (int)f.C,
                              (int)f.G, type_of(type), (int)v[1], (float)eps, pointer(ws), bytes, stream);
         Py_END_ALLOW_THREADS
-        return rc ? nullptr : wrap(y);
+        if (rc) return nullptr;
+        written(stats);
+        return wrap(y);
     });
 }
 

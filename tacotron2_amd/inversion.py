@@ -148,6 +148,13 @@ def _output(out, shape, dtype, device, what):
     return out, stride
 
 
+def _written(*tensors):
+    """Tells autograd that the caller's own tensors have changed: gradients that need what was in them are then refused."""
+    for t in tensors:
+        if t is not None and not t.is_inference():
+            torch.autograd.graph.increment_version(t)
+
+
 @functools.lru_cache(maxsize=4096)
 def _bytes_of(query, *args):
     """What a gl_*_workspace query says: a function of its arguments alone."""
@@ -285,6 +292,7 @@ def _dense(x, weight, bias, act, residual, out_dtype, out, preactivation, worksp
         _lib.check(_lib.lib().gl_dense(_p(x), x_stride, _p(weight), w_stride, _p(bias), _p(residual), r_stride, _p(y),
                                        y_stride, _p(z), z_stride, rows, K, N, d, od, act, _p(ws), ws_bytes,
                                        _stream(device)), "gl_dense")
+    _written(out, preactivation)
     return y
 
 
@@ -393,6 +401,7 @@ def _dense_backward(dy, x, weight, z, act, need, outs, workspace):
         _lib.check(_lib.lib().gl_dense_backward(_p(dy), dy_stride, _p(x), x_stride, _p(weight), w_stride, _p(z), z_stride,
                                                 _p(dx), dx_stride, _p(dw), dw_stride, _p(db), rows, K, N, d, od, act,
                                                 _p(ws), ws_bytes, _stream(device)), "gl_dense_backward")
+    _written(*outs)
     return dx, dw, db
 
 
@@ -473,6 +482,7 @@ def _group_norm(x, groups, weight, bias, eps, act, lengths, out, stats, workspac
         _lib.check(_lib.lib().gl_group_norm(_p(x), x_stride, _p(weight), _p(bias), _p(lens), _p(y), y_stride, _p(stats), B,
                                             T, C, groups, d, act, eps, _p(ws), ws_bytes, _stream(device)),
                    "gl_group_norm")
+    _written(out, stats)
     return y
 
 
@@ -563,6 +573,7 @@ def _group_norm_backward(dy, x, groups, stats, weight, bias, act, lengths, need,
         _lib.check(_lib.lib().gl_group_norm_backward(_p(dy), dy_stride, _p(x), x_stride, _p(stats), _p(weight), _p(bias),
                                                      _p(lens), _p(dx), dx_stride, _p(dg), _p(db), B, T, C, groups, d, act,
                                                      _p(ws), ws_bytes, _stream(device)), "gl_group_norm_backward")
+    _written(*outs)
     return dx, dg, db
 
 

@@ -74,6 +74,34 @@ def test_tangents_and_traces_are_refused(way):
         torch.jit.trace(net, torch.zeros(1, 5, 8, device="cuda"), check_trace=False)
 
 
+@gpu
+def test_gradients_that_need_an_overwritten_tensor_are_refused(way):
+    """What a call writes into the caller's tensor counts as a change of it."""
+    x, w, y = torch.randn(3, 4, device="cuda"), torch.randn(6, 4, device="cuda"), torch.randn(3, 6, device="cuda")
+    st, g, b = torch.ones(1, 2, 2, device="cuda"), torch.ones(4, device="cuda"), torch.zeros(6, device="cuda")
+    other = torch.randn(3, 6, device="cuda")
+    writes = [(lambda t: inv.dense(x, w, out=t), (3, 6)), (lambda t: inv.dense(x, w, preactivation=t, activation="silu"), (3, 6)),
+              (lambda t: inv.group_norm(x, 2, out=t), (3, 4)), (lambda t: inv.group_norm(x, 2, stats=t), (1, 2, 2)),
+              (lambda t: inv.dense_backward(y, x, w, dx=t), (3, 4)), (lambda t: inv.dense_backward(y, x, w, dweight=t), (6, 4)),
+              (lambda t: inv.dense_backward(y, x, w, dbias=t), (6,)), (lambda t: inv.group_norm_backward(x, x.clone(), 2, st, g, g, dx=t), (3, 4)),
+              (lambda t: inv.group_norm_backward(x, x.clone(), 2, st, g, g, dweight=t), (4,)),
+              (lambda t: inv.group_norm_backward(x, x.clone(), 2, st, g, g, dbias=t), (4,))]
+    for write, shape in writes:
+        leaf = torch.randn(shape, device="cuda", requires_grad=True)
+        square = leaf * leaf                                 # needs leaf's values
+        with torch.no_grad():
+            write(leaf.detach())
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            square.sum().backward()
+    with torch.inference_mode():                             # tensors without a count of changes
+        assert torch.equal(inv.dense(x, w, b, out=torch.empty(3, 6, device="cuda")), inv.dense(x, w, b))
+        assert torch.equal(inv.dense(x, w, b, preactivation=torch.empty_like(other), activation="relu"), inv.dense(x, w, b, activation="relu"))
+    z = torch.empty(3, 6, device="cuda")                     # and what a differentiable call keeps for itself is none
+    xg = x.clone().requires_grad_()
+    inv.group_norm(inv.dense(xg, w, b, activation="silu"), 2).sum().backward()
+    assert xg.grad is not None and z._version == 0
+
+
 def test_pointers_off_their_elements_are_refused():
     """Checked before anything runs: the pointers here are never followed.  Workspaces are large enough for all of them."""
     lib = _lib.lib()
