@@ -15,19 +15,20 @@ __device__ __forceinline__ float gl_to_f32(gl_f16 v) { return (float)v; }
 // FINE, here and below: for float32 results.  The rest is for 16-bit ones, next to whose half step (2^-12 and more) it errs little.
 
 // exp(z) = 2^(z log2 e).  The product's rounding moves the result by up to |z| 2^-24 of it; FINE takes what it lost along.
+// Subnormal results come out of a product that rounds them once: exp2 itself has none.
 template <bool FINE>
 __device__ __forceinline__ float gl_exp(float z) {
     constexpr float k = 1.44269504088896341f;
-    float t = z * k;
-    if constexpr (FINE) asm("" : "+v"(t));                   // the rounded product itself: never one operation with what is added below
-    const bool low = t < -120.0f;                            // subnormal results: 2^64 up, then down with one rounding
-    float e = __builtin_amdgcn_exp2f(t + (low ? 64.0f : 0.0f));
-    if constexpr (FINE) {
+    const float t = z * k;
+    const bool low = t < -120.0f;
+    if constexpr (!FINE) return __builtin_amdgcn_exp2f(t + (low ? 64.0f : 0.0f)) * (low ? 0x1p-64f : 1.0f);
+    else {
         constexpr float k_rest = (float)(1.44269504088896341 - (double)k);
         const float rest = fmaf(z, k_rest, fmaf(z, k, -t));
-        e = fabsf(t + 16.0f) < 144.0f ? fmaf(e, rest * 0.69314718055994531f, e) : e;        // not where e is infinite, or z
+        const float e = __builtin_amdgcn_exp2f(t * (low ? 0.5f : 1.0f));     // no sum with t: it would be one operation with z k
+        const float all = fabsf(t + 16.0f) < 144.0f ? fmaf(e, rest * 0.69314718055994531f, e) : e;  // not where e is infinite, or z
+        return all * (low ? e : 1.0f);
     }
-    return e * (low ? 0x1p-64f : 1.0f);
 }
 
 template <bool FINE>
