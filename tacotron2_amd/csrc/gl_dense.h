@@ -86,6 +86,9 @@ int gl_mm16(const gl_operand& P, const gl_operand& Q, gl_epilogue e, long long I
 template <typename T, typename TO>
 int gl_dense_join(const gl_epilogue& e, long long I, int J, int parts, hipStream_t st);
 
+// the same for float32 through planes; what those do not give is computed from the operands
+int gl_dense_join_planes(const gl_epilogue& e, long long I, int J, long long nq, const gl_mm_plan& p, hipStream_t st);
+
 // computes the 64 x 64 blocks that are flagged, on the float32 operands
 int gl_dense_flagged(const gl_epilogue& e, long long I, int J, long long nq, hipStream_t st);
 

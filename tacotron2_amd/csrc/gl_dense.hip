@@ -341,19 +341,96 @@ __global__ void __launch_bounds__(256) k_dense_join(Epilogue e, long long I, int
         const int j = (int)(at - i * J);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            float sum = s[v];
-            bool again = e.exact_p && !(fabsf(sum) < INFINITY);          // float32 through planes: once more from the operands
-            if (e.scale_p) {
-                const gl_scale p = {e.scale_p[i]}, q = {e.scale_q[j + v]};
-                again |= !gl_halves_give(ldexpf(sum, p.e() + q.e()), p, q, (float)e.exact_nq);
-            }
-            if (again) {
-                sum = 0.0f;
-                for (long long q = 0; q < e.exact_nq && sum == sum; ++q)
-                    sum = fmaf(e.exact_p[i * e.exact_p_is + q * e.exact_p_qs], e.exact_q[(j + v) * e.exact_q_is + q * e.exact_q_qs], sum);
-            }
-            gl_finish<T, TO>(e, i, j + v, sum);
+            gl_finish<T, TO>(e, i, j + v, s[v]);
         }
+    }
+}
+
+// The same for float32 through planes: a workgroup 16 rows of a 64 x 64 block, which are left as they were and flagged (a byte of
+// the block's flag) where the planes do not give one of their sums.  V divides J.
+constexpr int kJoinRows = 16;
+template <int V>
+__device__ __forceinline__ void join_rows(const Epilogue& e, long long i0, int j0, long long I, int J, int parts, unsigned char* flag) {
+    typedef typename vecn<float, V>::type vf;
+    constexpr int kAcross = kTile / V, kRows = 256 / kAcross, kEach = kJoinRows / kRows, kAtOnce = 12 / kEach;
+    const int j = j0 + (threadIdx.x % kAcross) * V;
+    const long long i1 = i0 + threadIdx.x / kAcross, n = I * J;
+    auto real = [&](int k) { return j < J && i1 + k * kRows < I; };
+    vf s[kEach];
+    const float* from[kEach];
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+        s[k] = vf{};
+        from[k] = e.partial + (real(k) ? (i1 + k * kRows) * J + j : 0);
+    }
+    for (int p = 0; p < parts; p += kAtOnce) {               // no branch around a load: one would have to wait for it
+        vf t[kAtOnce][kEach];
+#pragma unroll
+        for (int o = 0; o < kAtOnce; ++o)
+#pragma unroll
+            for (int k = 0; k < kEach; ++k) t[o][k] = *(const vf*)(from[k] + min(p + o, parts - 1) * n);
+#pragma unroll
+        for (int o = 0; o < kAtOnce; ++o)
+#pragma unroll
+            for (int k = 0; k < kEach; ++k) s[k] += p + o < parts ? t[o][k] : vf{};
+    }
+    if (flag) {
+        bool bad = false;
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+            if (!real(k)) continue;
+            const long long i = i1 + k * kRows;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                bad |= !(fabsf(s[k][v]) < INFINITY);
+                if (e.scale_p) {
+                    const gl_scale p = {e.scale_p[i]}, q = {e.scale_q[j + v]};
+                    bad |= !gl_halves_give(ldexpf(s[k][v], p.e() + q.e()), p, q, (float)e.exact_nq);
+                }
+            }
+        }
+        bad = __syncthreads_or(bad);
+        if (threadIdx.x == 0) *flag = bad;
+        if (bad) return;
+    }
+#pragma unroll
+    for (int k = 0; k < kEach; ++k)
+        if (real(k))
+#pragma unroll
+            for (int v = 0; v < V; ++v) gl_finish<float, float>(e, i1 + k * kRows, j + v, s[k][v]);
+}
+// grid (blocks, their runs of 16 rows)
+template <int V>
+__global__ void __launch_bounds__(256) k_dense_join_rows(Epilogue e, long long I, int J, int parts, int tiles_j) {
+    const int tile = blockIdx.x, run = blockIdx.y;
+    if (run == 0 && threadIdx.x == 0) e.flags[gridDim.x + tile] = 0;         // the count of k_dense_repair
+    join_rows<V>(e, (long long)(tile / tiles_j) * kTile + run * kJoinRows, tile % tiles_j * kTile, I, J, parts,
+                 (unsigned char*)(e.flags + tile) + run);
+}
+
+// And the flagged rows from the operands themselves, a block in as many parts, each a workgroup's: the one that ends last joins
+// them, in their order.  grid (workgroups, parts).  Nobody waits.
+template <int V>
+__global__ void __launch_bounds__(256) k_dense_repair(AnyArgs a, Epilogue e, int parts) {
+    __shared__ int last;
+    int set = 0;                                             // all of this workgroup's at once: there is hardly ever one
+    for (long long tile = blockIdx.x + (long long)threadIdx.x * gridDim.x; tile < a.n_tiles; tile += 256LL * gridDim.x) set |= e.flags[tile];
+    if (!__syncthreads_or(set)) return;
+    for (long long tile = blockIdx.x; tile < a.n_tiles; tile += gridDim.x) {
+        const unsigned flags = e.flags[tile];
+        if (!flags) continue;                                // uniform over the workgroup
+        any_tiles<float, float, float, 1, false, false>(a, tile, a.n_tiles, blockIdx.y, nullptr);
+        __threadfence();
+        __syncthreads();
+        if (threadIdx.x == 0) last = atomicAdd(e.flags + a.n_tiles + tile, 1) == parts - 1;
+        __syncthreads();
+        const bool mine = last;
+        __syncthreads();
+        if (!mine) continue;
+        __threadfence();
+        for (int run = 0; run < kTile / kJoinRows; ++run)
+            if (flags >> (8 * run) & 0xff)
+                join_rows<V>(e, tile / a.tiles_j * kTile + run * kJoinRows, (int)(tile % a.tiles_j) * kTile, a.I, a.J, parts, nullptr);
     }
 }
 
@@ -697,7 +774,8 @@ long long copy_bytes(int dtype, long long rows, int cols) {
     return gl_align16(rows * pad_to(cols) * (dtype == GL_F32 ? 6LL : 2LL));
 }
 long long halves_bytes(long long rows, int cols) { return gl_align16(rows * pad_to(cols) * 4LL); }
-long long flag_bytes(int dtype, long long I, int J) { return dtype == GL_F32 ? gl_align16(gl_ceil_div(I, 64) * gl_ceil_div(J, 64) * 4) : 0; }
+// a flag and a count for every 64 x 64 block
+long long flag_bytes(int dtype, long long I, int J) { return dtype == GL_F32 ? gl_align16(gl_ceil_div(I, 64) * gl_ceil_div(J, 64) * 8) : 0; }
 // flags and parts of a product, whichever kernel takes it
 long long partial_bytes(int dtype, long long I, int J, long long nq, bool any_q, bool fast) {
     const long long any = any_bytes(I, J, nq);
@@ -1066,6 +1144,23 @@ template int gl_dense_join<gl_bf16, gl_bf16>(const gl_epilogue&, long long, int,
 template int gl_dense_join<gl_bf16, float>(const gl_epilogue&, long long, int, int, hipStream_t);
 template int gl_dense_join<gl_f16, gl_f16>(const gl_epilogue&, long long, int, int, hipStream_t);
 template int gl_dense_join<gl_f16, float>(const gl_epilogue&, long long, int, int, hipStream_t);
+
+int gl_dense_join_planes(const gl_epilogue& e, long long I, int J, long long nq, const gl_mm_plan& p, hipStream_t st) {
+    const long long tiles = gl_ceil_div(I, kTile) * gl_ceil_div(J, kTile);
+    const int tiles_j = (int)gl_ceil_div(J, kTile);
+    const bool wide = J % 4 == 0;
+    hipLaunchKernelGGL((wide ? k_dense_join_rows<4> : k_dense_join_rows<1>), dim3((unsigned)tiles, kTile / kJoinRows), dim3(256), 0, st, e, I, J,
+                       p.parts, tiles_j);
+    GL_HIP_CHECK(hipGetLastError());
+    gl_epilogue f = {};
+    f.partial = e.partial;
+    const AnyArgs a = {{e.exact_p, e.exact_p_is, e.exact_p_qs}, {e.exact_q, e.exact_q_is, e.exact_q_qs}, {}, f, I, nq, p.per, J, tiles_j,
+                       (int)tiles, GL_ACT_NONE, e.exact_p_qs == 1, e.exact_q_qs == 1, nullptr, nullptr};
+    hipLaunchKernelGGL((wide ? k_dense_repair<4> : k_dense_repair<1>), dim3((unsigned)(tiles < 512 ? tiles : 512), p.parts), dim3(256), 0, st, a, e,
+                       p.parts);
+    GL_HIP_CHECK(hipGetLastError());
+    return 0;
+}
 
 int gl_dense_flagged(const gl_epilogue& e, long long I, int J, long long nq, hipStream_t st) {
     const long long tiles = gl_ceil_div(I, kTile) * gl_ceil_div(J, kTile);

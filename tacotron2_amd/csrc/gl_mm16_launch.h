@@ -76,7 +76,8 @@ int one(const gl_operand& P, const gl_operand& Q, const gl_epilogue& e, long lon
         if (rc) return rc;
         gl_epilogue j = e;
         j.partial = partial;
-        return gl_dense_join<TB, TO>(j, I, J, p.parts, st);
+        if constexpr (SEG > 2) return gl_dense_join_planes(j, I, J, nq, p, st);
+        else return gl_dense_join<TB, TO>(j, I, J, p.parts, st);
     }
     auto off4 = [](const void* q, long long stride) { return q && (stride % 2 || (uintptr_t)q % 4); };
     const int odd = sizeof(TO) == 2 && (off4(e.y, e.y_stride) || off4(e.z, e.z_stride) || off4(e.residual, e.r_stride));
