@@ -596,7 +596,9 @@ class MelInversion(torch.nn.Module):
 
     Parameters are of `dtype`; log-mels of another type are cast to it.  lengths (ragged batch): frames past an
     utterance's end do not reach the norms of the others; their magnitudes are for the caller to ignore
-    (``logmel_to_audio`` zeroes them).  A freshly made network starts at magnitudes around exp(out_bias)."""
+    (``logmel_to_audio`` zeroes them).  float16: the gradients between layers are float16 too and vanish below 6e-8, so scale the
+    loss (a mean over a batch's magnitudes by some 2**14) and divide the parameters' gradients; float32 and bfloat16 need none.
+    A freshly made network starts at magnitudes around exp(out_bias)."""
 
     def __init__(self, n_mels=80, n_bins=1025, channels=512, hidden=None, blocks=2, groups=32, dtype=torch.float32,
                  device=None, seed=0, out_bias=-3.0):
