@@ -591,8 +591,8 @@ __global__ void __launch_bounds__(256) k_dense_halves(Halves a, Halves b, int co
 }
 
 // dz = dy act'(z), as the products read it (splits_dz() says which): rounded to T, in two planes of T, or, float32, in three of
-// bfloat16 beside `exact`; zeros up to dz_stride columns, and column sums of the unrounded dz over this workgroup's frames.  grid (blocks of 64 V columns, parts of the frames); thread =
-// (V columns, one of 4 frame lanes).  dz is a pass of its own, since both products read it and one of them transposed; it is
+// bfloat16 beside `exact`; zeros up to dz_stride columns, and column sums of the unrounded dz over this workgroup's frames.
+// grid (blocks of 64 V columns, parts of the frames); thread = (V columns, one of 4 frame lanes).  dz is a pass of its own, since both products read it and one of them transposed; it is
 // bound by memory: 55 104 x 2048 bf16 gelu 129 us (677 MB, 5.2 TB/s).
 template <typename T, typename TO, int V, int PLANES>
 __global__ void __launch_bounds__(256) k_dense_dz(const TO* __restrict__ dy, long long dy_stride, const TO* __restrict__ z,
@@ -768,7 +768,7 @@ double small_layer(int dtype, int inputs, int outputs, bool back) {
 bool is_small(long long rows, int inputs, int outputs, int dtype, bool back) {
     return (double)rows * inputs * outputs < small_layer(dtype, inputs, outputs, back);
 }
-int pad_to(int n) { return (n + 63) / 64 * 64; }
+int pad_to(int n) { return (n + kPadded - 1) / kPadded * kPadded; }
 bool copies(int dtype, int width) { return dtype == GL_F32 || width % 8 != 0; }
 long long copy_bytes(int dtype, long long rows, int cols) {
     return gl_align16(rows * pad_to(cols) * (dtype == GL_F32 ? 6LL : 2LL));

@@ -17,7 +17,8 @@
 //   2: P in two planes of Q's own type (gl_split): low x Q first, times kSplitStep, then high x Q.
 // float32 operands: a block with a sum that the planes do not give is not written but flagged, and the float32 kernel computes it.
 //   3: two planes of f16 per row (gl_scale), where a row of either side is one of the contraction: h l, l h, then, with the
-//      sums times 2^-12, h h.  Left out is l l 2^-24 <= 2^-24 |x| |y|: with both sides' rounding three roundings a product.
+//      sums times 2^-12, h h.  Left out is l l 2^-24 <= 2^-22 |x| |y| (h rounds at 2^-11 of a value), and either side is off by up
+//      to 2^-23 of itself: 2^-21 |x| |y| in all at most, for a product whose both factors are the worst there are.
 //   6: three planes of bfloat16, x = h + m + l with h = bf16(x), m = bf16(x - h), l = bf16(x - h - m), which need no scale (an
 //      operand across the contraction has one per column): hh, hm, mh, mm, hl, lh; what is left out (ml, lm, ll) is below 2^-24
 //      of |x| |y|.  Sums that are not finite are flagged: an infinity times a zero plane would be NaN.

@@ -1,11 +1,12 @@
-// Launches of the 16-bit products (gl_mm16.h), instantiated once per element type (gl_dense_bf16.hip, gl_dense_f16.hip).
+// Launches of the 16-bit products (gl_mm16.h), instantiated once per element type (gl_dense_bf16.hip, gl_dense_f16.hip,
+// gl_dense_f32.hip: its planes).
 #pragma once
 #include "gl_dense.h"
 #include "gl_mm16.h"
 
 namespace gl_mm {
 
-// rows: of C on this side.  A padded operand contiguous in the contraction has nq rounded up to 32 of it, one contiguous
+// rows: of C on this side.  A padded operand contiguous in the contraction has nq rounded up to kPadded of it, one contiguous
 // across it may be read in whole chunks of 8.
 static inline Side side(const gl_operand& o, long long rows, long long nq, long long nq_padded) {
     const bool across = o.across();
@@ -14,7 +15,7 @@ static inline Side side(const gl_operand& o, long long rows, long long nq, long 
 }
 
 static inline long long padded_q(const gl_operand& P, long long nq) {
-    return P.padded && !P.across() ? (nq + 63) / 64 * 64 : nq;
+    return P.padded && !P.across() ? (nq + kPadded - 1) / kPadded * kPadded : nq;
 }
 
 template <typename T, typename TO, typename TB, int SEG, int ACT, bool EXTRA, bool LINES, int BM, bool PT, bool QT>

@@ -948,7 +948,7 @@ Cut cut_for(int B, int T, int C, int groups, int size, int V, int most, int row_
     int k = 1;
     while (k < groups && (n * k) % V) ++k;                   // whole groups on whole vectors
     if (n * k % V == 0 && threads_for(n * k / V, T, most) && lds_bytes(kMaxThreads, V, n * k, n, 2) <= kMaxLds) {
-        // more groups to a block, to 128 bytes a row, while the slab fits and the blocks fill the chip
+        // more groups to a block, to row_bytes a row, while the slab fits and the blocks fill the chip
         for (int m = 2 * k; m <= groups && (long long)n * k * size < row_bytes; m += k)
             if (groups % m == 0 && threads_for(n * m / V, T, most) && (long long)B * (groups / m) >= 256) k = m;
         c.kind = 0;

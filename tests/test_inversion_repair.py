@@ -61,3 +61,18 @@ def test_blocks_below_their_rows_range_in_parts(M, K, N):
     close(y[:M - 1], y64.cpu(), y_tol.cpu(), "y")
     for _ in range(3):
         assert torch.equal(y, inv.dense(x, w, activation="tanh", residual=keep))
+
+
+@gpu
+def test_planes_hold_float32_to_a_step():
+    """Values over all of a binade times one: 2^-23 of the planes, and 2^-23 of the sum, which a matrix instruction may cut off instead of
+    rounding it.  Times each other: 2^-23 of either side's planes, twice 2^-23 for the product of the lower planes that is left out
+    (2^-11 of a value each), 2^-23 of the sum: 5 of them (computed with exact planes and a cut-off sum on the CPU: 4.98)."""
+    M, N = 2048, 1024
+    steps = torch.arange(M * N, dtype=torch.float64).view(M, N) * 4 + 1
+    x = ((1 + steps * 2.0 ** -23) * 2.0 ** (torch.arange(M) % 31 - 15)[:, None]).float()
+    y = inv.dense(x.cuda(), torch.eye(N, device="cuda")).cpu()
+    assert ((y.double() - x.double()).abs() <= 2 * 2.0 ** -23 * x.double()).all()
+    both = (x.double() * x[0].double()[None, :])                                         # both factors rounded
+    y = inv.dense(x.cuda(), torch.diag(x[0]).cuda()).cpu()
+    assert ((y.double() - both).abs() <= 5 * 2.0 ** -23 * both).all()
