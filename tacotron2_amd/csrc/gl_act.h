@@ -6,28 +6,28 @@ typedef _Float16 gl_f16;
 typedef __bf16 gl_bf16;
 
 template <int N> struct gl_int { static constexpr int value = N; };
-template <typename T> constexpr bool gl_fine = __is_same(T, float);
 
 __device__ __forceinline__ float gl_to_f32(float v) { return v; }
 __device__ __forceinline__ float gl_to_f32(gl_bf16 v) { return (float)v; }
 __device__ __forceinline__ float gl_to_f32(gl_f16 v) { return (float)v; }
 
-// FINE, here and below: for float32 results.  The rest is for 16-bit ones, next to whose half step (2^-12 and more) it errs little.
+// R, here and below: the type of the results.  What is FINE is for float32; the rest is for 16-bit ones, next to whose half step
+// (2^-12, 2^-9) it errs little.
+template <typename R> constexpr bool gl_fine = __is_same(R, float);
 
-// exp(z) = 2^(z log2 e).  The product's rounding moves the result by up to |z| 2^-24 of it; FINE takes what it lost along.
-// Subnormal results come out of a product that rounds them once: exp2 itself has none.
+// exp(z) = 2^(z log2 e).  The product's rounding moves the result by up to |z| 2^-24 of it.  FINE: 2^n 2^f with a whole n, where f
+// takes along what the product and float32's log2 e lose; n stays within the range in which f alone makes infinity or zero.
 template <bool FINE>
 __device__ __forceinline__ float gl_exp(float z) {
     constexpr float k = 1.44269504088896341f;
-    const float t = z * k;
-    const bool low = t < -120.0f;
-    if constexpr (!FINE) return __builtin_amdgcn_exp2f(t + (low ? 64.0f : 0.0f)) * (low ? 0x1p-64f : 1.0f);
-    else {
+    if constexpr (FINE) {
         constexpr float k_rest = (float)(1.44269504088896341 - (double)k);
-        const float rest = fmaf(z, k_rest, fmaf(z, k, -t));
-        const float e = __builtin_amdgcn_exp2f(t * (low ? 0.5f : 1.0f));     // no sum with t: it would be one operation with z k
-        const float all = fabsf(t + 16.0f) < 144.0f ? fmaf(e, rest * 0.69314718055994531f, e) : e;  // not where e is infinite, or z
-        return all * (low ? e : 1.0f);
+        const float n = __builtin_amdgcn_fmed3f(__builtin_rintf(z * k), -200.0f, 200.0f);
+        return __builtin_amdgcn_ldexpf(__builtin_amdgcn_exp2f(fmaf(z, k_rest, fmaf(z, k, -n))), (int)n);
+    } else {
+        const float t = z * k;
+        const bool low = t < -120.0f;                        // subnormal results: 2^64 up, then down with one rounding
+        return __builtin_amdgcn_exp2f(t + (low ? 64.0f : 0.0f)) * (low ? 0x1p-64f : 1.0f);
     }
 }
 
@@ -39,17 +39,27 @@ __device__ __forceinline__ float gl_sigmoid(float z) {
 
 // Phi(-a) / exp(-a^2 / 2) for a >= 0, in the form of Hastings' approximations: t P(t), t = 1 / (1 + c a).  c and P are fitted by
 // weighted least squares (Lawson's weights) for the smallest relative error over a <= 14.6, where the result leaves float32's
-// range: 2^-24.9.  Eight terms would leave 2^-22.5, five 2^-14.9, which shows in float16.
+// range: 2^-24.9 with nine terms; 2^-14.9 with five, for bfloat16 (55 104 x 512 -> 2048: four terms more are 8 us of 155).
+template <int TERMS>
 __device__ __forceinline__ float gl_phi_ratio(float a) {
-    const float t = __builtin_amdgcn_rcpf(fmaf(a, 0.35f, 1.0f));
-    float p = fmaf(t, -2.915946483e-02f, 1.440387674e-01f);
-    p = fmaf(p, t, -2.558555896e-01f);
-    p = fmaf(p, t, 1.593390985e-01f);
-    p = fmaf(p, t, -2.322604228e-02f);
-    p = fmaf(p, t, 1.055584544e-01f);
-    p = fmaf(p, t, 1.198197353e-01f);
-    p = fmaf(p, t, 1.398637337e-01f);
-    p = fmaf(p, t, 1.396212914e-01f);
+    static_assert(TERMS == 9 || TERMS == 5);
+    const float t = __builtin_amdgcn_rcpf(fmaf(a, TERMS == 9 ? 0.35f : 0.375f, 1.0f));
+    float p;
+    if constexpr (TERMS == 9) {
+        p = fmaf(t, -2.915946483e-02f, 1.440387674e-01f);
+        p = fmaf(p, t, -2.558555896e-01f);
+        p = fmaf(p, t, 1.593390985e-01f);
+        p = fmaf(p, t, -2.322604228e-02f);
+        p = fmaf(p, t, 1.055584544e-01f);
+        p = fmaf(p, t, 1.198197353e-01f);
+        p = fmaf(p, t, 1.398637337e-01f);
+        p = fmaf(p, t, 1.396212914e-01f);
+    } else {
+        p = fmaf(t, -9.025423899e-02f, 1.994171632e-01f);
+        p = fmaf(p, t, 8.423240805e-02f);
+        p = fmaf(p, t, 1.575242494e-01f);
+        p = fmaf(p, t, 1.490832449e-01f);
+    }
     return t * p;
 }
 // exp(-a^2 / 2).  FINE: with what a^2 and its product with log2(e) / 2 lose; a is cut off where the result has long been zero.
@@ -69,13 +79,14 @@ __device__ __forceinline__ float gl_gauss(float a) {
 
 // act(z).  Every branch on `act` is uniform: a kernel argument or a template constant.  For many values at once take
 // gl_with_act around the loop: a branch a value scatters the code that runs over all activations of all values.
-template <bool FINE>
+template <typename R>
 __device__ __forceinline__ float gl_act(float z, int act) {
+    constexpr bool FINE = gl_fine<R>;
     switch (act) {
         case GL_ACT_RELU: return z < 0.0f ? 0.0f : z;                  // NaN stays NaN
         case GL_ACT_SILU: return z * gl_sigmoid<FINE>(z);
         case GL_ACT_GELU: {                                            // z Phi(z), Phi(z) = 1 - Phi(-z): no tail is a difference
-            const float h = gl_phi_ratio(fabsf(z)) * gl_gauss<FINE>(fabsf(z));
+            const float h = gl_phi_ratio<__is_same(R, gl_bf16) ? 5 : 9>(fabsf(z)) * gl_gauss<FINE>(fabsf(z));
             return z * (z > 0.0f ? 1.0f - h : h);
         }
         case GL_ACT_TANH: {
@@ -100,9 +111,10 @@ __device__ __forceinline__ float gl_act(float z, int act) {
     }
 }
 
-// act'(z).  FINE: of float32 gradients
-template <bool FINE>
+// act'(z).  R: the type of dy.  Phi has all its terms here: unrounded sums of gradients are made of it.
+template <typename R>
 __device__ __forceinline__ float gl_act_grad(float z, int act) {
+    constexpr bool FINE = gl_fine<R>;
     switch (act) {
         case GL_ACT_RELU: return z > 0.0f ? 1.0f : (z != z ? z : 0.0f);
         case GL_ACT_SILU: {
@@ -114,7 +126,7 @@ __device__ __forceinline__ float gl_act_grad(float z, int act) {
             return fmaf(z * s, 1.0f - s, s);
         }
         case GL_ACT_GELU: {                                            // Phi(z) + z phi(z)
-            const float a = fabsf(z), e = gl_gauss<FINE>(a), h = gl_phi_ratio(a) * e;
+            const float a = fabsf(z), e = gl_gauss<FINE>(a), h = gl_phi_ratio<9>(a) * e;
             return fmaf(z * e, 0.39894228040143268f, z < 0.0f ? h : 1.0f - h);
         }
         case GL_ACT_TANH: {                                            // 4 e / (1 + e)^2 with e = exp(-2 |z|)

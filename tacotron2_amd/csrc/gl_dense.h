@@ -100,7 +100,7 @@ __device__ __forceinline__ void gl_finish(const gl_epilogue& e, long long i, int
     float z = sum;
     if (e.bias) z += gl_to_f32(((const T*)e.bias)[j]);
     if (e.z) ((TO*)e.z)[i * e.z_stride + j] = (TO)z;
-    float y = gl_act<gl_fine<TO>>(z, e.act);
+    float y = gl_act<TO>(z, e.act);
     if (e.residual) y += gl_to_f32(((const TO*)e.residual)[i * e.r_stride + j]);
     ((TO*)e.y)[i * e.y_stride + j] = (TO)y;
 }

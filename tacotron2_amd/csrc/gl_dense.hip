@@ -139,7 +139,7 @@ __device__ __forceinline__ void any_tiles(const AnyArgs& a, long long first, lon
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
                         d[k] = gl_to_f32(t.p[k]);
-                        if constexpr (decltype(act)::value != GL_ACT_NONE) d[k] *= gl_act_grad<gl_fine<TD>>(gl_to_f32(t.z[k]), decltype(act)::value);
+                        if constexpr (decltype(act)::value != GL_ACT_NONE) d[k] *= gl_act_grad<TD>(gl_to_f32(t.z[k]), decltype(act)::value);
                     }
                 });
 #pragma unroll
@@ -250,7 +250,7 @@ __device__ __forceinline__ void any_tiles(const AnyArgs& a, long long first, lon
         if (e.z) quads([&](int j, int n, int r) { put((TY*)e.z + i * e.z_stride + j, n, r); });
         gl_with_act(e.act, [&](auto act) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) acc[r] = gl_act<gl_fine<TY>>(acc[r], decltype(act)::value);
+            for (int r = 0; r < 16; ++r) acc[r] = gl_act<TY>(acc[r], decltype(act)::value);
         });
         if (e.residual)
             quads([&](int j, int n, int r) {
@@ -622,7 +622,7 @@ __global__ void __launch_bounds__(256) k_dense_dz(const TO* __restrict__ dy, lon
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
                     d[v] = gl_to_f32(g[v]);
-                    if constexpr (ACT != GL_ACT_NONE) d[v] *= gl_act_grad<gl_fine<TO>>(gl_to_f32(zz[v]), ACT);
+                    if constexpr (ACT != GL_ACT_NONE) d[v] *= gl_act_grad<TO>(gl_to_f32(zz[v]), ACT);
                     sum[v] += d[v];
                 }
             }

@@ -378,7 +378,7 @@ __device__ __forceinline__ int epilogue(const Out& o, f32x4 (&acc)[MI][NI], long
 #pragma unroll
             for (int n = 0; n < NI; ++n) {
 #pragma unroll
-                for (int r = 0; r < 4; ++r) acc[m][n][r] = gl_act<gl_fine<TO>>(acc[m][n][r], decltype(act)::value);
+                for (int r = 0; r < 4; ++r) acc[m][n][r] = gl_act<TO>(acc[m][n][r], decltype(act)::value);
                 if (n & 1) __builtin_amdgcn_sched_barrier(0);    // keeps the block's temporaries few
             }
     };

@@ -315,7 +315,7 @@ __global__ void __launch_bounds__(kMaxThreads) k_norm_slab(const T* x, long long
             vT o = vT{};
             if (t < live)
 #pragma unroll
-                for (int k = 0; k < V; ++k) set<T, V>(o, k, gl_act<gl_fine<T>>(fmaf(get<T, V>(held[i], k) - mean[k], ga[k], be[k]), decltype(a)::value));
+                for (int k = 0; k < V; ++k) set<T, V>(o, k, gl_act<T>(fmaf(get<T, V>(held[i], k) - mean[k], ga[k], be[k]), decltype(a)::value));
             *(vT*)(yb + (long long)t * y_stride) = o;
         }
     });
@@ -456,7 +456,7 @@ __global__ void __launch_bounds__(kMaxThreads) k_norm_apply(const T* x, long lon
             if (t < live) {
                 const vT in = *(const vT*)(xb + (long long)t * x_stride);
 #pragma unroll
-                for (int k = 0; k < V; ++k) set<T, V>(o, k, gl_act<gl_fine<T>>(fmaf(get<T, V>(in, k) - mean[k], ga[k], be[k]), decltype(a)::value));
+                for (int k = 0; k < V; ++k) set<T, V>(o, k, gl_act<T>(fmaf(get<T, V>(in, k) - mean[k], ga[k], be[k]), decltype(a)::value));
             }
             *(vT*)(yb + (long long)t * y_stride) = o;
         }
@@ -470,7 +470,7 @@ template <typename T, int V, int ACT>
 __device__ __forceinline__ void du_d(const typename vec_of<T, V>::type& x, const typename vec_of<T, V>::type& dy, int k, float mean,
                                      float slope, float be, float& du, float& d) {
     d = get<T, V>(x, k) - mean;
-    du = get<T, V>(dy, k) * gl_act_grad<gl_fine<T>>(fmaf(d, slope, be), ACT);
+    du = get<T, V>(dy, k) * gl_act_grad<T>(fmaf(d, slope, be), ACT);
 }
 // dx = rstd (du gamma - p - xh q) = du slope + d cq + cp
 struct Back {
@@ -805,7 +805,7 @@ __global__ void __launch_bounds__(256) k_norm_plain_apply(const T* x, long long 
         if (t < live) {
             const float* st = stats + 2 * ((long long)b * G + c / n);
             const float xh = (gl_to_f32(x[row * x_stride + c]) - st[0]) * st[1];
-            v = gl_act<gl_fine<T>>(xh * (gamma ? gl_to_f32(gamma[c]) : 1.0f) + (beta ? gl_to_f32(beta[c]) : 0.0f), act);
+            v = gl_act<T>(xh * (gamma ? gl_to_f32(gamma[c]) : 1.0f) + (beta ? gl_to_f32(beta[c]) : 0.0f), act);
         }
         y[row * y_stride + c] = (T)v;
     }
@@ -830,7 +830,7 @@ __global__ void __launch_bounds__(256) k_norm_plain_back_chunk(const T* __restri
 #pragma unroll 4
     for (int t = 0; t < here; ++t) {
         const float d = gl_to_f32(xb[t * x_stride]) - mean;
-        const float du = gl_to_f32(db[t * dy_stride]) * gl_act_grad<gl_fine<T>>(fmaf(d, slope, be), act);
+        const float du = gl_to_f32(db[t * dy_stride]) * gl_act_grad<T>(fmaf(d, slope, be), act);
         a0 = fmaf(du, d, a0);
         a1 += du;
     }
@@ -881,7 +881,7 @@ __global__ void __launch_bounds__(256) k_norm_plain_back_apply(const T* dy, long
             const float* o = pq + 2 * ((long long)b * G + c / n);
             const float ga = gamma ? gl_to_f32(gamma[c]) : 1.0f, be = beta ? gl_to_f32(beta[c]) : 0.0f;
             const float xh = (gl_to_f32(x[row * x_stride + c]) - st[0]) * st[1];
-            const float du = gl_to_f32(dy[row * dy_stride + c]) * gl_act_grad<gl_fine<T>>(xh * ga + be, act);
+            const float du = gl_to_f32(dy[row * dy_stride + c]) * gl_act_grad<T>(xh * ga + be, act);
             v = st[1] * (du * ga - o[0] - xh * o[1]);
         }
         dx[row * dx_stride + c] = (T)v;
