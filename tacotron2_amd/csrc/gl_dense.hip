@@ -347,7 +347,8 @@ __global__ void __launch_bounds__(256) k_dense_join(Epilogue e, long long I, int
 }
 
 // The same for float32 through planes: a workgroup 16 rows of a 64 x 64 block, which are left as they were and flagged (a byte of
-// the block's flag) where the planes do not give one of their sums.  V divides J.
+// the block's flag) where the planes do not give one of their sums.  V divides J.  Bound by memory and, with few blocks, by how many
+// loads run at once: 264 x 512 in 42 parts 8 us (a workgroup a whole block: 15), 512 x 512 in 24 parts 6.
 constexpr int kJoinRows = 16;
 template <int V>
 __device__ __forceinline__ void join_rows(const Epilogue& e, long long i0, int j0, long long I, int J, int parts, unsigned char* flag) {
@@ -409,7 +410,8 @@ __global__ void __launch_bounds__(256) k_dense_join_rows(Epilogue e, long long I
 }
 
 // And the flagged rows from the operands themselves, a block in as many parts, each a workgroup's: the one that ends last joins
-// them, in their order.  grid (workgroups, parts).  Nobody waits.
+// them, in their order.  grid (workgroups, parts).  Nobody waits.  4.6 us where no flag is set; dweight of 40 000 x 512 -> 264 with
+// one infinite gradient 0.23 ms (a loop over the frames in one thread for every sum: 50 ms).
 template <int V>
 __global__ void __launch_bounds__(256) k_dense_repair(AnyArgs a, Epilogue e, int parts) {
     __shared__ int last;
@@ -592,8 +594,9 @@ __global__ void __launch_bounds__(256) k_dense_halves(Halves a, Halves b, int co
 
 // dz = dy act'(z), as the products read it (splits_dz() says which): rounded to T, in two planes of T, or, float32, in three of
 // bfloat16 beside `exact`; zeros up to dz_stride columns, and column sums of the unrounded dz over this workgroup's frames.
-// grid (blocks of 64 V columns, parts of the frames); thread = (V columns, one of 4 frame lanes).  dz is a pass of its own, since both products read it and one of them transposed; it is
-// bound by memory: 55 104 x 2048 bf16 gelu 129 us (677 MB, 5.2 TB/s).
+// grid (blocks of 64 V columns, parts of the frames); thread = (V columns, one of 4 frame lanes).  dz is a pass of its own, since
+// both products read it and one of them transposed; it is bound by memory: 55 104 x 2048 gelu bf16 129 us (677 MB, 5.2 TB/s), two
+// planes from float32 254 us (1.35 GB, 5.3 TB/s), from f16 164.
 template <typename T, typename TO, int V, int PLANES>
 __global__ void __launch_bounds__(256) k_dense_dz(const TO* __restrict__ dy, long long dy_stride, const TO* __restrict__ z,
                                                   long long z_stride, void* __restrict__ dz_, long long dz_stride, long long plane,
@@ -968,11 +971,11 @@ SmallSplit small_split(long long I, int J, long long nq) {
 // Whether 16-bit products take dz in two planes.  bfloat16 with a dy of its own type: once rounded (half a step a term, what dy
 // itself has lost already: the gradients' error against 64 bits is 0.0023 of them where their own rounding makes 0.0017, and
 // 55 104 x 512 -> 2048 gelu takes 374 us where two planes take 614).  A caller who keeps dy and z in float32 keeps dz to 2^-18
-// of it (676 us, rounded once 463).  float16: dz falls below the type's
-// range where dy does not (a mean over a batch's magnitudes has gradients of 2e-8, and act' makes them smaller), and sums over
-// frames bring it back: two planes reach 2^-48.  dy itself serves without an activation, where it is of the products' type.
+// of it (676 us, rounded once 463).  float16: dz falls below the type's range where dy does not (a mean over a batch's magnitudes
+// has gradients of 2e-8, and act' makes them smaller), and sums over frames bring it back: two planes reach 2^-48 (633 us, rounded
+// once 380).  Without an activation and with relu dz is dy or zero: it serves as it is where dy is of the products' type.
 bool splits_dz(int dtype, int out_dtype, int act) {
-    return dtype != GL_F32 && (out_dtype == GL_F32 || (dtype == GL_F16 && act != GL_ACT_NONE));
+    return dtype != GL_F32 && (out_dtype == GL_F32 || (dtype == GL_F16 && act > GL_ACT_RELU));
 }
 
 // workspace of a small layer: [parts of dx] [parts of dweight] [parts of dbias]; else
