@@ -39,11 +39,11 @@ __device__ __forceinline__ float gl_sigmoid(float z) {
 
 // Phi(-a) / exp(-a^2 / 2) for a >= 0, in the form of Hastings' approximations: t P(t), t = 1 / (1 + c a).  c and P are fitted by
 // weighted least squares (Lawson's weights) for the smallest relative error over a <= 14.6, where the result leaves float32's
-// range: 2^-24.9 with nine terms; 2^-14.9 with five, for bfloat16 (55 104 x 512 -> 2048: four terms more are 8 us of 155).
+// range: 2^-24.9 with nine terms; 2^-20.6 with seven, for bfloat16 (55 104 x 512 -> 2048: two terms are 4 us of 155).
 template <int TERMS>
 __device__ __forceinline__ float gl_phi_ratio(float a) {
-    static_assert(TERMS == 9 || TERMS == 5);
-    const float t = __builtin_amdgcn_rcpf(fmaf(a, TERMS == 9 ? 0.35f : 0.375f, 1.0f));
+    static_assert(TERMS == 9 || TERMS == 7);
+    const float t = __builtin_amdgcn_rcpf(fmaf(a, TERMS == 9 ? 0.35f : 0.265f, 1.0f));
     float p;
     if constexpr (TERMS == 9) {
         p = fmaf(t, -2.915946483e-02f, 1.440387674e-01f);
@@ -55,10 +55,12 @@ __device__ __forceinline__ float gl_phi_ratio(float a) {
         p = fmaf(p, t, 1.398637337e-01f);
         p = fmaf(p, t, 1.396212914e-01f);
     } else {
-        p = fmaf(t, -9.025423899e-02f, 1.994171632e-01f);
-        p = fmaf(p, t, 8.423240805e-02f);
-        p = fmaf(p, t, 1.575242494e-01f);
-        p = fmaf(p, t, 1.490832449e-01f);
+        p = fmaf(t, -6.778700520e-02f, 1.952730320e-01f);
+        p = fmaf(p, t, -6.636279412e-02f);
+        p = fmaf(p, t, 1.424932325e-01f);
+        p = fmaf(p, t, 8.294662721e-02f);
+        p = fmaf(p, t, 1.078367668e-01f);
+        p = fmaf(p, t, 1.055998295e-01f);
     }
     return t * p;
 }
@@ -86,7 +88,7 @@ __device__ __forceinline__ float gl_act(float z, int act) {
         case GL_ACT_RELU: return z < 0.0f ? 0.0f : z;                  // NaN stays NaN
         case GL_ACT_SILU: return z * gl_sigmoid<FINE>(z);
         case GL_ACT_GELU: {                                            // z Phi(z), Phi(z) = 1 - Phi(-z): no tail is a difference
-            const float h = gl_phi_ratio<__is_same(R, gl_bf16) ? 5 : 9>(fabsf(z)) * gl_gauss<FINE>(fabsf(z));
+            const float h = gl_phi_ratio<__is_same(R, gl_bf16) ? 7 : 9>(fabsf(z)) * gl_gauss<FINE>(fabsf(z));
             return z * (z > 0.0f ? 1.0f - h : h);
         }
         case GL_ACT_TANH: {

@@ -60,6 +60,9 @@ def test_gelu_at_its_ends():
     z = torch.tensor([float("inf"), 3e38, 1e30, -1e30, -40.0, 0.0, float("nan")])
     y = through(z, "gelu")
     assert torch.equal(y[:3], z.double()[:3]) and not y[3:6].any() and y[6].isnan()
+    for dtype in (F32, BF16, F16):
+        ends = through(torch.tensor([float("inf"), -float("inf"), float("nan")]).to(dtype), "gelu")
+        assert ends[0] == float("inf") and ends[1].isnan() and ends[2].isnan()       # as -inf times zero is
 
 
 @gpu
