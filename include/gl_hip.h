@@ -303,9 +303,10 @@ int gl_dense(const void* x, long long x_stride, const void* weight, long long w_
              long long z_stride, long long rows, int inputs, int outputs, int dtype, int out_dtype, int activation,
              void* workspace, long long workspace_bytes, void* stream);
 
-/* Gradients of gl_dense: dz = dy * act'(preactivation).  The products take dz as 16-bit matrix instructions do: bf16 dy: rounded
- *   to bf16; f16 dy: as it is without an activation and with relu, else within 2^-23 |dz| + 2^-49; GL_F32 dy to a 16-bit dtype: within 2^-18 |dz|
- *   (bf16) or as above (f16).  f16 from |dz| = 8 on: half a step of f16; past 65504 infinite.
+/* Gradients of gl_dense: dz = dy * act'(preactivation).  The products take it in 16 bits where dtype has those: bf16 dy: rounded
+ *   to bf16; f16 dy: as it is without an activation and with relu, else within 2^-23 |dz| + min(2^-37, 2^-11 |dz|) + 2^-45;
+ *   GL_F32 dy to a 16-bit dtype: within 2^-17 |dz| (bf16) or as above (f16).  f16 from |dz| = 128 on: half a step of f16; past
+ *   65504 infinite.
  *   dx[r][k] = sum_n dz[r][n] weight[n][k],  dweight[n][k] = sum_r dz[r][n] x[r][k],  dbias[n] = sum_r dz[r][n]
  *   (of the unrounded dz).  dx, dweight, dbias: NULL = not wanted (x may be NULL without dweight, weight without dx).
  *   The residual's gradient is dy.  preactivation may be NULL for GL_ACT_NONE.  rows == 0 writes zero sums.       */

@@ -49,15 +49,15 @@ __device__ __forceinline__ bool gl_halves_give(float sum, gl_scale p, gl_scale q
 }
 
 // A float32 value in two planes of a 16-bit type: v = high + low kSplitStep.  bfloat16 has the range for low to be what high leaves:
-// off by 2^-18 |v|.  float16: what high leaves, 2^24 up, so that values far below high's range stay: off by 2^-23 |v| or 2^-49 where
-// |v| < 8; above, where 2^24 times the rest may not fit, by half a step of float16.  Infinities, NaN and what rounds to infinity
-// stay in high alone.
-template <typename T> constexpr float kSplitStep = __is_same(T, gl_f16) ? 0x1p-24f : 1.0f;
+// off by 2^-17 |v| at most.  float16: what high leaves, 2^20 up, so that values below high's range stay: off by 2^-23 |v| from
+// 2^-14, where high has all its bits, to 128; below, by min(2^-37, 2^-11 |v|), and 2^-45 where low runs out of bits too; above, where
+// 2^20 times the rest may not fit, by half a step of float16.  Infinities, NaN and what rounds to infinity stay in high alone.
+template <typename T> constexpr float kSplitStep = __is_same(T, gl_f16) ? 0x1p-20f : 1.0f;
 template <typename T>
 __device__ __forceinline__ void gl_split(float v, T& high, T& low) {
     high = (T)v;
     float rest = v - (float)high;                            // exact where it is finite
-    if constexpr (__is_same(T, gl_f16)) rest = __builtin_amdgcn_fmed3f(rest * 0x1p24f, -65504.0f, 65504.0f);
+    if constexpr (__is_same(T, gl_f16)) rest = __builtin_amdgcn_fmed3f(rest * 0x1p20f, -65504.0f, 65504.0f);
     low = (T)(fabsf((float)high) < INFINITY ? rest : 0.0f);
 }
 

@@ -970,9 +970,9 @@ SmallSplit small_split(long long I, int J, long long nq) {
 
 // Whether 16-bit products take dz in two planes.  bfloat16 with a dy of its own type: once rounded (half a step a term, what dy
 // itself has lost already: the gradients' error against 64 bits is 0.0023 of them where their own rounding makes 0.0017, and
-// 55 104 x 512 -> 2048 gelu takes 374 us where two planes take 614).  A caller who keeps dy and z in float32 keeps dz to 2^-18
+// 55 104 x 512 -> 2048 gelu takes 374 us where two planes take 614).  A caller who keeps dy and z in float32 keeps dz to 2^-17
 // of it (676 us, rounded once 463).  float16: dz falls below the type's range where dy does not (a mean over a batch's magnitudes
-// has gradients of 2e-8, and act' makes them smaller), and sums over frames bring it back: two planes reach 2^-48 (633 us, rounded
+// has gradients of 2e-8, and act' makes them smaller), and sums over frames bring it back: two planes reach 2^-44 (633 us, rounded
 // once 380).  Without an activation and with relu dz is dy or zero: it serves as it is where dy is of the products' type.
 bool splits_dz(int dtype, int out_dtype, int act) {
     return dtype != GL_F32 && (out_dtype == GL_F32 || (dtype == GL_F16 && act > GL_ACT_RELU));

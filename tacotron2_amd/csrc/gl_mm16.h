@@ -518,8 +518,8 @@ k_mm16(Side P, Side Q, Out o, long long I, int J, long long nq, long long q_per_
 // 256 x 256 tiles of 8 waves: a wave of 128 x 64 needs 12 KiB of LDS reads for 32 matrix instructions, which leaves room under
 // the LDS rate; 4 stages, one barrier a step.  Two workgroups a CU on 256 x 128 tiles, to cover the epilogue, read half again
 // as much from the L2s: 150 us where this one takes 124, and 181 with gelu where this one takes 179.
-// Measured, bf16: 55 104 x 512 x 2048 124 us (930 TF; 1200 without results), with gelu 155 to 175 (two transcendental
-// and eleven other operations a result, which no product runs under: the wave of both SIMD slots is in its epilogue then);
+// Measured, bf16: 55 104 x 512 x 2048 124 us (930 TF; 1200 without results), with gelu 151 to 163 (two transcendental
+// and fifteen other operations a result, which no product runs under: the wave of both SIMD slots is in its epilogue then);
 // x 1025 exp to float32 89 us for the first 1024; gradients: dx 55 104 x 2048 x 512 115 us (1000 TF), dweight in 16 parts 114 to 124.
 template <typename T, typename TO, typename TB, int SEG, int ACT, bool EXTRA, bool LINES, int BM, int BN, int WM, int WN, int RING, bool PT, bool QT>
 __global__ void __launch_bounds__(64 * (BM / WM) * (BN / WN), (BM / WM) * (BN / WN) / 4)

@@ -410,7 +410,7 @@ def dense_backward(dy, x, weight, preactivation=None, *, activation=None, needs=
     """Gradients (dx, dweight, dbias) of :func:`dense` (gl_dense_backward); the residual's gradient is dy itself.
 
     dy, preactivation: (..., outputs), of dense's result type.  dz = dy * act'(preactivation) goes into the products rounded to
-    bfloat16 where dy is bfloat16, in two planes (2^-18 of it) where float32 dy meets 16-bit weights, and in float16 in two planes
+    bfloat16 where dy is bfloat16, in two planes (2^-17 of it) where float32 dy meets 16-bit weights, and in float16 in two planes
     that reach far below the type's range: gradients too small for float16 count in sums over frames.  needs: which of the three are wanted (None comes back
     for the others).  dx, dweight, dbias: tensors that receive them."""
     return _dense_backward(dy, x, weight, preactivation, _activation(activation), needs, (dx, dweight, dbias), workspace)

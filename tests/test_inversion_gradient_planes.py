@@ -1,9 +1,10 @@
 """Gradients of 16-bit dense layers whose dz = dy act'(z) does not fit the type: dy and z kept in float32, and float16's range.
 
 Tolerances.  dz goes into the products in two planes of the type: bfloat16 within (2^-8)^2 |dz| (half a step of what half a step
-left), float16 within (2^-11)^2 |dz| + 2^-49 while |dz| < 8 (the lower plane counts 2^-24; its own half step below the normal
-range is 2^-25).  act' is evaluated to 2^-20 of its scale, sums of n are off by (n + 16) 2^-23 of their magnitudes, and the result
-is rounded once; nothing else is."""
+left), float16 within (2^-11)^2 |dz| while 2^-14 <= |dz| < 128.  Below 2^-14 the higher plane leaves up to 2^-25, or all of dz, of
+which the lower one, counting 2^-20, keeps 11 bits: min(2^-25 2^-12, 2^-11 |dz|), and 2^-45 (half its own smallest step, 2^-24)
+where those run out.  act' is evaluated to 2^-20 of its scale, sums of n are off by (n + 16) 2^-23 of their magnitudes, and the
+result is rounded once; nothing else is."""
 import pytest
 import torch
 
@@ -18,7 +19,9 @@ def gradients64(dy, x, w, z, name, dtype):
     dy, x, w = dy.double(), x.double(), w.double()
     dz = dy * slope64(z.double(), name)
     raw = dy.abs() * scale64(z.double(), name) * 2.0 ** -20 if name else torch.zeros_like(dz)
-    off = raw + u(dtype) ** 2 * dz.abs() + (2.0 ** -49 if dtype == F16 else 0.0)
+    off = raw + u(dtype) ** 2 * dz.abs()
+    if dtype == F16:
+        off = off + (2.0 ** -11 * dz.abs()).clamp(max=2.0 ** -37) + 2.0 ** -45
     M, N = dz.shape
     sums = ((dz @ w, off @ w.abs() + (N + 16) * 2.0 ** -23 * (dz.abs() @ w.abs())),
             (dz.t() @ x, off.t() @ x.abs() + (M + 16) * 2.0 ** -23 * (dz.abs().t() @ x.abs())),
