@@ -37,6 +37,7 @@ import argparse
 import hashlib
 import json
 import os
+import struct
 import subprocess
 import sys
 import time
@@ -90,6 +91,27 @@ def file_sha256(path):
         for blk in iter(lambda: fh.read(1 << 20), b""):
             h.update(blk)
     return h.hexdigest()
+
+
+def kernel_code_sha256(lib_path, kernel):
+    """sha256 of the gfx950 code object inside the library that holds `kernel`: what a stored measurement of it belongs to,
+    whatever other kernels are built into the library beside it.  None if there is none."""
+    with open(lib_path, "rb") as fh:
+        data = fh.read()
+    magic = b"__CLANG_OFFLOAD_BUNDLE__"            # magic, u64 entries, then per entry u64 offset, size, length of its triple
+    at = data.find(magic)
+    while at >= 0:
+        entries, = struct.unpack_from("<Q", data, at + len(magic))
+        p = at + len(magic) + 8
+        for _ in range(entries):
+            off, size, length = struct.unpack_from("<QQQ", data, p)
+            triple = data[p + 24:p + 24 + length]
+            p += 24 + length
+            code = data[at + off:at + off + size]
+            if triple.endswith(b"gfx950") and kernel.encode() in code:
+                return hashlib.sha256(code).hexdigest()
+        at = data.find(magic, p)
+    return None
 
 
 def cpu_baseline_and_parity(mags, x0s, gpu_x, N, H, iters, budget_s):
@@ -153,9 +175,9 @@ def cpu_baseline_all_cores(N, H, T, iters, budget_s, per_utt_s):
 def traffic_for(lib_path, default_cfg, fused):
     """HBM bytes per launch of the dominant kernel from the PMC passes (FETCH_SIZE x2 gfx950 correction +
     WRITE_SIZE, separate rocprofv3 --pmc runs of this same command; tools_pmc_mem.sh), and the MFMA counters of the
-    mel inversion on the bench path (tools_pmc_k1.sh).  Stored measurements: they are stamped only on the headline
-    workload and only when they were taken with the very library this run loaded (sha256 recorded beside them);
-    otherwise null with the reason.  Returns (traffic, note, k1 record or None)."""
+    mel inversion on the bench path (tools_pmc_k1.sh).  Stored measurements: each is stamped only on the headline
+    workload and only when it was taken with the very code of its kernel that this run loaded (sha256 recorded beside
+    it); otherwise null with the reason.  Returns (traffic, note, k1 record or None)."""
     tpath = os.path.join(ROOT, "profiles", "r3_traffic.json")
     if not (default_cfg and fused):
         return None, "only measured for the headline workload on the fused path", None
@@ -163,12 +185,17 @@ def traffic_for(lib_path, default_cfg, fused):
         return None, "profiles/r3_traffic.json absent", None
     with open(tpath) as fh:
         rec = json.load(fh)
-    sha = file_sha256(lib_path)
-    if rec.get("lib_sha256") != sha:
-        return None, (f"profiles/r3_traffic.json was measured with libgl_hip.so sha256 {str(rec.get('lib_sha256'))[:12]}..., "
-                      f"this run loaded {sha[:12]}...: not stamped"), None
-    note = f"rocprofv3 PMC passes of this library (sha256 {sha[:12]}..., git {rec.get('git_head', '?')[:9]})"
-    return rec.get("hbm_bytes_per_launch"), note, rec.get("k1")
+    stored = rec.get("code_sha256", {})
+    code = {k: kernel_code_sha256(lib_path, k) for k in stored}
+    same = {k: code[k] is not None and code[k] == stored[k] for k in stored}
+    k1 = rec.get("k1") if same.get("k_mel_to_mag") else None
+    if not same.get("k_gl2048_regring"):
+        return None, (f"profiles/r3_traffic.json was measured with other code of the loop kernel "
+                      f"({str(stored.get('k_gl2048_regring'))[:12]}..., this run loaded "
+                      f"{str(code.get('k_gl2048_regring'))[:12]}...): not stamped"), k1
+    note = (f"rocprofv3 PMC passes of this kernel's code (code object sha256 {code['k_gl2048_regring'][:12]}..., "
+            f"git {rec.get('git_head', '?')[:9]})")
+    return rec.get("hbm_bytes_per_launch"), note, k1
 
 
 def _events_ms(fn, reps):
@@ -560,7 +587,7 @@ def main():
                 "mfma_flops_issued_per_launch": k1.get("mfma_flops_issued_per_launch"),
                 "mfma_busy_share_of_simd_time": (c["SQ_VALU_MFMA_BUSY_CYCLES"] / (4.0 * c["SQ_BUSY_CU_CYCLES"])
                                                if c.get("SQ_BUSY_CU_CYCLES") else None),
-                "source": "stored rocprofv3 record of this library (kernel trace + --pmc pass, profiles/r3_traffic.json: "
+                "source": "stored rocprofv3 record of this kernel's code (kernel trace + --pmc pass, profiles/r3_traffic.json: "
                           "k1); fp32-input MFMA peak = the fp32 vector peak on gfx950"}
         if rccl is not None:
             out["rccl"] = rccl

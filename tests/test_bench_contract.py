@@ -89,3 +89,23 @@ def test_traffic_record_belongs_to_the_library_in_the_tree():
         pytest.skip("libgl_hip.so changed after the PMC passes: traffic record is stale")
     for f in rec["files"]:
         assert os.path.exists(os.path.join(ROOT, f)), f
+
+
+def test_traffic_record_survives_changes_of_other_kernels(tmp_path):
+    """The record belongs to the code of the kernels it measured, not to everything that is built into the library."""
+    import bench
+    lib = os.path.join(ROOT, "tacotron2_amd", "libgl_hip.so")
+    if not os.path.exists(lib):
+        pytest.skip("library not built")
+    with open(os.path.join(ROOT, "profiles", "r3_traffic.json")) as fh:
+        rec = json.load(fh)
+    data = open(lib, "rb").read()
+    traffic, note, k1 = bench.traffic_for(lib, True, True)
+    assert traffic == rec["hbm_bytes_per_launch"] and k1 == rec["k1"], note
+    other = tmp_path / "other.so"
+    other.write_bytes(data + b"another kernel's code")
+    assert bench.traffic_for(str(other), True, True)[0] == traffic
+    at = data.find(b"k_gl2048_regring", data.find(b"__CLANG_OFFLOAD_BUNDLE__"))
+    other.write_bytes(data[:at] + b"K" + data[at + 1:])              # its own code: no longer the measured one
+    assert bench.traffic_for(str(other), True, True)[0] is None
+    assert bench.traffic_for(lib, False, True)[0] is None and bench.kernel_code_sha256(lib, "k_no_such_kernel") is None

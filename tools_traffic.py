@@ -5,8 +5,8 @@
 
 HBM bytes per launch of the dominant kernel = 2 x FETCH_SIZE (gfx950 counts a 128-byte read request as 64,
 MI355X_MICROARCH.md, HBM section) + WRITE_SIZE, both in KB per dispatch, averaged over the run's 60 dispatches.
-The record names the library it was measured with (sha256 of libgl_hip.so) and the git head: bench.py stamps the
-figure only into runs that loaded that very library.
+The record names the library it was measured with (sha256 of libgl_hip.so), the code objects of the two kernels inside it
+and the git head: bench.py stamps a figure only into runs that loaded that very code.
 """
 import hashlib
 import json
@@ -16,6 +16,9 @@ import subprocess
 import sys
 
 ROOT = os.path.dirname(os.path.abspath(__file__))
+sys.path.insert(0, ROOT)
+from bench import kernel_code_sha256  # noqa: E402
+
 tag = sys.argv[1]
 
 
@@ -40,6 +43,7 @@ rec = {
                   "reads; WRITE_SIZE exact",
     "hbm_bytes_per_launch": int(round((2.0 * fetch_kb + write_kb) * 1024.0)),
     "algorithmic_bytes_per_launch": B * (T * F * 4 + 2 * L * 4),
+    "code_sha256": {k: kernel_code_sha256(lib, k) for k in ("k_gl2048_regring", "k_mel_to_mag")},
     "lib_sha256": hashlib.sha256(open(lib, "rb").read()).hexdigest(),
     "git_head": subprocess.run(["git", "-C", ROOT, "rev-parse", "HEAD"], capture_output=True, text=True).stdout.strip(),
     "files": [f"profiles/{tag}_pmc_mem_pass1.txt", f"profiles/{tag}_pmc_mem_pass2.txt"],
