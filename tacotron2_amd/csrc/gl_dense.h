@@ -32,8 +32,9 @@ struct gl_epilogue {
 };
 
 // A row of a float32 matrix in two planes of f16: x 2^e = h + l 2^-12 with h = f16(x 2^e), l = f16((x 2^e - h) 2^12) and the row's
-// largest |x| 2^e in [2^14, 2^15).  Values of at least 2^-13 have 23 bits in it (float32's last one may be lost: 2^-23 of the value), smaller ones are off by
-// 2^-37 at most: `small` says that there are such.  `wild`: the row holds an infinity or a NaN, and its planes zeros.
+// largest |x| 2^e in [2^14, 2^15).  Values of at least 2^-13 have 23 bits in it (float32's last one may be lost: 2^-23 of the
+// value), smaller ones are off by 2^-37 at most: `small` says that there are such.  `wild`: the row holds an infinity or a NaN,
+// and its planes zeros.
 struct gl_scale {
     int bits;                    // e, small, wild
     static __host__ __device__ gl_scale of(int e, bool small, bool wild) { return {e * 4 + (small ? 1 : 0) + (wild ? 2 : 0)}; }

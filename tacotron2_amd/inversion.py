@@ -211,7 +211,7 @@ def _needs_grad(*tensors):
     return False
 
 
-def _plain_call(what, *tensors):
+def _refuse_transforms(what, *tensors):
     """Refuses what would lose a derivative or the call itself without a word: tangents, and torch.jit.trace."""
     if torch._C._get_tracing_state() is not None:
         raise RuntimeError(f"{what}() cannot be traced: torch.jit.trace would record its empty result alone")
@@ -334,7 +334,7 @@ def dense(x, weight, bias=None, *, activation=None, residual=None, out_dtype=Non
             y = calls.dense(x, weight, bias, residual, preactivation, out_dtype, act)
             if y is not None:
                 return y
-    _plain_call("dense", x, weight, bias, residual)
+    _refuse_transforms("dense", x, weight, bias, residual)
     if _needs_grad(x, weight, bias, residual):
         if out is not None or preactivation is not None:
             raise ValueError("out= and preactivation= belong to the form without gradients: use torch.no_grad()")
@@ -357,7 +357,7 @@ def _dense_backward(dy, x, weight, z, act, need, outs, workspace):
             grads = calls.dense_backward(dy, x, weight, z, act, bool(need[0]), bool(need[1]), bool(need[2]))
             if grads is not None:
                 return grads
-    _plain_call("dense_backward", dy, x, weight, z)
+    _refuse_transforms("dense_backward", dy, x, weight, z)
     _tensor(x, "x")
     if x.dim() < 1 or not isinstance(weight, torch.Tensor) or weight.dim() != 2:
         raise ValueError("x must be (..., inputs) and weight (outputs, inputs)")
@@ -411,8 +411,8 @@ def dense_backward(dy, x, weight, preactivation=None, *, activation=None, needs=
 
     dy, preactivation: (..., outputs), of dense's result type.  dz = dy * act'(preactivation) goes into the products rounded to
     bfloat16 where dy is bfloat16, in two planes (2^-17 of it) where float32 dy meets 16-bit weights, and in float16 in two planes
-    that reach far below the type's range: gradients too small for float16 count in sums over frames.  needs: which of the three are wanted (None comes back
-    for the others).  dx, dweight, dbias: tensors that receive them."""
+    that reach far below the type's range: gradients too small for float16 count in sums over frames.  needs: which of the
+    three are wanted (None comes back for the others).  dx, dweight, dbias: tensors that receive them."""
     return _dense_backward(dy, x, weight, preactivation, _activation(activation), needs, (dx, dweight, dbias), workspace)
 
 
@@ -524,7 +524,7 @@ def group_norm(x, groups, weight=None, bias=None, *, eps=1e-5, activation=None, 
             y = calls.group_norm(x, weight, bias, lengths, stats, int(groups), act, eps)
             if y is not None:
                 return y
-    _plain_call("group_norm", x, weight, bias)
+    _refuse_transforms("group_norm", x, weight, bias)
     if _needs_grad(x, weight, bias):
         if out is not None or stats is not None:
             raise ValueError("out= and stats= belong to the form without gradients: use torch.no_grad()")
@@ -541,7 +541,7 @@ def _group_norm_backward(dy, x, groups, stats, weight, bias, act, lengths, need,
                                               bool(need[2]))
             if grads is not None:
                 return grads
-    _plain_call("group_norm_backward", dy, x, stats, weight, bias)
+    _refuse_transforms("group_norm_backward", dy, x, stats, weight, bias)
     groups, B, T, C, lens = _norm_args(x, groups, weight, bias, lengths)
     device, dtype = x.device, x.dtype
     _tensor(dy, "dy", device, dtype, x.shape)
