@@ -82,6 +82,17 @@ def test_float16_layers_round_their_results_alone(M, K, N, name):
 
 
 @gpu
+@pytest.mark.parametrize("dtype,od", [(F16, F16), (BF16, F32)])
+@pytest.mark.parametrize("M", [32980, 32960, 33025])
+def test_planes_change_inside_a_pair_of_steps(M, dtype, od):
+    """The walking kernel takes steps of 32 frames in twos; the last part of these has an odd number of them a plane."""
+    K, N = 512, 2048
+    x, w = randn((M, K), dtype, 1).cuda(), randn((N, K), dtype, 2, K ** -0.5).cuda()
+    z, dy = randn((M, N), od, 3).cuda(), randn((M, N), od, 4, 0.1).cuda()
+    check(dy, x, w, z, "silu", dtype)
+
+
+@gpu
 @pytest.mark.parametrize("dy_dtype,size", [(F32, 1.8e-8), (F16, 4e-6)])
 @pytest.mark.parametrize("M,K,N", [(3000, 64, 64), (30000, 512, 513), (30000, 512, 512), (30000, 72, 256)])
 def test_float16_gradients_below_its_range_reach_the_sums(M, K, N, dy_dtype, size):
